@@ -197,7 +197,7 @@ def _plain_keep(x, form, group):
     v[:, :width] = x
     v = v.reshape(rows, parts, group)
     scale = v.abs().amax(-1, keepdim=True) / QMAX[form]
-    u = torch.where(scale > 0, v / scale, torch.zeros_like(v))
+    u = torch.where(scale > 0, v * (1 / scale), torch.zeros_like(v))
     u = u.round() if form == "int8" else u.to(torch.float8_e4m3fn).float()
     back = (u * scale).reshape(rows, parts * group)[:, :width]
     return back, scale[..., 0]

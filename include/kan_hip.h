@@ -35,6 +35,8 @@ extern "C" {
 /* dtype codes */
 #define KAN_DTYPE_F32 0
 #define KAN_DTYPE_F64 1
+#define KAN_DTYPE_BF16 2 /* residual norm, 8-bit activations and grouped products only */
+#define KAN_DTYPE_F16 3  /* as KAN_DTYPE_BF16 */
 
 /* status codes */
 #define KAN_OK 0
@@ -393,6 +395,84 @@ int kan_hip_refit_gram(int dtype, const void* x_t, const void* grid_old, const v
                        double* gram, double* cross, int64_t n, int64_t in_features,
                        int64_t grid_size_old, int64_t grid_size_new, int64_t spline_order,
                        void* stream);
+
+/* ---- operators of a residual stack of routed experts ----------------------
+ * No reference counterpart (the reference has single layers and plain stacks).
+ * Types: KAN_DTYPE_F32, KAN_DTYPE_BF16, KAN_DTYPE_F16; sums and statistics are
+ * held in FP32.  Nothing waits for the host, and no sum uses atomics. */
+
+/* Residual norm: the norm after a block, its gate and residual scale, and the
+ * norm before the next block, over n rows of C values:
+ *   u  = post_weight * y / sqrt(mean(y^2) + eps)    (u = y without post_weight)
+ *   x' = x + scale * act(gate) * u
+ *   h  = pre_weight * x' / sqrt(mean(x'^2) + eps)
+ * x, x_out are in xdtype (ydtype or FP32); y, gate, h_out in ydtype;
+ * post_weight, pre_weight, scale [C] in wdtype (scale NULL: scale_const).  y
+ * may be NULL (x' = x, then x_out too is NULL).  gate [gate_rows, gate_cols]:
+ * gate_rows divides n, a gate row serves n / gate_rows consecutive rows;
+ * gate_cols is 1 or C.  h_out and pre_weight go together.  rstd [2, n]
+ * (optional) receives 1 / sqrt(mean(y^2) + eps) and 1 / sqrt(mean(x'^2) + eps),
+ * each where its norm is taken; the backward reads it. */
+#define KAN_GATE_IDENTITY 0
+#define KAN_GATE_SIGMOID 1
+#define KAN_GATE_TANH 2
+#define KAN_GATE_SILU 3
+int kan_hip_residual_norm(int xdtype, int ydtype, int wdtype, const void* x, const void* y,
+                          const void* gate, const void* post_weight, const void* pre_weight,
+                          const void* scale, double scale_const, int gate_act, int64_t gate_rows,
+                          int64_t gate_cols, int64_t n, int64_t C, double eps, void* x_out,
+                          void* h_out, float* rstd, void* stream);
+/* Its gradients, from those of x' (grad_x_out) and h (grad_h), either of which
+ * may be NULL for zeros, and the forward's inputs (x' itself is not needed).
+ * Any output may be NULL.  grad_gate has the gate's shape.  gate_rows 0 in the
+ * workspace query: no gate.  With n = 0 nothing is written. */
+int kan_hip_residual_norm_backward_workspace(int64_t gate_rows, int64_t gate_cols, int64_t n,
+                                             int64_t C, size_t* bytes);
+int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const void* grad_x_out,
+                                   const void* grad_h, const void* x, const void* y,
+                                   const void* gate, const void* post_weight,
+                                   const void* pre_weight, const void* scale, double scale_const,
+                                   int gate_act, int64_t gate_rows, int64_t gate_cols, int64_t n,
+                                   int64_t C, const float* rstd, void* grad_x, void* grad_y,
+                                   void* grad_gate, void* grad_post, void* grad_pre,
+                                   void* grad_scale, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* Activations kept in 8 bits: rows of C values cut into groups of `group` (32,
+ * 64, 128 or 256; the last of a row may be short), scale [rows,
+ * ceil(C / group)] = max|x| / qmax (127 for int8, 448 for e4m3) and q [rows, C]
+ * = round(x * (1 / scale)).  A scale below the smallest normal float is kept as
+ * 0 (the group comes back as zeros); a group with an infinity or NaN gets
+ * scale NaN and comes back as NaN.  row_stride: elements between x's rows. */
+#define KAN_ACT8_NONE 0
+#define KAN_ACT8_INT8 1
+#define KAN_ACT8_E4M3 2
+int kan_hip_act8_quantize(int dtype, int format, const void* x, int64_t row_stride, int64_t rows,
+                          int64_t C, int64_t group, void* q, float* scale, void* stream);
+int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* scale, int64_t rows,
+                            int64_t C, int64_t group, void* out, void* stream);
+
+/* Products grouped by expert: rows sorted by expert, expert e having the rows
+ * offsets[e] .. offsets[e + 1] - 1 of T (offsets [E + 1] on the device, int32
+ * or int64, ascending from 0; each is taken within 0 .. T and as the running
+ * maximum, so that no value of theirs leads outside the operands).  With
+ * weights w [E, N, K]:
+ *   KAN_GROUPED_FORWARD  a = x [T, K],  b = w:  out y [T, N],  y[t] = w[e] x[t]
+ *   KAN_GROUPED_INPUT    a = dy [T, N], b = w:  out dx [T, K], dx[t] = w[e]^T dy[t]
+ *   KAN_GROUPED_WEIGHT   a = dy [T, N], b = x:  out dw [E, N, K], the sum of
+ *                        dy[t] x[t]^T over the expert's rows (zeros without any)
+ * Rows from offsets[E] on get zeros.  The weight product also takes b as 8-bit
+ * rows (b_format, with b_scale and b_group as kan_hip_act8_quantize keeps
+ * them; KAN_ACT8_NONE otherwise). */
+#define KAN_GROUPED_FORWARD 0
+#define KAN_GROUPED_INPUT 1
+#define KAN_GROUPED_WEIGHT 2
+int kan_hip_grouped_matmul_workspace(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K,
+                                     size_t* bytes);
+int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
+                           const float* b_scale, int64_t b_group, const void* offsets,
+                           int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
 
 /* Kernel-level timing (measurement support; no counterpart in the
  * reference, whose benchmarks time with torch.profiler,

@@ -1,0 +1,290 @@
+"""grouped_linear against products in float64, forward and gradients.
+
+Bounds: a sum of L products in float32 is off by at most L + 16 roundings of
+2^-24 of the sum of magnitudes (16: what a matrix instruction truncates inside),
+plus one rounding to the result's type."""
+
+import pytest
+import torch
+
+from torchsplinekan_amd import grouped_linear, quantize_activation
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+HALF_ULP = {F32: 2.0 ** -24, BF16: 2.0 ** -8, F16: 2.0 ** -11}
+DTYPES = [F32, BF16, F16]
+
+
+def _offsets(counts, dtype=torch.int32):
+    return torch.tensor([0] + list(counts)).cumsum(0).to(dtype)
+
+
+def _counts(T, E, seed):
+    g = torch.Generator().manual_seed(seed)
+    p = torch.softmax(torch.randn(E, generator=g) * 1.5, 0)
+    return torch.bincount(torch.multinomial(p, T, replacement=True, generator=g),
+                          minlength=E).tolist()
+
+
+def _bound(got, want, mag, terms, what):
+    got = got.detach().cpu()
+    assert got.shape == want.shape, what
+    fp32 = (terms + 16) * 2.0 ** -24 * mag
+    tol = fp32 + HALF_ULP[got.dtype] * (want.abs() + fp32)
+    if got.dtype == F16:
+        tol = tol + 2.0 ** -25
+    bad = (got.double() - want).abs() > tol
+    assert not bool(bad.any()), f"{what}: {int(bad.sum())} of {bad.numel()} outside the bound"
+
+
+def _inputs(T, E, K, N, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(T, K, generator=g).to(dtype)
+    w = (torch.randn(E, N, K, generator=g) * max(K, 1) ** -0.5).to(dtype)
+    dy = torch.randn(T, N, generator=g).to(dtype)
+    return x, w, dy
+
+
+def _check(x, w, dy, offsets, ends=None, checkpoint=None, group=128):
+    """ends: where the groups end, when the offsets themselves do not say."""
+    T, K = x.shape
+    E, N, _ = w.shape
+    xd, wd = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = grouped_linear(xd, wd, offsets.cuda(), checkpoint=checkpoint, group=group)
+    assert y.dtype == x.dtype
+    dx, dw = torch.autograd.grad(y, [xd, wd], dy.cuda())
+    with torch.no_grad():
+        assert torch.equal(grouped_linear(xd, wd, offsets.cuda()), y)
+    kept = x if checkpoint is None else quantize_activation(x, group, checkpoint).dequantize(F32)
+    ends = offsets.tolist()[1:] if ends is None else ends
+    X, W, D, Q = x.double(), w.double(), dy.double(), kept.double()
+    # (a value q * scale takes part in the 16-bit products rounded to their type)
+    extra = 0.0 if checkpoint is None or x.dtype == F32 else HALF_ULP[x.dtype]
+    lo = 0
+    for e in range(E):
+        hi = max(lo, ends[e])
+        r = slice(lo, hi)
+        _bound(y[r], X[r] @ W[e].t(), X[r].abs() @ W[e].abs().t(), K, f"y of {e}")
+        _bound(dx[r], D[r] @ W[e], D[r].abs() @ W[e].abs(), N, f"dx of {e}")
+        mag = D[r].abs().t() @ Q[r].abs()
+        _bound(dw[e], D[r].t() @ Q[r], mag * (1 + extra * 2.0 ** 24 / (hi - lo + 16)), hi - lo,
+               f"dw of {e}")
+        lo = hi
+    assert not bool(y[lo:].any()) and not bool(dx[lo:].any())
+
+
+# ---------------------------------------------------------------------------
+# CPU
+# ---------------------------------------------------------------------------
+
+def test_cpu_path_against_differences():
+    x, w, dy = _inputs(9, 3, 4, 5, torch.float64)
+    off = _offsets([4, 0, 3])
+    x.requires_grad_(), w.requires_grad_()
+    torch.autograd.gradcheck(lambda a, b: grouped_linear(a, b, off), (x, w))
+    y = grouped_linear(x, w, off)
+    torch.testing.assert_close(y[:4], x[:4] @ w[0].t())
+    assert not bool(y[7:].any())
+
+
+def test_cpu_checkpoint():
+    x, w, dy = _inputs(9, 2, 40, 5, F32)
+    off = _offsets([4, 5])
+    x.requires_grad_(), w.requires_grad_()
+    y = grouped_linear(x, w, off, checkpoint="int8", group=32)
+    assert torch.equal(y, grouped_linear(x, w, off))
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    kept = quantize_activation(x[:4], 32).dequantize()
+    torch.testing.assert_close(dw[0], dy[:4].t() @ kept)
+    torch.testing.assert_close(dx[4:], dy[4:] @ w[1])
+
+
+@pytest.mark.parametrize("x,w,off,kw,text", [
+    (torch.zeros(4), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32), {}, "must be"),
+    (torch.zeros(4, 5), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32), {}, "equal K"),
+    (torch.zeros(4, 4), torch.zeros(2, 3, 4).bfloat16(), torch.zeros(3, dtype=torch.int32), {},
+     "share a dtype"),
+    (torch.zeros(4, 4), torch.zeros(2, 3, 4), torch.zeros(2, dtype=torch.int32), {}, "offsets must"),
+    (torch.zeros(4, 4), torch.zeros(2, 3, 4), torch.zeros(3), {}, "int32 or int64"),
+    (torch.zeros(4, 4), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32),
+     dict(checkpoint="int4"), "format must"),
+    (torch.zeros(4, 4), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32),
+     dict(checkpoint="int8", group=100), "group must"),
+])
+def test_refusals(x, w, off, kw, text):
+    with pytest.raises(RuntimeError, match=text):
+        grouped_linear(x, w, off, **kw)
+
+
+def test_c_entry_refusals():
+    lib = pytest.importorskip("torchsplinekan_amd._lib")
+    f = lib.LIB.kan_hip_grouped_matmul
+    p = 4096
+    tail = (8, 2, 16, 16, p, None, 0, None)
+    assert f(1, 0, p, p, 0, None, 0, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 3, p, p, 0, None, 0, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 0, p, p, 1, p, 128, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert "weight product only" in lib.last_error()
+    assert f(2, 2, p, p, 5, p, 128, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 2, p, p, 1, p, 100, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 2, p, p, 1, None, 128, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 0, None, p, 0, None, 0, p, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 0, p, p, 0, None, 0, None, 0, *tail) == lib.KAN_ERR_INVALID
+    assert f(2, 0, p, p, 0, None, 0, p, 0, -1, 2, 16, 16, p, None, 0, None) == lib.KAN_ERR_INVALID
+    assert f(2, 0, p, p, 0, None, 0, p, 0, 8, 1 << 21, 16, 16, p, None, 0,
+             None) == lib.KAN_ERR_LIMIT
+    assert f(2, 0, None, None, 0, None, 0, None, 0, 0, 2, 16, 16, None, None, 0,
+             None) == lib.KAN_OK
+
+
+# ---------------------------------------------------------------------------
+# GPU
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(1, 1), (1, 70), (33, 1), (8, 8), (16, 48), (64, 64), (100, 60),
+                                 (301, 257), (136, 520), (128, 1032)])
+@pytest.mark.parametrize("counts", [[1], [5, 0, 1, 40], [0, 0, 70, 0], [64, 128, 130], [300, 3]])
+def test_sizes(counts, K, N, dtype):
+    x, w, dy = _inputs(sum(counts), len(counts), K, N, dtype)
+    _check(x, w, dy, _offsets(counts))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("E", [1, 2, 16, 63, 64, 65, 130])
+@pytest.mark.parametrize("T", [1, 7, 200, 1500])
+def test_experts(T, E, dtype):
+    """Numbers of experts on either side of a wave's 64 lanes, most of them
+    without rows where T is small."""
+    x, w, dy = _inputs(T, E, 40, 72, dtype, seed=E)
+    _check(x, w, dy, _offsets(_counts(T, E, seed=T + E), torch.int64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,E,K,N", [(3000, 5, 512, 320), (2500, 3, 257, 1000),
+                                     (700, 2, 2048, 96), (5000, 4, 96, 2000)])
+def test_larger(T, E, K, N, dtype):
+    x, w, dy = _inputs(T, E, K, N, dtype)
+    _check(x, w, dy, _offsets(_counts(T, E, seed=1)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("K,N,group", [(1, 3, 32), (100, 60, 64), (136, 128, 32), (301, 257, 128),
+                                       (512, 320, 256), (129, 72, 128)])
+def test_kept_rows(K, N, group, format, dtype):
+    counts = [37, 0, 200, 1, 64]
+    x, w, dy = _inputs(sum(counts), len(counts), K, N, dtype)
+    _check(x, w, dy, _offsets(counts), checkpoint=format, group=group)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offsets,ends", [
+    ([0, 10, 30, 30], [10, 30, 30]),          # rows past the last group
+    ([0, 0, 0, 0], [0, 0, 0]),                # no group has any
+    ([0, 40, 20, 70], [40, 40, 70]),          # descending: the running maximum
+    ([0, -5, 200, 90], [0, 90, 90]),          # outside 0 .. T
+])
+def test_offsets(offsets, ends, dtype):
+    x, w, dy = _inputs(90, 3, 72, 80, dtype)
+    for t in (torch.int32, torch.int64):
+        _check(x, w, dy, torch.tensor(offsets, dtype=t), ends=ends)
+
+
+@pytest.mark.gpu
+def test_empty():
+    off = _offsets([0, 0]).cuda()
+    for T, K, N, E in [(0, 8, 8, 2), (5, 0, 8, 2), (5, 8, 0, 2)]:
+        x = torch.randn(T, K, device="cuda", requires_grad=True)
+        w = torch.randn(E, N, K, device="cuda", requires_grad=True)
+        y = grouped_linear(x, w, off)
+        assert y.shape == (T, N) and not bool(y.any())
+        dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+        assert not bool(dx.any()) and not bool(dw.any())
+    y = grouped_linear(torch.randn(5, 8, device="cuda"), torch.randn(0, 3, 8, device="cuda"),
+                       _offsets([]).cuda())
+    assert y.shape == (5, 3) and not bool(y.any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_alignment(dtype):
+    """Views: rows that start off 16 bytes, transposed weights, transposed
+    gradients, and another stream."""
+    x, w, dy = _inputs(150, 3, 64, 72, dtype)
+    off = _offsets([50, 20, 80]).cuda()
+    want = grouped_linear(x.cuda(), w.cuda(), off)
+    big = torch.zeros(150 * 64 + 1, dtype=dtype, device="cuda")
+    big[1:] = x.cuda().reshape(-1)
+    xv = big[1:].view(150, 64)
+    wv = w.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = grouped_linear(xv, wv, off)
+    torch.cuda.current_stream().wait_stream(side)
+    tol = 80 * 2.0 ** -24 + 2 * HALF_ULP[dtype]
+    mag = x.double().abs() @ w.double().abs().amax(0).t()
+    assert bool(((got.double() - want.double()).abs().cpu() <= tol * mag).all())
+    xg, wg = xv.detach().requires_grad_(), w.cuda().requires_grad_()
+    dyt = dy.cuda().t().contiguous().t()
+    dx, dw = torch.autograd.grad(grouped_linear(xg, wg, off), [xg, wg], dyt)
+    lo = 0
+    for e, c in enumerate([50, 20, 80]):
+        r = slice(lo, lo + c)
+        D, X = dy[r].double(), x[r].double()
+        _bound(dx[r], D @ w[e].double(), D.abs() @ w[e].double().abs(), 72, "dx")
+        _bound(dw[e], D.t() @ X, D.abs().t() @ X.abs(), c, "dw")
+        lo += c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("K,N", [(64, 64), (77, 65)])
+def test_values_that_are_not_finite(K, N, dtype):
+    """A row's infinity or NaN reaches that row's outputs and its expert's
+    weight gradient, nothing else."""
+    counts = [30, 40, 50]
+    x, w, dy = _inputs(120, 3, K, N, dtype)
+    x[29, 3] = float("nan")           # the last row of expert 0
+    x[30, 5] = float("inf")           # the first of expert 1
+    w[1, :, 5] = w[1, :, 5].abs() + 1
+    xd, wd = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = grouped_linear(xd, wd, _offsets(counts).cuda())
+    dx, dw = torch.autograd.grad(y, [xd, wd], dy.cuda())
+    bad = ~y.isfinite().all(1).cpu()
+    assert bad.nonzero().flatten().tolist() == [29, 30]
+    assert bool(y[29].isnan().all()) and bool((y[30] == float("inf")).all())
+    assert bool(dx.isfinite().all())
+    finite = dw.isfinite().cpu()
+    assert bool(finite[2].all())
+    assert bool(dw[0, :, 3].isnan().all()) and bool(finite[0, :, 4:].all())
+    assert not bool(finite[1, :, 5].any()) and bool(finite[1, :, 6:].all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_same_bits_every_time(dtype):
+    x, w, dy = _inputs(2000, 9, 200, 264, dtype)
+    off = _offsets(_counts(2000, 9, 4)).cuda()
+    runs = []
+    for _ in range(2):
+        xd, wd = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+        y = grouped_linear(xd, wd, off, checkpoint="int8")
+        runs.append([y, *torch.autograd.grad(y, [xd, wd], dy.cuda())])
+    for u, v in zip(*runs):
+        assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+def test_float64_and_other_devices_are_refused():
+    x = torch.zeros(2, 4, dtype=torch.float64, device="cuda")
+    off = _offsets([2]).cuda()
+    with pytest.raises(RuntimeError, match="FP32, BF16 and FP16"):
+        grouped_linear(x, torch.zeros(1, 3, 4, dtype=torch.float64, device="cuda"), off)
+    with pytest.raises(RuntimeError, match="one device"):
+        grouped_linear(x.float(), torch.zeros(1, 3, 4), off)

@@ -19,6 +19,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libkan_hip.
 
 KAN_DTYPE_F32 = 0
 KAN_DTYPE_F64 = 1
+KAN_DTYPE_BF16 = 2  # the operators beside the KAN layers only
+KAN_DTYPE_F16 = 3
 KAN_OK = 0
 KAN_ERR_INVALID = 1
 KAN_ERR_LIMIT = 2
@@ -30,6 +32,7 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
+_dbl = ctypes.c_double
 
 # name -> (restype, argtypes)
 SIGNATURES = {
@@ -95,6 +98,16 @@ SIGNATURES = {
                                 _vp]),
     "kan_hip_edge_reg_backward": (_int, [_int, _vp, _vp, _i64, ctypes.c_double, ctypes.c_double,
                                          _vp, _sz, _vp, _vp]),
+    "kan_hip_residual_norm": (_int, [_int] * 3 + [_vp] * 6 + [_dbl, _int] + [_i64] * 4 + [_dbl]
+                              + [_vp] * 4),
+    "kan_hip_residual_norm_backward_workspace": (_int, [_i64] * 4 + [ctypes.POINTER(_sz)]),
+    "kan_hip_residual_norm_backward": (_int, [_int] * 3 + [_vp] * 8 + [_dbl, _int] + [_i64] * 4
+                                       + [_vp] * 8 + [_sz, _vp]),
+    "kan_hip_act8_quantize": (_int, [_int, _int, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "kan_hip_act8_dequantize": (_int, [_int, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "kan_hip_grouped_matmul_workspace": (_int, [_int, _int] + [_i64] * 4 + [ctypes.POINTER(_sz)]),
+    "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
+                               + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
     "kan_hip_timing_enable": (_int, [_int]),
     "kan_hip_timing_read": (_int, [_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i64),
                                    ctypes.POINTER(ctypes.c_double)]),
@@ -150,6 +163,19 @@ def dtype_code(dtype: torch.dtype) -> int:
     if dtype == torch.float64:
         return KAN_DTYPE_F64
     raise RuntimeError(f"only FP32 and FP64 inputs are supported, got {dtype}")
+
+
+OPERATOR_DTYPES = {torch.float32: KAN_DTYPE_F32, torch.bfloat16: KAN_DTYPE_BF16,
+                   torch.float16: KAN_DTYPE_F16}
+
+
+def operator_dtype_code(dtype: torch.dtype, who: str) -> int:
+    """dtype code of the operators beside the KAN layers (residual norm, 8-bit
+    activations, grouped products)."""
+    code = OPERATOR_DTYPES.get(dtype)
+    if code is None:
+        raise RuntimeError(f"{who}: only FP32, BF16 and FP16 tensors are supported, got {dtype}")
+    return code
 
 
 def ptr(t):

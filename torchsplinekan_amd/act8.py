@@ -1,0 +1,164 @@
+"""Activations kept in 8 bits between the forward and the backward pass (no
+reference counterpart; the reference bounds memory by recomputation only).
+
+``quantize_activation`` keeps a tensor as 8-bit values with one float32 scale
+for every group of its last axis; ``checkpoint_8bit`` runs a layer that keeps
+nothing but its input, in 8 bits, and runs again in the backward pass: a KAN
+layer then holds 1 byte an input instead of the 4 (R + 1) of its basis.
+Device tensors run on the kernels of csrc/kan_act8.hip, CPU tensors on the same
+formulas in torch.
+"""
+
+from dataclasses import dataclass
+from typing import Callable, Optional, Sequence
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import fused as _fused
+
+_C = _fused._C
+FORMATS = {"int8": (1, 127.0, torch.int8), "e4m3": (2, 448.0, torch.float8_e4m3fn)}
+GROUPS = (32, 64, 128, 256)
+
+
+def _req(cond: bool, *msg) -> None:
+    if not cond:
+        raise RuntimeError("".join(str(m) for m in msg))
+
+
+def check_format(who: str, group: int, format: str) -> None:
+    _req(format in FORMATS, who, ": format must be 'int8' or 'e4m3', got ", repr(format))
+    _req(group in GROUPS, who, ": group must be 32, 64, 128 or 256, got ", group)
+
+
+def _native(who: str):
+    if _C is None:
+        raise RuntimeError(f"{who}: device tensors need libkan_hip.so; build it with "
+                           "`python -m torchsplinekan_amd.build_lib`")
+    return _C._lib
+
+
+@dataclass
+class Activation8:
+    """A tensor in 8 bits: q (int8 or float8_e4m3fn, the tensor's shape), scale
+    [..., ceil(C / group)] float32, and the type it had.  A group that held an
+    infinity or a NaN has scale NaN and comes back as NaN; one whose scale
+    would be below the smallest normal float32 comes back as zeros."""
+
+    q: torch.Tensor
+    scale: torch.Tensor
+    group: int
+    format: str
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.q.numel() + 4 * self.scale.numel()
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """The tensor, each value q * scale rounded to dtype (default: its own)."""
+        dtype = self.dtype if dtype is None else dtype
+        if not self.q.is_cuda or self.q.numel() == 0:
+            return _dequantize_cpu(self, dtype)
+        lib = _native("dequantize_activation")
+        out = torch.empty(self.q.shape, dtype=dtype, device=self.q.device)
+        C = out.shape[-1]
+        with torch.cuda.device(out.device):
+            lib.check(lib.LIB.kan_hip_act8_dequantize(
+                lib.operator_dtype_code(dtype, "dequantize_activation"), FORMATS[self.format][0],
+                lib.ptr(self.q), lib.ptr(self.scale), out.numel() // C, C, self.group,
+                lib.ptr(out), lib.stream_of(out.device)))
+        return out
+
+
+def _quantize_cpu(x, group, format):
+    _, qmax, qdtype = FORMATS[format]
+    C = x.shape[-1]
+    parts = -(-C // group)
+    v = torch.nn.functional.pad(x.float(), (0, parts * group - C)).reshape(*x.shape[:-1], parts,
+                                                                           group)
+    finite = v.isfinite().all(-1, keepdim=True)
+    scale = v.abs().amax(-1, keepdim=True) / qmax
+    scale = torch.where(scale < torch.finfo(torch.float32).tiny, 0.0, scale)
+    u = torch.where((scale > 0) & finite, v * (1 / scale), torch.zeros(()))
+    u = u.round() if format == "int8" else u
+    q = u.reshape(*x.shape[:-1], parts * group)[..., :C].to(qdtype).contiguous()
+    return q, torch.where(finite, scale, torch.nan)[..., 0]
+
+
+def _dequantize_cpu(a, dtype):
+    C = a.q.shape[-1]
+    scale = a.scale.repeat_interleave(a.group, -1)[..., :C]
+    return (a.q.float() * scale).to(dtype)
+
+
+@torch.no_grad()
+def quantize_activation(x: torch.Tensor, group: int = 128, format: str = "int8") -> Activation8:
+    """x [..., C] in 8 bits: for every group of `group` (32, 64, 128 or 256)
+    consecutive values of the last axis, scale = max|x| / qmax (127 for "int8",
+    448 for "e4m3") and q = round(x * (1 / scale)) to nearest, ties to even."""
+    who = "quantize_activation"
+    check_format(who, group, format)
+    _req(x.dim() >= 1, who, ": x must have at least one dimension")
+    _req(x.dtype in (torch.float32, torch.bfloat16, torch.float16), who,
+         ": only FP32, BF16 and FP16 tensors are supported, got ", x.dtype)
+    if not x.is_cuda or x.numel() == 0:
+        q, scale = _quantize_cpu(x, group, format)
+        return Activation8(q, scale, group, format, x.dtype)
+    lib = _native(who)
+    C = x.shape[-1]
+    rows = x.numel() // C
+    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C):
+        x = x.contiguous()
+    ldx = x.stride(0) if x.dim() == 2 else C
+    code, _, qdtype = FORMATS[format]
+    q = torch.empty(x.shape, dtype=qdtype, device=x.device)
+    scale = torch.empty(*x.shape[:-1], -(-C // group), dtype=torch.float32, device=x.device)
+    with torch.cuda.device(x.device):
+        lib.check(lib.LIB.kan_hip_act8_quantize(
+            lib.OPERATOR_DTYPES[x.dtype], code, lib.ptr(x), ldx, rows, C, group, lib.ptr(q),
+            lib.ptr(scale), lib.stream_of(x.device)))
+    return Activation8(q, scale, group, format, x.dtype)
+
+
+class _Checkpoint8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, fn, args, group, format, x, *params):
+        ctx.fn, ctx.args = fn, args
+        ctx.kept = quantize_activation(x, group, format)
+        ctx.params = params
+        with torch.no_grad():
+            return fn(x, *args)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        x = ctx.kept.dequantize().requires_grad_(ctx.needs_input_grad[4])
+        with torch.enable_grad():
+            out = ctx.fn(x, *ctx.args)
+        outs = [out] if isinstance(out, torch.Tensor) else list(out)
+        pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
+        wanted = [t for t, need in zip((x, *ctx.params), ctx.needs_input_grad[4:]) if need]
+        got = iter(torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs],
+                                       allow_unused=True) if pairs and wanted
+                   else [None] * len(wanted))
+        return (None, None, None, None,
+                *(next(got) if need else None for need in ctx.needs_input_grad[4:]))
+
+
+def checkpoint_8bit(fn: Callable, x: torch.Tensor, *args, group: int = 128, format: str = "int8",
+                    params: Optional[Sequence[torch.Tensor]] = None):
+    """fn(x, *args), keeping x in 8 bits for the backward pass and nothing that
+    fn makes: the backward restores x and runs fn again, so gradients are those
+    of fn at the restored x (the output is exact).  Gradients reach x and
+    `params` (default: fn.parameters() of a module; args are taken as
+    constants).  fn must give the same result each time: no random numbers."""
+    check_format("checkpoint_8bit", group, format)
+    if params is None:
+        params = tuple(fn.parameters()) if isinstance(fn, nn.Module) else ()
+    params = tuple(p for p in params if p.requires_grad)
+    if not (torch.is_grad_enabled() and (x.requires_grad or params)):
+        return fn(x, *args)
+    return _Checkpoint8.apply(fn, args, group, format, x, *params)

@@ -1,0 +1,485 @@
+// The norm after a block, its gate and residual scale, and the norm before
+// the next block, in one pass over the rows of a residual stream:
+//   u  = post * y r1,           r1 = (mean(y^2) + eps)^(-1/2)    (u = y without post)
+//   x' = x + s a(g) u,          a = identity, sigmoid, tanh or silu
+//   h  = pre * x' r2,           r2 = (mean(x'^2) + eps)^(-1/2)
+// and its backward pass: with t = dh pre, xh = x' r2 and yh = y r1,
+//   D  = dx' + r2 (t - xh mean(t xh)),   dx = D,   dpre = sum_rows dh xh
+//   v  = D s a(g),  w = v post
+//   dy = r1 (w - yh mean(w yh)),         dpost = sum_rows v yh     (dy = v without post)
+//   dg = D s u a'(g), summed over what g is broadcast over;  ds = sum_rows D a(g) u.
+//
+// All arithmetic is in float32, rounded once where a result is stored: x' is
+// recomputed from x and y in the backward (the same bytes as reading x'), so
+// both passes see the unrounded stream.  Sums over rows go through one partial
+// row per block and are added in block order: no atomics, the same bits every
+// time.
+#include "kan_types.h"
+
+namespace kan {
+
+namespace {
+
+enum GateKind {
+  kGateNone = 0,
+  kGateElement = 1,   // [n, C]
+  kGateToken = 2,     // [n]
+  kGateRows = 3,      // [n / L, C]: one row of the gate for L rows, L > 1
+  kGateScalars = 4    // [n / L]: one value for L rows, L > 1
+};
+
+struct NormParams {
+  const void *x, *y, *gate, *post, *pre, *scale;
+  void *x_out, *h_out;
+  float* rstd;             // [2, n]: r1, r2 (optional in the forward)
+  const void *dxo, *dh;    // backward: gradients of x' and h, either may be null
+  void *dx, *dy, *dgate;
+  float *part_pre, *part_post, *part_scale;  // [blocks, C]
+  float* part_gate;        // kGateRows: [n / L * nchunk, C]; kGateScalars: [n]
+  int64_t n, C, L;
+  int64_t chunk, nchunk, seg_rows;  // rows of a block; see row_range
+  float scale_const, eps;
+  int gate_kind, act, wdtype;
+};
+
+// The rows of block b.  A gate row's rows are either cut into nchunk blocks
+// (seg_rows = L) or handled whole, several gate rows to a block (nchunk = 1,
+// chunk a multiple of L); any other gate has one segment of n rows.
+struct RowRange {
+  int64_t lo, hi;
+};
+__device__ __forceinline__ RowRange row_range(const NormParams& p, int64_t b) {
+  RowRange r;
+  const int64_t seg = b / p.nchunk;
+  r.lo = seg * p.seg_rows + (b - seg * p.nchunk) * p.chunk;
+  const int64_t end = p.nchunk > 1 ? min(p.n, (seg + 1) * p.seg_rows) : p.n;
+  r.hi = min(end, r.lo + p.chunk);
+  return r;
+}
+
+__device__ __forceinline__ float sigmoid_of(float v) { return 1.0f / (1.0f + expf(-v)); }
+
+__device__ __forceinline__ float act_of(float g, int act) {
+  switch (act) {
+    case KAN_GATE_SIGMOID: return sigmoid_of(g);
+    case KAN_GATE_TANH: return tanhf(g);
+    case KAN_GATE_SILU: return g * sigmoid_of(g);
+    default: return g;
+  }
+}
+__device__ __forceinline__ float act_slope(float g, int act) {
+  switch (act) {
+    case KAN_GATE_SIGMOID: {
+      const float s = sigmoid_of(g);
+      return s * (1.0f - s);
+    }
+    case KAN_GATE_TANH: {
+      const float t = tanhf(g);
+      return 1.0f - t * t;
+    }
+    case KAN_GATE_SILU: {
+      const float s = sigmoid_of(g);
+      return s * (1.0f + g * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---- rows of any width ------------------------------------------------------
+// One block per row at a time, its values read again in every pass.
+constexpr int kRowThreads = 256;
+
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  float s = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kRowThreads / 64; ++w) s += red[w];
+  return s;
+}
+
+template <typename TX, typename TY>
+struct RowView {
+  const NormParams& p;
+  const TX* x;
+  const TY *y, *gate;
+  int64_t gstep;  // 0: one value for the row
+  float r1;
+  __device__ RowView(const NormParams& p_, int64_t row) : p(p_), r1(1.0f) {
+    x = static_cast<const TX*>(p.x) + row * p.C;
+    y = p.y == nullptr ? nullptr : static_cast<const TY*>(p.y) + row * p.C;
+    gate = nullptr;
+    gstep = 0;
+    if (p.gate_kind != kGateNone) {
+      gstep = p.gate_kind == kGateElement || p.gate_kind == kGateRows;
+      gate = static_cast<const TY*>(p.gate) + (row / p.L) * (gstep ? p.C : 1);
+    }
+  }
+  __device__ __forceinline__ float scale(int64_t c) const {
+    return p.scale == nullptr ? p.scale_const : load_any(p.scale, c, p.wdtype);
+  }
+  __device__ __forceinline__ float post(int64_t c) const { return load_any(p.post, c, p.wdtype); }
+  __device__ __forceinline__ float g(int64_t c) const { return (float)gate[c * gstep]; }
+  __device__ __forceinline__ float a(int64_t c) const {
+    return gate == nullptr ? 1.0f : act_of(g(c), p.act);
+  }
+  __device__ __forceinline__ float u(int64_t c) const {
+    return p.post == nullptr ? (float)y[c] : (float)y[c] * r1 * post(c);
+  }
+  __device__ __forceinline__ float stream(int64_t c) const {
+    const float v = (float)x[c];
+    return y == nullptr ? v : v + scale(c) * a(c) * u(c);
+  }
+};
+
+template <typename TX, typename TY>
+__global__ __launch_bounds__(kRowThreads) void norm_rows_kernel(NormParams p) {
+  __shared__ float red[kRowThreads / 64];
+  const float inv_c = 1.0f / (float)p.C;
+  for (int64_t row = blockIdx.x; row < p.n; row += gridDim.x) {
+    RowView<TX, TY> v(p, row);
+    if (v.y != nullptr && p.post != nullptr) {
+      float s = 0.0f;
+      for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
+        const float t = (float)v.y[c];
+        s += t * t;
+      }
+      v.r1 = 1.0f / sqrtf(block_sum(s, red) * inv_c + p.eps);
+      if (p.rstd != nullptr && threadIdx.x == 0) p.rstd[row] = v.r1;
+    }
+    float s = 0.0f;
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
+      const float t = v.stream(c);
+      s += t * t;
+      if (p.x_out != nullptr) static_cast<TX*>(p.x_out)[row * p.C + c] = (TX)t;
+    }
+    if (p.h_out == nullptr) continue;
+    const float r2 = 1.0f / sqrtf(block_sum(s, red) * inv_c + p.eps);
+    if (p.rstd != nullptr && threadIdx.x == 0) p.rstd[p.n + row] = r2;
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads)
+      static_cast<TY*>(p.h_out)[row * p.C + c] =
+          (TY)(v.stream(c) * r2 * load_any(p.pre, c, p.wdtype));
+  }
+}
+
+// A thread owns the columns c = threadIdx.x + i kRowThreads of every row of
+// its block, so a block's partial sums are plain reads and writes of its own.
+__device__ __forceinline__ void add_part(float* part, int64_t at, bool first, float v) {
+  if (part != nullptr) part[at] = first ? v : part[at] + v;
+}
+
+template <typename TX, typename TY>
+__global__ __launch_bounds__(kRowThreads) void norm_rows_grad_kernel(NormParams p) {
+  __shared__ float red[kRowThreads / 64];
+  const float inv_c = 1.0f / (float)p.C;
+  const RowRange rr = row_range(p, blockIdx.x);
+  const int64_t b = blockIdx.x;
+  for (int64_t row = rr.lo; row < rr.hi; ++row) {
+    RowView<TX, TY> v(p, row);
+    const bool first = row == rr.lo;
+    const bool gate_rows = p.gate_kind == kGateRows;
+    const bool gate_first = gate_rows && (first || row % p.L == 0);
+    const int64_t gate_at =
+        (p.nchunk > 1 ? b : row / p.L) * p.C;  // (kGateRows: its partial row)
+    const TX* dxo = p.dxo == nullptr ? nullptr : static_cast<const TX*>(p.dxo) + row * p.C;
+    const TY* dh = p.dh == nullptr ? nullptr : static_cast<const TY*>(p.dh) + row * p.C;
+    if (v.y != nullptr && p.post != nullptr) v.r1 = p.rstd[row];
+    float r2 = 0.0f, m2 = 0.0f;
+    if (dh != nullptr) {
+      r2 = p.rstd[p.n + row];
+      float s = 0.0f;
+      for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads)
+        s += (float)dh[c] * load_any(p.pre, c, p.wdtype) * (v.stream(c) * r2);
+      m2 = block_sum(s, red) * inv_c;
+    }
+    auto total = [&](int64_t c) {  // D
+      float d = dxo == nullptr ? 0.0f : (float)dxo[c];
+      if (dh != nullptr)
+        d += r2 * ((float)dh[c] * load_any(p.pre, c, p.wdtype) - v.stream(c) * r2 * m2);
+      return d;
+    };
+    float s1 = 0.0f, sg = 0.0f;
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
+      const float d = total(c);
+      if (p.dx != nullptr) static_cast<TX*>(p.dx)[row * p.C + c] = (TX)d;
+      if (dh != nullptr) add_part(p.part_pre, b * p.C + c, first, (float)dh[c] * v.stream(c) * r2);
+      if (v.y == nullptr) continue;
+      const float a = v.a(c), u = v.u(c), sc = v.scale(c), vv = d * sc * a;
+      add_part(p.part_scale, b * p.C + c, first, d * a * u);
+      if (p.post != nullptr) {
+        const float yh = (float)v.y[c] * v.r1;
+        add_part(p.part_post, b * p.C + c, first, vv * yh);
+        s1 += vv * v.post(c) * yh;
+      } else if (p.dy != nullptr) {
+        static_cast<TY*>(p.dy)[row * p.C + c] = (TY)vv;
+      }
+      if (p.dgate != nullptr) {
+        const float dg = d * sc * u * act_slope(v.g(c), p.act);
+        if (p.gate_kind == kGateElement) static_cast<TY*>(p.dgate)[row * p.C + c] = (TY)dg;
+        else if (gate_rows) add_part(p.part_gate, gate_at + c, gate_first, dg);
+        else sg += dg;
+      }
+    }
+    if (v.y == nullptr) continue;
+    if (p.dgate != nullptr && (p.gate_kind == kGateToken || p.gate_kind == kGateScalars)) {
+      sg = block_sum(sg, red);
+      if (threadIdx.x == 0) {
+        if (p.gate_kind == kGateToken) static_cast<TY*>(p.dgate)[row] = (TY)sg;
+        else p.part_gate[row] = sg;
+      }
+    }
+    if (p.post == nullptr || p.dy == nullptr) continue;
+    const float m1 = block_sum(s1, red) * inv_c;
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
+      const float yh = (float)v.y[c] * v.r1;
+      const float w = total(c) * v.scale(c) * v.a(c) * v.post(c);
+      static_cast<TY*>(p.dy)[row * p.C + c] = (TY)(v.r1 * (w - yh * m1));
+    }
+  }
+}
+
+// out[g, c] = sum over r < rows of part[g rows + r, c], in a fixed order:
+// 16 lanes of rows a column, their sums added in order.
+constexpr int kSumRowLanes = 16;
+__global__ __launch_bounds__(64 * kSumRowLanes) void sum_rows_kernel(
+    const float* __restrict__ part, int64_t rows, int64_t C, void* __restrict__ out, int dtype) {
+  __shared__ float red[kSumRowLanes][64];
+  const int lane = threadIdx.x & 63, rl = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane, g = blockIdx.y;
+  float s = 0.0f;
+  if (c < C) {
+    const float* src = part + g * rows * C + c;
+#pragma unroll 4
+    for (int64_t r = rl; r < rows; r += kSumRowLanes) s += src[r * C];
+  }
+  red[rl][lane] = s;
+  __syncthreads();
+  if (rl != 0 || c >= C) return;
+#pragma unroll
+  for (int w = 1; w < kSumRowLanes; ++w) s += red[w][lane];
+  store_any(out, g * C + c, dtype, s);
+}
+
+// out[g] = sum of part[g rows .. (g + 1) rows), one wave a sum.
+__global__ __launch_bounds__(64) void sum_runs_kernel(const float* __restrict__ part, int64_t rows,
+                                                      void* __restrict__ out, int dtype) {
+  const int64_t g = blockIdx.x;
+  float s = 0.0f;
+  for (int64_t r = threadIdx.x; r < rows; r += 64) s += part[g * rows + r];
+  s = wave_sum(s);
+  if (threadIdx.x == 0) store_any(out, g, dtype, s);
+}
+
+constexpr int64_t kMaxGridY = 65535;
+
+// How the rows of the backward are dealt to blocks, and the partial sums.
+struct GradPlan {
+  int64_t blocks, chunk, nchunk, seg_rows, gate_rows;  // gate_rows of part_gate
+  size_t bytes;
+};
+GradPlan grad_plan(int64_t n, int64_t C, int kind, int64_t L) {
+  const int64_t target = 2 * (int64_t)device_cu_count();
+  GradPlan g{};
+  const int64_t want = std::max<int64_t>(1, ceil_div(n, target));
+  if (kind == kGateRows && L > want) {
+    g.nchunk = ceil_div(L, want);
+    g.chunk = ceil_div(L, g.nchunk);
+    g.nchunk = ceil_div(L, g.chunk);
+    g.seg_rows = L;
+    g.blocks = n / L * g.nchunk;
+    g.gate_rows = g.blocks;
+  } else {
+    g.nchunk = 1;
+    g.chunk = kind == kGateRows ? want / L * L : want;
+    g.seg_rows = g.chunk;
+    g.blocks = ceil_div(n, g.chunk);
+    g.gate_rows = kind == kGateRows ? n / L : 0;
+  }
+  size_t floats = (size_t)(3 * g.blocks + g.gate_rows) * (size_t)C;
+  if (kind == kGateScalars) floats += (size_t)n;
+  g.bytes = 4 * floats;
+  return g;
+}
+
+template <typename TX, typename TY>
+int launch_forward(const NormParams& p, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(p.n, 16 * (int64_t)device_cu_count());
+  norm_rows_kernel<TX, TY><<<dim3((unsigned)blocks), kRowThreads, 0, st>>>(p);
+  return check_launch("residual_norm");
+}
+template <typename TX, typename TY>
+int launch_grad(const NormParams& p, int64_t blocks, hipStream_t st) {
+  norm_rows_grad_kernel<TX, TY><<<dim3((unsigned)blocks), kRowThreads, 0, st>>>(p);
+  return check_launch("residual_norm_backward");
+}
+
+int check_norm(const char* who, int xdtype, int ydtype, int wdtype, const void* x, const void* y,
+               const void* gate, const void* post, const void* scale, int gate_act,
+               int64_t gate_rows, int64_t gate_cols, int64_t n, int64_t C, NormParams* p) {
+  if (!dtype_is_operator(xdtype) || !dtype_is_operator(ydtype) || !dtype_is_operator(wdtype))
+    return set_error(KAN_ERR_INVALID, "%s: dtype codes must be FP32, BF16 or FP16", who);
+  if (xdtype != ydtype && xdtype != KAN_DTYPE_F32)
+    return set_error(KAN_ERR_INVALID, "%s: the stream is in the branch's type or in FP32", who);
+  if (n < 0 || C < 0) return set_error(KAN_ERR_INVALID, "%s: negative size", who);
+  if (gate_act < KAN_GATE_IDENTITY || gate_act > KAN_GATE_SILU)
+    return set_error(KAN_ERR_INVALID, "%s: unknown gate activation %d", who, gate_act);
+  if (y == nullptr && (gate != nullptr || post != nullptr || scale != nullptr))
+    return set_error(KAN_ERR_INVALID, "%s: gate, post_weight and scale need a branch", who);
+  p->gate_kind = kGateNone;
+  p->L = 1;
+  if (gate != nullptr) {
+    if (gate_rows < 1 || n % gate_rows != 0 || (gate_cols != 1 && gate_cols != C))
+      return set_error(KAN_ERR_INVALID,
+                       "%s: a gate has rows that divide n and 1 or C columns, got [%lld, %lld]", who,
+                       (long long)gate_rows, (long long)gate_cols);
+    p->L = n / gate_rows;
+    if (gate_cols == C && C > 1) p->gate_kind = p->L == 1 ? kGateElement : kGateRows;
+    else p->gate_kind = p->L == 1 ? kGateToken : kGateScalars;
+  }
+  p->x = x;
+  p->y = y;
+  p->gate = gate;
+  p->post = post;
+  p->scale = scale;
+  p->act = gate_act;
+  p->wdtype = wdtype;
+  p->n = n;
+  p->C = C;
+  return KAN_OK;
+}
+
+#define KAN_NORM_TYPES(xd, yd, CALL)                                          \
+  (xd == KAN_DTYPE_F32 ? (yd == KAN_DTYPE_F32    ? CALL(float, float)         \
+                          : yd == KAN_DTYPE_BF16 ? CALL(float, bf16)          \
+                                                 : CALL(float, f16))          \
+   : xd == KAN_DTYPE_BF16 ? CALL(bf16, bf16)                                  \
+                          : CALL(f16, f16))
+
+}  // namespace
+}  // namespace kan
+
+using namespace kan;
+
+extern "C" {
+
+int kan_hip_residual_norm(int xdtype, int ydtype, int wdtype, const void* x, const void* y,
+                          const void* gate, const void* post_weight, const void* pre_weight,
+                          const void* scale, double scale_const, int gate_act, int64_t gate_rows,
+                          int64_t gate_cols, int64_t n, int64_t C, double eps, void* x_out,
+                          void* h_out, float* rstd, void* stream) {
+  NormParams p{};
+  const int rc = check_norm("residual_norm", xdtype, ydtype, wdtype, x, y, gate, post_weight, scale,
+                            gate_act, gate_rows, gate_cols, n, C, &p);
+  if (rc != KAN_OK) return rc;
+  if (n == 0 || C == 0) return KAN_OK;
+  if (x == nullptr) return set_error(KAN_ERR_INVALID, "residual_norm: x must not be NULL");
+  if ((h_out == nullptr) != (pre_weight == nullptr))
+    return set_error(KAN_ERR_INVALID, "residual_norm: h_out and pre_weight go together");
+  if (x_out == nullptr && h_out == nullptr) return KAN_OK;
+  p.pre = pre_weight;
+  p.x_out = x_out;
+  p.h_out = h_out;
+  p.rstd = rstd;
+  p.scale_const = (float)scale_const;
+  p.eps = (float)eps;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const double moved = (double)n * C *
+                       (dtype_bytes(xdtype) * (x_out != nullptr ? 2 : 1) +
+                        dtype_bytes(ydtype) * ((y != nullptr) + (h_out != nullptr)));
+  TimedLaunch timed(kClassOther, st, moved);
+#define KAN_CALL(TX, TY) launch_forward<TX, TY>(p, st)
+  return KAN_NORM_TYPES(xdtype, ydtype, KAN_CALL);
+#undef KAN_CALL
+}
+
+int kan_hip_residual_norm_backward_workspace(int64_t gate_rows, int64_t gate_cols, int64_t n,
+                                             int64_t C, size_t* bytes) {
+  if (bytes == nullptr)
+    return set_error(KAN_ERR_INVALID, "residual_norm_backward_workspace: bytes must not be NULL");
+  NormParams p{};
+  const int rc = check_norm("residual_norm_backward", KAN_DTYPE_F32, KAN_DTYPE_F32, KAN_DTYPE_F32,
+                            &p, &p, gate_rows > 0 ? &p : nullptr, nullptr, nullptr, 0, gate_rows,
+                            gate_cols, n, C, &p);
+  if (rc != KAN_OK) return rc;
+  *bytes = n == 0 || C == 0 ? 0 : grad_plan(n, C, p.gate_kind, p.L).bytes;
+  return KAN_OK;
+}
+
+int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const void* grad_x_out,
+                                   const void* grad_h, const void* x, const void* y,
+                                   const void* gate, const void* post_weight,
+                                   const void* pre_weight, const void* scale, double scale_const,
+                                   int gate_act, int64_t gate_rows, int64_t gate_cols, int64_t n,
+                                   int64_t C, const float* rstd, void* grad_x, void* grad_y,
+                                   void* grad_gate, void* grad_post, void* grad_pre,
+                                   void* grad_scale, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  const char* who = "residual_norm_backward";
+  NormParams p{};
+  const int rc = check_norm(who, xdtype, ydtype, wdtype, x, y, gate, post_weight, scale, gate_act,
+                            gate_rows, gate_cols, n, C, &p);
+  if (rc != KAN_OK) return rc;
+  if ((grad_y != nullptr && y == nullptr) || (grad_gate != nullptr && gate == nullptr) ||
+      (grad_post != nullptr && post_weight == nullptr) ||
+      (grad_scale != nullptr && scale == nullptr) || (grad_pre != nullptr && grad_h == nullptr) ||
+      (grad_h != nullptr && pre_weight == nullptr))
+    return set_error(KAN_ERR_INVALID, "%s: a gradient of an absent operand", who);
+  if (n == 0 || C == 0) return KAN_OK;
+  if (x == nullptr || rstd == nullptr)
+    return set_error(KAN_ERR_INVALID, "%s: x and rstd must not be NULL", who);
+  const GradPlan g = grad_plan(n, C, p.gate_kind, p.L);
+  if (workspace == nullptr || workspace_bytes < g.bytes)
+    return set_error(KAN_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, g.bytes,
+                     workspace == nullptr ? (size_t)0 : workspace_bytes);
+  float* ws = static_cast<float*>(workspace);
+  const int64_t row_part = g.blocks * C;
+  p.pre = grad_h == nullptr ? nullptr : pre_weight;
+  p.part_pre = grad_pre == nullptr ? nullptr : ws;
+  p.part_post = grad_post == nullptr ? nullptr : ws + row_part;
+  p.part_scale = grad_scale == nullptr ? nullptr : ws + 2 * row_part;
+  p.part_gate = grad_gate == nullptr ? nullptr : ws + 3 * row_part;
+  p.dxo = grad_x_out;
+  p.dh = grad_h;
+  p.dx = grad_x;
+  p.dy = grad_y;
+  p.dgate = grad_gate;
+  p.rstd = const_cast<float*>(rstd);
+  p.chunk = g.chunk;
+  p.nchunk = g.nchunk;
+  p.seg_rows = g.seg_rows;
+  p.scale_const = (float)scale_const;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const double moved =
+      (double)n * C *
+      (dtype_bytes(xdtype) * (1 + (grad_x_out != nullptr) + (grad_x != nullptr)) +
+       dtype_bytes(ydtype) * ((y != nullptr) + (grad_h != nullptr) + (grad_y != nullptr)));
+  {
+    TimedLaunch timed(kClassOther, st, moved);
+#define KAN_CALL(TX, TY) launch_grad<TX, TY>(p, g.blocks, st)
+    const int e = KAN_NORM_TYPES(xdtype, ydtype, KAN_CALL);
+#undef KAN_CALL
+    if (e != KAN_OK) return e;
+  }
+  const unsigned cols = (unsigned)ceil_div(C, 64);
+  auto sum_rows = [&](const float* part, int64_t groups, int64_t rows, void* out, int dtype) {
+    for (int64_t g0 = 0; g0 < groups; g0 += kMaxGridY) {
+      const int64_t cnt = std::min(kMaxGridY, groups - g0);
+      char* dst = static_cast<char*>(out) + (size_t)(g0 * C) * dtype_bytes(dtype);
+      sum_rows_kernel<<<dim3(cols, (unsigned)cnt), 64 * kSumRowLanes, 0, st>>>(
+          part + g0 * rows * C, rows, C, dst, dtype);
+    }
+  };
+  TimedLaunch timed(kClassOther, st, (double)g.bytes);
+  if (grad_pre != nullptr) sum_rows(p.part_pre, 1, g.blocks, grad_pre, wdtype);
+  if (grad_post != nullptr) sum_rows(p.part_post, 1, g.blocks, grad_post, wdtype);
+  if (grad_scale != nullptr) sum_rows(p.part_scale, 1, g.blocks, grad_scale, wdtype);
+  if (grad_gate != nullptr && p.gate_kind == kGateRows)
+    sum_rows(p.part_gate, n / p.L, g.nchunk, grad_gate, ydtype);
+  if (grad_gate != nullptr && p.gate_kind == kGateScalars)
+    sum_runs_kernel<<<dim3((unsigned)(n / p.L)), 64, 0, st>>>(p.part_gate, p.L, grad_gate, ydtype);
+  return check_launch(who);
+}
+
+}  // extern "C"

@@ -1,0 +1,80 @@
+// The 16-bit types of the operators beside the KAN layers (residual norm,
+// 8-bit activations, grouped products): storage types, conversions, vectors
+// and wave sums.
+#pragma once
+
+#include "kan_common.h"
+
+namespace kan {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+inline size_t dtype_bytes(int code) {
+  return code == KAN_DTYPE_F64 ? 8 : code == KAN_DTYPE_F32 ? 4 : 2;
+}
+inline bool dtype_is_operator(int code) {
+  return code == KAN_DTYPE_F32 || code == KAN_DTYPE_BF16 || code == KAN_DTYPE_F16;
+}
+
+template <typename T, int V>
+struct VecOf {
+  typedef T type __attribute__((ext_vector_type(V)));
+};
+
+// V consecutive values as floats.  p is aligned to the whole vector.
+template <typename T, int V>
+__device__ __forceinline__ void load_f32(const T* __restrict__ p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = (float)p[0];
+  } else {
+    const auto u = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = (float)u[j];
+  }
+}
+
+// The same rounded to T (to nearest, ties to even).
+template <typename T, int V>
+__device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    p[0] = (T)v[0];
+  } else {
+    typename VecOf<T, V>::type u;
+#pragma unroll
+    for (int j = 0; j < V; ++j) u[j] = (T)v[j];
+    *reinterpret_cast<typename VecOf<T, V>::type*>(p) = u;
+  }
+}
+
+// One value of an array whose type is known at run time (the short vectors of
+// weights, read once a row or less).
+__device__ __forceinline__ float load_any(const void* __restrict__ p, int64_t i, int dtype) {
+  if (dtype == KAN_DTYPE_F32) return static_cast<const float*>(p)[i];
+  if (dtype == KAN_DTYPE_BF16) return (float)static_cast<const bf16*>(p)[i];
+  return (float)static_cast<const f16*>(p)[i];
+}
+__device__ __forceinline__ void store_any(void* __restrict__ p, int64_t i, int dtype, float v) {
+  if (dtype == KAN_DTYPE_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == KAN_DTYPE_BF16) static_cast<bf16*>(p)[i] = (bf16)v;
+  else static_cast<f16*>(p)[i] = (f16)v;
+}
+
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ float dpp_or_zero(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROW_MASK, 0xf, false));
+}
+
+// Sum over the wave, in every lane (a fixed tree: the same bits every time).
+__device__ __forceinline__ float wave_sum(float v) {
+  v += dpp_or_zero<0xB1>(v);         // lane ^ 1
+  v += dpp_or_zero<0x4E>(v);         // lane ^ 2
+  v += dpp_or_zero<0x141>(v);        // mirrored half rows: the other 4 of 8
+  v += dpp_or_zero<0x140>(v);        // mirrored rows: the other 8 of 16
+  v += dpp_or_zero<0x142, 0xa>(v);   // row 0 into 1, row 2 into 3
+  v += dpp_or_zero<0x143, 0xc>(v);   // rows 0 and 1 into 2 and 3
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+}  // namespace kan

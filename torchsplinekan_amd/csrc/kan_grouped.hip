@@ -10,6 +10,8 @@
 // Sums are in float32, rounded once.  A grid covers the largest number of
 // row tiles T rows can make of E groups (T / BM + E + 1); a block finds its
 // group from the offsets, and blocks past the last tile end at once.
+#include <type_traits>
+
 #include "kan_types.h"
 
 namespace kan {
@@ -213,6 +215,456 @@ int launch_plain(int op, const GroupedParams& p, hipStream_t st) {
   return check_launch("grouped_matmul");
 }
 
+// ---- 16-bit products on MFMA ------------------------------------------------
+// Block tiles of BM x BN outputs, 64 deep, WM x WN waves; v_mfma_f32_32x32x16
+// on bf16 or f16 operands.
+//
+// An operand's slab lies in LDS in 16-byte chunks of 8 values, in the layout of
+// its rows in memory: K-contiguous operands as [row][8 chunks of k], the others
+// as [64 k][chunks of rows].  A thread's chunks are the same in every slab, so
+// their offsets are set once and a slab costs one scalar addition.  Whole slabs
+// go from memory to LDS without passing registers (a wave's 64 chunks of 16
+// bytes lie in a row there, so the chunks are exchanged on the memory side:
+// chunk c of row r at position c ^ (r & 7), of k row k at c ^ 4 (k & 3), which
+// spreads the fragments' reads over the banks).  K-contiguous fragments are
+// one 16-byte read a lane, the others two 8-byte reads that transpose 4 x 16
+// values across the lanes of a row.  Last slabs, rows off 16 bytes and 8-bit
+// rows pass registers.
+//
+// Rows and columns past a tile's last repeat an earlier one: their products
+// are not stored.  k past the last is zero in both operands, as what lies there
+// (another expert's rows) may be anything.
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <typename T>
+struct Half;
+template <>
+struct Half<bf16> {
+  typedef bf16 frag __attribute__((ext_vector_type(8)));
+  __device__ static __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Half<f16> {
+  typedef f16 frag __attribute__((ext_vector_type(8)));
+  __device__ static __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+constexpr int kDepth = 64;  // k of a slab
+
+template <int BM_, int BN_, int WM_, int WN_>
+struct TileCfg {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM * WN;
+  static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
+  static constexpr int kBuf = (BM + BN) * kDepth * 2;  // bytes of one slab pair
+};
+using TileBig = TileCfg<256, 256, 2, 4>;
+using TileSmall = TileCfg<128, 128, 2, 2>;
+
+// How an operand reaches LDS.
+enum OperandMode { kDirect = 0, kGuarded = 1, kInt8 = 2, kE4m3 = 3 };
+
+// Values of 16 bytes (of 2 where rows are not aligned): memcpy keeps the
+// load's alignment honest.
+struct __attribute__((packed, aligned(2))) Loose16 {
+  u32x4 v;
+};
+struct __attribute__((packed, aligned(1))) Loose8 {
+  uint2 v;
+};
+
+template <typename T, int ROWS, bool KCONT, int MODE, int NT>
+struct Operand {
+  static constexpr int kPer = ROWS * (kDepth / 8) / NT;  // chunks of a thread
+  static constexpr int kRowChunks = KCONT ? kDepth / 8 : ROWS / 8;
+  static constexpr int kValue = MODE >= kInt8 ? 1 : 2;   // bytes of a value in memory
+  static_assert(ROWS * (kDepth / 8) % NT == 0, "whole rounds of chunks");
+  static_assert(MODE < kInt8 || !KCONT, "8-bit rows are the weight product's");
+
+  const char* base;  // of the tile's first row (KCONT) or column, at k = 0
+  int64_t ld;        // bytes between rows
+  int rows;          // valid rows (KCONT) or columns from the tile's first on
+  uint32_t off[kPer];
+  u32x4 reg[kPer];
+  // 8-bit rows
+  const float* scale;
+  int64_t parts;
+  int group, col0;
+  float step[MODE >= kInt8 ? kPer : 1];
+
+  // Row of the thread's chunk p in the slab's layout, and the chunk of that
+  // row which belongs at the thread's position.
+  __device__ __forceinline__ static int chunk_row(int p) {
+    return (p * NT + (int)threadIdx.x) / kRowChunks;
+  }
+  __device__ __forceinline__ static int chunk_col(int p) {
+    const int r = chunk_row(p), pos = (p * NT + (int)threadIdx.x) % kRowChunks;
+    return KCONT ? pos ^ (r & 7) : pos ^ ((r & 3) << 2);
+  }
+
+  __device__ __forceinline__ void init(const void* src, int64_t ld_values, int64_t first,
+                                       int64_t valid) {
+    ld = ld_values * kValue;
+    rows = (int)min(valid, (int64_t)ROWS);
+    base = static_cast<const char*>(src) + (KCONT ? first * ld : first * kValue);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int r = chunk_row(p), c = 8 * chunk_col(p);
+      off[p] = KCONT ? (uint32_t)(min(r, rows - 1) * ld) + (uint32_t)(c * kValue)
+                     : (uint32_t)(r * ld) + (uint32_t)((c < rows ? c : 0) * kValue);
+    }
+  }
+  __device__ __forceinline__ const char* slab(int64_t k0) const {
+    return base + (KCONT ? k0 * kValue : k0 * ld);
+  }
+
+  // A whole slab straight into LDS.  (In assembly: the compiler would wait for
+  // these loads before any transposing LDS read, taking it for a read of the
+  // same bytes; slab_barrier waits for them.  They write no register.)
+  __device__ __forceinline__ void issue(int64_t k0, char* lds) const {
+    const char* src = slab(k0);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + (threadIdx.x >> 6) * 1024);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p)
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                       to + p * NT * 16),
+                   "v"(off[p]), "s"(src));
+  }
+
+  // A slab into registers; k from kend on is zero.
+  __device__ __forceinline__ void load(int64_t k0, int64_t kend) {
+    const char* src = slab(k0);
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      const int r = chunk_row(p), c = 8 * chunk_col(p);
+      // how many of the chunk's values exist: k for KCONT, columns otherwise
+      const int64_t left = KCONT ? kend - k0 - c : (int64_t)(rows - c);
+      const int n = (!KCONT && k0 + r >= kend) || left <= 0 ? 0 : (int)min(left, (int64_t)8);
+      u32x4 v = {0, 0, 0, 0};
+      if constexpr (MODE >= kInt8) {
+        if (n == 8) {
+          const uint2 u = reinterpret_cast<const Loose8*>(src + off[p])->v;
+          v[0] = u.x;
+          v[1] = u.y;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < n) v[j >> 2] |= (uint32_t)(uint8_t)src[off[p] + j] << (8 * (j & 3));
+        }
+        step[p] = n > 0 ? scale[(k0 + r) * parts + (col0 + c) / group] : 0.0f;
+      } else if (n == 8) {
+        if constexpr (MODE == kGuarded) v = reinterpret_cast<const Loose16*>(src + off[p])->v;
+        else v = *reinterpret_cast<const u32x4*>(src + off[p]);
+      } else if constexpr (MODE == kGuarded) {  // (aligned rows end with whole chunks)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < n)
+            v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(src + off[p])[j]
+                         << (16 * (j & 1));
+      }
+      reg[p] = v;
+    }
+  }
+
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int p = 0; p < kPer; ++p) {
+      u32x4 v = reg[p];
+      if constexpr (MODE >= kInt8) v = restore(v, step[p]);
+      *reinterpret_cast<u32x4*>(lds + (p * NT + threadIdx.x) * 16) = v;
+    }
+  }
+  // 8 values q * scale rounded to T.
+  __device__ __forceinline__ static u32x4 restore(u32x4 q, float s) {
+    typename Half<T>::frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = q[j >> 2];
+      float u;
+      if constexpr (MODE == kInt8) {
+        u = (float)(int8_t)(w >> (8 * (j & 3)));
+      } else {
+        switch (j & 3) {
+          case 0: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 0); break;
+          case 1: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 1); break;
+          case 2: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 2); break;
+          default: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 3); break;
+        }
+      }
+      f[j] = (T)(u * s);
+    }
+    return __builtin_bit_cast(u32x4, f);
+  }
+};
+
+// Fragments of 32 rows x 16 k of a slab in LDS (ROWS rows in all, the wave's
+// FR x 32 from `first` on): lane l has row l & 31 and k 8 (l >> 5) .. + 7.
+template <typename T, int ROWS, int FR, bool KCONT>
+struct Fragments {
+  typedef typename Half<T>::frag frag;
+  uint32_t at[KCONT ? 4 : FR];  // by k step, or by group of 32 rows
+  __device__ __forceinline__ void init(int first) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (KCONT) {
+      const int r = first + (lane & 31);
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        at[s] = (uint32_t)(r * 128 + (((2 * s + (lane >> 5)) ^ (r & 7)) << 4));
+    } else {
+      // 16 lanes read 4 k rows of 16 columns, 4 columns each, and lane l then
+      // holds column l & 15 of the 4 k rows
+      const int k = 8 * (lane >> 5) + ((lane & 15) >> 2);
+#pragma unroll
+      for (int i = 0; i < FR; ++i) {
+        const int col = first + 32 * i + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        at[i] = (uint32_t)(k * ROWS * 2 + (((col >> 3) ^ ((k & 3) << 2)) << 4) +
+                           ((col >> 2) & 1) * 8);
+      }
+    }
+  }
+  __device__ __forceinline__ frag read(const char* lds, int i, int s) const {
+    if constexpr (KCONT) {
+      return *reinterpret_cast<const frag*>(lds + at[s] + i * 32 * 128);
+    } else {
+      typedef __attribute__((address_space(3))) s16x4* lds4;
+      const char* p = lds + at[i] + 16 * s * ROWS * 2;
+      struct {
+        s16x4 lo, hi;
+      } v;
+      v.lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p));
+      v.hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * ROWS * 2));
+      return __builtin_bit_cast(frag, v);
+    }
+  }
+};
+
+// Every wave's slab loads and LDS accesses are done, then every wave goes on.
+__device__ __forceinline__ void slab_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+constexpr int kGroupedM = 8;  // row tiles that walk the columns together
+
+template <typename T, class G, int OP, int MA, int MB>
+__global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, int tiles_m,
+                                                             int tiles_n, int store_vec) {
+  constexpr bool KA = OP != 2, KB = OP == 0;
+  constexpr int BM = G::BM, BN = G::BN, FM = G::FM, FN = G::FN;
+  __shared__ __align__(16) char lds[2 * G::kBuf];
+
+  // the tile: rows [m0, m_end) and columns [n0, n_end) of the output, k range
+  int e, tm, tn;
+  int64_t m0, m_end, kbeg = 0, kend;
+  if constexpr (OP == 2) {
+    const int id = xcd_remap(blockIdx.x, gridDim.x), per = tiles_m * tiles_n;
+    e = __builtin_amdgcn_readfirstlane(id / per);
+    const int t = id - e * per;
+    tm = __builtin_amdgcn_readfirstlane(t / tiles_n);
+    tn = __builtin_amdgcn_readfirstlane(t % tiles_n);
+    int lo = 0, hi = 0;
+    group_rows(p, e, &lo, &hi);
+    kbeg = lo;
+    kend = hi;
+    m0 = (int64_t)tm * BM;
+    m_end = p.N;
+  } else {
+    tiles_m = count_tiles(p, BM);
+    const int total = tiles_m * tiles_n;
+    if ((int)blockIdx.x >= total) return;
+    const int id = xcd_remap(blockIdx.x, total), group = kGroupedM * tiles_n;
+    const int first = id / group * kGroupedM, in = id % group;
+    const int gm = min(tiles_m - first, kGroupedM);
+    tm = __builtin_amdgcn_readfirstlane(first + in % gm);
+    tn = __builtin_amdgcn_readfirstlane(in / gm);
+    const RowTile rt = find_tile(p, tm, BM);
+    e = rt.e;
+    m0 = rt.m0;
+    m_end = rt.m1;
+    kend = e == p.E ? 0 : OP == 0 ? p.K : p.N;
+  }
+  const int64_t n_end = OP == 0 ? p.N : p.K, n0 = (int64_t)tn * BN;
+  const int64_t weight = (int64_t)e * p.N * p.K;
+
+  Operand<T, BM, KA, MA, G::NT> a;
+  Operand<T, BN, KB, MB, G::NT> b;
+  a.init(p.A, OP == 0 ? p.K : p.N, m0, m_end - m0);
+  b.init(OP == 2 ? p.B : static_cast<const T*>(p.B) + weight, p.K, n0, n_end - n0);
+  if constexpr (MB >= kInt8) {
+    b.scale = p.b_scale;
+    b.group = p.group;
+    b.parts = (p.K + p.group - 1) / p.group;
+    b.col0 = (int)n0;
+  }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / G::WN, wn = wave % G::WN, lane = threadIdx.x & 63;
+  Fragments<T, BM, FM, KA> fa;
+  Fragments<T, BN, FN, KB> fb;
+  fa.init(wm * FM * 32);
+  fb.init(wn * FN * 32);
+
+  f32x16 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+
+  constexpr int kB = BM * kDepth * 2;  // B's slab lies behind A's
+  auto compute = [&](const char* cur) __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < kDepth / 16; ++s) {
+      typename Half<T>::frag av[FM], bv[FN];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) bv[j] = fb.read(cur + kB, j, s);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) av[i] = fa.read(cur, i, s);
+      // (B first: a lane then holds 4 columns of one row of the output)
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = Half<T>::mma(bv[j], av[i], acc[i][j]);
+    }
+  };
+
+  const int slabs = (int)((kend - kbeg + kDepth - 1) / kDepth);
+  const int whole = (int)((kend - kbeg) / kDepth);
+  if (slabs > 0) {
+    // before: starts slab kt on its way into buf; after: finishes it.  (whole_c:
+    // all its k exist)
+    auto before = [&](int kt, char* buf, auto whole_c) __attribute__((always_inline)) {
+      constexpr bool kWhole = decltype(whole_c)::value;
+      const int64_t k0 = kbeg + (int64_t)kt * kDepth;
+      if constexpr (MA == kDirect && kWhole) a.issue(k0, buf);
+      else a.load(k0, kend);
+      if constexpr (MB == kDirect && kWhole) b.issue(k0, buf + kB);
+      else b.load(k0, kend);
+    };
+    auto after = [&](char* buf, auto whole_c) __attribute__((always_inline)) {
+      constexpr bool kWhole = decltype(whole_c)::value;
+      if constexpr (MA != kDirect || !kWhole) a.store(buf);
+      if constexpr (MB != kDirect || !kWhole) b.store(buf + kB);
+    };
+    constexpr std::true_type yes{};
+    constexpr std::false_type no{};
+    if (whole > 0) {
+      before(0, lds, yes);
+      after(lds, yes);
+    } else {
+      before(0, lds, no);
+      after(lds, no);
+    }
+    slab_barrier();
+    int kt = 0;
+    for (; kt + 1 < whole; ++kt) {
+      char* nxt = lds + ((kt + 1) & 1) * G::kBuf;
+      before(kt + 1, nxt, yes);
+      compute(lds + (kt & 1) * G::kBuf);
+      after(nxt, yes);
+      slab_barrier();
+    }
+    if (kt + 1 < slabs) {
+      char* nxt = lds + ((kt + 1) & 1) * G::kBuf;
+      before(kt + 1, nxt, no);
+      compute(lds + (kt & 1) * G::kBuf);
+      after(nxt, no);
+      slab_barrier();
+      ++kt;
+    }
+    compute(lds + (kt & 1) * G::kBuf);
+  }
+
+  // The wave's outputs go through LDS to become whole 16-byte pieces of rows.
+  __syncthreads();
+  T* out = static_cast<T*>(p.C) + (OP == 2 ? weight : 0);
+  constexpr int kWaveRows = FM * 32, kRowBytes = FN * 64, kChunks = kRowBytes / 16;
+  char* stage = lds + wave * kWaveRows * kRowBytes;
+  typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int r = i * 32 + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        t4 v;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = (T)acc[i][j][4 * q + u];
+        const int c = (4 * j + q) ^ (r & (kChunks - 1));
+        *reinterpret_cast<t4*>(stage + r * kRowBytes + c * 16 + (lane >> 5) * 8) = v;
+      }
+  }
+  const int64_t row0 = m0 + wm * kWaveRows, col0 = n0 + wn * FN * 32;
+  constexpr int kStep = 64 / kChunks;  // rows a wave stores at once
+#pragma unroll 4
+  for (int it = 0; it < kWaveRows / kStep; ++it) {
+    const int r = it * kStep + lane / kChunks, c = lane % kChunks;
+    const u32x4 v =
+        *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + ((c ^ (r & (kChunks - 1))) * 16));
+    const int64_t row = row0 + r, col = col0 + 8 * c;
+    if (row >= m_end || col >= n_end) continue;
+    T* dst = out + row * n_end + col;
+    if (store_vec) {
+      *reinterpret_cast<u32x4*>(dst) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (col + j < n_end)
+          reinterpret_cast<uint16_t*>(dst)[j] = (uint16_t)(v[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T, class G, int OP, int MA, int MB>
+int launch_tile(const GroupedParams& p, hipStream_t st) {
+  const int64_t cols = OP == 0 ? p.N : p.K;
+  const int64_t tiles_n = ceil_div(cols, G::BN);
+  const int64_t tiles_m = OP == 2 ? ceil_div(p.N, G::BM) : p.T / G::BM + p.E + 1;
+  const int64_t blocks = tiles_n * tiles_m * (OP == 2 ? p.E : 1);
+  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  grouped_tile_kernel<T, G, OP, MA, MB><<<dim3((unsigned)blocks), G::NT, 0, st>>>(
+      p, (int)tiles_m, (int)tiles_n, cols % 8 == 0 && aligned16(p.C) ? 1 : 0);
+  return check_launch("grouped_matmul");
+}
+
+template <typename T, class G>
+int launch_half_cfg(int op, const GroupedParams& p, hipStream_t st) {
+  const bool a16 = aligned16(p.A) && (op == 0 ? p.K : p.N) % 8 == 0;
+  const bool b16 = aligned16(p.B) && p.K % 8 == 0;
+  if (op == 0)
+    return a16 && b16 ? launch_tile<T, G, 0, kDirect, kDirect>(p, st)
+                      : launch_tile<T, G, 0, kGuarded, kGuarded>(p, st);
+  if (op == 1)
+    return a16 && b16 ? launch_tile<T, G, 1, kDirect, kDirect>(p, st)
+                      : launch_tile<T, G, 1, kGuarded, kGuarded>(p, st);
+  if (p.format == KAN_ACT8_INT8)
+    return a16 ? launch_tile<T, G, 2, kDirect, kInt8>(p, st)
+               : launch_tile<T, G, 2, kGuarded, kInt8>(p, st);
+  if (p.format == KAN_ACT8_E4M3)
+    return a16 ? launch_tile<T, G, 2, kDirect, kE4m3>(p, st)
+               : launch_tile<T, G, 2, kGuarded, kE4m3>(p, st);
+  return a16 && b16 ? launch_tile<T, G, 2, kDirect, kDirect>(p, st)
+                    : launch_tile<T, G, 2, kGuarded, kGuarded>(p, st);
+}
+
+template <typename T>
+int launch_half(int op, const GroupedParams& p, hipStream_t st) {
+  const int64_t rows = op == 2 ? p.N : p.T / std::max(p.E, 1), cols = op == 0 ? p.N : p.K;
+  const int64_t big = ceil_div(rows, 256) * ceil_div(cols, 256) * std::max(p.E, 1);
+  return big >= device_cu_count() ? launch_half_cfg<T, TileBig>(op, p, st)
+                                  : launch_half_cfg<T, TileSmall>(op, p, st);
+}
+
 int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K) {
   if (!dtype_is_operator(dtype))
     return set_error(KAN_ERR_INVALID, "grouped_matmul: dtype must be FP32, BF16 or FP16 (code %d)",
@@ -221,9 +673,10 @@ int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K)
     return set_error(KAN_ERR_INVALID, "grouped_matmul: unknown product %d", op);
   if (T < 0 || E < 0 || N < 0 || K < 0)
     return set_error(KAN_ERR_INVALID, "grouped_matmul: negative size");
-  constexpr int64_t kMost = 0x7fffffff - 4096;  // (tile ends are held in 32 bits)
-  if (T > kMost || N > kMost || K > kMost || E > (1 << 20))
-    return set_error(KAN_ERR_LIMIT, "grouped_matmul: at most 2^31 - 4097 rows and columns and 2^20 experts");
+  // (tile ends are held in 32 bits, as are the bytes from a tile's first row)
+  if (T > 0x7fffffff - 4096 || N > (1 << 22) || K > (1 << 22) || E > (1 << 20))
+    return set_error(KAN_ERR_LIMIT,
+                     "grouped_matmul: at most 2^31 - 4097 rows, 2^22 columns and 2^20 experts");
   return KAN_OK;
 }
 
@@ -285,8 +738,8 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * N * K);
   if (dtype == KAN_DTYPE_F32) return launch_plain<float>(op, p, st);
-  if (dtype == KAN_DTYPE_BF16) return launch_plain<bf16>(op, p, st);
-  return launch_plain<f16>(op, p, st);
+  if (dtype == KAN_DTYPE_BF16) return launch_half<bf16>(op, p, st);
+  return launch_half<f16>(op, p, st);
 }
 
 }  // extern "C"

@@ -225,8 +225,8 @@ int launch_plain(int op, const GroupedParams& p, hipStream_t st) {
 // their offsets are set once and a slab costs one scalar addition.  Whole slabs
 // go from memory to LDS without passing registers (a wave's 64 chunks of 16
 // bytes lie in a row there, so the chunks are exchanged on the memory side:
-// chunk c of row r at position c ^ (r & 7), of k row k at c ^ 4 (k & 3), which
-// spreads the fragments' reads over the banks).  K-contiguous fragments are
+// chunk c of row r at position c ^ (r / 2 % 8), of k row k at c ^ 4 (k % 4),
+// which spreads 16 lanes' reads over all 64 banks).  K-contiguous fragments are
 // one 16-byte read a lane, the others two 8-byte reads that transpose 4 x 16
 // values across the lanes of a row.  Last slabs, rows off 16 bytes and 8-bit
 // rows pass registers.
@@ -304,7 +304,7 @@ struct Operand {
   }
   __device__ __forceinline__ static int chunk_col(int p) {
     const int r = chunk_row(p), pos = (p * NT + (int)threadIdx.x) % kRowChunks;
-    return KCONT ? pos ^ (r & 7) : pos ^ ((r & 3) << 2);
+    return KCONT ? pos ^ ((r >> 1) & 7) : pos ^ ((r & 3) << 2);
   }
 
   __device__ __forceinline__ void init(const void* src, int64_t ld_values, int64_t first,
@@ -415,7 +415,7 @@ struct Fragments {
       const int r = first + (lane & 31);
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        at[s] = (uint32_t)(r * 128 + (((2 * s + (lane >> 5)) ^ (r & 7)) << 4));
+        at[s] = (uint32_t)(r * 128 + (((2 * s + (lane >> 5)) ^ ((r >> 1) & 7)) << 4));
     } else {
       // 16 lanes read 4 k rows of 16 columns, 4 columns each, and lane l then
       // holds column l & 15 of the 4 k rows
@@ -519,67 +519,89 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
       for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
 
   constexpr int kB = BM * kDepth * 2;  // B's slab lies behind A's
-  auto compute = [&](const char* cur) __attribute__((always_inline)) {
+  constexpr int kSteps = kDepth / 16;
+  typename Half<T>::frag av[2][FM], bv[2][FN];  // by the parity of the k step
+  auto read_step = [&](const char* buf, int st) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < kDepth / 16; ++s) {
-      typename Half<T>::frag av[FM], bv[FN];
+    for (int j = 0; j < FN; ++j) bv[st & 1][j] = fb.read(buf + kB, j, st);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) bv[j] = fb.read(cur + kB, j, s);
+    for (int i = 0; i < FM; ++i) av[st & 1][i] = fa.read(buf, i, st);
+    __builtin_amdgcn_sched_barrier(0);  // (left alone, reads sink below the MFMAs)
+  };
+  auto mma_step = [&](int st) __attribute__((always_inline)) {
+    // (B first: a lane then holds 4 columns of one row of the output)
 #pragma unroll
-      for (int i = 0; i < FM; ++i) av[i] = fa.read(cur, i, s);
-      // (B first: a lane then holds 4 columns of one row of the output)
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = Half<T>::mma(bv[j], av[i], acc[i][j]);
-    }
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = Half<T>::mma(bv[st & 1][j], av[st & 1][i], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
   const int slabs = (int)((kend - kbeg + kDepth - 1) / kDepth);
-  const int whole = (int)((kend - kbeg) / kDepth);
-  if (slabs > 0) {
-    // before: starts slab kt on its way into buf; after: finishes it.  (whole_c:
-    // all its k exist)
-    auto before = [&](int kt, char* buf, auto whole_c) __attribute__((always_inline)) {
-      constexpr bool kWhole = decltype(whole_c)::value;
-      const int64_t k0 = kbeg + (int64_t)kt * kDepth;
-      if constexpr (MA == kDirect && kWhole) a.issue(k0, buf);
-      else a.load(k0, kend);
-      if constexpr (MB == kDirect && kWhole) b.issue(k0, buf + kB);
-      else b.load(k0, kend);
-    };
-    auto after = [&](char* buf, auto whole_c) __attribute__((always_inline)) {
-      constexpr bool kWhole = decltype(whole_c)::value;
-      if constexpr (MA != kDirect || !kWhole) a.store(buf);
-      if constexpr (MB != kDirect || !kWhole) b.store(buf + kB);
-    };
-    constexpr std::true_type yes{};
-    constexpr std::false_type no{};
-    if (whole > 0) {
-      before(0, lds, yes);
-      after(lds, yes);
+  const int whole = MA == kDirect || MB == kDirect ? (int)((kend - kbeg) / kDepth) : slabs;
+  // start: sends slab kt on its way into buf; a last slab (rest) of an operand
+  // that goes straight to LDS is there when it returns.  finish: stores what
+  // passes registers.
+  auto start = [&](int kt, char* buf, auto rest) __attribute__((always_inline)) {
+    constexpr bool kRest = decltype(rest)::value;
+    const int64_t k0 = kbeg + (int64_t)kt * kDepth;
+    if constexpr (MA != kDirect) {
+      a.load(k0, kend);
+    } else if constexpr (kRest) {
+      a.load(k0, kend);
+      a.store(buf);
     } else {
-      before(0, lds, no);
-      after(lds, no);
+      a.issue(k0, buf);
     }
+    if constexpr (MB != kDirect) {
+      b.load(k0, kend);
+    } else if constexpr (kRest) {
+      b.load(k0, kend);
+      b.store(buf + kB);
+    } else {
+      b.issue(k0, buf + kB);
+    }
+  };
+  auto finish = [&](char* buf) __attribute__((always_inline)) {
+    if constexpr (MA != kDirect) a.store(buf);
+    if constexpr (MB != kDirect) b.store(buf + kB);
+  };
+  // One slab.  The fragments of a k step are read under the step before it;
+  // the last step's MFMAs cover the barrier that publishes the next slab, its
+  // first reads, and the start of the slab after it, which takes the buffer
+  // that every wave has just read for the last time.
+  auto slab = [&](int kt, bool next, bool third, auto rest) __attribute__((always_inline)) {
+    char* cur = lds + (kt & 1) * G::kBuf;
+    char* nxt = lds + ((kt + 1) & 1) * G::kBuf;
+#pragma unroll
+    for (int st = 0; st + 1 < kSteps; ++st) {
+      read_step(cur, st + 1);
+      mma_step(st);
+    }
+    if (next) {
+      finish(nxt);
+      slab_barrier();
+      if (third) start(kt + 2, cur, rest);
+      read_step(nxt, 0);
+    }
+    mma_step(kSteps - 1);
+  };
+  if (slabs > 0) {
+    constexpr std::true_type rest{};
+    constexpr std::false_type full{};
+    if (whole > 0) start(0, lds, full);
+    else start(0, lds, rest);
+    finish(lds);
     slab_barrier();
+    if (whole > 1) start(1, lds + G::kBuf, full);
+    else if (slabs > 1) start(1, lds + G::kBuf, rest);
+    read_step(lds, 0);
     int kt = 0;
-    for (; kt + 1 < whole; ++kt) {
-      char* nxt = lds + ((kt + 1) & 1) * G::kBuf;
-      before(kt + 1, nxt, yes);
-      compute(lds + (kt & 1) * G::kBuf);
-      after(nxt, yes);
-      slab_barrier();
-    }
-    if (kt + 1 < slabs) {
-      char* nxt = lds + ((kt + 1) & 1) * G::kBuf;
-      before(kt + 1, nxt, no);
-      compute(lds + (kt & 1) * G::kBuf);
-      after(nxt, no);
-      slab_barrier();
-      ++kt;
-    }
-    compute(lds + (kt & 1) * G::kBuf);
+#pragma unroll 1
+    for (; kt + 2 < whole; ++kt) slab(kt, true, true, full);
+#pragma unroll 1
+    for (; kt < slabs; ++kt) slab(kt, kt + 1 < slabs, kt + 2 < slabs, rest);
   }
 
   // The wave's outputs go through LDS to become whole 16-byte pieces of rows.

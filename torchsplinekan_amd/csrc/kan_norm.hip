@@ -34,7 +34,7 @@ struct NormParams {
   float* rstd;             // [2, n]: r1, r2 (optional in the forward)
   const void *dxo, *dh;    // backward: gradients of x' and h, either may be null
   void *dx, *dy, *dgate;
-  float *part_pre, *part_post, *part_scale;  // [blocks, C]
+  float *part_pre, *part_branch;  // [blocks, C]: sums of dh xh and of D a(g) yh
   float* part_gate;        // kGateRows: [n / L * nchunk, C]; kGateScalars: [n]
   int64_t n, C, L;
   int64_t chunk, nchunk, seg_rows;  // rows of a block; see row_range
@@ -207,10 +207,9 @@ __global__ __launch_bounds__(kRowThreads) void norm_rows_grad_kernel(NormParams 
       if (dh != nullptr) add_part(p.part_pre, b * p.C + c, first, (float)dh[c] * v.stream(c) * r2);
       if (v.y == nullptr) continue;
       const float a = v.a(c), u = v.u(c), sc = v.scale(c), vv = d * sc * a;
-      add_part(p.part_scale, b * p.C + c, first, d * a * u);
+      const float yh = (float)v.y[c] * v.r1;
+      add_part(p.part_branch, b * p.C + c, first, d * a * yh);
       if (p.post != nullptr) {
-        const float yh = (float)v.y[c] * v.r1;
-        add_part(p.part_post, b * p.C + c, first, vv * yh);
         s1 += vv * v.post(c) * yh;
       } else if (p.dy != nullptr) {
         static_cast<TY*>(p.dy)[row * p.C + c] = (TY)vv;
@@ -240,26 +239,330 @@ __global__ __launch_bounds__(kRowThreads) void norm_rows_grad_kernel(NormParams 
   }
 }
 
-// out[g, c] = sum over r < rows of part[g rows + r, c], in a fixed order:
-// 16 lanes of rows a column, their sums added in order.
+// ---- rows held in registers ---------------------------------------------------
+// TPR lanes share a row, each with 8 of its values in NV pieces of VEC; a block
+// is one row's lanes, or four waves with a row each, and runs through its rows,
+// the weights staying in registers.  Every value is read once: the
+// passes above happen on registers, a row's sums cross its waves through LDS.
+template <int TPR>
+struct RowShape {
+  static constexpr int kThreads = TPR == 64 ? 256 : TPR;
+  static constexpr int kRows = kThreads / TPR;  // rows at once
+  static constexpr int kWaves = TPR / 64;       // of a row
+  static_assert(kRows == 1 || kWaves == 1, "rows side by side share no barrier");
+};
+
+// Sums of M values over a row's lanes.  Rows of several waves take two buffers
+// in turn, so that one barrier a sum is enough: a wave that writes a buffer
+// again has passed the barrier after which all had read it.
+template <int TPR, int M>
+__device__ __forceinline__ void row_sums(float (&v)[M], float* red, int& turn) {
+#pragma unroll
+  for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
+  constexpr int W = RowShape<TPR>::kWaves;
+  if constexpr (W > 1) {
+    float* buf = red + turn * (2 * W) + 0;
+    turn ^= 1;
+    const int w = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int m = 0; m < M; ++m) buf[m * W + w] = v[m];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < W; ++i) s += buf[m * W + i];
+      v[m] = s;
+    }
+  }
+}
+
+#define KAN_EACH                     \
+  _Pragma("unroll") for (int i = 0; i < NV; ++i) _Pragma("unroll") for (int j = 0; j < VEC; ++j)
+
+// The lane's pieces of a row of C values: piece i starts at (i TPR + lane) VEC.
+// Pieces past the row's end are zero and not stored.
+template <typename T, int TPR, int VEC, int NV>
+struct Pieces {
+  __device__ __forceinline__ static int64_t at(int i) {
+    return (int64_t)(i * TPR + (int)threadIdx.x % TPR) * VEC;
+  }
+  __device__ __forceinline__ static void load(float (&v)[NV][VEC], const T* __restrict__ row,
+                                              int64_t C) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (at(i) < C) {
+        load_f32<T, VEC>(row + at(i), v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+      }
+    }
+  }
+  __device__ __forceinline__ static void store(const float (&v)[NV][VEC], T* __restrict__ row,
+                                               int64_t C) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (at(i) < C) store_f32<T, VEC>(row + at(i), v[i]);
+  }
+};
+
+// The lane's pieces of a weight vector (of `none` where there is no vector).
+template <int TPR, int VEC, int NV>
+__device__ __forceinline__ void load_weight(float (&v)[NV][VEC], const void* __restrict__ w,
+                                            int dtype, int64_t C, float none) {
+  if (w == nullptr) {
+    KAN_EACH v[i][j] = none;
+  } else if (dtype == KAN_DTYPE_F32) {
+    Pieces<float, TPR, VEC, NV>::load(v, static_cast<const float*>(w), C);
+  } else if (dtype == KAN_DTYPE_BF16) {
+    Pieces<bf16, TPR, VEC, NV>::load(v, static_cast<const bf16*>(w), C);
+  } else {
+    Pieces<f16, TPR, VEC, NV>::load(v, static_cast<const f16*>(w), C);
+  }
+}
+
+// GATED: the gate has a value for every column.
+template <typename TX, typename TY, int TPR, int VEC, int NV, bool GATED>
+__global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_kernel(NormParams p) {
+  typedef RowShape<TPR> S;
+  typedef Pieces<TX, TPR, VEC, NV> PX;
+  typedef Pieces<TY, TPR, VEC, NV> PY;
+  __shared__ float red[4 * S::kWaves];
+  int turn = 0;
+  const float inv_c = 1.0f / (float)p.C;
+  const bool branch = p.y != nullptr, normed = p.post != nullptr;
+  float sp[NV][VEC], pre[NV][VEC];  // scale * post; pre
+  if (branch) {
+    load_weight<TPR>(sp, p.post, p.wdtype, p.C, 1.0f);
+    load_weight<TPR>(pre, p.scale, p.wdtype, p.C, p.scale_const);
+    KAN_EACH sp[i][j] *= pre[i][j];
+  }
+  if (p.h_out != nullptr) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
+  // (every wave of a row takes the same number of turns)
+  for (int64_t r0 = (int64_t)blockIdx.x * S::kRows; r0 < p.n; r0 += (int64_t)gridDim.x * S::kRows) {
+    const int64_t row = r0 + threadIdx.x / TPR;
+    if (S::kRows > 1 && row >= p.n) break;
+    float x[NV][VEC];
+    PX::load(x, static_cast<const TX*>(p.x) + row * p.C, p.C);
+    if (branch) {
+      float y[NV][VEC], g[NV][VEC];
+      PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
+      float r1 = 1.0f;
+      if constexpr (GATED) PY::load(g, static_cast<const TY*>(p.gate) + row / p.L * p.C, p.C);
+      if (normed) {
+        float s[1] = {0.0f};
+        KAN_EACH s[0] += y[i][j] * y[i][j];
+        row_sums<TPR>(s, red, turn);
+        r1 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
+        if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[row] = r1;
+      }
+      if (!GATED && p.gate_kind != kGateNone)
+        r1 *= act_of((float)static_cast<const TY*>(p.gate)[row / p.L], p.act);
+      KAN_EACH {
+        float u = y[i][j] * r1 * sp[i][j];
+        if constexpr (GATED) u *= act_of(g[i][j], p.act);
+        x[i][j] += u;
+      }
+      if (p.x_out != nullptr) PX::store(x, static_cast<TX*>(p.x_out) + row * p.C, p.C);
+    }
+    if (p.h_out == nullptr) continue;
+    float s[1] = {0.0f};
+    KAN_EACH s[0] += x[i][j] * x[i][j];
+    row_sums<TPR>(s, red, turn);
+    const float r2 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
+    if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[p.n + row] = r2;
+    KAN_EACH x[i][j] *= r2 * pre[i][j];
+    PY::store(x, static_cast<TY*>(p.h_out) + row * p.C, p.C);
+  }
+}
+
+// This block's column sums into one partial row: rows that were handled side
+// by side are added through LDS in order.
+template <int TPR, int VEC, int NV>
+__device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __restrict__ out,
+                                              int64_t C, float* lds) {
+  typedef RowShape<TPR> S;
+  const int r = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  if constexpr (S::kRows > 1) {
+    __syncthreads();
+    KAN_EACH lds[(i * VEC + j) * S::kThreads + threadIdx.x] = v[i][j];
+    __syncthreads();
+    if (r != 0) return;
+    KAN_EACH {
+#pragma unroll
+      for (int q = 1; q < S::kRows; ++q)
+        v[i][j] += lds[(i * VEC + j) * S::kThreads + q * TPR + t];
+    }
+  }
+  Pieces<float, TPR, VEC, NV>::store(v, out, C);
+}
+
+// dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
+// sum serves both, and a weight's factor is applied after it, so a lane keeps
+// only pre and scale * post, and two sums (three with a gate row's).
+template <typename TX, typename TY, int TPR, int VEC, int NV, bool GATED>
+__global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(NormParams p) {
+  typedef RowShape<TPR> S;
+  typedef Pieces<TX, TPR, VEC, NV> PX;
+  typedef Pieces<TY, TPR, VEC, NV> PY;
+  constexpr int kCols = S::kRows > 1 ? NV * VEC * S::kThreads : 1;
+  __shared__ float red[4 * S::kWaves];
+  __shared__ float cols[kCols];
+  int turn = 0;
+  const float inv_c = 1.0f / (float)p.C;
+  const bool branch = p.y != nullptr, normed = p.post != nullptr, with_h = p.dh != nullptr;
+  const bool one = !GATED && p.gate_kind != kGateNone;
+  const bool gate_rows = GATED && p.gate_kind == kGateRows;
+  float sp[NV][VEC], pre[NV][VEC];
+  float s_pre[NV][VEC] = {}, s_branch[NV][VEC] = {}, s_gate[NV][VEC] = {};
+  if (branch) {
+    load_weight<TPR>(sp, p.post, p.wdtype, p.C, 1.0f);
+    load_weight<TPR>(pre, p.scale, p.wdtype, p.C, p.scale_const);
+    KAN_EACH sp[i][j] *= pre[i][j];
+  }
+  if (with_h) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
+  const RowRange rr = row_range(p, blockIdx.x);
+  for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
+    const int64_t end = gate_rows ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
+    for (int64_t r0 = seg; r0 < end; r0 += S::kRows) {
+      const int64_t row = r0 + threadIdx.x / TPR;
+      if (S::kRows > 1 && row >= end) break;
+      float d[NV][VEC], x[NV][VEC], y[NV][VEC], dh[NV][VEC], a[NV][VEC], slope[NV][VEC];
+      float r1 = 1.0f, r2 = 0.0f, a1 = 1.0f, slope1 = 0.0f;
+      if (p.dxo != nullptr) PX::load(d, static_cast<const TX*>(p.dxo) + row * p.C, p.C);
+      else KAN_EACH d[i][j] = 0.0f;
+      if (with_h) {
+        PX::load(x, static_cast<const TX*>(p.x) + row * p.C, p.C);
+        PY::load(dh, static_cast<const TY*>(p.dh) + row * p.C, p.C);
+        r2 = p.rstd[p.n + row];
+      }
+      if (branch) {
+        PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
+        if (normed) r1 = p.rstd[row];
+        if constexpr (GATED) {
+          PY::load(a, static_cast<const TY*>(p.gate) + row / p.L * p.C, p.C);
+          KAN_EACH {
+            slope[i][j] = act_slope(a[i][j], p.act);
+            a[i][j] = act_of(a[i][j], p.act);
+          }
+        } else if (one) {
+          const float g = (float)static_cast<const TY*>(p.gate)[row / p.L];
+          a1 = act_of(g, p.act);
+          slope1 = act_slope(g, p.act);
+        }
+        KAN_EACH y[i][j] *= r1;  // yh (y itself without post)
+      }
+      auto gate_of = [&](int i, int j) __attribute__((always_inline)) {
+        if constexpr (GATED) return a[i][j];
+        else return a1;
+      };
+      if (with_h) {
+        float s[1] = {0.0f};
+        KAN_EACH {
+          if (branch) x[i][j] += gate_of(i, j) * (y[i][j] * sp[i][j]);
+          x[i][j] *= r2;  // xh
+          s_pre[i][j] += dh[i][j] * x[i][j];
+          dh[i][j] *= pre[i][j];  // t
+          s[0] += dh[i][j] * x[i][j];
+        }
+        row_sums<TPR>(s, red, turn);
+        const float m2 = s[0] * inv_c;
+        KAN_EACH d[i][j] += r2 * (dh[i][j] - x[i][j] * m2);
+      }
+      if (p.dx != nullptr) PX::store(d, static_cast<TX*>(p.dx) + row * p.C, p.C);
+      if (!branch) continue;
+      float s[2] = {0.0f, 0.0f};  // of w yh; of the gate's gradient
+      KAN_EACH {
+        const float da = d[i][j] * gate_of(i, j);
+        s_branch[i][j] += da * y[i][j];
+        if constexpr (GATED) slope[i][j] *= d[i][j] * y[i][j];
+        else s[1] += d[i][j] * y[i][j] * sp[i][j];
+        d[i][j] = da * sp[i][j];  // w
+        s[0] += d[i][j] * y[i][j];
+      }
+      if constexpr (GATED) {
+        if (gate_rows) {
+          KAN_EACH s_gate[i][j] += slope[i][j];
+        } else if (p.dgate != nullptr) {
+          KAN_EACH slope[i][j] *= sp[i][j];
+          PY::store(slope, static_cast<TY*>(p.dgate) + row * p.C, p.C);
+        }
+      }
+      if (normed || one) row_sums<TPR>(s, red, turn);
+      if (one && p.dgate != nullptr && threadIdx.x % TPR == 0) {
+        if (p.gate_kind == kGateToken) static_cast<TY*>(p.dgate)[row] = (TY)(s[1] * slope1);
+        else p.part_gate[row] = s[1] * slope1;
+      }
+      if (p.dy == nullptr) continue;
+      const float m1 = normed ? s[0] * inv_c : 0.0f;
+      KAN_EACH d[i][j] = r1 * (d[i][j] - y[i][j] * m1);
+      PY::store(d, static_cast<TY*>(p.dy) + row * p.C, p.C);
+    }
+    if (gate_rows && p.dgate != nullptr) {
+      const int64_t at = p.nchunk > 1 ? (int64_t)blockIdx.x : seg / p.L;
+      KAN_EACH s_gate[i][j] *= sp[i][j];
+      flush_columns<TPR>(s_gate, p.part_gate + at * p.C, p.C, cols);
+      KAN_EACH s_gate[i][j] = 0.0f;
+    }
+    seg = end;
+  }
+  const int64_t at = (int64_t)blockIdx.x * p.C;
+  if (p.part_pre != nullptr) flush_columns<TPR>(s_pre, p.part_pre + at, p.C, cols);
+  if (p.part_branch != nullptr) flush_columns<TPR>(s_branch, p.part_branch + at, p.C, cols);
+}
+
+// Column sums of partial rows in a fixed order: 16 lanes of rows a column,
+// their sums added in order.
 constexpr int kSumRowLanes = 16;
-__global__ __launch_bounds__(64 * kSumRowLanes) void sum_rows_kernel(
-    const float* __restrict__ part, int64_t rows, int64_t C, void* __restrict__ out, int dtype) {
+__device__ __forceinline__ bool column_sum(const float* __restrict__ part, int64_t rows, int64_t C,
+                                           int64_t* col, float* sum) {
   __shared__ float red[kSumRowLanes][64];
   const int lane = threadIdx.x & 63, rl = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane, g = blockIdx.y;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
   float s = 0.0f;
   if (c < C) {
-    const float* src = part + g * rows * C + c;
 #pragma unroll 4
-    for (int64_t r = rl; r < rows; r += kSumRowLanes) s += src[r * C];
+    for (int64_t r = rl; r < rows; r += kSumRowLanes) s += part[r * C + c];
   }
   red[rl][lane] = s;
   __syncthreads();
-  if (rl != 0 || c >= C) return;
+  if (rl != 0 || c >= C) return false;
 #pragma unroll
   for (int w = 1; w < kSumRowLanes; ++w) s += red[w][lane];
-  store_any(out, g * C + c, dtype, s);
+  *col = c;
+  *sum = s;
+  return true;
+}
+
+// grid y 0: dpre; 1: dpost and dscale from their common sum.
+__global__ __launch_bounds__(64 * kSumRowLanes) void norm_weights_kernel(
+    NormParams p, int64_t rows, void* __restrict__ dpre, void* __restrict__ dpost,
+    void* __restrict__ dscale) {
+  int64_t c;
+  float s;
+  if (blockIdx.y == 0) {
+    if (p.part_pre != nullptr && column_sum(p.part_pre, rows, p.C, &c, &s))
+      store_any(dpre, c, p.wdtype, s);
+  } else if (p.part_branch != nullptr && column_sum(p.part_branch, rows, p.C, &c, &s)) {
+    if (dpost != nullptr)
+      store_any(dpost, c, p.wdtype,
+                s * (p.scale == nullptr ? p.scale_const : load_any(p.scale, c, p.wdtype)));
+    if (dscale != nullptr)
+      store_any(dscale, c, p.wdtype, p.post == nullptr ? s : s * load_any(p.post, c, p.wdtype));
+  }
+}
+
+// dgate[g, c] = sum of the gate row's `rows` partial rows.
+__global__ __launch_bounds__(64 * kSumRowLanes) void norm_gate_kernel(
+    const float* __restrict__ part, int64_t rows, int64_t C, int64_t g0, void* __restrict__ dgate,
+    int dtype) {
+  const int64_t g = g0 + blockIdx.y;
+  int64_t c;
+  float s;
+  if (column_sum(part + g * rows * C, rows, C, &c, &s)) store_any(dgate, g * C + c, dtype, s);
 }
 
 // out[g] = sum of part[g rows .. (g + 1) rows), one wave a sum.
@@ -274,13 +577,26 @@ __global__ __launch_bounds__(64) void sum_runs_kernel(const float* __restrict__ 
 
 constexpr int64_t kMaxGridY = 65535;
 
+// Lanes that share a row of C values, 8 each (rows past kMaxHeld stay in memory,
+// on blocks of 256).
+constexpr int64_t kMaxHeld = 8192;
+int held_tpr(int64_t C) {
+  if (C > kMaxHeld) return 256;
+  int tpr = 64;
+  while (tpr * 8 < C) tpr *= 2;
+  return tpr;
+}
+
 // How the rows of the backward are dealt to blocks, and the partial sums.
 struct GradPlan {
   int64_t blocks, chunk, nchunk, seg_rows, gate_rows;  // gate_rows of part_gate
   size_t bytes;
 };
 GradPlan grad_plan(int64_t n, int64_t C, int kind, int64_t L) {
-  const int64_t target = 2 * (int64_t)device_cu_count();
+  // 16 waves a CU (one block of the widest shape)
+  const int tpr = held_tpr(C);
+  const int threads = tpr == 64 ? 256 : tpr, at_once = threads / tpr;
+  const int64_t target = device_cu_count() * (int64_t)(1024 / threads);
   GradPlan g{};
   const int64_t want = std::max<int64_t>(1, ceil_div(n, target));
   if (kind == kGateRows && L > want) {
@@ -292,27 +608,81 @@ GradPlan grad_plan(int64_t n, int64_t C, int kind, int64_t L) {
     g.gate_rows = g.blocks;
   } else {
     g.nchunk = 1;
-    g.chunk = kind == kGateRows ? want / L * L : want;
+    g.chunk = kind == kGateRows ? want / L * L : round_up(want, at_once);
     g.seg_rows = g.chunk;
     g.blocks = ceil_div(n, g.chunk);
     g.gate_rows = kind == kGateRows ? n / L : 0;
   }
-  size_t floats = (size_t)(3 * g.blocks + g.gate_rows) * (size_t)C;
+  size_t floats = (size_t)(2 * g.blocks + g.gate_rows) * (size_t)C;
   if (kind == kGateScalars) floats += (size_t)n;
   g.bytes = 4 * floats;
   return g;
 }
 
+// Rows of whole vectors (16 bytes of the branch's type) that start on whole
+// vectors take those; other rows single values.
+bool whole_vectors(const NormParams& p, int vec, size_t xb, size_t yb) {
+  if (p.C % vec != 0) return false;
+  auto ok = [](const void* q, size_t bytes) {
+    return reinterpret_cast<uintptr_t>(q) % (bytes < 16 ? bytes : 16) == 0;
+  };
+  return ok(p.x, vec * xb) && ok(p.x_out, vec * xb) && ok(p.dxo, vec * xb) && ok(p.dx, vec * xb) &&
+         ok(p.y, vec * yb) && ok(p.gate, p.gate_kind == kGateToken || p.gate_kind == kGateScalars
+                                             ? 1 : vec * yb) &&
+         ok(p.h_out, vec * yb) && ok(p.dh, vec * yb) && ok(p.dy, vec * yb) &&
+         ok(p.dgate, p.gate_kind == kGateElement ? vec * yb : 1) && ok(p.post, 16) &&
+         ok(p.pre, 16) && ok(p.scale, 16);
+}
+
+template <typename TX, typename TY, int TPR, int VEC, bool GATED>
+int launch_held(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+  typedef RowShape<TPR> S;
+  if (grad_blocks > 0) {
+    norm_grad_kernel<TX, TY, TPR, VEC, 8 / VEC, GATED>
+        <<<dim3((unsigned)grad_blocks), S::kThreads, 0, st>>>(p);
+    return check_launch("residual_norm_backward");
+  }
+  const int64_t blocks = std::min<int64_t>(ceil_div(p.n, S::kRows),
+                                           device_cu_count() * (int64_t)(2048 / S::kThreads));
+  norm_kernel<TX, TY, TPR, VEC, 8 / VEC, GATED>
+      <<<dim3((unsigned)blocks), S::kThreads, 0, st>>>(p);
+  return check_launch("residual_norm");
+}
+
+template <typename TX, typename TY, int VEC, bool GATED>
+int launch_tpr(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+  switch (held_tpr(p.C)) {
+    case 64: return launch_held<TX, TY, 64, VEC, GATED>(p, grad_blocks, st);
+    case 128: return launch_held<TX, TY, 128, VEC, GATED>(p, grad_blocks, st);
+    case 256: return launch_held<TX, TY, 256, VEC, GATED>(p, grad_blocks, st);
+    case 512: return launch_held<TX, TY, 512, VEC, GATED>(p, grad_blocks, st);
+    default: return launch_held<TX, TY, 1024, VEC, GATED>(p, grad_blocks, st);
+  }
+}
+
+template <typename TX, typename TY, int VEC>
+int launch_vec(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+  return p.gate_kind == kGateElement || p.gate_kind == kGateRows
+             ? launch_tpr<TX, TY, VEC, true>(p, grad_blocks, st)
+             : launch_tpr<TX, TY, VEC, false>(p, grad_blocks, st);
+}
+
+// grad_blocks > 0: the backward, on that many blocks.
 template <typename TX, typename TY>
-int launch_forward(const NormParams& p, hipStream_t st) {
+int launch_norm(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+  if (p.C <= kMaxHeld) {
+    constexpr int kVec = sizeof(TY) == 2 ? 8 : 4;
+    return whole_vectors(p, kVec, sizeof(TX), sizeof(TY))
+               ? launch_vec<TX, TY, kVec>(p, grad_blocks, st)
+               : launch_vec<TX, TY, 1>(p, grad_blocks, st);
+  }
+  if (grad_blocks > 0) {
+    norm_rows_grad_kernel<TX, TY><<<dim3((unsigned)grad_blocks), kRowThreads, 0, st>>>(p);
+    return check_launch("residual_norm_backward");
+  }
   const int64_t blocks = std::min<int64_t>(p.n, 16 * (int64_t)device_cu_count());
   norm_rows_kernel<TX, TY><<<dim3((unsigned)blocks), kRowThreads, 0, st>>>(p);
   return check_launch("residual_norm");
-}
-template <typename TX, typename TY>
-int launch_grad(const NormParams& p, int64_t blocks, hipStream_t st) {
-  norm_rows_grad_kernel<TX, TY><<<dim3((unsigned)blocks), kRowThreads, 0, st>>>(p);
-  return check_launch("residual_norm_backward");
 }
 
 int check_norm(const char* who, int xdtype, int ydtype, int wdtype, const void* x, const void* y,
@@ -389,7 +759,7 @@ int kan_hip_residual_norm(int xdtype, int ydtype, int wdtype, const void* x, con
                        (dtype_bytes(xdtype) * (x_out != nullptr ? 2 : 1) +
                         dtype_bytes(ydtype) * ((y != nullptr) + (h_out != nullptr)));
   TimedLaunch timed(kClassOther, st, moved);
-#define KAN_CALL(TX, TY) launch_forward<TX, TY>(p, st)
+#define KAN_CALL(TX, TY) launch_norm<TX, TY>(p, 0, st)
   return KAN_NORM_TYPES(xdtype, ydtype, KAN_CALL);
 #undef KAN_CALL
 }
@@ -437,9 +807,8 @@ int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const voi
   const int64_t row_part = g.blocks * C;
   p.pre = grad_h == nullptr ? nullptr : pre_weight;
   p.part_pre = grad_pre == nullptr ? nullptr : ws;
-  p.part_post = grad_post == nullptr ? nullptr : ws + row_part;
-  p.part_scale = grad_scale == nullptr ? nullptr : ws + 2 * row_part;
-  p.part_gate = grad_gate == nullptr ? nullptr : ws + 3 * row_part;
+  p.part_branch = grad_post == nullptr && grad_scale == nullptr ? nullptr : ws + row_part;
+  p.part_gate = grad_gate == nullptr ? nullptr : ws + 2 * row_part;
   p.dxo = grad_x_out;
   p.dh = grad_h;
   p.dx = grad_x;
@@ -457,26 +826,22 @@ int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const voi
        dtype_bytes(ydtype) * ((y != nullptr) + (grad_h != nullptr) + (grad_y != nullptr)));
   {
     TimedLaunch timed(kClassOther, st, moved);
-#define KAN_CALL(TX, TY) launch_grad<TX, TY>(p, g.blocks, st)
+#define KAN_CALL(TX, TY) launch_norm<TX, TY>(p, g.blocks, st)
     const int e = KAN_NORM_TYPES(xdtype, ydtype, KAN_CALL);
 #undef KAN_CALL
     if (e != KAN_OK) return e;
   }
   const unsigned cols = (unsigned)ceil_div(C, 64);
-  auto sum_rows = [&](const float* part, int64_t groups, int64_t rows, void* out, int dtype) {
-    for (int64_t g0 = 0; g0 < groups; g0 += kMaxGridY) {
-      const int64_t cnt = std::min(kMaxGridY, groups - g0);
-      char* dst = static_cast<char*>(out) + (size_t)(g0 * C) * dtype_bytes(dtype);
-      sum_rows_kernel<<<dim3(cols, (unsigned)cnt), 64 * kSumRowLanes, 0, st>>>(
-          part + g0 * rows * C, rows, C, dst, dtype);
-    }
-  };
   TimedLaunch timed(kClassOther, st, (double)g.bytes);
-  if (grad_pre != nullptr) sum_rows(p.part_pre, 1, g.blocks, grad_pre, wdtype);
-  if (grad_post != nullptr) sum_rows(p.part_post, 1, g.blocks, grad_post, wdtype);
-  if (grad_scale != nullptr) sum_rows(p.part_scale, 1, g.blocks, grad_scale, wdtype);
-  if (grad_gate != nullptr && p.gate_kind == kGateRows)
-    sum_rows(p.part_gate, n / p.L, g.nchunk, grad_gate, ydtype);
+  if (p.part_pre != nullptr || p.part_branch != nullptr)
+    norm_weights_kernel<<<dim3(cols, 2), 64 * kSumRowLanes, 0, st>>>(p, g.blocks, grad_pre,
+                                                                    grad_post, grad_scale);
+  if (grad_gate != nullptr && p.gate_kind == kGateRows) {
+    for (int64_t g0 = 0; g0 < n / p.L; g0 += kMaxGridY)
+      norm_gate_kernel<<<dim3(cols, (unsigned)std::min(kMaxGridY, n / p.L - g0)),
+                         64 * kSumRowLanes, 0, st>>>(p.part_gate, g.nchunk, C, g0, grad_gate,
+                                                     ydtype);
+  }
   if (grad_gate != nullptr && p.gate_kind == kGateScalars)
     sum_runs_kernel<<<dim3((unsigned)(n / p.L)), 64, 0, st>>>(p.part_gate, p.L, grad_gate, ydtype);
   return check_launch(who);

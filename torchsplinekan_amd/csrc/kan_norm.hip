@@ -67,22 +67,32 @@ __device__ __forceinline__ float act_of(float g, int act) {
     default: return g;
   }
 }
-__device__ __forceinline__ float act_slope(float g, int act) {
+// a(g) and a'(g) from one evaluation.
+__device__ __forceinline__ void act_both(float g, int act, float* a, float* slope) {
   switch (act) {
-    case KAN_GATE_SIGMOID: {
-      const float s = sigmoid_of(g);
-      return s * (1.0f - s);
-    }
-    case KAN_GATE_TANH: {
-      const float t = tanhf(g);
-      return 1.0f - t * t;
-    }
+    case KAN_GATE_SIGMOID:
+      *a = sigmoid_of(g);
+      *slope = *a * (1.0f - *a);
+      break;
+    case KAN_GATE_TANH:
+      *a = tanhf(g);
+      *slope = 1.0f - *a * *a;
+      break;
     case KAN_GATE_SILU: {
       const float s = sigmoid_of(g);
-      return s * (1.0f + g * (1.0f - s));
+      *a = g * s;
+      *slope = s * (1.0f + g * (1.0f - s));
+      break;
     }
-    default: return 1.0f;
+    default:
+      *a = g;
+      *slope = 1.0f;
   }
+}
+__device__ __forceinline__ float act_slope(float g, int act) {
+  float a, slope;
+  act_both(g, act, &a, &slope);
+  return slope;
 }
 
 // ---- rows of any width ------------------------------------------------------
@@ -324,8 +334,9 @@ __device__ __forceinline__ void load_weight(float (&v)[NV][VEC], const void* __r
   }
 }
 
-// GATED: the gate has a value for every column.
-template <typename TX, typename TY, int TPR, int VEC, int NV, bool GATED>
+// GATE: 0 none or one value a row, 1 a value for every element, 2 a row of
+// values for L rows, evaluated once for all of them that a block has.
+template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE>
 __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_kernel(NormParams p) {
   typedef RowShape<TPR> S;
   typedef Pieces<TX, TPR, VEC, NV> PX;
@@ -334,48 +345,58 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_kernel(NormParam
   int turn = 0;
   const float inv_c = 1.0f / (float)p.C;
   const bool branch = p.y != nullptr, normed = p.post != nullptr;
-  float sp[NV][VEC], pre[NV][VEC];  // scale * post; pre
+  float sp[NV][VEC], pre[NV][VEC], gate[NV][VEC];  // scale * post; pre; scale * post * a(g)
   if (branch) {
     load_weight<TPR>(sp, p.post, p.wdtype, p.C, 1.0f);
     load_weight<TPR>(pre, p.scale, p.wdtype, p.C, p.scale_const);
     KAN_EACH sp[i][j] *= pre[i][j];
   }
   if (p.h_out != nullptr) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
-  // (every wave of a row takes the same number of turns)
-  for (int64_t r0 = (int64_t)blockIdx.x * S::kRows; r0 < p.n; r0 += (int64_t)gridDim.x * S::kRows) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    if (S::kRows > 1 && row >= p.n) break;
-    float x[NV][VEC];
-    PX::load(x, static_cast<const TX*>(p.x) + row * p.C, p.C);
-    if (branch) {
-      float y[NV][VEC], g[NV][VEC];
-      PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
-      float r1 = 1.0f;
-      if constexpr (GATED) PY::load(g, static_cast<const TY*>(p.gate) + row / p.L * p.C, p.C);
-      if (normed) {
-        float s[1] = {0.0f};
-        KAN_EACH s[0] += y[i][j] * y[i][j];
-        row_sums<TPR>(s, red, turn);
-        r1 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
-        if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[row] = r1;
-      }
-      if (!GATED && p.gate_kind != kGateNone)
-        r1 *= act_of((float)static_cast<const TY*>(p.gate)[row / p.L], p.act);
-      KAN_EACH {
-        float u = y[i][j] * r1 * sp[i][j];
-        if constexpr (GATED) u *= act_of(g[i][j], p.act);
-        x[i][j] += u;
-      }
-      if (p.x_out != nullptr) PX::store(x, static_cast<TX*>(p.x_out) + row * p.C, p.C);
+  const RowRange rr = row_range(p, blockIdx.x);
+  for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
+    const int64_t end = GATE == 2 ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
+    if constexpr (GATE == 2) {
+      PY::load(gate, static_cast<const TY*>(p.gate) + seg / p.L * p.C, p.C);
+      KAN_EACH gate[i][j] = act_of(gate[i][j], p.act) * sp[i][j];
     }
-    if (p.h_out == nullptr) continue;
-    float s[1] = {0.0f};
-    KAN_EACH s[0] += x[i][j] * x[i][j];
-    row_sums<TPR>(s, red, turn);
-    const float r2 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
-    if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[p.n + row] = r2;
-    KAN_EACH x[i][j] *= r2 * pre[i][j];
-    PY::store(x, static_cast<TY*>(p.h_out) + row * p.C, p.C);
+    // (every wave of a row takes the same number of turns)
+    for (int64_t r0 = seg; r0 < end; r0 += S::kRows) {
+      const int64_t row = r0 + threadIdx.x / TPR;
+      if (S::kRows > 1 && row >= end) break;
+      float x[NV][VEC];
+      PX::load(x, static_cast<const TX*>(p.x) + row * p.C, p.C);
+      if (branch) {
+        float y[NV][VEC];
+        PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
+        float r1 = 1.0f;
+        if constexpr (GATE == 1) PY::load(gate, static_cast<const TY*>(p.gate) + row * p.C, p.C);
+        if (normed) {
+          float s[1] = {0.0f};
+          KAN_EACH s[0] += y[i][j] * y[i][j];
+          row_sums<TPR>(s, red, turn);
+          r1 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
+          if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[row] = r1;
+        }
+        if (GATE == 0 && p.gate_kind != kGateNone)
+          r1 *= act_of((float)static_cast<const TY*>(p.gate)[row / p.L], p.act);
+        KAN_EACH {
+          if constexpr (GATE == 0) x[i][j] += y[i][j] * r1 * sp[i][j];
+          else if constexpr (GATE == 1)
+            x[i][j] += y[i][j] * r1 * sp[i][j] * act_of(gate[i][j], p.act);
+          else x[i][j] += y[i][j] * r1 * gate[i][j];
+        }
+        if (p.x_out != nullptr) PX::store(x, static_cast<TX*>(p.x_out) + row * p.C, p.C);
+      }
+      if (p.h_out == nullptr) continue;
+      float s[1] = {0.0f};
+      KAN_EACH s[0] += x[i][j] * x[i][j];
+      row_sums<TPR>(s, red, turn);
+      const float r2 = 1.0f / sqrtf(s[0] * inv_c + p.eps);
+      if (p.rstd != nullptr && threadIdx.x % TPR == 0) p.rstd[p.n + row] = r2;
+      KAN_EACH x[i][j] *= r2 * pre[i][j];
+      PY::store(x, static_cast<TY*>(p.h_out) + row * p.C, p.C);
+    }
+    seg = end;
   }
 }
 
@@ -403,8 +424,9 @@ __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __rest
 // dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
 // sum serves both, and a weight's factor is applied after it, so a lane keeps
 // only pre and scale * post, and two sums (three with a gate row's).
-template <typename TX, typename TY, int TPR, int VEC, int NV, bool GATED>
-__global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(NormParams p) {
+template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE>
+__global__ __launch_bounds__(RowShape<TPR>::kThreads) __attribute__((amdgpu_waves_per_eu(4))) void
+norm_grad_kernel(NormParams p) {
   typedef RowShape<TPR> S;
   typedef Pieces<TX, TPR, VEC, NV> PX;
   typedef Pieces<TY, TPR, VEC, NV> PY;
@@ -414,8 +436,8 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(Norm
   int turn = 0;
   const float inv_c = 1.0f / (float)p.C;
   const bool branch = p.y != nullptr, normed = p.post != nullptr, with_h = p.dh != nullptr;
-  const bool one = !GATED && p.gate_kind != kGateNone;
-  const bool gate_rows = GATED && p.gate_kind == kGateRows;
+  const bool one = GATE == 0 && p.gate_kind != kGateNone;
+  float a[NV][VEC], slope[NV][VEC];
   float sp[NV][VEC], pre[NV][VEC];
   float s_pre[NV][VEC] = {}, s_branch[NV][VEC] = {}, s_gate[NV][VEC] = {};
   if (branch) {
@@ -426,11 +448,15 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(Norm
   if (with_h) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
   const RowRange rr = row_range(p, blockIdx.x);
   for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
-    const int64_t end = gate_rows ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
+    const int64_t end = GATE == 2 ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
+    if constexpr (GATE == 2) {
+      PY::load(a, static_cast<const TY*>(p.gate) + seg / p.L * p.C, p.C);
+      KAN_EACH act_both(a[i][j], p.act, &a[i][j], &slope[i][j]);
+    }
     for (int64_t r0 = seg; r0 < end; r0 += S::kRows) {
       const int64_t row = r0 + threadIdx.x / TPR;
       if (S::kRows > 1 && row >= end) break;
-      float d[NV][VEC], x[NV][VEC], y[NV][VEC], dh[NV][VEC], a[NV][VEC], slope[NV][VEC];
+      float d[NV][VEC], x[NV][VEC], y[NV][VEC], dh[NV][VEC];
       float r1 = 1.0f, r2 = 0.0f, a1 = 1.0f, slope1 = 0.0f;
       if (p.dxo != nullptr) PX::load(d, static_cast<const TX*>(p.dxo) + row * p.C, p.C);
       else KAN_EACH d[i][j] = 0.0f;
@@ -442,21 +468,16 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(Norm
       if (branch) {
         PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
         if (normed) r1 = p.rstd[row];
-        if constexpr (GATED) {
-          PY::load(a, static_cast<const TY*>(p.gate) + row / p.L * p.C, p.C);
-          KAN_EACH {
-            slope[i][j] = act_slope(a[i][j], p.act);
-            a[i][j] = act_of(a[i][j], p.act);
-          }
+        if constexpr (GATE == 1) {
+          PY::load(a, static_cast<const TY*>(p.gate) + row * p.C, p.C);
+          KAN_EACH act_both(a[i][j], p.act, &a[i][j], &slope[i][j]);
         } else if (one) {
-          const float g = (float)static_cast<const TY*>(p.gate)[row / p.L];
-          a1 = act_of(g, p.act);
-          slope1 = act_slope(g, p.act);
+          act_both((float)static_cast<const TY*>(p.gate)[row / p.L], p.act, &a1, &slope1);
         }
         KAN_EACH y[i][j] *= r1;  // yh (y itself without post)
       }
       auto gate_of = [&](int i, int j) __attribute__((always_inline)) {
-        if constexpr (GATED) return a[i][j];
+        if constexpr (GATE != 0) return a[i][j];
         else return a1;
       };
       if (with_h) {
@@ -478,18 +499,14 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(Norm
       KAN_EACH {
         const float da = d[i][j] * gate_of(i, j);
         s_branch[i][j] += da * y[i][j];
-        if constexpr (GATED) slope[i][j] *= d[i][j] * y[i][j];
-        else s[1] += d[i][j] * y[i][j] * sp[i][j];
+        if constexpr (GATE == 0) s[1] += d[i][j] * y[i][j] * sp[i][j];
+        else if constexpr (GATE == 1) slope[i][j] *= d[i][j] * y[i][j] * sp[i][j];
+        else s_gate[i][j] += d[i][j] * y[i][j];
         d[i][j] = da * sp[i][j];  // w
         s[0] += d[i][j] * y[i][j];
       }
-      if constexpr (GATED) {
-        if (gate_rows) {
-          KAN_EACH s_gate[i][j] += slope[i][j];
-        } else if (p.dgate != nullptr) {
-          KAN_EACH slope[i][j] *= sp[i][j];
-          PY::store(slope, static_cast<TY*>(p.dgate) + row * p.C, p.C);
-        }
+      if constexpr (GATE == 1) {
+        if (p.dgate != nullptr) PY::store(slope, static_cast<TY*>(p.dgate) + row * p.C, p.C);
       }
       if (normed || one) row_sums<TPR>(s, red, turn);
       if (one && p.dgate != nullptr && threadIdx.x % TPR == 0) {
@@ -501,9 +518,9 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_grad_kernel(Norm
       KAN_EACH d[i][j] = r1 * (d[i][j] - y[i][j] * m1);
       PY::store(d, static_cast<TY*>(p.dy) + row * p.C, p.C);
     }
-    if (gate_rows && p.dgate != nullptr) {
+    if (GATE == 2 && p.dgate != nullptr) {
       const int64_t at = p.nchunk > 1 ? (int64_t)blockIdx.x : seg / p.L;
-      KAN_EACH s_gate[i][j] *= sp[i][j];
+      KAN_EACH s_gate[i][j] *= sp[i][j] * slope[i][j];
       flush_columns<TPR>(s_gate, p.part_gate + at * p.C, p.C, cols);
       KAN_EACH s_gate[i][j] = 0.0f;
     }
@@ -587,17 +604,17 @@ int held_tpr(int64_t C) {
   return tpr;
 }
 
-// How the rows of the backward are dealt to blocks, and the partial sums.
-struct GradPlan {
+// How rows are dealt to blocks, and the backward's partial sums.
+struct RowPlan {
   int64_t blocks, chunk, nchunk, seg_rows, gate_rows;  // gate_rows of part_gate
   size_t bytes;
 };
-GradPlan grad_plan(int64_t n, int64_t C, int kind, int64_t L) {
-  // 16 waves a CU (one block of the widest shape)
+constexpr int kGradWaves = 16;  // waves a CU (one block of the widest shape)
+RowPlan row_plan(int64_t n, int64_t C, int kind, int64_t L, int waves_per_cu) {
   const int tpr = held_tpr(C);
   const int threads = tpr == 64 ? 256 : tpr, at_once = threads / tpr;
-  const int64_t target = device_cu_count() * (int64_t)(1024 / threads);
-  GradPlan g{};
+  const int64_t target = device_cu_count() * (int64_t)std::max(1, 64 * waves_per_cu / threads);
+  RowPlan g{};
   const int64_t want = std::max<int64_t>(1, ceil_div(n, target));
   if (kind == kGateRows && L > want) {
     g.nchunk = ceil_div(L, want);
@@ -634,37 +651,39 @@ bool whole_vectors(const NormParams& p, int vec, size_t xb, size_t yb) {
          ok(p.pre, 16) && ok(p.scale, 16);
 }
 
-template <typename TX, typename TY, int TPR, int VEC, bool GATED>
-int launch_held(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+template <typename TX, typename TY, int TPR, int VEC, int GATE>
+int launch_held(NormParams p, int64_t grad_blocks, hipStream_t st) {
   typedef RowShape<TPR> S;
   if (grad_blocks > 0) {
-    norm_grad_kernel<TX, TY, TPR, VEC, 8 / VEC, GATED>
+    norm_grad_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE>
         <<<dim3((unsigned)grad_blocks), S::kThreads, 0, st>>>(p);
     return check_launch("residual_norm_backward");
   }
-  const int64_t blocks = std::min<int64_t>(ceil_div(p.n, S::kRows),
-                                           device_cu_count() * (int64_t)(2048 / S::kThreads));
-  norm_kernel<TX, TY, TPR, VEC, 8 / VEC, GATED>
-      <<<dim3((unsigned)blocks), S::kThreads, 0, st>>>(p);
+  const RowPlan g = row_plan(p.n, p.C, p.gate_kind, p.L, 32);
+  p.chunk = g.chunk;
+  p.nchunk = g.nchunk;
+  p.seg_rows = g.seg_rows;
+  norm_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE>
+      <<<dim3((unsigned)g.blocks), S::kThreads, 0, st>>>(p);
   return check_launch("residual_norm");
 }
 
-template <typename TX, typename TY, int VEC, bool GATED>
+template <typename TX, typename TY, int VEC, int GATE>
 int launch_tpr(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
   switch (held_tpr(p.C)) {
-    case 64: return launch_held<TX, TY, 64, VEC, GATED>(p, grad_blocks, st);
-    case 128: return launch_held<TX, TY, 128, VEC, GATED>(p, grad_blocks, st);
-    case 256: return launch_held<TX, TY, 256, VEC, GATED>(p, grad_blocks, st);
-    case 512: return launch_held<TX, TY, 512, VEC, GATED>(p, grad_blocks, st);
-    default: return launch_held<TX, TY, 1024, VEC, GATED>(p, grad_blocks, st);
+    case 64: return launch_held<TX, TY, 64, VEC, GATE>(p, grad_blocks, st);
+    case 128: return launch_held<TX, TY, 128, VEC, GATE>(p, grad_blocks, st);
+    case 256: return launch_held<TX, TY, 256, VEC, GATE>(p, grad_blocks, st);
+    case 512: return launch_held<TX, TY, 512, VEC, GATE>(p, grad_blocks, st);
+    default: return launch_held<TX, TY, 1024, VEC, GATE>(p, grad_blocks, st);
   }
 }
 
 template <typename TX, typename TY, int VEC>
 int launch_vec(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
-  return p.gate_kind == kGateElement || p.gate_kind == kGateRows
-             ? launch_tpr<TX, TY, VEC, true>(p, grad_blocks, st)
-             : launch_tpr<TX, TY, VEC, false>(p, grad_blocks, st);
+  if (p.gate_kind == kGateElement) return launch_tpr<TX, TY, VEC, 1>(p, grad_blocks, st);
+  if (p.gate_kind == kGateRows) return launch_tpr<TX, TY, VEC, 2>(p, grad_blocks, st);
+  return launch_tpr<TX, TY, VEC, 0>(p, grad_blocks, st);
 }
 
 // grad_blocks > 0: the backward, on that many blocks.
@@ -773,7 +792,7 @@ int kan_hip_residual_norm_backward_workspace(int64_t gate_rows, int64_t gate_col
                             &p, &p, gate_rows > 0 ? &p : nullptr, nullptr, nullptr, 0, gate_rows,
                             gate_cols, n, C, &p);
   if (rc != KAN_OK) return rc;
-  *bytes = n == 0 || C == 0 ? 0 : grad_plan(n, C, p.gate_kind, p.L).bytes;
+  *bytes = n == 0 || C == 0 ? 0 : row_plan(n, C, p.gate_kind, p.L, kGradWaves).bytes;
   return KAN_OK;
 }
 
@@ -799,7 +818,7 @@ int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const voi
   if (n == 0 || C == 0) return KAN_OK;
   if (x == nullptr || rstd == nullptr)
     return set_error(KAN_ERR_INVALID, "%s: x and rstd must not be NULL", who);
-  const GradPlan g = grad_plan(n, C, p.gate_kind, p.L);
+  const RowPlan g = row_plan(n, C, p.gate_kind, p.L, kGradWaves);
   if (workspace == nullptr || workspace_bytes < g.bytes)
     return set_error(KAN_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, g.bytes,
                      workspace == nullptr ? (size_t)0 : workspace_bytes);

@@ -293,8 +293,10 @@ __device__ __forceinline__ void row_sums(float (&v)[M], float* red, int& turn) {
   _Pragma("unroll") for (int i = 0; i < NV; ++i) _Pragma("unroll") for (int j = 0; j < VEC; ++j)
 
 // The lane's pieces of a row of C values: piece i starts at (i TPR + lane) VEC.
-// Pieces past the row's end are zero and not stored.
-template <typename T, int TPR, int VEC, int NV>
+// Values past the row's end are zero and not stored.  WHOLE: rows are whole
+// vectors, on 16 bytes; otherwise vectors lie anywhere, and a row's last piece
+// goes value by value.
+template <typename T, int TPR, int VEC, int NV, bool WHOLE>
 struct Pieces {
   __device__ __forceinline__ static int64_t at(int i) {
     return (int64_t)(i * TPR + (int)threadIdx.x % TPR) * VEC;
@@ -303,55 +305,62 @@ struct Pieces {
                                               int64_t C) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (at(i) < C) {
-        load_f32<T, VEC>(row + at(i), v[i]);
+      if (at(i) + VEC <= C) {
+        load_f32<T, VEC, WHOLE>(row + at(i), v[i]);
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = 0.0f;
+        for (int j = 0; j < VEC; ++j) v[i][j] = !WHOLE && at(i) + j < C ? (float)row[at(i) + j] : 0.0f;
       }
     }
   }
   __device__ __forceinline__ static void store(const float (&v)[NV][VEC], T* __restrict__ row,
                                                int64_t C) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (at(i) < C) store_f32<T, VEC>(row + at(i), v[i]);
+    for (int i = 0; i < NV; ++i) {
+      if (at(i) + VEC <= C) {
+        store_f32<T, VEC, WHOLE>(row + at(i), v[i]);
+      } else if constexpr (!WHOLE) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (at(i) + j < C) row[at(i) + j] = (T)v[i][j];
+      }
+    }
   }
 };
 
 // The lane's pieces of a weight vector (of `none` where there is no vector).
-template <int TPR, int VEC, int NV>
+template <int TPR, bool WHOLE, int VEC, int NV>
 __device__ __forceinline__ void load_weight(float (&v)[NV][VEC], const void* __restrict__ w,
                                             int dtype, int64_t C, float none) {
   if (w == nullptr) {
     KAN_EACH v[i][j] = none;
   } else if (dtype == KAN_DTYPE_F32) {
-    Pieces<float, TPR, VEC, NV>::load(v, static_cast<const float*>(w), C);
+    Pieces<float, TPR, VEC, NV, WHOLE>::load(v, static_cast<const float*>(w), C);
   } else if (dtype == KAN_DTYPE_BF16) {
-    Pieces<bf16, TPR, VEC, NV>::load(v, static_cast<const bf16*>(w), C);
+    Pieces<bf16, TPR, VEC, NV, WHOLE>::load(v, static_cast<const bf16*>(w), C);
   } else {
-    Pieces<f16, TPR, VEC, NV>::load(v, static_cast<const f16*>(w), C);
+    Pieces<f16, TPR, VEC, NV, WHOLE>::load(v, static_cast<const f16*>(w), C);
   }
 }
 
 // GATE: 0 none or one value a row, 1 a value for every element, 2 a row of
 // values for L rows, evaluated once for all of them that a block has.
-template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE>
+template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_kernel(NormParams p) {
   typedef RowShape<TPR> S;
-  typedef Pieces<TX, TPR, VEC, NV> PX;
-  typedef Pieces<TY, TPR, VEC, NV> PY;
+  typedef Pieces<TX, TPR, VEC, NV, WHOLE> PX;
+  typedef Pieces<TY, TPR, VEC, NV, WHOLE> PY;
   __shared__ float red[4 * S::kWaves];
   int turn = 0;
   const float inv_c = 1.0f / (float)p.C;
   const bool branch = p.y != nullptr, normed = p.post != nullptr;
   float sp[NV][VEC], pre[NV][VEC], gate[NV][VEC];  // scale * post; pre; scale * post * a(g)
   if (branch) {
-    load_weight<TPR>(sp, p.post, p.wdtype, p.C, 1.0f);
-    load_weight<TPR>(pre, p.scale, p.wdtype, p.C, p.scale_const);
+    load_weight<TPR, WHOLE>(sp, p.post, p.wdtype, p.C, 1.0f);
+    load_weight<TPR, WHOLE>(pre, p.scale, p.wdtype, p.C, p.scale_const);
     KAN_EACH sp[i][j] *= pre[i][j];
   }
-  if (p.h_out != nullptr) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
+  if (p.h_out != nullptr) load_weight<TPR, WHOLE>(pre, p.pre, p.wdtype, p.C, 1.0f);
   const RowRange rr = row_range(p, blockIdx.x);
   for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
     const int64_t end = GATE == 2 ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void norm_kernel(NormParam
 
 // This block's column sums into one partial row: rows that were handled side
 // by side are added through LDS in order.
-template <int TPR, int VEC, int NV>
+template <int TPR, bool WHOLE, int VEC, int NV>
 __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __restrict__ out,
                                               int64_t C, float* lds) {
   typedef RowShape<TPR> S;
@@ -418,18 +427,20 @@ __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __rest
         v[i][j] += lds[(i * VEC + j) * S::kThreads + q * TPR + t];
     }
   }
-  Pieces<float, TPR, VEC, NV>::store(v, out, C);
+  Pieces<float, TPR, VEC, NV, WHOLE>::store(v, out, C);
 }
 
-// dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
+// Four waves a SIMD (128 registers; a float32 row of 512 lanes with a gate would
+// spill there and takes two).  dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
 // sum serves both, and a weight's factor is applied after it, so a lane keeps
 // only pre and scale * post, and two sums (three with a gate row's).
-template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE>
-__global__ __launch_bounds__(RowShape<TPR>::kThreads) __attribute__((amdgpu_waves_per_eu(4))) void
+template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE, bool WHOLE>
+__global__ __launch_bounds__(RowShape<TPR>::kThreads) __attribute__((
+    amdgpu_waves_per_eu(sizeof(TY) == 4 && TPR == 512 && GATE != 0 ? 2 : 4))) void
 norm_grad_kernel(NormParams p) {
   typedef RowShape<TPR> S;
-  typedef Pieces<TX, TPR, VEC, NV> PX;
-  typedef Pieces<TY, TPR, VEC, NV> PY;
+  typedef Pieces<TX, TPR, VEC, NV, WHOLE> PX;
+  typedef Pieces<TY, TPR, VEC, NV, WHOLE> PY;
   constexpr int kCols = S::kRows > 1 ? NV * VEC * S::kThreads : 1;
   __shared__ float red[4 * S::kWaves];
   __shared__ float cols[kCols];
@@ -441,11 +452,11 @@ norm_grad_kernel(NormParams p) {
   float sp[NV][VEC], pre[NV][VEC];
   float s_pre[NV][VEC] = {}, s_branch[NV][VEC] = {}, s_gate[NV][VEC] = {};
   if (branch) {
-    load_weight<TPR>(sp, p.post, p.wdtype, p.C, 1.0f);
-    load_weight<TPR>(pre, p.scale, p.wdtype, p.C, p.scale_const);
+    load_weight<TPR, WHOLE>(sp, p.post, p.wdtype, p.C, 1.0f);
+    load_weight<TPR, WHOLE>(pre, p.scale, p.wdtype, p.C, p.scale_const);
     KAN_EACH sp[i][j] *= pre[i][j];
   }
-  if (with_h) load_weight<TPR>(pre, p.pre, p.wdtype, p.C, 1.0f);
+  if (with_h) load_weight<TPR, WHOLE>(pre, p.pre, p.wdtype, p.C, 1.0f);
   const RowRange rr = row_range(p, blockIdx.x);
   for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
     const int64_t end = GATE == 2 ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
@@ -521,14 +532,14 @@ norm_grad_kernel(NormParams p) {
     if (GATE == 2 && p.dgate != nullptr) {
       const int64_t at = p.nchunk > 1 ? (int64_t)blockIdx.x : seg / p.L;
       KAN_EACH s_gate[i][j] *= sp[i][j] * slope[i][j];
-      flush_columns<TPR>(s_gate, p.part_gate + at * p.C, p.C, cols);
+      flush_columns<TPR, WHOLE>(s_gate, p.part_gate + at * p.C, p.C, cols);
       KAN_EACH s_gate[i][j] = 0.0f;
     }
     seg = end;
   }
   const int64_t at = (int64_t)blockIdx.x * p.C;
-  if (p.part_pre != nullptr) flush_columns<TPR>(s_pre, p.part_pre + at, p.C, cols);
-  if (p.part_branch != nullptr) flush_columns<TPR>(s_branch, p.part_branch + at, p.C, cols);
+  if (p.part_pre != nullptr) flush_columns<TPR, WHOLE>(s_pre, p.part_pre + at, p.C, cols);
+  if (p.part_branch != nullptr) flush_columns<TPR, WHOLE>(s_branch, p.part_branch + at, p.C, cols);
 }
 
 // Column sums of partial rows in a fixed order: 16 lanes of rows a column,
@@ -636,8 +647,8 @@ RowPlan row_plan(int64_t n, int64_t C, int kind, int64_t L, int waves_per_cu) {
   return g;
 }
 
-// Rows of whole vectors (16 bytes of the branch's type) that start on whole
-// vectors take those; other rows single values.
+// Whether rows are whole vectors (16 bytes of the branch's type) and every
+// operand lies on 16 bytes.
 bool whole_vectors(const NormParams& p, int vec, size_t xb, size_t yb) {
   if (p.C % vec != 0) return false;
   auto ok = [](const void* q, size_t bytes) {
@@ -651,11 +662,12 @@ bool whole_vectors(const NormParams& p, int vec, size_t xb, size_t yb) {
          ok(p.pre, 16) && ok(p.scale, 16);
 }
 
-template <typename TX, typename TY, int TPR, int VEC, int GATE>
+template <typename TX, typename TY, int TPR, int GATE, bool WHOLE>
 int launch_held(NormParams p, int64_t grad_blocks, hipStream_t st) {
   typedef RowShape<TPR> S;
+  constexpr int VEC = sizeof(TY) == 2 ? 8 : 4;
   if (grad_blocks > 0) {
-    norm_grad_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE>
+    norm_grad_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE, WHOLE>
         <<<dim3((unsigned)grad_blocks), S::kThreads, 0, st>>>(p);
     return check_launch("residual_norm_backward");
   }
@@ -663,38 +675,36 @@ int launch_held(NormParams p, int64_t grad_blocks, hipStream_t st) {
   p.chunk = g.chunk;
   p.nchunk = g.nchunk;
   p.seg_rows = g.seg_rows;
-  norm_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE>
+  norm_kernel<TX, TY, TPR, VEC, 8 / VEC, GATE, WHOLE>
       <<<dim3((unsigned)g.blocks), S::kThreads, 0, st>>>(p);
   return check_launch("residual_norm");
 }
 
-template <typename TX, typename TY, int VEC, int GATE>
+template <typename TX, typename TY, int GATE, bool WHOLE>
 int launch_tpr(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
   switch (held_tpr(p.C)) {
-    case 64: return launch_held<TX, TY, 64, VEC, GATE>(p, grad_blocks, st);
-    case 128: return launch_held<TX, TY, 128, VEC, GATE>(p, grad_blocks, st);
-    case 256: return launch_held<TX, TY, 256, VEC, GATE>(p, grad_blocks, st);
-    case 512: return launch_held<TX, TY, 512, VEC, GATE>(p, grad_blocks, st);
-    default: return launch_held<TX, TY, 1024, VEC, GATE>(p, grad_blocks, st);
+    case 64: return launch_held<TX, TY, 64, GATE, WHOLE>(p, grad_blocks, st);
+    case 128: return launch_held<TX, TY, 128, GATE, WHOLE>(p, grad_blocks, st);
+    case 256: return launch_held<TX, TY, 256, GATE, WHOLE>(p, grad_blocks, st);
+    case 512: return launch_held<TX, TY, 512, GATE, WHOLE>(p, grad_blocks, st);
+    default: return launch_held<TX, TY, 1024, GATE, WHOLE>(p, grad_blocks, st);
   }
 }
 
-template <typename TX, typename TY, int VEC>
-int launch_vec(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
-  if (p.gate_kind == kGateElement) return launch_tpr<TX, TY, VEC, 1>(p, grad_blocks, st);
-  if (p.gate_kind == kGateRows) return launch_tpr<TX, TY, VEC, 2>(p, grad_blocks, st);
-  return launch_tpr<TX, TY, VEC, 0>(p, grad_blocks, st);
+template <typename TX, typename TY, bool WHOLE>
+int launch_gate(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
+  if (p.gate_kind == kGateElement) return launch_tpr<TX, TY, 1, WHOLE>(p, grad_blocks, st);
+  if (p.gate_kind == kGateRows) return launch_tpr<TX, TY, 2, WHOLE>(p, grad_blocks, st);
+  return launch_tpr<TX, TY, 0, WHOLE>(p, grad_blocks, st);
 }
 
 // grad_blocks > 0: the backward, on that many blocks.
 template <typename TX, typename TY>
 int launch_norm(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
-  if (p.C <= kMaxHeld) {
-    constexpr int kVec = sizeof(TY) == 2 ? 8 : 4;
-    return whole_vectors(p, kVec, sizeof(TX), sizeof(TY))
-               ? launch_vec<TX, TY, kVec>(p, grad_blocks, st)
-               : launch_vec<TX, TY, 1>(p, grad_blocks, st);
-  }
+  if (p.C <= kMaxHeld)
+    return whole_vectors(p, sizeof(TY) == 2 ? 8 : 4, sizeof(TX), sizeof(TY))
+               ? launch_gate<TX, TY, true>(p, grad_blocks, st)
+               : launch_gate<TX, TY, false>(p, grad_blocks, st);
   if (grad_blocks > 0) {
     norm_rows_grad_kernel<TX, TY><<<dim3((unsigned)grad_blocks), kRowThreads, 0, st>>>(p);
     return check_launch("residual_norm_backward");

@@ -22,29 +22,32 @@ struct VecOf {
   typedef T type __attribute__((ext_vector_type(V)));
 };
 
-// V consecutive values as floats.  p is aligned to the whole vector.
+// A vector at an address that is aligned to one value only (the hardware
+// takes it; the compiler must not assume more).
 template <typename T, int V>
+struct __attribute__((packed, aligned(sizeof(T)))) LooseVec {
+  typename VecOf<T, V>::type v;
+};
+
+// V consecutive values as floats.  WHOLE: p is aligned to 16 bytes, or to the
+// vector if that is shorter.
+template <typename T, int V, bool WHOLE = true>
 __device__ __forceinline__ void load_f32(const T* __restrict__ p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = (float)p[0];
-  } else {
-    const auto u = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+  typename VecOf<T, V>::type u;
+  if constexpr (WHOLE) u = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+  else u = reinterpret_cast<const LooseVec<T, V>*>(p)->v;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = (float)u[j];
-  }
+  for (int j = 0; j < V; ++j) v[j] = (float)u[j];
 }
 
 // The same rounded to T (to nearest, ties to even).
-template <typename T, int V>
+template <typename T, int V, bool WHOLE = true>
 __device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    p[0] = (T)v[0];
-  } else {
-    typename VecOf<T, V>::type u;
+  typename VecOf<T, V>::type u;
 #pragma unroll
-    for (int j = 0; j < V; ++j) u[j] = (T)v[j];
-    *reinterpret_cast<typename VecOf<T, V>::type*>(p) = u;
-  }
+  for (int j = 0; j < V; ++j) u[j] = (T)v[j];
+  if constexpr (WHOLE) *reinterpret_cast<typename VecOf<T, V>::type*>(p) = u;
+  else reinterpret_cast<LooseVec<T, V>*>(p)->v = u;
 }
 
 // One value of an array whose type is known at run time (the short vectors of

@@ -461,14 +461,14 @@ int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* s
  *   KAN_GROUPED_INPUT    a = dy [T, N], b = w:  out dx [T, K], dx[t] = w[e]^T dy[t]
  *   KAN_GROUPED_WEIGHT   a = dy [T, N], b = x:  out dw [E, N, K], the sum of
  *                        dy[t] x[t]^T over the expert's rows (zeros without any)
- * Rows from offsets[E] on get zeros.  The weight product also takes b as 8-bit
+ * Rows from offsets[E] on get zeros.  T < 2^30, N and K <= 2^22, E <= 65535.  The weight product also takes b as 8-bit
  * rows (b_format, with b_scale and b_group as kan_hip_act8_quantize keeps
  * them; KAN_ACT8_NONE otherwise). */
 #define KAN_GROUPED_FORWARD 0
 #define KAN_GROUPED_INPUT 1
 #define KAN_GROUPED_WEIGHT 2
-int kan_hip_grouped_matmul_workspace(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K,
-                                     size_t* bytes);
+int kan_hip_grouped_matmul_workspace(int dtype, int op, int b_format, int64_t T, int64_t E,
+                                     int64_t N, int64_t K, size_t* bytes);
 int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,

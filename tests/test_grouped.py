@@ -130,7 +130,7 @@ def test_c_entry_refusals():
     assert f(2, 0, None, p, 0, None, 0, p, 0, *tail) == lib.KAN_ERR_INVALID
     assert f(2, 0, p, p, 0, None, 0, None, 0, *tail) == lib.KAN_ERR_INVALID
     assert f(2, 0, p, p, 0, None, 0, p, 0, -1, 2, 16, 16, p, None, 0, None) == lib.KAN_ERR_INVALID
-    assert f(2, 0, p, p, 0, None, 0, p, 0, 8, 1 << 21, 16, 16, p, None, 0,
+    assert f(2, 0, p, p, 0, None, 0, p, 0, 8, 1 << 16, 16, 16, p, None, 0,
              None) == lib.KAN_ERR_LIMIT
     assert f(2, 0, None, None, 0, None, 0, None, 0, 0, 2, 16, 16, None, None, 0,
              None) == lib.KAN_OK

@@ -50,6 +50,7 @@
 #include <type_traits>
 
 #include "kan_common.h"
+#include "kan_grouped.h"
 #include "kan_spline.h"
 
 namespace kan {
@@ -1023,18 +1024,16 @@ struct SplitLds {
   static constexpr int kBytes = EPIK == 0 || kStage + kSide < kBase ? kBase : kStage + kSide;
 };
 
+// One tile of a split product (lds: SplitLds<C, AK, BKC, EPIK>::kBytes).
 template <class C, bool AK, bool BKC, int EPIK>
-__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-gemm_split_kernel(GemmParams<float> p, DxParams e) {
+__device__ __forceinline__ void split_tile(const GemmParams<float>& p, const TileCoords& tc,
+                                           const DxParams& e, char* lds) {
   constexpr int BM = C::BM, BN = C::BN, NT = C::kThreads;
   constexpr int FM = C::FM, FN = C::FN;
   typedef SplitLoader<BM, AK, NT> LA;
   typedef SplitLoader<BN, BKC, NT> LB;
   typedef SplitLds<C, AK, BKC, EPIK> Lds;
   static_assert(C::BK == kSplitBK, "one MFMA deep");
-  __shared__ __align__(16) char lds[Lds::kBytes];
-
-  const TileCoords tc = tile_coords<C>(p);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wm = wave / C::WN, wn = wave % C::WN;
 
@@ -1222,6 +1221,53 @@ gemm_split_kernel(GemmParams<float> p, DxParams e) {
     else
       ecomp_epilogue<C, -EPIK>(p, e, tc, acc, back, stage, side, kSide, wave, wm, wn, lane);
   }
+}
+
+template <class C, bool AK, bool BKC, int EPIK>
+__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+gemm_split_kernel(GemmParams<float> p, DxParams e) {
+  __shared__ __align__(16) char lds[SplitLds<C, AK, BKC, EPIK>::kBytes];
+  split_tile<C, AK, BKC, EPIK>(p, tile_coords<C>(p), e, lds);
+}
+
+// The same tiles over rows grouped by expert (kan_grouped.h): a block's tile of
+// its expert's product, as one product of that expert's operands.
+template <class C, int OP>
+__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+grouped_split_kernel(GroupedParams g, int tiles_m, int tiles_n, int buf) {
+  constexpr bool AK = OP != 2, BKC = OP == 0;
+  __shared__ __align__(16) char lds[SplitLds<C, AK, BKC, 0>::kBytes];
+  GemmParams<float> p{};
+  TileCoords tc{};
+  p.A = static_cast<const float*>(g.A);
+  p.B = static_cast<const float*>(g.B);
+  p.lda = OP == 0 ? g.K : g.N;
+  p.ldb = g.K;
+  p.N = p.ldc = OP == 0 ? g.N : g.K;
+  p.buf = buf;
+  const int64_t weights = g.N * g.K;
+  if constexpr (OP == 2) {
+    WeightTile t;
+    if (!weight_tile(g, tiles_m, tiles_n, &t)) return;
+    tc.m0 = (int64_t)t.tm * C::BM;
+    tc.n0 = (int64_t)t.tn * C::BN;
+    tc.kbeg = t.lo;
+    tc.kend = t.hi;
+    p.M = g.N;
+    p.C = t.slot >= 0 ? g.part + t.slot * weights : static_cast<float*>(g.C) + t.e * weights;
+  } else {
+    RowTile t;
+    int tn;
+    if (!row_tile(g, C::BM, tiles_n, &t, &tn)) return;
+    tc.m0 = t.m0;
+    tc.n0 = (int64_t)tn * C::BN;
+    tc.kend = t.e == g.E ? 0 : OP == 0 ? g.K : g.N;
+    p.M = t.m1;
+    p.B += t.e * weights;
+    p.C = static_cast<float*>(g.C);
+  }
+  tc.nkt = (int)ceil_div(tc.kend - tc.kbeg, C::BK);
+  split_tile<C, AK, BKC, 0>(p, tc, DxParams{}, lds);
 }
 
 template <class C, bool AK, bool BKC>
@@ -2149,6 +2195,61 @@ inline unsigned flat_blocks(int64_t count) {
   return (unsigned)(b < 1 ? 1 : b);
 }
 }  // namespace
+
+namespace {
+// The large tile where its tiles fill the chip; the narrow one for up to 64
+// columns.  (Half of a group's last row tile is empty on average.)
+int grouped_cfg_f32(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+  const int64_t cols = op == 0 ? N : K;
+  if (cols <= 64) return 2;
+  const int64_t tiles_m = op == 2 ? ceil_div(N, 256) * E : T / 256 + E / 2;
+  return tiles_m * ceil_div(cols, 256) >= device_cu_count() ? 0 : 1;
+}
+
+template <class C, int OP>
+int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
+  const int64_t cols = OP == 0 ? p.N : p.K, lda = OP == 0 ? p.K : p.N;
+  const int64_t tiles_n = ceil_div(cols, C::BN), tiles_m = ceil_div(p.N, C::BM);
+  const int64_t blocks = OP == 2 ? weight_grid(p, tiles_m * tiles_n) : row_grid(p, C::BM, tiles_n);
+  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  // whole-slab byte offsets in 31 bits, as launch_cfg
+  auto span_ok = [](bool kcont, int rows, int64_t ld) {
+    return ((kcont ? rows * ld + C::BK : C::BK * ld + rows) * 4) < (int64_t)1 << 31;
+  };
+  const int buf = span_ok(OP != 2, C::BM, lda) && span_ok(OP == 0, C::BN, p.K);
+  hipLaunchKernelGGL((grouped_split_kernel<C, OP>), dim3((unsigned)blocks), dim3(C::kThreads), 0,
+                     st, p, (int)tiles_m, (int)tiles_n, buf);
+  return check_launch("grouped_matmul");
+}
+
+template <class C>
+int launch_grouped_op(int op, const GroupedParams& p, hipStream_t st) {
+  if (op == 0) return launch_grouped_cfg<C, 0>(p, st);
+  if (op == 1) return launch_grouped_cfg<C, 1>(p, st);
+  return launch_grouped_cfg<C, 2>(p, st);
+}
+}  // namespace
+
+// (a tile's share of the engine's 220 TFLOP/s, 150 on the narrow tile)
+int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K) {
+  const int cus = device_cu_count();
+  switch (grouped_cfg_f32(2, T, E, N, K)) {
+    case 0:
+      return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 256), {cus, 0.15, 10.0});
+    case 1:
+      return weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.076, 5.0});
+    default:
+      return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 64), {2 * cus, 0.11, 5.0});
+  }
+}
+
+int launch_grouped_f32(int op, const GroupedParams& p, hipStream_t st) {
+  const int cfg = grouped_cfg_f32(op, p.T, p.E, p.N, p.K);
+  const int rc = cfg == 0   ? launch_grouped_op<CfgF32Big>(op, p, st)
+                 : cfg == 1 ? launch_grouped_op<CfgF32Small>(op, p, st)
+                            : launch_grouped_op<CfgF32Narrow>(op, p, st);
+  return rc != KAN_OK || op != 2 ? rc : launch_grouped_sum<float>(p, st);
+}
 
 template <typename T>
 int64_t matmul_ws_elems(int layout, int64_t M, int64_t N, int64_t K, int64_t max_slice_elems) {

@@ -12,208 +12,11 @@
 // group from the offsets, and blocks past the last tile end at once.
 #include <type_traits>
 
-#include "kan_types.h"
+#include "kan_grouped.h"
 
 namespace kan {
 
 namespace {
-
-struct GroupedParams {
-  const void *A, *B;      // op 0: x, w; 1: dy, w; 2: dy, x
-  const float* b_scale;   // op 2 with 8-bit rows: [T, ceil(K / group)]
-  void* C;
-  const void* offsets;
-  int offsets64;
-  int E;
-  int64_t T, N, K;
-  int group, format;      // of 8-bit rows (KAN_ACT8_NONE: B is in the products' type)
-};
-
-// ---- which rows a tile has --------------------------------------------------
-
-template <int CTRL, int ROW_MASK = 0xf>
-__device__ __forceinline__ int dpp_int(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
-}
-// inclusive scans over the wave, of values that are not negative
-__device__ __forceinline__ int scan_add(int v) {
-  v += dpp_int<0x111>(v);
-  v += dpp_int<0x112>(v);
-  v += dpp_int<0x114>(v);
-  v += dpp_int<0x118>(v);
-  v += dpp_int<0x142, 0xa>(v);
-  v += dpp_int<0x143, 0xc>(v);
-  return v;
-}
-__device__ __forceinline__ int scan_max(int v) {
-  v = max(v, dpp_int<0x111>(v));
-  v = max(v, dpp_int<0x112>(v));
-  v = max(v, dpp_int<0x114>(v));
-  v = max(v, dpp_int<0x118>(v));
-  v = max(v, dpp_int<0x142, 0xa>(v));
-  v = max(v, dpp_int<0x143, 0xc>(v));
-  return v;
-}
-
-// End of group e's rows as stored, within 0 .. T; the rows past the last
-// group's are a group E of their own that ends at T.
-__device__ __forceinline__ int group_end(const GroupedParams& p, int e) {
-  if (e >= p.E) return (int)p.T;
-  const int64_t v = p.offsets64 ? static_cast<const int64_t*>(p.offsets)[e + 1]
-                                : (int64_t)static_cast<const int*>(p.offsets)[e + 1];
-  return (int)max((int64_t)0, min(p.T, v));
-}
-
-// Offsets that do not ascend are taken as their running maximum, so that
-// every row belongs to one group whatever the offsets hold.
-struct GroupScan {
-  int begin, end, tiles, last;  // of this lane's group; last: tiles up to and with it
-  int carry_end = 0, carry_tiles = 0;
-  __device__ __forceinline__ void step(const GroupedParams& p, int base, int bm) {
-    const int lane = threadIdx.x & 63, e = base + lane;
-    end = max(carry_end, scan_max(e <= p.E ? group_end(p, e) : 0));
-    begin = __shfl_up(end, 1);
-    if (lane == 0) begin = carry_end;
-    tiles = (end - begin + bm - 1) / bm;
-    last = carry_tiles + scan_add(tiles);
-    carry_end = __builtin_amdgcn_readlane(end, 63);
-    carry_tiles = __builtin_amdgcn_readlane(last, 63);
-  }
-};
-
-// Number of row tiles of all groups.
-__device__ __forceinline__ int count_tiles(const GroupedParams& p, int bm) {
-  GroupScan s;
-  for (int base = 0; base <= p.E; base += 64) s.step(p, base, bm);
-  return s.carry_tiles;
-}
-
-// Group (E: none) and rows [m0, m1) of a row tile.
-struct RowTile {
-  int e, m0, m1;
-};
-__device__ __forceinline__ RowTile find_tile(const GroupedParams& p, int tile, int bm) {
-  GroupScan s;
-  RowTile r{p.E, 0, 0};
-  for (int base = 0; base <= p.E; base += 64) {
-    s.step(p, base, bm);
-    if (tile >= s.carry_tiles) continue;
-    const int l = __builtin_ctzll(__ballot(tile < s.last));
-    r.e = base + l;
-    const int before = __builtin_amdgcn_readlane(s.last - s.tiles, l);
-    r.m0 = __builtin_amdgcn_readlane(s.begin, l) + (tile - before) * bm;
-    r.m1 = min(__builtin_amdgcn_readlane(s.end, l), r.m0 + bm);
-    break;
-  }
-  return r;
-}
-
-// Rows [begin, end) of group e.
-__device__ __forceinline__ void group_rows(const GroupedParams& p, int e, int* begin, int* end) {
-  GroupScan s;
-  for (int base = 0; base <= e; base += 64) {
-    s.step(p, base, 1);
-    if (e < base + 64) {
-      *begin = __builtin_amdgcn_readlane(s.begin, e - base);
-      *end = __builtin_amdgcn_readlane(s.end, e - base);
-    }
-  }
-}
-
-// ---- plain tiles ------------------------------------------------------------
-
-__device__ __forceinline__ float kept_value(const GroupedParams& p, int64_t t, int64_t k) {
-  const uint8_t b = static_cast<const uint8_t*>(p.B)[t * p.K + k];
-  const float s = p.b_scale[t * ((p.K + p.group - 1) / p.group) + k / p.group];
-  const float q = p.format == KAN_ACT8_INT8 ? (float)(int8_t)b
-                                            : __builtin_amdgcn_cvt_f32_fp8((int)b, 0);
-  return q * s;
-}
-
-// 64 x 64 outputs a block, 4 x 4 a thread, 16 deep.
-constexpr int kPlainTile = 64, kPlainDepth = 16;
-template <typename T, int OP>
-__global__ __launch_bounds__(256) void grouped_plain_kernel(GroupedParams p, int tiles_m,
-                                                            int tiles_n) {
-  __shared__ float la[kPlainDepth][kPlainTile + 4], lb[kPlainDepth][kPlainTile + 4];
-  const int tile = blockIdx.x / tiles_n, n0 = (blockIdx.x % tiles_n) * kPlainTile;
-  RowTile rt;
-  int64_t kbeg = 0, kend, m_end, n_end, ldc;
-  const T *A = static_cast<const T*>(p.A), *B = static_cast<const T*>(p.B);
-  T* C = static_cast<T*>(p.C);
-  if constexpr (OP == 2) {
-    rt.e = tile / tiles_m;
-    rt.m0 = (tile % tiles_m) * kPlainTile;
-    int lo = 0, hi = 0;
-    group_rows(p, rt.e, &lo, &hi);
-    kbeg = lo;
-    kend = hi;
-    m_end = p.N;
-    n_end = ldc = p.K;
-    C += (int64_t)rt.e * p.N * p.K;
-  } else {
-    if (tile >= count_tiles(p, kPlainTile)) return;
-    rt = find_tile(p, tile, kPlainTile);
-    kend = rt.e == p.E ? 0 : OP == 0 ? p.K : p.N;
-    m_end = rt.m1;
-    n_end = ldc = OP == 0 ? p.N : p.K;
-    B += (int64_t)rt.e * p.N * p.K;
-  }
-  float acc[4][4] = {};
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int64_t k0 = kbeg; k0 < kend; k0 += kPlainDepth) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kPlainTile * kPlainDepth; i += 256) {
-      const int r = OP == 2 ? i % kPlainTile : i / kPlainDepth;
-      const int d = OP == 2 ? i / kPlainTile : i % kPlainDepth;
-      const int64_t m = rt.m0 + r, k = k0 + d;
-      float v = 0.0f;
-      if (m < m_end && k < kend)
-        v = (float)(OP == 0 ? A[m * p.K + k] : OP == 1 ? A[m * p.N + k] : A[k * p.N + m]);
-      la[d][r] = v;
-    }
-    for (int i = threadIdx.x; i < kPlainTile * kPlainDepth; i += 256) {
-      const int r = OP == 0 ? i / kPlainDepth : i % kPlainTile;
-      const int d = OP == 0 ? i % kPlainDepth : i / kPlainTile;
-      const int64_t n = n0 + r, k = k0 + d;
-      float v = 0.0f;
-      if (n < n_end && k < kend) {
-        if (OP == 2 && p.format != KAN_ACT8_NONE) v = kept_value(p, k, n);
-        else v = (float)(OP == 0 ? B[n * p.K + k] : B[k * p.K + n]);
-      }
-      lb[d][r] = v;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int d = 0; d < kPlainDepth; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_fmaf(la[d][ty * 4 + i], lb[d][tx * 4 + j], acc[i][j]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = rt.m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m < m_end && n < n_end) C[m * ldc + n] = (T)acc[i][j];
-    }
-}
-
-template <typename T>
-int launch_plain(int op, const GroupedParams& p, hipStream_t st) {
-  const int64_t cols = op == 0 ? p.N : p.K;
-  const int64_t tiles_n = ceil_div(cols, kPlainTile);
-  const int64_t tiles_m = op == 2 ? ceil_div(p.N, kPlainTile) : p.T / kPlainTile + p.E + 1;
-  const int64_t blocks = tiles_n * tiles_m * (op == 2 ? p.E : 1);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
-  const dim3 g((unsigned)blocks);
-  if (op == 0) grouped_plain_kernel<T, 0><<<g, 256, 0, st>>>(p, (int)tiles_m, (int)tiles_n);
-  else if (op == 1) grouped_plain_kernel<T, 1><<<g, 256, 0, st>>>(p, (int)tiles_m, (int)tiles_n);
-  else grouped_plain_kernel<T, 2><<<g, 256, 0, st>>>(p, (int)tiles_m, (int)tiles_n);
-  return check_launch("grouped_matmul");
-}
 
 // ---- 16-bit products on MFMA ------------------------------------------------
 // Block tiles of BM x BN outputs, 64 deep, WM x WN waves; v_mfma_f32_32x32x16
@@ -292,10 +95,19 @@ struct Operand {
   uint32_t off[kPer];
   u32x4 reg[kPer];
   // 8-bit rows
-  const float* scale;
-  int64_t parts;
-  int group, col0;
+  const float* scale;               // of row 0
+  int64_t parts;                    // scales of a row
+  uint32_t part[MODE >= kInt8 ? kPer : 1];  // the chunk's, from the slab's first row on
   float step[MODE >= kInt8 ? kPer : 1];
+
+  __device__ __forceinline__ void init_scale(const float* src, int64_t parts_, int group,
+                                             int64_t col0) {
+    scale = src;
+    parts = parts_;
+#pragma unroll
+    for (int p = 0; p < kPer; ++p)
+      part[p] = (uint32_t)(chunk_row(p) * parts) + ((uint32_t)col0 + 8 * chunk_col(p)) / group;
+  }
 
   // Row of the thread's chunk p in the slab's layout, and the chunk of that
   // row which belongs at the thread's position.
@@ -357,7 +169,7 @@ struct Operand {
           for (int j = 0; j < 8; ++j)
             if (j < n) v[j >> 2] |= (uint32_t)(uint8_t)src[off[p] + j] << (8 * (j & 3));
         }
-        step[p] = n > 0 ? scale[(k0 + r) * parts + (col0 + c) / group] : 0.0f;
+        step[p] = n > 0 ? (scale + k0 * parts)[part[p]] : 0.0f;
       } else if (n == 8) {
         if constexpr (MODE == kGuarded) v = reinterpret_cast<const Loose16*>(src + off[p])->v;
         else v = *reinterpret_cast<const u32x4*>(src + off[p]);
@@ -380,24 +192,28 @@ struct Operand {
       *reinterpret_cast<u32x4*>(lds + (p * NT + threadIdx.x) * 16) = v;
     }
   }
-  // 8 values q * scale rounded to T.
+  // 8 values q * scale rounded to T.  (int8: the bytes plus 128 convert in one
+  // operation each; (q + 128) s - 128 s in one rounding is q s.)
   __device__ __forceinline__ static u32x4 restore(u32x4 q, float s) {
     typename Half<T>::frag f;
+    if constexpr (MODE == kInt8) {
+      const float back = -128.0f * s;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t w = q[j >> 2];
-      float u;
-      if constexpr (MODE == kInt8) {
-        u = (float)(int8_t)(w >> (8 * (j & 3)));
-      } else {
-        switch (j & 3) {
-          case 0: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 0); break;
-          case 1: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 1); break;
-          case 2: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 2); break;
-          default: u = __builtin_amdgcn_cvt_f32_fp8((int)w, 3); break;
-        }
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t w = q[j >> 2] ^ 0x80808080u;
+        f[j] = (T)__builtin_fmaf((float)(uint8_t)(w >> (8 * (j & 3))), s, back);
       }
-      f[j] = (T)(u * s);
+    } else {
+      typedef float f32x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[j], false);
+        const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[j], true);
+        f[4 * j] = (T)(lo[0] * s);
+        f[4 * j + 1] = (T)(lo[1] * s);
+        f[4 * j + 2] = (T)(hi[0] * s);
+        f[4 * j + 3] = (T)(hi[1] * s);
+      }
     }
     return __builtin_bit_cast(u32x4, f);
   }
@@ -451,8 +267,6 @@ __device__ __forceinline__ void slab_barrier() {
   asm volatile("" ::: "memory");
 }
 
-constexpr int kGroupedM = 8;  // row tiles that walk the columns together
-
 template <typename T, class G, int OP, int MA, int MB>
 __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, int tiles_m,
                                                              int tiles_n, int store_vec) {
@@ -461,33 +275,24 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
   __shared__ __align__(16) char lds[2 * G::kBuf];
 
   // the tile: rows [m0, m_end) and columns [n0, n_end) of the output, k range
-  int e, tm, tn;
+  int e, tn, slot = -1;
   int64_t m0, m_end, kbeg = 0, kend;
   if constexpr (OP == 2) {
-    const int id = xcd_remap(blockIdx.x, gridDim.x), per = tiles_m * tiles_n;
-    e = __builtin_amdgcn_readfirstlane(id / per);
-    const int t = id - e * per;
-    tm = __builtin_amdgcn_readfirstlane(t / tiles_n);
-    tn = __builtin_amdgcn_readfirstlane(t % tiles_n);
-    int lo = 0, hi = 0;
-    group_rows(p, e, &lo, &hi);
-    kbeg = lo;
-    kend = hi;
-    m0 = (int64_t)tm * BM;
+    WeightTile t;
+    if (!weight_tile(p, tiles_m, tiles_n, &t)) return;
+    e = t.e;
+    tn = t.tn;
+    slot = t.slot;
+    kbeg = t.lo;
+    kend = t.hi;
+    m0 = (int64_t)t.tm * BM;
     m_end = p.N;
   } else {
-    tiles_m = count_tiles(p, BM);
-    const int total = tiles_m * tiles_n;
-    if ((int)blockIdx.x >= total) return;
-    const int id = xcd_remap(blockIdx.x, total), group = kGroupedM * tiles_n;
-    const int first = id / group * kGroupedM, in = id % group;
-    const int gm = min(tiles_m - first, kGroupedM);
-    tm = __builtin_amdgcn_readfirstlane(first + in % gm);
-    tn = __builtin_amdgcn_readfirstlane(in / gm);
-    const RowTile rt = find_tile(p, tm, BM);
-    e = rt.e;
-    m0 = rt.m0;
-    m_end = rt.m1;
+    RowTile t;
+    if (!row_tile(p, BM, tiles_n, &t, &tn)) return;
+    e = t.e;
+    m0 = t.m0;
+    m_end = t.m1;
     kend = e == p.E ? 0 : OP == 0 ? p.K : p.N;
   }
   const int64_t n_end = OP == 0 ? p.N : p.K, n0 = (int64_t)tn * BN;
@@ -497,12 +302,8 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
   Operand<T, BN, KB, MB, G::NT> b;
   a.init(p.A, OP == 0 ? p.K : p.N, m0, m_end - m0);
   b.init(OP == 2 ? p.B : static_cast<const T*>(p.B) + weight, p.K, n0, n_end - n0);
-  if constexpr (MB >= kInt8) {
-    b.scale = p.b_scale;
-    b.group = p.group;
-    b.parts = (p.K + p.group - 1) / p.group;
-    b.col0 = (int)n0;
-  }
+  if constexpr (MB >= kInt8)
+    b.init_scale(p.b_scale, (p.K + p.group - 1) / p.group, p.group, n0);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / G::WN, wn = wave % G::WN, lane = threadIdx.x & 63;
   Fragments<T, BM, FM, KA> fa;
@@ -604,6 +405,20 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     for (; kt < slabs; ++kt) slab(kt, kt + 1 < slabs, kt + 2 < slabs, rest);
   }
 
+  if (OP == 2 && slot >= 0) {  // the sums of an item of several
+    float* part = p.part + (int64_t)slot * p.N * p.K;
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int64_t row = m0 + (wm * FM + i) * 32 + (lane & 31);
+          const int64_t col = n0 + (wn * FN + j) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
+          if (row < m_end && col < n_end) part[row * n_end + col] = acc[i][j][v];
+        }
+    return;
+  }
   // The wave's outputs go through LDS to become whole 16-byte pieces of rows.
   __syncthreads();
   T* out = static_cast<T*>(p.C) + (OP == 2 ? weight : 0);
@@ -650,13 +465,13 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 template <typename T, class G, int OP, int MA, int MB>
 int launch_tile(const GroupedParams& p, hipStream_t st) {
   const int64_t cols = OP == 0 ? p.N : p.K;
-  const int64_t tiles_n = ceil_div(cols, G::BN);
-  const int64_t tiles_m = OP == 2 ? ceil_div(p.N, G::BM) : p.T / G::BM + p.E + 1;
-  const int64_t blocks = tiles_n * tiles_m * (OP == 2 ? p.E : 1);
+  const int64_t tiles_n = ceil_div(cols, G::BN), tiles_m = ceil_div(p.N, G::BM);
+  const int64_t blocks = OP == 2 ? weight_grid(p, tiles_m * tiles_n) : row_grid(p, G::BM, tiles_n);
   if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
   grouped_tile_kernel<T, G, OP, MA, MB><<<dim3((unsigned)blocks), G::NT, 0, st>>>(
       p, (int)tiles_m, (int)tiles_n, cols % 8 == 0 && aligned16(p.C) ? 1 : 0);
-  return check_launch("grouped_matmul");
+  const int rc = check_launch("grouped_matmul");
+  return rc != KAN_OK || OP != 2 ? rc : launch_grouped_sum<T>(p, st);
 }
 
 template <typename T, class G>
@@ -679,12 +494,25 @@ int launch_half_cfg(int op, const GroupedParams& p, hipStream_t st) {
                     : launch_tile<T, G, 2, kGuarded, kGuarded>(p, st);
 }
 
+// The large tile where its tiles (half of a group's last row tile is empty on
+// average) fill the chip.
+bool half_takes_big(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+  const int64_t tiles_m = op == 2 ? ceil_div(N, 256) * E : T / 256 + E / 2;
+  return tiles_m * ceil_div(op == 0 ? N : K, 256) >= device_cu_count();
+}
+// (16384 rows, 8 experts of 4096 x 4096: 64 rows of the large tile in 1.0 us;
+// of the small one, two blocks a CU, in 0.65)
+int half_run(int64_t T, int64_t E, int64_t N, int64_t K) {
+  const int cus = device_cu_count();
+  if (half_takes_big(2, T, E, N, K))
+    return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 256), {cus, 0.016, 5.0});
+  return weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.010, 4.0});
+}
+
 template <typename T>
 int launch_half(int op, const GroupedParams& p, hipStream_t st) {
-  const int64_t rows = op == 2 ? p.N : p.T / std::max(p.E, 1), cols = op == 0 ? p.N : p.K;
-  const int64_t big = ceil_div(rows, 256) * ceil_div(cols, 256) * std::max(p.E, 1);
-  return big >= device_cu_count() ? launch_half_cfg<T, TileBig>(op, p, st)
-                                  : launch_half_cfg<T, TileSmall>(op, p, st);
+  return half_takes_big(op, p.T, p.E, p.N, p.K) ? launch_half_cfg<T, TileBig>(op, p, st)
+                                                : launch_half_cfg<T, TileSmall>(op, p, st);
 }
 
 int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K) {
@@ -696,10 +524,23 @@ int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K)
   if (T < 0 || E < 0 || N < 0 || K < 0)
     return set_error(KAN_ERR_INVALID, "grouped_matmul: negative size");
   // (tile ends are held in 32 bits, as are the bytes from a tile's first row)
-  if (T > 0x7fffffff - 4096 || N > (1 << 22) || K > (1 << 22) || E > (1 << 20))
+  if (T > 0x3fffffff || N > (1 << 22) || K > (1 << 22) || E > 65535)
     return set_error(KAN_ERR_LIMIT,
-                     "grouped_matmul: at most 2^31 - 4097 rows, 2^22 columns and 2^20 experts");
+                     "grouped_matmul: at most 2^30 - 1 rows, 2^22 columns and 65535 experts");
   return KAN_OK;
+}
+
+// Workspace of the weight gradient: the items' partial sums and, in fp32, the
+// 8-bit rows as floats (the engine takes fp32 operands).
+int run_of(int dtype, int64_t T, int64_t E, int64_t N, int64_t K) {
+  return dtype == KAN_DTYPE_F32 ? grouped_f32_run(T, E, N, K) : half_run(T, E, N, K);
+}
+size_t workspace_bytes_of(int dtype, int op, int format, int64_t T, int64_t E, int64_t N,
+                          int64_t K) {
+  if (op != KAN_GROUPED_WEIGHT || T * E * N * K == 0) return 0;
+  int64_t elems = weight_part_elems(T, E, N, K, run_of(dtype, T, E, N, K));
+  if (dtype == KAN_DTYPE_F32 && format != KAN_ACT8_NONE) elems += T * K;
+  return 4 * (size_t)elems;
 }
 
 }  // namespace
@@ -709,13 +550,13 @@ using namespace kan;
 
 extern "C" {
 
-int kan_hip_grouped_matmul_workspace(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K,
+int kan_hip_grouped_matmul_workspace(int dtype, int op, int b_format, int64_t T, int64_t E, int64_t N, int64_t K,
                                      size_t* bytes) {
   if (bytes == nullptr)
     return set_error(KAN_ERR_INVALID, "grouped_matmul_workspace: bytes must not be NULL");
   const int rc = check_grouped(dtype, op, T, E, N, K);
   if (rc != KAN_OK) return rc;
-  *bytes = 0;
+  *bytes = workspace_bytes_of(dtype, op, b_format, T, E, N, K);
   return KAN_OK;
 }
 
@@ -742,8 +583,10 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   const bool some = op == KAN_GROUPED_WEIGHT ? T > 0 : E * N * K > 0;  // any term to add up
   if (out == nullptr || (some && (a == nullptr || b == nullptr)) || (E > 0 && offsets == nullptr))
     return set_error(KAN_ERR_INVALID, "grouped_matmul: operands must not be NULL");
-  (void)workspace;
-  (void)workspace_bytes;
+  const size_t need = workspace_bytes_of(dtype, op, b_format, T, E, N, K);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return set_error(KAN_ERR_WORKSPACE, "grouped_matmul: needs %zu bytes of workspace, got %zu",
+                     need, workspace == nullptr ? (size_t)0 : workspace_bytes);
   GroupedParams p{};
   p.A = a;
   p.B = b;
@@ -759,7 +602,22 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   p.format = b_format;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * N * K);
-  if (dtype == KAN_DTYPE_F32) return launch_plain<float>(op, p, st);
+  p.run = kNoRuns;
+  int64_t part = 0;
+  if (op == KAN_GROUPED_WEIGHT && T > 0) {
+    p.run = run_of(dtype, T, E, N, K);
+    part = weight_part_elems(T, E, N, K, p.run);
+    if (part > 0) p.part = static_cast<float*>(workspace);
+  }
+  if (dtype == KAN_DTYPE_F32) {
+    if (b_format != KAN_ACT8_NONE && T > 0) {
+      float* rows = static_cast<float*>(workspace) + part;
+      const int e = kan_hip_act8_dequantize(dtype, b_format, b, b_scale, T, K, b_group, rows, stream);
+      if (e != KAN_OK) return e;
+      p.B = rows;
+    }
+    return launch_grouped_f32(op, p, st);
+  }
   if (dtype == KAN_DTYPE_BF16) return launch_half<bf16>(op, p, st);
   return launch_half<f16>(op, p, st);
 }

@@ -40,7 +40,7 @@ def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
     ptr = lib.ptr
     nbytes = ctypes.c_size_t()
     with torch.cuda.device(out.device):
-        lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(code, op, T, E, N, K,
+        lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(code, op, form, T, E, N, K,
                                                            ctypes.byref(nbytes)))
         ws = torch.empty(nbytes.value, dtype=torch.uint8, device=out.device) \
             if nbytes.value else None

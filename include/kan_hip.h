@@ -440,7 +440,7 @@ int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const voi
 
 /* Activations kept in 8 bits: rows of C values cut into groups of `group` (32,
  * 64, 128 or 256; the last of a row may be short), scale [rows,
- * ceil(C / group)] = max|x| / qmax (127 for int8, 448 for e4m3) and q [rows, C]
+ * ceil(C / group)] = max|x| * (1 / qmax) (127 for int8, 448 for e4m3) and q [rows, C]
  * = round(x * (1 / scale)).  A scale below the smallest normal float is kept as
  * 0 (the group comes back as zeros); a group with an infinity or NaN gets
  * scale NaN and comes back as NaN.  row_stride: elements between x's rows. */

@@ -190,6 +190,24 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(fn, device: torch.device, *args) -> None:
+    """fn(*args, stream) on `device` and its current stream, with the status
+    checked.  (Short calls are bound by their host time: the stream's handle is
+    taken without building a Stream object, and the device is switched only
+    where it is another one.)"""
+    if device.index == torch.cuda.current_device():
+        stream = stream_of(device) if _raw_stream is None else _raw_stream(device.index)
+        status = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, stream_of(device))
+    if status != KAN_OK:
+        check(status)
+
+
 # routing switches of kan_hip_set_route (KAN_ROUTE_* in include/kan_hip.h) and
 # the values each takes
 ROUTES = {"fused_dx": 0, "compact_e": 1, "edge_fused": 2, "gemm_tile": 3}

@@ -65,11 +65,10 @@ class Activation8:
         lib = _native("dequantize_activation")
         out = torch.empty(self.q.shape, dtype=dtype, device=self.q.device)
         C = out.shape[-1]
-        with torch.cuda.device(out.device):
-            lib.check(lib.LIB.kan_hip_act8_dequantize(
-                lib.operator_dtype_code(dtype, "dequantize_activation"), FORMATS[self.format][0],
-                lib.ptr(self.q), lib.ptr(self.scale), out.numel() // C, C, self.group,
-                lib.ptr(out), lib.stream_of(out.device)))
+        lib.launch(lib.LIB.kan_hip_act8_dequantize, out.device,
+                   lib.operator_dtype_code(dtype, "dequantize_activation"),
+                   FORMATS[self.format][0], self.q.data_ptr(), self.scale.data_ptr(),
+                   out.numel() // C, C, self.group, out.data_ptr())
         return out
 
 
@@ -80,7 +79,7 @@ def _quantize_cpu(x, group, format):
     v = torch.nn.functional.pad(x.float(), (0, parts * group - C)).reshape(*x.shape[:-1], parts,
                                                                            group)
     finite = v.isfinite().all(-1, keepdim=True)
-    scale = v.abs().amax(-1, keepdim=True) / qmax
+    scale = v.abs().amax(-1, keepdim=True) * (1 / qmax)
     scale = torch.where(scale < torch.finfo(torch.float32).tiny, 0.0, scale)
     u = torch.where((scale > 0) & finite, v * (1 / scale), torch.zeros(()))
     u = u.round() if format == "int8" else u
@@ -94,32 +93,31 @@ def _dequantize_cpu(a, dtype):
     return (a.q.float() * scale).to(dtype)
 
 
-@torch.no_grad()
 def quantize_activation(x: torch.Tensor, group: int = 128, format: str = "int8") -> Activation8:
     """x [..., C] in 8 bits: for every group of `group` (32, 64, 128 or 256)
-    consecutive values of the last axis, scale = max|x| / qmax (127 for "int8",
-    448 for "e4m3") and q = round(x * (1 / scale)) to nearest, ties to even."""
+    consecutive values of the last axis, scale = max|x| * (1 / qmax) (127 for
+    "int8", 448 for "e4m3") and q = round(x * (1 / scale)) to nearest, ties to even."""
     who = "quantize_activation"
     check_format(who, group, format)
     _req(x.dim() >= 1, who, ": x must have at least one dimension")
     _req(x.dtype in (torch.float32, torch.bfloat16, torch.float16), who,
          ": only FP32, BF16 and FP16 tensors are supported, got ", x.dtype)
     if not x.is_cuda or x.numel() == 0:
-        q, scale = _quantize_cpu(x, group, format)
+        q, scale = _quantize_cpu(x.detach(), group, format)
         return Activation8(q, scale, group, format, x.dtype)
     lib = _native(who)
     C = x.shape[-1]
-    rows = x.numel() // C
-    if not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C):
-        x = x.contiguous()
-    ldx = x.stride(0) if x.dim() == 2 else C
+    rows, ldx = x.numel() // C, C
+    if not x.is_contiguous():
+        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C:
+            ldx = x.stride(0)
+        else:
+            x = x.contiguous()
     code, _, qdtype = FORMATS[format]
     q = torch.empty(x.shape, dtype=qdtype, device=x.device)
-    scale = torch.empty(*x.shape[:-1], -(-C // group), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        lib.check(lib.LIB.kan_hip_act8_quantize(
-            lib.OPERATOR_DTYPES[x.dtype], code, lib.ptr(x), ldx, rows, C, group, lib.ptr(q),
-            lib.ptr(scale), lib.stream_of(x.device)))
+    scale = torch.empty(x.shape[:-1] + (-(-C // group),), dtype=torch.float32, device=x.device)
+    lib.launch(lib.LIB.kan_hip_act8_quantize, x.device, lib.OPERATOR_DTYPES[x.dtype], code,
+               x.data_ptr(), ldx, rows, C, group, q.data_ptr(), scale.data_ptr())
     return Activation8(q, scale, group, format, x.dtype)
 
 

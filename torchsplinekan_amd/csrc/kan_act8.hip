@@ -2,7 +2,7 @@
 // Every row is cut into groups of G = 32, 64, 128 or 256 values along its
 // last axis (the last group of a row may be short).  With m = max |x| of the
 // group:
-//   scale = m / qmax  (qmax 127 for int8, 448 for e4m3), float32
+//   scale = m * (1 / qmax)  (qmax 127 for int8, 448 for e4m3), float32
 //   q     = round(x * (1 / scale))  to nearest, ties to even
 //   x     ~ q * scale
 // A group whose scale would lie below the smallest normal float32 (m below
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kActThreads) void quantize_kernel(Act8Params p) {
   for (int j = 0; j < kActVals; ++j) m = max(m, __float_as_int(v[j]) & 0x7fffffff);
   for (int d = p.group / kActVals / 2; d > 0; d >>= 1) m = max(m, __shfl_xor(m, d));
   if (!in) return;
-  float scale = __int_as_float(m) / F::kMax, inv = 0.0f;
+  float scale = __int_as_float(m) * (1.0f / F::kMax), inv = 0.0f;
   if (m >= 0x7f800000) scale = __int_as_float(0x7fc00000);
   else if (scale < 1.17549435e-38f) scale = 0.0f;
   else inv = 1.0f / scale;

@@ -86,6 +86,7 @@ struct Operand {
   static constexpr int kPer = ROWS * (kDepth / 8) / NT;  // chunks of a thread
   static constexpr int kRowChunks = KCONT ? kDepth / 8 : ROWS / 8;
   static constexpr int kValue = MODE >= kInt8 ? 1 : 2;   // bytes of a value in memory
+  static constexpr int kMode = MODE;
   static_assert(ROWS * (kDepth / 8) % NT == 0, "whole rounds of chunks");
   static_assert(MODE < kInt8 || !KCONT, "8-bit rows are the weight product's");
 
@@ -149,15 +150,20 @@ struct Operand {
                    "v"(off[p]), "s"(src));
   }
 
-  // A slab into registers; k from kend on is zero.
+  // A slab into registers.  GUARD: k from kend on is zero, and chunks that lie
+  // partly outside the operand go value by value; otherwise every chunk of the
+  // slab exists.
+  template <bool GUARD>
   __device__ __forceinline__ void load(int64_t k0, int64_t kend) {
     const char* src = slab(k0);
 #pragma unroll
     for (int p = 0; p < kPer; ++p) {
-      const int r = chunk_row(p), c = 8 * chunk_col(p);
-      // how many of the chunk's values exist: k for KCONT, columns otherwise
-      const int64_t left = KCONT ? kend - k0 - c : (int64_t)(rows - c);
-      const int n = (!KCONT && k0 + r >= kend) || left <= 0 ? 0 : (int)min(left, (int64_t)8);
+      int n = 8;  // how many of the chunk's values exist: k for KCONT, columns otherwise
+      if constexpr (GUARD) {
+        const int r = chunk_row(p), c = 8 * chunk_col(p);
+        const int64_t left = KCONT ? kend - k0 - c : (int64_t)(rows - c);
+        n = (!KCONT && k0 + r >= kend) || left <= 0 ? 0 : (int)min(left, (int64_t)8);
+      }
       u32x4 v = {0, 0, 0, 0};
       if constexpr (MODE >= kInt8) {
         if (n == 8) {
@@ -182,6 +188,10 @@ struct Operand {
       }
       reg[p] = v;
     }
+  }
+  // Whether a slab whose k all exist needs no guard.
+  __device__ __forceinline__ bool interior() const {
+    return MODE == kDirect || KCONT || rows == ROWS;
   }
 
   __device__ __forceinline__ void store(char* lds) const {
@@ -340,29 +350,29 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
   };
 
   const int slabs = (int)((kend - kbeg + kDepth - 1) / kDepth);
-  const int whole = MA == kDirect || MB == kDirect ? (int)((kend - kbeg) / kDepth) : slabs;
-  // start: sends slab kt on its way into buf; a last slab (rest) of an operand
-  // that goes straight to LDS is there when it returns.  finish: stores what
-  // passes registers.
-  auto start = [&](int kt, char* buf, auto rest) __attribute__((always_inline)) {
+  // slabs whose chunks all exist
+  const int whole = a.interior() && b.interior() ? (int)((kend - kbeg) / kDepth) : 0;
+  // start: sends slab kt on its way into buf; one of the others (rest) of an
+  // operand that goes straight to LDS is there when it returns.  finish: stores
+  // what passes registers.
+  auto start_one = [&](auto& x, int64_t k0, char* buf, auto rest) __attribute__((always_inline)) {
+    typedef typename std::remove_reference<decltype(x)>::type X;
     constexpr bool kRest = decltype(rest)::value;
+    if constexpr (X::kMode != kDirect) {
+      x.template load<kRest>(k0, kend);
+    } else if constexpr (!kRest) {
+      x.issue(k0, buf);
+    } else if (k0 + kDepth <= kend) {
+      x.issue(k0, buf);
+    } else {
+      x.template load<true>(k0, kend);
+      x.store(buf);
+    }
+  };
+  auto start = [&](int kt, char* buf, auto rest) __attribute__((always_inline)) {
     const int64_t k0 = kbeg + (int64_t)kt * kDepth;
-    if constexpr (MA != kDirect) {
-      a.load(k0, kend);
-    } else if constexpr (kRest) {
-      a.load(k0, kend);
-      a.store(buf);
-    } else {
-      a.issue(k0, buf);
-    }
-    if constexpr (MB != kDirect) {
-      b.load(k0, kend);
-    } else if constexpr (kRest) {
-      b.load(k0, kend);
-      b.store(buf + kB);
-    } else {
-      b.issue(k0, buf + kB);
-    }
+    start_one(a, k0, buf, rest);
+    start_one(b, k0, buf + kB, rest);
   };
   auto finish = [&](char* buf) __attribute__((always_inline)) {
     if constexpr (MA != kDirect) a.store(buf);

@@ -35,19 +35,20 @@ def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
     if out.numel() == 0:
         return out
     code = lib.OPERATOR_DTYPES[out.dtype]
-    kept = isinstance(b, Activation8)
-    form, scale, group = (FORMATS[b.format][0], b.scale, b.group) if kept else (0, None, 0)
-    ptr = lib.ptr
-    nbytes = ctypes.c_size_t()
-    with torch.cuda.device(out.device):
+    form, scale, group, ws, size = 0, None, 0, None, 0
+    if op == WEIGHT:  # (the other products take no workspace)
+        if isinstance(b, Activation8):
+            form, scale, group, b = FORMATS[b.format][0], b.scale, b.group, b.q
+        nbytes = ctypes.c_size_t()
         lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(code, op, form, T, E, N, K,
                                                            ctypes.byref(nbytes)))
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=out.device) \
-            if nbytes.value else None
-        lib.check(lib.LIB.kan_hip_grouped_matmul(
-            code, op, ptr(a), ptr(b.q if kept else b), form, ptr(scale), group, ptr(offsets),
-            int(offsets.dtype == torch.int64), T, E, N, K, ptr(out), ptr(ws), nbytes.value,
-            lib.stream_of(out.device)))
+        size = nbytes.value
+        if size:
+            ws = torch.empty(size, dtype=torch.uint8, device=out.device)
+    ptr = lib.ptr
+    lib.launch(lib.LIB.kan_hip_grouped_matmul, out.device, code, op, ptr(a), ptr(b), form,
+               ptr(scale), group, ptr(offsets), int(offsets.dtype == torch.int64), T, E, N, K,
+               out.data_ptr(), ptr(ws), size)
     return out
 
 

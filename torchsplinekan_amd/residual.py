@@ -46,23 +46,21 @@ def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, post, pre, scale, gate_rows, scale_const, act, eps, dtype, save):
+    def forward(ctx, x, y, gate, post, pre, scale, gate_rows, scale_const, act, eps, dtype, wdtype,
+                save):
         lib = _native()
         C = x.shape[-1]
         n = x.numel() // C
         new = None if y is None else torch.empty_like(x)
         h = None if pre is None else torch.empty(x.shape, dtype=dtype, device=x.device)
         rstd = torch.empty(2, n, dtype=torch.float32, device=x.device) if save else None
-        weight = next((t for t in (pre, post, scale) if t is not None), None)
-        codes = (lib.OPERATOR_DTYPES[x.dtype], lib.OPERATOR_DTYPES[dtype],
-                 lib.OPERATOR_DTYPES[torch.float32 if weight is None else weight.dtype])
+        code = lib.OPERATOR_DTYPES
+        codes = (code[x.dtype], code[dtype], code.get(wdtype, lib.KAN_DTYPE_F32))
         gate_cols = 0 if gate is None else gate.shape[-1]
-        ptr = lib.ptr
-        with torch.cuda.device(x.device):
-            lib.check(lib.LIB.kan_hip_residual_norm(
-                *codes, ptr(x), ptr(y), ptr(gate), ptr(post), ptr(pre), ptr(scale), scale_const,
-                act, gate_rows, gate_cols, n, C, eps, ptr(new), ptr(h), ptr(rstd),
-                lib.stream_of(x.device)))
+        at = [None if t is None else t.data_ptr()
+              for t in (x, y, gate, post, pre, scale, new, h, rstd)]
+        lib.launch(lib.LIB.kan_hip_residual_norm, x.device, *codes, *at[:6], scale_const, act,
+                   gate_rows, gate_cols, n, C, eps, *at[6:])
         if save:
             ctx.save_for_backward(x, y, gate, post, pre, scale, rstd)
             ctx.args = (codes, gate_rows, gate_cols, scale_const, act, n, C)
@@ -83,17 +81,15 @@ class _ResidualNorm(torch.autograd.Function):
             grads[4].zero_()
         gpre = None if gh is None else grads[4]
         nbytes = ctypes.c_size_t()
-        ptr = lib.ptr
-        with torch.cuda.device(x.device):
-            lib.check(lib.LIB.kan_hip_residual_norm_backward_workspace(
-                gate_rows, gate_cols, n, C, ctypes.byref(nbytes)))
-            ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
-            lib.check(lib.LIB.kan_hip_residual_norm_backward(
-                *codes, ptr(gnew), ptr(gh), ptr(x), ptr(y), ptr(gate), ptr(post), ptr(pre),
-                ptr(scale), scale_const, act, gate_rows, gate_cols, n, C, ptr(rstd), ptr(grads[0]),
-                ptr(grads[1]), ptr(grads[2]), ptr(grads[3]), ptr(gpre), ptr(grads[5]), ptr(ws),
-                nbytes.value, lib.stream_of(x.device)))
-        return (*grads, None, None, None, None, None, None)
+        lib.check(lib.LIB.kan_hip_residual_norm_backward_workspace(
+            gate_rows, gate_cols, n, C, ctypes.byref(nbytes)))
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+        at = [None if t is None else t.data_ptr()
+              for t in (gnew, gh, x, y, gate, post, pre, scale, rstd, *grads[:4], gpre, grads[5],
+                        ws)]
+        lib.launch(lib.LIB.kan_hip_residual_norm_backward, x.device, *codes, *at[:8], scale_const,
+                   act, gate_rows, gate_cols, n, C, *at[8:], nbytes.value)
+        return (*grads, None, None, None, None, None, None, None)
 
 
 def _composite(x, y, gate, post, pre, scale, scale_const, act, eps, dtype):
@@ -138,60 +134,68 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *,
     gradients reach every tensor; x' is not kept for them (the backward
     evaluates it again from x and y)."""
     _req(x.dim() >= 1, "x must have at least one dimension")
-    C = x.shape[-1]
+    shape, C, device = x.shape, x.shape[-1], x.device
     _req(gate_act in GATE_ACTS, "gate_act must be None, 'sigmoid', 'tanh' or 'silu', got ",
          repr(gate_act))
     if y is None:
         _req(post_weight is None and gate is None and scale is None,
              "post_weight, gate and scale need a branch y")
         dtype = x.dtype if dtype is None else dtype
+        if pre_weight is None:
+            return x, None
     else:
-        _req(y.shape == x.shape, "y must have x's shape ", list(x.shape), ", got ", list(y.shape))
+        _req(y.shape == shape, "y must have x's shape ", list(shape), ", got ", list(y.shape))
         _req(dtype is None or dtype == y.dtype, "with y, h is in y's type ", y.dtype)
         dtype = y.dtype
+        _req(y.device == device, "tensors must be on one device")
     _req(gate is not None or gate_act is None, "gate_act needs a gate")
     _req(x.dtype == dtype or x.dtype == torch.float32,
          "x must be in the branch's type or float32, got ", x.dtype, " and ", dtype)
-    scale_t = scale if isinstance(scale, torch.Tensor) else None
-    scale_const = 1.0 if scale is None or scale_t is not None else float(scale)
-    weights = [(n, t) for n, t in (("post_weight", post_weight), ("pre_weight", pre_weight),
-                                   ("scale", scale_t)) if t is not None]
-    for name, t in weights:
-        _req(tuple(t.shape) == (C,), name, " must have shape [", C, "], got ", list(t.shape))
-        _req(t.dtype == weights[0][1].dtype, "post_weight, pre_weight and scale must share a dtype")
+    scale_t, scale_const = None, 1.0
+    if isinstance(scale, torch.Tensor):
+        scale_t = scale
+    elif scale is not None:
+        scale_const = float(scale)
+    wdtype = None
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("scale", scale_t)):
+        if t is None:
+            continue
+        _req(t.dim() == 1 and t.shape[0] == C, name, " must have shape [", C, "], got ",
+             list(t.shape))
+        _req(wdtype is None or t.dtype == wdtype,
+             "post_weight, pre_weight and scale must share a dtype")
+        _req(t.device == device, "tensors must be on one device")
+        wdtype = t.dtype
     gate_rows = 0
     if gate is not None:
         _req(gate.dtype == dtype, "gate must be in the branch's type ", dtype, ", got ", gate.dtype)
         _req(1 <= gate.dim() <= x.dim() and gate.shape[-1] in (1, C)
-             and all(g in (1, s) for g, s in zip(gate.shape[-2::-1], x.shape[-2::-1])),
-             "gate of shape ", list(gate.shape), " does not broadcast against ", list(x.shape))
-    for t in (y, gate, *(t for _, t in weights)):
-        _req(t is None or t.device == x.device, "tensors must be on one device")
-    if y is None and pre_weight is None:
-        return x, None
+             and all(g in (1, s) for g, s in zip(gate.shape[-2::-1], shape[-2::-1])),
+             "gate of shape ", list(gate.shape), " does not broadcast against ", list(shape))
+        _req(gate.device == device, "tensors must be on one device")
     if not x.is_cuda or x.numel() == 0:
         return _composite(x, y, gate, post_weight, pre_weight, scale_t, scale_const, gate_act, eps,
                           dtype)
     lib = _native()
-    for t in (x, y, gate, *(t for _, t in weights)):
-        if t is not None:
-            lib.operator_dtype_code(t.dtype, "residual_norm")
-    lib.operator_dtype_code(dtype, "residual_norm")
+    for t in (x.dtype, dtype, wdtype):
+        if t is not None and t not in lib.OPERATOR_DTYPES:
+            lib.operator_dtype_code(t, "residual_norm")  # (raises)
     if gate is not None:
-        gate = gate.reshape((1,) * (x.dim() - gate.dim()) + tuple(gate.shape))
+        if gate.dim() < x.dim():
+            gate = gate.reshape((1,) * (x.dim() - gate.dim()) + tuple(gate.shape))
         gate_rows = _gate_rows(gate, x)
         if gate_rows == 0:
             # broadcast over leading dimensions: one gate row for every row of
             # x, in float32, so that its gradient is rounded once, after the sum
             new, h = residual_norm(
                 x.float(), y.float(), post_weight=post_weight, pre_weight=pre_weight,
-                gate=gate.float().expand(*x.shape[:-1], gate.shape[-1]), gate_act=gate_act,
+                gate=gate.float().expand(*shape[:-1], gate.shape[-1]), gate_act=gate_act,
                 scale=scale, eps=eps)
             return new.to(x.dtype), None if h is None else h.to(dtype)
-    tensors = [None if t is None else t.contiguous()
+    tensors = [t if t is None or t.is_contiguous() else t.contiguous()
                for t in (x, y, gate, post_weight, pre_weight, scale_t)]
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-    args = (gate_rows, scale_const, GATE_ACTS[gate_act], float(eps), dtype, save)
+    args = (gate_rows, scale_const, GATE_ACTS[gate_act], float(eps), dtype, wdtype, save)
     if save:
         new, h = _ResidualNorm.apply(*tensors, *args)
     else:

@@ -463,12 +463,13 @@ int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* s
  *                        dy[t] x[t]^T over the expert's rows (zeros without any)
  * Rows from offsets[E] on get zeros.  T < 2^30, N and K <= 2^22, E <= 65535.  The weight product also takes b as 8-bit
  * rows (b_format, with b_scale and b_group as kan_hip_act8_quantize keeps
- * them; KAN_ACT8_NONE otherwise). */
+ * them; KAN_ACT8_NONE otherwise).  The workspace depends on the operands'
+ * alignment, so its query takes their addresses (which it does not read). */
 #define KAN_GROUPED_FORWARD 0
 #define KAN_GROUPED_INPUT 1
 #define KAN_GROUPED_WEIGHT 2
-int kan_hip_grouped_matmul_workspace(int dtype, int op, int b_format, int64_t T, int64_t E,
-                                     int64_t N, int64_t K, size_t* bytes);
+int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const void* b, int b_format,
+                                     int64_t T, int64_t E, int64_t N, int64_t K, size_t* bytes);
 int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,

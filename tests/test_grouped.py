@@ -172,6 +172,44 @@ def test_larger(T, E, K, N, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,E,K,N", [(40, 5, 4096, 72), (40, 5, 72, 4096), (300, 2, 2051, 130),
+                                     (1, 1, 8000, 8), (130, 3, 9, 3001)])
+def test_few_tiles_with_long_sums(T, E, K, N, dtype):
+    """Outputs of few tiles: their sums are cut into several."""
+    x, w, dy = _inputs(T, E, K, N, dtype)
+    _check(x, w, dy, _offsets(_counts(T, E, seed=2)))
+    off = [0] + [T // 2] * E                      # rows past the last group
+    _check(x, w, dy, torch.tensor(off, dtype=torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,E,K,N", [(12000, 2, 2047, 1027), (9000, 3, 1536, 2045),
+                                     (20001, 2, 1283, 1024)])
+def test_large_products_of_rows_off_16_bytes(T, E, K, N, dtype):
+    """Products that are long enough to bring their rows onto 16 bytes first."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(T, K, generator=g, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn(E, N, K, generator=g, device="cuda") * K ** -0.5).to(dtype).requires_grad_()
+    dy = torch.randn(T, N, generator=g, device="cuda").to(dtype)
+    counts = _counts(T, E, seed=3)
+    off = _offsets(counts).cuda()
+    y = grouped_linear(x, w, off)
+    dx, dw = torch.autograd.grad(y, [x, w], dy)
+    lo = 0
+    for e, c in enumerate(counts):
+        r = slice(lo, lo + c)
+        X, W, D = x[r].detach().double(), w[e].detach().double(), dy[r].double()
+        for got, a, b, terms in ((y[r], X, W.t(), K), (dx[r], D, W, N), (dw[e], D.t(), X, c)):
+            want, mag = torch.mm(a, b), torch.mm(a.abs(), b.abs())
+            tol = (terms + 16) * 2.0 ** -24 * mag * (1 + HALF_ULP[dtype])
+            tol = tol + HALF_ULP[dtype] * want.abs() + 2.0 ** -25
+            assert bool(((got.double() - want).abs() <= tol).all())
+        lo += c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("format", ["int8", "e4m3"])
 @pytest.mark.parametrize("K,N,group", [(1, 3, 32), (100, 60, 64), (136, 128, 32), (301, 257, 128),
                                        (512, 320, 256), (129, 72, 128)])

@@ -105,7 +105,8 @@ SIGNATURES = {
                                        + [_vp] * 8 + [_sz, _vp]),
     "kan_hip_act8_quantize": (_int, [_int, _int, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
     "kan_hip_act8_dequantize": (_int, [_int, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
-    "kan_hip_grouped_matmul_workspace": (_int, [_int] * 3 + [_i64] * 4 + [ctypes.POINTER(_sz)]),
+    "kan_hip_grouped_matmul_workspace": (_int, [_int, _int, _vp, _vp, _int] + [_i64] * 4
+                                         + [ctypes.POINTER(_sz)]),
     "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
                                + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
     "kan_hip_timing_enable": (_int, [_int]),

@@ -1262,9 +1262,14 @@ grouped_split_kernel(GroupedParams g, int tiles_m, int tiles_n, int buf) {
     tc.m0 = t.m0;
     tc.n0 = (int64_t)tn * C::BN;
     tc.kend = t.e == g.E ? 0 : OP == 0 ? g.K : g.N;
+    cut_range(g, &tc.kbeg, &tc.kend);
     p.M = t.m1;
     p.B += t.e * weights;
-    p.C = static_cast<float*>(g.C);
+    p.C = g.cuts > 1 ? g.part : static_cast<float*>(g.C);
+    if (g.cuts > 1) {
+      tc.split = blockIdx.y;
+      p.split_stride = g.T * p.N;
+    }
   }
   tc.nkt = (int)ceil_div(tc.kend - tc.kbeg, C::BK);
   split_tile<C, AK, BKC, 0>(p, tc, DxParams{}, lds);
@@ -2217,8 +2222,8 @@ int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
     return ((kcont ? rows * ld + C::BK : C::BK * ld + rows) * 4) < (int64_t)1 << 31;
   };
   const int buf = span_ok(OP != 2, C::BM, lda) && span_ok(OP == 0, C::BN, p.K);
-  hipLaunchKernelGGL((grouped_split_kernel<C, OP>), dim3((unsigned)blocks), dim3(C::kThreads), 0,
-                     st, p, (int)tiles_m, (int)tiles_n, buf);
+  hipLaunchKernelGGL((grouped_split_kernel<C, OP>), dim3((unsigned)blocks, OP == 2 ? 1 : p.cuts),
+                     dim3(C::kThreads), 0, st, p, (int)tiles_m, (int)tiles_n, buf);
   return check_launch("grouped_matmul");
 }
 
@@ -2243,12 +2248,23 @@ int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K) {
   }
 }
 
+// (16 k of a 128 x 128 or 256 x 64 tile alone take about 0.9 us)
+int grouped_f32_cuts(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+  const int cfg = grouped_cfg_f32(op, T, E, N, K);
+  if (cfg == 0) return 1;
+  const int64_t cols = op == 0 ? N : K, depth = op == 0 ? K : N;
+  const double tiles = row_tiles(T, E, cfg == 1 ? 128 : 256) * (double)ceil_div(cols, cfg == 1 ? 128 : 64);
+  return sum_cuts(tiles, 2 * device_cu_count(), ceil_div(depth, 64), 3.6);
+}
+
 int launch_grouped_f32(int op, const GroupedParams& p, hipStream_t st) {
   const int cfg = grouped_cfg_f32(op, p.T, p.E, p.N, p.K);
   const int rc = cfg == 0   ? launch_grouped_op<CfgF32Big>(op, p, st)
                  : cfg == 1 ? launch_grouped_op<CfgF32Small>(op, p, st)
                             : launch_grouped_op<CfgF32Narrow>(op, p, st);
-  return rc != KAN_OK || op != 2 ? rc : launch_grouped_sum<float>(p, st);
+  if (rc != KAN_OK) return rc;
+  return op == 2 ? launch_grouped_sum<float>(p, st)
+                 : launch_grouped_cuts<float>(p, op == 0 ? p.N : p.K, st);
 }
 
 template <typename T>

@@ -2,6 +2,8 @@
 // block finds the rows its tile has from offsets that lie on the device.
 #pragma once
 
+#include <cmath>
+
 #include "kan_types.h"
 
 namespace kan {
@@ -14,9 +16,12 @@ struct GroupedParams {
   int offsets64;
   int E;
   int64_t T, N, K;
+  int64_t lda, ldb;       // values between rows of A and B
   int group, format;      // of 8-bit rows (KAN_ACT8_NONE: B is in the products' type)
   int run;                // op 2: rows of an item of work; the sums of a group of
   float* part;            // several items go to part [T / run + E, N, K]
+  int cuts;               // op 0, 1: the sums are cut into this many (grid y), whose
+                          // results go to part [cuts, T, columns] if there are several
 };
 
 // ---- which rows a tile has --------------------------------------------------
@@ -284,10 +289,59 @@ __device__ __forceinline__ bool row_tile(const GroupedParams& p, int bm, int til
 inline int64_t row_grid(const GroupedParams& p, int64_t bm, int64_t tiles_n) {
   return (p.T / bm + p.E + 1) * tiles_n;
 }
+// About how many row tiles T rows of E groups make: half of a group's last one
+// is empty, and no more groups have rows than there are rows.
+inline double row_tiles(int64_t T, int64_t E, int64_t bm) {
+  return (double)(T / bm) + std::max(0.5, 0.5 * (double)std::min(E, T));
+}
+// Rounds of `places` blocks at once that `blocks` equal ones take.  (The last
+// round, where it is not full, runs at a higher clock: half way to whole rounds.)
+inline double rounds(double blocks, double places) {
+  const double x = blocks / places;
+  return 0.5 * (x + std::max(1.0, std::ceil(x)));
+}
+// Cuts of the sums (`slabs` of them) of `tiles` tiles that would leave places
+// idle: to fill them once, a cut of 4 slabs at least.  The cuts' results are
+// written, read and added by one more launch of about 5 us, so they have to save
+// more than that: slab_us is the time of a slab.
+inline int sum_cuts(double tiles, int places, int64_t slabs, double slab_us) {
+  const int64_t cuts = std::min<int64_t>((int64_t)(places / std::max(tiles, 1.0)), slabs / 4);
+  if (cuts < 2 || (double)(slabs - slabs / cuts) * slab_us < 10.0) return 1;
+  return (int)std::min<int64_t>(cuts, 32);
+}
+// The k range of this block's cut, whole slabs of 64.
+__device__ __forceinline__ void cut_range(const GroupedParams& p, int64_t* kbeg, int64_t* kend) {
+  if (p.cuts <= 1) return;
+  const int64_t each = ((*kend + p.cuts - 1) / p.cuts + 63) / 64 * 64;
+  *kbeg = min(*kend, (int64_t)blockIdx.y * each);
+  *kend = min(*kend, *kbeg + each);
+}
 
-// fp32 products on the split contraction engine's tiles (kan_gemm.hip), and
-// the rows of an item there.
+// out = the sum of `cuts` slices of `count` values, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_cuts_kernel(const float* __restrict__ part, int cuts,
+                                                           int64_t count, T* __restrict__ out) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count;
+       i += (int64_t)gridDim.x * 256) {
+    float v = part[i];
+#pragma unroll 8
+    for (int q = 1; q < cuts; ++q) v += part[q * count + i];
+    out[i] = (T)v;
+  }
+}
+template <typename T>
+int launch_grouped_cuts(const GroupedParams& p, int64_t cols, hipStream_t st) {
+  if (p.cuts <= 1) return KAN_OK;
+  const int64_t count = p.T * cols;
+  grouped_cuts_kernel<T><<<dim3((unsigned)std::min<int64_t>(ceil_div(count, 256), 8192)), 256, 0,
+                           st>>>(p.part, p.cuts, count, static_cast<T*>(p.C));
+  return check_launch("grouped_matmul sum");
+}
+
+// fp32 products on the split contraction engine's tiles (kan_gemm.hip); the rows
+// of an item and the cuts of a sum there.
 int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K);
+int grouped_f32_cuts(int op, int64_t T, int64_t E, int64_t N, int64_t K);
 int launch_grouped_f32(int op, const GroupedParams& p, hipStream_t st);
 
 }  // namespace kan

@@ -67,6 +67,7 @@ struct TileCfg {
   static constexpr int kBuf = (BM + BN) * kDepth * 2;  // bytes of one slab pair
 };
 using TileBig = TileCfg<256, 256, 2, 4>;
+using TileMid = TileCfg<192, 256, 2, 4>;  // (rows of K-contiguous operands only)
 using TileSmall = TileCfg<128, 128, 2, 2>;
 
 // How an operand reaches LDS.
@@ -163,6 +164,8 @@ struct Operand {
         const int r = chunk_row(p), c = 8 * chunk_col(p);
         const int64_t left = KCONT ? kend - k0 - c : (int64_t)(rows - c);
         n = (!KCONT && k0 + r >= kend) || left <= 0 ? 0 : (int)min(left, (int64_t)8);
+        // (aligned rows end with whole chunks: their own, or zeros up to ld)
+        if (MODE == kDirect && n > 0) n = 8;
       }
       u32x4 v = {0, 0, 0, 0};
       if constexpr (MODE >= kInt8) {
@@ -179,7 +182,7 @@ struct Operand {
       } else if (n == 8) {
         if constexpr (MODE == kGuarded) v = reinterpret_cast<const Loose16*>(src + off[p])->v;
         else v = *reinterpret_cast<const u32x4*>(src + off[p]);
-      } else if constexpr (MODE == kGuarded) {  // (aligned rows end with whole chunks)
+      } else if constexpr (MODE == kGuarded) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           if (j < n)
@@ -304,14 +307,15 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     m0 = t.m0;
     m_end = t.m1;
     kend = e == p.E ? 0 : OP == 0 ? p.K : p.N;
+    cut_range(p, &kbeg, &kend);
   }
   const int64_t n_end = OP == 0 ? p.N : p.K, n0 = (int64_t)tn * BN;
-  const int64_t weight = (int64_t)e * p.N * p.K;
+  const int64_t weight = (int64_t)e * p.N * (OP == 2 ? p.K : p.ldb);
 
   Operand<T, BM, KA, MA, G::NT> a;
   Operand<T, BN, KB, MB, G::NT> b;
-  a.init(p.A, OP == 0 ? p.K : p.N, m0, m_end - m0);
-  b.init(OP == 2 ? p.B : static_cast<const T*>(p.B) + weight, p.K, n0, n_end - n0);
+  a.init(p.A, p.lda, m0, m_end - m0);
+  b.init(OP == 2 ? p.B : static_cast<const T*>(p.B) + weight, p.ldb, n0, n_end - n0);
   if constexpr (MB >= kInt8)
     b.init_scale(p.b_scale, (p.K + p.group - 1) / p.group, p.group, n0);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -337,7 +341,6 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     for (int j = 0; j < FN; ++j) bv[st & 1][j] = fb.read(buf + kB, j, st);
 #pragma unroll
     for (int i = 0; i < FM; ++i) av[st & 1][i] = fa.read(buf, i, st);
-    __builtin_amdgcn_sched_barrier(0);  // (left alone, reads sink below the MFMAs)
   };
   auto mma_step = [&](int st) __attribute__((always_inline)) {
     // (B first: a lane then holds 4 columns of one row of the output)
@@ -346,6 +349,14 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
 #pragma unroll
       for (int j = 0; j < FN; ++j)
         acc[i][j] = Half<T>::mma(bv[st & 1][j], av[st & 1][i], acc[i][j]);
+    // the step's reads one by one between its MFMAs (left alone they sink below
+    // them; all of them first: 1 to 5 % slower)
+#pragma unroll
+    for (int q = 0; q < FM + FN; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, KA && KB ? 1 : 2, 0);  // LDS reads
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                 // MFMA
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, FM * FN, 0);
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -415,8 +426,9 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     for (; kt < slabs; ++kt) slab(kt, kt + 1 < slabs, kt + 2 < slabs, rest);
   }
 
-  if (OP == 2 && slot >= 0) {  // the sums of an item of several
-    float* part = p.part + (int64_t)slot * p.N * p.K;
+  if (OP == 2 ? slot >= 0 : p.cuts > 1) {  // an item of several, a cut of several
+    float* part =
+        p.part + (OP == 2 ? (int64_t)slot * p.N * p.K : (int64_t)blockIdx.y * p.T * n_end);
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -478,51 +490,157 @@ int launch_tile(const GroupedParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(cols, G::BN), tiles_m = ceil_div(p.N, G::BM);
   const int64_t blocks = OP == 2 ? weight_grid(p, tiles_m * tiles_n) : row_grid(p, G::BM, tiles_n);
   if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
-  grouped_tile_kernel<T, G, OP, MA, MB><<<dim3((unsigned)blocks), G::NT, 0, st>>>(
+  grouped_tile_kernel<T, G, OP, MA, MB><<<dim3((unsigned)blocks, OP == 2 ? 1 : p.cuts), G::NT, 0,
+                                         st>>>(
       p, (int)tiles_m, (int)tiles_n, cols % 8 == 0 && aligned16(p.C) ? 1 : 0);
   const int rc = check_launch("grouped_matmul");
-  return rc != KAN_OK || OP != 2 ? rc : launch_grouped_sum<T>(p, st);
+  if (rc != KAN_OK) return rc;
+  return OP == 2 ? launch_grouped_sum<T>(p, st) : launch_grouped_cuts<T>(p, cols, st);
 }
 
-template <typename T, class G>
-int launch_half_cfg(int op, const GroupedParams& p, hipStream_t st) {
-  const bool a16 = aligned16(p.A) && (op == 0 ? p.K : p.N) % 8 == 0;
-  const bool b16 = aligned16(p.B) && p.K % 8 == 0;
-  if (op == 0)
-    return a16 && b16 ? launch_tile<T, G, 0, kDirect, kDirect>(p, st)
-                      : launch_tile<T, G, 0, kGuarded, kGuarded>(p, st);
-  if (op == 1)
-    return a16 && b16 ? launch_tile<T, G, 1, kDirect, kDirect>(p, st)
-                      : launch_tile<T, G, 1, kGuarded, kGuarded>(p, st);
-  if (p.format == KAN_ACT8_INT8)
-    return a16 ? launch_tile<T, G, 2, kDirect, kInt8>(p, st)
-               : launch_tile<T, G, 2, kGuarded, kInt8>(p, st);
-  if (p.format == KAN_ACT8_E4M3)
-    return a16 ? launch_tile<T, G, 2, kDirect, kE4m3>(p, st)
-               : launch_tile<T, G, 2, kGuarded, kE4m3>(p, st);
-  return a16 && b16 ? launch_tile<T, G, 2, kDirect, kDirect>(p, st)
-                    : launch_tile<T, G, 2, kGuarded, kGuarded>(p, st);
+// Operands are read straight into LDS where their rows are whole 16 bytes.
+bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+template <typename T, class G, int OP>
+int launch_half_op(const GroupedParams& p, hipStream_t st) {
+  const bool a16 = whole_rows(p.A, p.lda), b16 = whole_rows(p.B, p.ldb);
+  if constexpr (OP == 2) {
+    if (p.format == KAN_ACT8_INT8)
+      return a16 ? launch_tile<T, G, 2, kDirect, kInt8>(p, st)
+                 : launch_tile<T, G, 2, kGuarded, kInt8>(p, st);
+    if (p.format == KAN_ACT8_E4M3)
+      return a16 ? launch_tile<T, G, 2, kDirect, kE4m3>(p, st)
+                 : launch_tile<T, G, 2, kGuarded, kE4m3>(p, st);
+  }
+  return a16 && b16 ? launch_tile<T, G, OP, kDirect, kDirect>(p, st)
+                    : launch_tile<T, G, OP, kGuarded, kGuarded>(p, st);
 }
 
-// The large tile where its tiles (half of a group's last row tile is empty on
-// average) fill the chip.
-bool half_takes_big(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
-  const int64_t tiles_m = op == 2 ? ceil_div(N, 256) * E : T / 256 + E / 2;
-  return tiles_m * ceil_div(op == 0 ? N : K, 256) >= device_cu_count();
-}
-// (16384 rows, 8 experts of 4096 x 4096: 64 rows of the large tile in 1.0 us;
-// of the small one, two blocks a CU, in 0.65)
-int half_run(int64_t T, int64_t E, int64_t N, int64_t K) {
+enum HalfCfg { kBig, kMid, kSmall };
+
+// What a product in 16 bits runs on.  Time of a round of each tile, 16384 rows
+// over 8 equal groups, 4096 x 4096 in bf16: 111 us on 256 x 256, 88 on 192 x
+// 256, 73 on two 128 x 128 a CU.  (32768 rows over 16 groups, 4096 -> 1024: 314
+// us on 256 rows, 285 on 192; 16384 over 8, 4096 -> 4096: 510 and 528.)
+struct HalfPlan {
+  HalfCfg cfg;
+  int cuts, run;
+};
+HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
   const int cus = device_cu_count();
-  if (half_takes_big(2, T, E, N, K))
-    return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 256), {cus, 0.016, 5.0});
-  return weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.010, 4.0});
+  HalfPlan pl{kSmall, 1, kNoRuns};
+  if (op == 2) {
+    const int64_t big = ceil_div(N, 256) * ceil_div(K, 256);
+    // (64 rows of the large tile take 1.0 us, of the small one 0.65)
+    if (big * E >= cus) {
+      pl.cfg = kBig;
+      pl.run = weight_run(T, E, N, K, big, {cus, 0.016, 5.0});
+    } else {
+      pl.run = weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.010, 4.0});
+    }
+    return pl;
+  }
+  const int64_t cols = op == 0 ? N : K, depth = op == 0 ? K : N;
+  const double wide = (double)ceil_div(cols, 256);
+  const double small = row_tiles(T, E, 128) * (double)ceil_div(cols, 128);
+  const double t[3] = {1.0 * rounds(row_tiles(T, E, 256) * wide, cus),
+                       0.8 * rounds(row_tiles(T, E, 192) * wide, cus),
+                       0.65 * rounds(small, 2.0 * cus)};
+  for (int c = 0; c < 2; ++c)
+    if (t[c] < t[pl.cfg]) pl.cfg = (HalfCfg)c;
+  if (pl.cfg == kSmall) pl.cuts = sum_cuts(small, 2 * cus, ceil_div(depth, kDepth), 0.7);
+  return pl;
+}
+
+// Rows of [rows, C] at any address onto whole 16 bytes: out [rows, ld], ld a
+// multiple of 8, the rest of a row zero.
+template <typename T>
+__global__ __launch_bounds__(256) void align_rows_kernel(const T* __restrict__ x, int64_t rows,
+                                                         int64_t C, int64_t ld,
+                                                         T* __restrict__ out) {
+  const int64_t chunks = ld / 8, total = rows * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / chunks, c = 8 * (i - r * chunks);
+    const T* src = x + r * C + c;
+    u32x4 v = {0, 0, 0, 0};
+    if (c + 8 <= C) {
+      v = reinterpret_cast<const Loose16*>(src)->v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < C)
+          v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[j] << (16 * (j & 1));
+    }
+    *reinterpret_cast<u32x4*>(out + i * 8) = v;
+  }
+}
+template <typename T>
+int launch_align(const void* x, int64_t rows, int64_t C, int64_t ld, void* out, hipStream_t st) {
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows * (ld / 8), 256), 1 << 16);
+  align_rows_kernel<T><<<dim3((unsigned)blocks), 256, 0, st>>>(static_cast<const T*>(x), rows, C,
+                                                               ld, static_cast<T*>(out));
+  return check_launch("grouped_matmul rows");
+}
+
+// Operands with rows off 16 bytes are brought onto them first where the
+// products then save more than the copies take: at 32768 rows, 16 groups of
+// 1023 -> 4095 the products took 636 (forward), 937 (input) and 1015 us
+// (weight) on rows as they were, against 293, 323 and 262 on aligned ones; a
+// copy moves its rows twice at about 4 TB/s, and takes 5 us at least.
+struct AlignPlan {
+  bool a, b;
+  int64_t a_rows, a_cols, b_rows, b_cols;
+  size_t a_bytes, b_bytes;
+};
+AlignPlan align_plan(int op, int format, const void* A, const void* B, int64_t T, int64_t E,
+                     int64_t N, int64_t K) {
+  AlignPlan pl{};
+  pl.a_rows = T;
+  pl.a_cols = op == 0 ? K : N;
+  pl.b_rows = op == 2 ? T : E * N;
+  pl.b_cols = K;
+  pl.a = !whole_rows(A, pl.a_cols);
+  pl.b = format == KAN_ACT8_NONE && !whole_rows(B, pl.b_cols);
+  const double extra[3] = {1.2, 1.9, 2.9};  // of the aligned product's time
+  const double saved_us = extra[op] * 2.0 * (double)T * (double)N * (double)K / 1.0e9;
+  double copies_us = 0.0;
+  if (pl.a) copies_us += 5.0 + 4.0 * (double)(pl.a_rows * pl.a_cols) / 4.0e6;
+  if (pl.b) copies_us += 5.0 + 4.0 * (double)(pl.b_rows * pl.b_cols) / 4.0e6;
+  if (saved_us <= copies_us) pl.a = pl.b = false;
+  if (pl.a) pl.a_bytes = 2 * (size_t)(pl.a_rows * round_up(pl.a_cols, 8));
+  if (pl.b) pl.b_bytes = 2 * (size_t)(pl.b_rows * round_up(pl.b_cols, 8));
+  return pl;
 }
 
 template <typename T>
-int launch_half(int op, const GroupedParams& p, hipStream_t st) {
-  return half_takes_big(op, p.T, p.E, p.N, p.K) ? launch_half_cfg<T, TileBig>(op, p, st)
-                                                : launch_half_cfg<T, TileSmall>(op, p, st);
+int launch_half(int op, GroupedParams p, const HalfPlan& plan, const AlignPlan& al, char* ws,
+                hipStream_t st) {
+  if (al.a) {
+    const int64_t ld = round_up(al.a_cols, 8);
+    const int rc = launch_align<T>(p.A, al.a_rows, al.a_cols, ld, ws, st);
+    if (rc != KAN_OK) return rc;
+    p.A = ws;
+    p.lda = ld;
+    ws += al.a_bytes;
+  }
+  if (al.b) {
+    const int64_t ld = round_up(al.b_cols, 8);
+    const int rc = launch_align<T>(p.B, al.b_rows, al.b_cols, ld, ws, st);
+    if (rc != KAN_OK) return rc;
+    p.B = ws;
+    p.ldb = ld;
+  }
+  if (op == 2)
+    return plan.cfg == kBig ? launch_half_op<T, TileBig, 2>(p, st)
+                            : launch_half_op<T, TileSmall, 2>(p, st);
+  if (op == 0)
+    return plan.cfg == kBig   ? launch_half_op<T, TileBig, 0>(p, st)
+           : plan.cfg == kMid ? launch_half_op<T, TileMid, 0>(p, st)
+                              : launch_half_op<T, TileSmall, 0>(p, st);
+  return plan.cfg == kBig   ? launch_half_op<T, TileBig, 1>(p, st)
+         : plan.cfg == kMid ? launch_half_op<T, TileMid, 1>(p, st)
+                            : launch_half_op<T, TileSmall, 1>(p, st);
 }
 
 int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K) {
@@ -540,17 +658,32 @@ int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K)
   return KAN_OK;
 }
 
-// Workspace of the weight gradient: the items' partial sums and, in fp32, the
-// 8-bit rows as floats (the engine takes fp32 operands).
-int run_of(int dtype, int64_t T, int64_t E, int64_t N, int64_t K) {
-  return dtype == KAN_DTYPE_F32 ? grouped_f32_run(T, E, N, K) : half_run(T, E, N, K);
-}
-size_t workspace_bytes_of(int dtype, int op, int format, int64_t T, int64_t E, int64_t N,
-                          int64_t K) {
-  if (op != KAN_GROUPED_WEIGHT || T * E * N * K == 0) return 0;
-  int64_t elems = weight_part_elems(T, E, N, K, run_of(dtype, T, E, N, K));
-  if (dtype == KAN_DTYPE_F32 && format != KAN_ACT8_NONE) elems += T * K;
-  return 4 * (size_t)elems;
+// A call's workspace: rows brought onto 16 bytes (16-bit types) or restored from
+// 8 bits (fp32, whose engine takes floats), then the partial sums.
+struct Workspace {
+  HalfPlan plan;
+  AlignPlan align;
+  size_t rows_bytes, part_bytes;  // (part from a multiple of 16 bytes on)
+};
+Workspace plan_call(int dtype, int op, int format, const void* A, const void* B, int64_t T,
+                    int64_t E, int64_t N, int64_t K) {
+  Workspace w{};
+  w.plan = {kSmall, 1, kNoRuns};
+  if (T * E * N * K == 0) return w;
+  if (dtype == KAN_DTYPE_F32) {
+    if (op == KAN_GROUPED_WEIGHT) w.plan.run = grouped_f32_run(T, E, N, K);
+    else w.plan.cuts = grouped_f32_cuts(op, T, E, N, K);
+    if (format != KAN_ACT8_NONE) w.rows_bytes = 4 * (size_t)(T * K);
+  } else {
+    w.plan = half_plan(op, T, E, N, K);
+    w.align = align_plan(op, format, A, B, T, E, N, K);
+    w.rows_bytes = w.align.a_bytes + w.align.b_bytes;
+  }
+  w.rows_bytes = (size_t)round_up((int64_t)w.rows_bytes, 16);
+  if (op == KAN_GROUPED_WEIGHT) w.part_bytes = 4 * (size_t)weight_part_elems(T, E, N, K, w.plan.run);
+  else if (w.plan.cuts > 1)
+    w.part_bytes = 4 * (size_t)w.plan.cuts * (size_t)(T * (op == KAN_GROUPED_FORWARD ? N : K));
+  return w;
 }
 
 }  // namespace
@@ -560,13 +693,14 @@ using namespace kan;
 
 extern "C" {
 
-int kan_hip_grouped_matmul_workspace(int dtype, int op, int b_format, int64_t T, int64_t E, int64_t N, int64_t K,
-                                     size_t* bytes) {
+int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const void* b, int b_format,
+                                     int64_t T, int64_t E, int64_t N, int64_t K, size_t* bytes) {
   if (bytes == nullptr)
     return set_error(KAN_ERR_INVALID, "grouped_matmul_workspace: bytes must not be NULL");
   const int rc = check_grouped(dtype, op, T, E, N, K);
   if (rc != KAN_OK) return rc;
-  *bytes = workspace_bytes_of(dtype, op, b_format, T, E, N, K);
+  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
+  *bytes = w.rows_bytes + w.part_bytes;
   return KAN_OK;
 }
 
@@ -593,10 +727,12 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   const bool some = op == KAN_GROUPED_WEIGHT ? T > 0 : E * N * K > 0;  // any term to add up
   if (out == nullptr || (some && (a == nullptr || b == nullptr)) || (E > 0 && offsets == nullptr))
     return set_error(KAN_ERR_INVALID, "grouped_matmul: operands must not be NULL");
-  const size_t need = workspace_bytes_of(dtype, op, b_format, T, E, N, K);
+  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
+  const size_t need = w.rows_bytes + w.part_bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(KAN_ERR_WORKSPACE, "grouped_matmul: needs %zu bytes of workspace, got %zu",
                      need, workspace == nullptr ? (size_t)0 : workspace_bytes);
+  char* ws = static_cast<char*>(workspace);
   GroupedParams p{};
   p.A = a;
   p.B = b;
@@ -612,24 +748,22 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   p.format = b_format;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * N * K);
-  p.run = kNoRuns;
-  int64_t part = 0;
-  if (op == KAN_GROUPED_WEIGHT && T > 0) {
-    p.run = run_of(dtype, T, E, N, K);
-    part = weight_part_elems(T, E, N, K, p.run);
-    if (part > 0) p.part = static_cast<float*>(workspace);
-  }
+  p.lda = op == KAN_GROUPED_FORWARD ? K : N;
+  p.ldb = K;
+  p.run = w.plan.run;
+  p.cuts = w.plan.cuts;
+  if (w.part_bytes > 0) p.part = reinterpret_cast<float*>(ws + w.rows_bytes);
   if (dtype == KAN_DTYPE_F32) {
-    if (b_format != KAN_ACT8_NONE && T > 0) {
-      float* rows = static_cast<float*>(workspace) + part;
-      const int e = kan_hip_act8_dequantize(dtype, b_format, b, b_scale, T, K, b_group, rows, stream);
+    if (w.rows_bytes > 0) {
+      const int e =
+          kan_hip_act8_dequantize(dtype, b_format, b, b_scale, T, K, b_group, ws, stream);
       if (e != KAN_OK) return e;
-      p.B = rows;
+      p.B = ws;
     }
     return launch_grouped_f32(op, p, st);
   }
-  if (dtype == KAN_DTYPE_BF16) return launch_half<bf16>(op, p, st);
-  return launch_half<f16>(op, p, st);
+  return dtype == KAN_DTYPE_BF16 ? launch_half<bf16>(op, p, w.plan, w.align, ws, st)
+                                 : launch_half<f16>(op, p, w.plan, w.align, ws, st);
 }
 
 }  // extern "C"

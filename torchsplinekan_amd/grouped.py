@@ -35,20 +35,18 @@ def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
     if out.numel() == 0:
         return out
     code = lib.OPERATOR_DTYPES[out.dtype]
-    form, scale, group, ws, size = 0, None, 0, None, 0
-    if op == WEIGHT:  # (the other products take no workspace)
-        if isinstance(b, Activation8):
-            form, scale, group, b = FORMATS[b.format][0], b.scale, b.group, b.q
-        nbytes = ctypes.c_size_t()
-        lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(code, op, form, T, E, N, K,
-                                                           ctypes.byref(nbytes)))
-        size = nbytes.value
-        if size:
-            ws = torch.empty(size, dtype=torch.uint8, device=out.device)
-    ptr = lib.ptr
-    lib.launch(lib.LIB.kan_hip_grouped_matmul, out.device, code, op, ptr(a), ptr(b), form,
-               ptr(scale), group, ptr(offsets), int(offsets.dtype == torch.int64), T, E, N, K,
-               out.data_ptr(), ptr(ws), size)
+    form, scale, group, ws = 0, None, 0, None
+    if isinstance(b, Activation8):
+        form, scale, group, b = FORMATS[b.format][0], b.scale.data_ptr(), b.group, b.q
+    pa, pb = lib.ptr(a), lib.ptr(b)
+    nbytes = ctypes.c_size_t()
+    lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(code, op, pa, pb, form, T, E, N, K,
+                                                       ctypes.byref(nbytes)))
+    if nbytes.value:
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=out.device)
+    lib.launch(lib.LIB.kan_hip_grouped_matmul, out.device, code, op, pa, pb, form, scale, group,
+               lib.ptr(offsets), int(offsets.dtype == torch.int64), T, E, N, K, out.data_ptr(),
+               lib.ptr(ws), nbytes.value)
     return out
 
 

@@ -1265,11 +1265,7 @@ grouped_split_kernel(GroupedParams g, int tiles_m, int tiles_n, int buf) {
     cut_range(g, &tc.kbeg, &tc.kend);
     p.M = t.m1;
     p.B += t.e * weights;
-    p.C = g.cuts > 1 ? g.part : static_cast<float*>(g.C);
-    if (g.cuts > 1) {
-      tc.split = blockIdx.y;
-      p.split_stride = g.T * p.N;
-    }
+    p.C = g.cuts > 1 ? g.part + blockIdx.y * (g.T * p.N) : static_cast<float*>(g.C);
   }
   tc.nkt = (int)ceil_div(tc.kend - tc.kbeg, C::BK);
   split_tile<C, AK, BKC, 0>(p, tc, DxParams{}, lds);

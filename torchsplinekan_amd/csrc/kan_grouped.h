@@ -312,9 +312,10 @@ inline int sum_cuts(double tiles, int places, int64_t slabs, double slab_us) {
 // The k range of this block's cut, whole slabs of 64.
 __device__ __forceinline__ void cut_range(const GroupedParams& p, int64_t* kbeg, int64_t* kend) {
   if (p.cuts <= 1) return;
-  const int64_t each = ((*kend + p.cuts - 1) / p.cuts + 63) / 64 * 64;
-  *kbeg = min(*kend, (int64_t)blockIdx.y * each);
-  *kend = min(*kend, *kbeg + each);
+  const int k = (int)*kend, each = ((k + p.cuts - 1) / p.cuts + 63) / 64 * 64;
+  // (uniform values: the division runs in vector registers)
+  *kbeg = __builtin_amdgcn_readfirstlane(min(k, (int)blockIdx.y * each));
+  *kend = __builtin_amdgcn_readfirstlane(min(k, (int)*kbeg + each));
 }
 
 // out = the sum of `cuts` slices of `count` values, in order.

@@ -37,7 +37,6 @@ namespace {
 // Rows and columns past a tile's last repeat an earlier one: their products
 // are not stored.  k past the last is zero in both operands, as what lies there
 // (another expert's rows) may be anything.
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -107,8 +106,10 @@ struct Operand {
     scale = src;
     parts = parts_;
 #pragma unroll
-    for (int p = 0; p < kPer; ++p)
-      part[p] = (uint32_t)(chunk_row(p) * parts) + ((uint32_t)col0 + 8 * chunk_col(p)) / group;
+    for (int p = 0; p < kPer; ++p) {
+      const int c = 8 * chunk_col(p);
+      part[p] = (uint32_t)(chunk_row(p) * parts) + ((uint32_t)col0 + (c < rows ? c : 0)) / group;
+    }
   }
 
   // Row of the thread's chunk p in the slab's layout, and the chunk of that
@@ -192,9 +193,10 @@ struct Operand {
       reg[p] = v;
     }
   }
-  // Whether a slab whose k all exist needs no guard.
+  // Whether a slab whose k all exist needs no guard: chunks past the last column
+  // repeat the first, and rows of whole chunks have no part of one.
   __device__ __forceinline__ bool interior() const {
-    return MODE == kDirect || KCONT || rows == ROWS;
+    return MODE == kDirect || KCONT || rows == ROWS || (MODE >= kInt8 && ld % 8 == 0);
   }
 
   __device__ __forceinline__ void store(char* lds) const {
@@ -473,6 +475,8 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     T* dst = out + row * n_end + col;
     if (store_vec) {
       *reinterpret_cast<u32x4*>(dst) = v;
+    } else if (col + 8 <= n_end) {
+      reinterpret_cast<Loose16*>(dst)->v = v;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -498,6 +502,144 @@ int launch_tile(const GroupedParams& p, hipStream_t st) {
   return OP == 2 ? launch_grouped_sum<T>(p, st) : launch_grouped_cuts<T>(p, cols, st);
 }
 
+// ---- few rows ---------------------------------------------------------------
+// The forward of groups of a few rows (single tokens): bound by the weights'
+// bytes, which a 128-row tile would hold up behind MFMAs on rows that do not
+// exist.  A block has 16 rows and 16 columns; its four waves take the k in
+// turns, each lane 64 consecutive bytes of one weight row (and of one x row),
+// straight from memory into v_mfma_f32_16x16 operands: which k a lane's values
+// are does not matter as long as both operands agree.  The waves' sums are added
+// through LDS in order.
+// (8 rows at 16 experts of 1024 -> 4096: fp32 66 us on tiles, bf16 rows of 1023
+// 33 us.)
+template <typename T>
+struct RowsMma;
+template <>
+struct RowsMma<float> {
+  typedef float vec __attribute__((ext_vector_type(4)));
+  typedef float acc_t __attribute__((ext_vector_type(4)));
+  __device__ static __forceinline__ acc_t mma(vec a, vec b, acc_t c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+template <>
+struct RowsMma<bf16> {
+  typedef bf16 vec __attribute__((ext_vector_type(8)));
+  typedef float acc_t __attribute__((ext_vector_type(4)));
+  __device__ static __forceinline__ acc_t mma(vec a, vec b, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct RowsMma<f16> {
+  typedef f16 vec __attribute__((ext_vector_type(8)));
+  typedef float acc_t __attribute__((ext_vector_type(4)));
+  __device__ static __forceinline__ acc_t mma(vec a, vec b, acc_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+constexpr int kFewRows = 16;
+template <typename T, int NC, bool WHOLE>
+__global__ __launch_bounds__(256) void grouped_few_kernel(GroupedParams p, int tiles_n) {
+  typedef RowsMma<T> M;
+  constexpr int V = 16 / sizeof(T), U = 4;  // values of a load, loads of a lane's turn
+  constexpr int kCols = 16 * NC;
+  __shared__ float red[4][kFewRows][kCols + 1];
+  RowTile t;
+  int tn;
+  if (!row_tile(p, kFewRows, tiles_n, &t, &tn)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n0 = tn * kCols;
+  typename M::acc_t acc[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) acc[c] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (t.e < p.E) {
+    const int m = min(t.m0 + (lane & 15), t.m1 - 1);
+    const T* x = static_cast<const T*>(p.A) + (int64_t)m * p.K;
+    const T* w[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      w[c] = static_cast<const T*>(p.B) +
+             ((int64_t)t.e * p.N + min((int64_t)(n0 + 16 * c + (lane & 15)), p.N - 1)) * p.K;
+    auto load = [](const T* q) __attribute__((always_inline)) {
+      if constexpr (sizeof(T) == 2 && !WHOLE)
+        return __builtin_bit_cast(typename M::vec, load16_even(q));
+      else
+        return reinterpret_cast<const LooseVec<T, V>*>(q)->v;
+    };
+    constexpr int kTurn = 4 * U * V;
+    for (int64_t k0 = wave * kTurn; k0 < p.K; k0 += 4 * kTurn) {
+      typename M::vec a[NC][U], b[U];
+      const int64_t k = k0 + (lane >> 4) * V;
+      if (k0 + kTurn <= p.K) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            a[c][u] = load(w[c] + k + u * 4 * V);
+          b[u] = load(x + k + u * 4 * V);
+        }
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int j = 0; j < V; ++j) {
+            const int64_t at = k + u * 4 * V + j;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) a[c][u][j] = at < p.K ? w[c][at] : (T)0.0f;
+            b[u][j] = at < p.K ? x[at] : (T)0.0f;
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[c] = M::mma(a[c][u], b[u], acc[c]);
+    }
+  }
+  // lane l has row l & 15 and columns 4 (l >> 4) .. + 3 of each 16
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) red[wave][lane & 15][16 * c + 4 * (lane >> 4) + v] = acc[c][v];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int at = i * 256 + threadIdx.x, m = at / kCols, n = at % kCols;
+    const float s = red[0][m][n] + red[1][m][n] + red[2][m][n] + red[3][m][n];
+    if (t.m0 + m < t.m1 && n0 + n < p.N)
+      static_cast<T*>(p.C)[(int64_t)(t.m0 + m) * p.N + n0 + n] = (T)s;
+  }
+}
+
+template <typename T, int NC, bool WHOLE>
+int launch_few_cols(const GroupedParams& p, hipStream_t st) {
+  const int64_t tiles_n = ceil_div(p.N, 16 * NC), blocks = row_grid(p, kFewRows, tiles_n);
+  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  grouped_few_kernel<T, NC, WHOLE><<<dim3((unsigned)blocks), 256, 0, st>>>(p, (int)tiles_n);
+  return check_launch("grouped_matmul");
+}
+
+// Groups of up to 8 rows on average in 16 bits, 32 in fp32 (whose tiles multiply
+// six times): 128 rows, 16 experts of 1024 x 1024, 8.4 us against 11.9 on tiles
+// in bf16, 14.8 against 32 in fp32; at 16 rows a group (64 rows, 4 experts of
+// 4096 x 4096, bf16) 42 against 33, at 32 in fp32 (512 rows, 16 experts of 1024 x
+// 1024) 30.6 against 35.5.
+bool takes_few(int dtype, int op, int64_t T, int64_t E) {
+  return op == KAN_GROUPED_FORWARD && T <= (dtype == KAN_DTYPE_F32 ? 32 : 8) * E;
+}
+// 32 columns a block (the x rows are read once for both halves) where such
+// blocks number two a CU: 16 experts of 1024 x 1024 and 128 rows 9.9 -> 8.4 us;
+// one expert of 4096 x 4096 and one row 7.9 us on 16 columns, 11.3 on 32.
+template <typename T>
+int launch_few(const GroupedParams& p, hipStream_t st) {
+  const bool wide = std::min<int64_t>(p.E, p.T) * ceil_div(p.N, 32) >= 2 * device_cu_count();
+  if (sizeof(T) == 2 && !(aligned16(p.A) && aligned16(p.B) && p.K % 8 == 0))
+    return wide ? launch_few_cols<T, 2, false>(p, st) : launch_few_cols<T, 1, false>(p, st);
+  return wide ? launch_few_cols<T, 2, true>(p, st) : launch_few_cols<T, 1, true>(p, st);
+}
+
 // Operands are read straight into LDS where their rows are whole 16 bytes.
 bool whole_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
@@ -516,7 +658,7 @@ int launch_half_op(const GroupedParams& p, hipStream_t st) {
                     : launch_tile<T, G, OP, kGuarded, kGuarded>(p, st);
 }
 
-enum HalfCfg { kBig, kMid, kSmall };
+enum HalfCfg { kBig, kMid, kSmall, kFew };
 
 // What a product in 16 bits runs on.  Time of a round of each tile, 16384 rows
 // over 8 equal groups, 4096 x 4096 in bf16: 111 us on 256 x 256, 88 on 192 x
@@ -552,34 +694,35 @@ HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
   return pl;
 }
 
-// Rows of [rows, C] at any address onto whole 16 bytes: out [rows, ld], ld a
-// multiple of 8, the rest of a row zero.
-template <typename T>
-__global__ __launch_bounds__(256) void align_rows_kernel(const T* __restrict__ x, int64_t rows,
+// Rows of [rows, C] at any address onto whole chunks of 8 values: out [rows, ld],
+// ld a multiple of 8, the rest of a row zero.  (U: an integer of a value's size.)
+template <typename U>
+__global__ __launch_bounds__(256) void align_rows_kernel(const U* __restrict__ x, int64_t rows,
                                                          int64_t C, int64_t ld,
-                                                         T* __restrict__ out) {
+                                                         U* __restrict__ out) {
+  typedef typename std::conditional<sizeof(U) == 2, Loose16, Loose8>::type Loose;
+  typedef decltype(Loose::v) Chunk;
   const int64_t chunks = ld / 8, total = rows * chunks;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
        i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / chunks, c = 8 * (i - r * chunks);
-    const T* src = x + r * C + c;
-    u32x4 v = {0, 0, 0, 0};
+    const U* src = x + r * C + c;
+    U v[8] = {};
     if (c + 8 <= C) {
-      v = reinterpret_cast<const Loose16*>(src)->v;
+      *reinterpret_cast<Chunk*>(v) = reinterpret_cast<const Loose*>(src)->v;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (c + j < C)
-          v[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(src)[j] << (16 * (j & 1));
+        if (c + j < C) v[j] = src[j];
     }
-    *reinterpret_cast<u32x4*>(out + i * 8) = v;
+    *reinterpret_cast<Chunk*>(out + i * 8) = *reinterpret_cast<const Chunk*>(v);
   }
 }
-template <typename T>
+template <typename U>
 int launch_align(const void* x, int64_t rows, int64_t C, int64_t ld, void* out, hipStream_t st) {
   const int64_t blocks = std::min<int64_t>(ceil_div(rows * (ld / 8), 256), 1 << 16);
-  align_rows_kernel<T><<<dim3((unsigned)blocks), 256, 0, st>>>(static_cast<const T*>(x), rows, C,
-                                                               ld, static_cast<T*>(out));
+  align_rows_kernel<U><<<dim3((unsigned)blocks), 256, 0, st>>>(static_cast<const U*>(x), rows, C,
+                                                               ld, static_cast<U*>(out));
   return check_launch("grouped_matmul rows");
 }
 
@@ -600,16 +743,18 @@ AlignPlan align_plan(int op, int format, const void* A, const void* B, int64_t T
   pl.a_cols = op == 0 ? K : N;
   pl.b_rows = op == 2 ? T : E * N;
   pl.b_cols = K;
+  const int64_t b_value = format == KAN_ACT8_NONE ? 2 : 1;
   pl.a = !whole_rows(A, pl.a_cols);
-  pl.b = format == KAN_ACT8_NONE && !whole_rows(B, pl.b_cols);
+  pl.b = format == KAN_ACT8_NONE ? !whole_rows(B, pl.b_cols)
+                                 : pl.b_cols % 8 != 0 || reinterpret_cast<uintptr_t>(B) % 8 != 0;
   const double extra[3] = {1.2, 1.9, 2.9};  // of the aligned product's time
   const double saved_us = extra[op] * 2.0 * (double)T * (double)N * (double)K / 1.0e9;
   double copies_us = 0.0;
   if (pl.a) copies_us += 5.0 + 4.0 * (double)(pl.a_rows * pl.a_cols) / 4.0e6;
-  if (pl.b) copies_us += 5.0 + 4.0 * (double)(pl.b_rows * pl.b_cols) / 4.0e6;
+  if (pl.b) copies_us += 5.0 + 2.0 * b_value * (double)(pl.b_rows * pl.b_cols) / 4.0e6;
   if (saved_us <= copies_us) pl.a = pl.b = false;
-  if (pl.a) pl.a_bytes = 2 * (size_t)(pl.a_rows * round_up(pl.a_cols, 8));
-  if (pl.b) pl.b_bytes = 2 * (size_t)(pl.b_rows * round_up(pl.b_cols, 8));
+  if (pl.a) pl.a_bytes = (size_t)(2 * pl.a_rows * round_up(pl.a_cols, 8));
+  if (pl.b) pl.b_bytes = (size_t)(b_value * pl.b_rows * round_up(pl.b_cols, 8));
   return pl;
 }
 
@@ -618,7 +763,7 @@ int launch_half(int op, GroupedParams p, const HalfPlan& plan, const AlignPlan& 
                 hipStream_t st) {
   if (al.a) {
     const int64_t ld = round_up(al.a_cols, 8);
-    const int rc = launch_align<T>(p.A, al.a_rows, al.a_cols, ld, ws, st);
+    const int rc = launch_align<uint16_t>(p.A, al.a_rows, al.a_cols, ld, ws, st);
     if (rc != KAN_OK) return rc;
     p.A = ws;
     p.lda = ld;
@@ -626,7 +771,9 @@ int launch_half(int op, GroupedParams p, const HalfPlan& plan, const AlignPlan& 
   }
   if (al.b) {
     const int64_t ld = round_up(al.b_cols, 8);
-    const int rc = launch_align<T>(p.B, al.b_rows, al.b_cols, ld, ws, st);
+    const int rc = p.format == KAN_ACT8_NONE
+                       ? launch_align<uint16_t>(p.B, al.b_rows, al.b_cols, ld, ws, st)
+                       : launch_align<uint8_t>(p.B, al.b_rows, al.b_cols, ld, ws, st);
     if (rc != KAN_OK) return rc;
     p.B = ws;
     p.ldb = ld;
@@ -670,6 +817,10 @@ Workspace plan_call(int dtype, int op, int format, const void* A, const void* B,
   Workspace w{};
   w.plan = {kSmall, 1, kNoRuns};
   if (T * E * N * K == 0) return w;
+  if (takes_few(dtype, op, T, E)) {
+    w.plan.cfg = kFew;
+    return w;
+  }
   if (dtype == KAN_DTYPE_F32) {
     if (op == KAN_GROUPED_WEIGHT) w.plan.run = grouped_f32_run(T, E, N, K);
     else w.plan.cuts = grouped_f32_cuts(op, T, E, N, K);
@@ -753,6 +904,10 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   p.run = w.plan.run;
   p.cuts = w.plan.cuts;
   if (w.part_bytes > 0) p.part = reinterpret_cast<float*>(ws + w.rows_bytes);
+  if (w.plan.cfg == kFew)
+    return dtype == KAN_DTYPE_F32    ? launch_few<float>(p, st)
+           : dtype == KAN_DTYPE_BF16 ? launch_few<bf16>(p, st)
+                                     : launch_few<f16>(p, st);
   if (dtype == KAN_DTYPE_F32) {
     if (w.rows_bytes > 0) {
       const int e =

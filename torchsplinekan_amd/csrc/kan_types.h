@@ -50,6 +50,27 @@ __device__ __forceinline__ void store_f32(T* __restrict__ p, const float (&v)[V]
   else reinterpret_cast<LooseVec<T, V>*>(p)->v = u;
 }
 
+// 16 bytes from an address that is even only.  The hardware takes such a load,
+// several times slower than one of whole words: 5 words and a shift.  (Nothing
+// past the word of the last byte is read.)
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(4))) Words4 {
+  u32x4 v;
+};
+__device__ __forceinline__ u32x4 load16_even(const void* p) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+  const uint32_t shift = (uint32_t)(at & 2) * 8;
+  const u32x4 w = reinterpret_cast<const Words4*>(words)->v;
+  const uint32_t last = words[3 + (shift >> 4)];
+  u32x4 v;
+  v[0] = __builtin_amdgcn_alignbit(w[1], w[0], shift);
+  v[1] = __builtin_amdgcn_alignbit(w[2], w[1], shift);
+  v[2] = __builtin_amdgcn_alignbit(w[3], w[2], shift);
+  v[3] = __builtin_amdgcn_alignbit(last, w[3], shift);
+  return v;
+}
+
 // One value of an array whose type is known at run time (the short vectors of
 // weights, read once a row or less).
 __device__ __forceinline__ float load_any(const void* __restrict__ p, int64_t i, int dtype) {

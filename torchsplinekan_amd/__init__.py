@@ -8,6 +8,7 @@ same API, backed by ``torchsplinekan_amd._C`` (the replacement of
 from .kan_linear import KANLinear
 from .kan import KAN
 from .pruning import PruneResult, prune_nodes
+from .experts import KANExperts, KANExpertStack
 from .act8 import Activation8, checkpoint_8bit, quantize_activation
 from .grouped import grouped_linear
 from .residual import residual_norm
@@ -15,4 +16,5 @@ from .residual import residual_norm
 __version__ = "0.1.0"
 
 __all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "Activation8", "checkpoint_8bit",
-           "quantize_activation", "grouped_linear", "residual_norm", "__version__"]
+           "quantize_activation", "grouped_linear", "residual_norm", "KANExperts",
+           "KANExpertStack", "__version__"]

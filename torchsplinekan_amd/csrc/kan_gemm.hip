@@ -1024,16 +1024,70 @@ struct SplitLds {
   static constexpr int kBytes = EPIK == 0 || kStage + kSide < kBase ? kBase : kStage + kSide;
 };
 
-// One tile of a split product (lds: SplitLds<C, AK, BKC, EPIK>::kBytes).
-template <class C, bool AK, bool BKC, int EPIK>
-__device__ __forceinline__ void split_tile(const GemmParams<float>& p, const TileCoords& tc,
-                                           const DxParams& e, char* lds) {
+// A product grouped by expert as one of these kernels' parameters: a block
+// fills in its expert's operands (grouped_coords).
+template <int OP_>
+struct GroupedGemm : GemmParams<float> {
+  static constexpr int OP = OP_;
+  GroupedParams g;
+};
+
+// The block's tile (split -1: none) of rows grouped by expert (kan_grouped.h).
+template <class C, int OP>
+__device__ __forceinline__ TileCoords grouped_coords(GroupedGemm<OP>& p) {
+  const GroupedParams& g = p.g;
+  TileCoords tc{};
+  const int64_t weights = g.N * g.K;
+  if constexpr (OP == 2) {
+    WeightTile t;
+    if (!weight_tile(g, p.tiles_m, p.tiles_n, &t)) {
+      tc.split = -1;
+      return tc;
+    }
+    tc.m0 = (int64_t)t.tm * C::BM;
+    tc.n0 = (int64_t)t.tn * C::BN;
+    tc.kbeg = t.lo;
+    tc.kend = t.hi;
+    p.C = t.slot >= 0 ? g.part + t.slot * weights : p.C + t.e * weights;
+  } else {
+    RowTile t;
+    int tn;
+    if (!row_tile(g, C::BM, p.tiles_n, &t, &tn)) {
+      tc.split = -1;
+      return tc;
+    }
+    tc.m0 = t.m0;
+    tc.n0 = (int64_t)tn * C::BN;
+    tc.kend = t.e == g.E ? 0 : OP == 0 ? g.K : g.N;
+    cut_range(g, &tc.kbeg, &tc.kend);
+    p.M = t.m1;
+    p.B += t.e * weights;
+    if (g.cuts > 1) p.C = g.part + blockIdx.y * (g.T * p.N);
+  }
+  tc.nkt = (int)ceil_div(tc.kend - tc.kbeg, C::BK);
+  return tc;
+}
+
+template <class C, bool AK, bool BKC, int EPIK, class P = GemmParams<float>>
+__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+gemm_split_kernel(P p, DxParams e) {
   constexpr int BM = C::BM, BN = C::BN, NT = C::kThreads;
   constexpr int FM = C::FM, FN = C::FN;
   typedef SplitLoader<BM, AK, NT> LA;
   typedef SplitLoader<BN, BKC, NT> LB;
   typedef SplitLds<C, AK, BKC, EPIK> Lds;
   static_assert(C::BK == kSplitBK, "one MFMA deep");
+  __shared__ __align__(16) char lds[Lds::kBytes];
+
+  constexpr bool kGrouped = !std::is_same<P, GemmParams<float>>::value;
+  TileCoords tc;
+  if constexpr (kGrouped) {
+    tc = grouped_coords<C>(p);
+    if (tc.split < 0) return;
+    tc.split = 0;
+  } else {
+    tc = tile_coords<C>(p);
+  }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int wm = wave / C::WN, wn = wave % C::WN;
 
@@ -1221,54 +1275,6 @@ __device__ __forceinline__ void split_tile(const GemmParams<float>& p, const Til
     else
       ecomp_epilogue<C, -EPIK>(p, e, tc, acc, back, stage, side, kSide, wave, wm, wn, lane);
   }
-}
-
-template <class C, bool AK, bool BKC, int EPIK>
-__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-gemm_split_kernel(GemmParams<float> p, DxParams e) {
-  __shared__ __align__(16) char lds[SplitLds<C, AK, BKC, EPIK>::kBytes];
-  split_tile<C, AK, BKC, EPIK>(p, tile_coords<C>(p), e, lds);
-}
-
-// The same tiles over rows grouped by expert (kan_grouped.h): a block's tile of
-// its expert's product, as one product of that expert's operands.
-template <class C, int OP>
-__global__ __launch_bounds__(C::kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void
-grouped_split_kernel(GroupedParams g, int tiles_m, int tiles_n, int buf) {
-  constexpr bool AK = OP != 2, BKC = OP == 0;
-  __shared__ __align__(16) char lds[SplitLds<C, AK, BKC, 0>::kBytes];
-  GemmParams<float> p{};
-  TileCoords tc{};
-  p.A = static_cast<const float*>(g.A);
-  p.B = static_cast<const float*>(g.B);
-  p.lda = OP == 0 ? g.K : g.N;
-  p.ldb = g.K;
-  p.N = p.ldc = OP == 0 ? g.N : g.K;
-  p.buf = buf;
-  const int64_t weights = g.N * g.K;
-  if constexpr (OP == 2) {
-    WeightTile t;
-    if (!weight_tile(g, tiles_m, tiles_n, &t)) return;
-    tc.m0 = (int64_t)t.tm * C::BM;
-    tc.n0 = (int64_t)t.tn * C::BN;
-    tc.kbeg = t.lo;
-    tc.kend = t.hi;
-    p.M = g.N;
-    p.C = t.slot >= 0 ? g.part + t.slot * weights : static_cast<float*>(g.C) + t.e * weights;
-  } else {
-    RowTile t;
-    int tn;
-    if (!row_tile(g, C::BM, tiles_n, &t, &tn)) return;
-    tc.m0 = t.m0;
-    tc.n0 = (int64_t)tn * C::BN;
-    tc.kend = t.e == g.E ? 0 : OP == 0 ? g.K : g.N;
-    cut_range(g, &tc.kbeg, &tc.kend);
-    p.M = t.m1;
-    p.B += t.e * weights;
-    p.C = g.cuts > 1 ? g.part + blockIdx.y * (g.T * p.N) : static_cast<float*>(g.C);
-  }
-  tc.nkt = (int)ceil_div(tc.kend - tc.kbeg, C::BK);
-  split_tile<C, AK, BKC, 0>(p, tc, DxParams{}, lds);
 }
 
 template <class C, bool AK, bool BKC>
@@ -2217,9 +2223,21 @@ int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
   auto span_ok = [](bool kcont, int rows, int64_t ld) {
     return ((kcont ? rows * ld + C::BK : C::BK * ld + rows) * 4) < (int64_t)1 << 31;
   };
-  const int buf = span_ok(OP != 2, C::BM, lda) && span_ok(OP == 0, C::BN, p.K);
-  hipLaunchKernelGGL((grouped_split_kernel<C, OP>), dim3((unsigned)blocks, OP == 2 ? 1 : p.cuts),
-                     dim3(C::kThreads), 0, st, p, (int)tiles_m, (int)tiles_n, buf);
+  GroupedGemm<OP> q{};
+  q.A = static_cast<const float*>(p.A);
+  q.B = static_cast<const float*>(p.B);
+  q.C = static_cast<float*>(p.C);
+  q.M = p.N;  // (of the weight gradient; a row tile sets its own)
+  q.N = q.ldc = cols;
+  q.lda = lda;
+  q.ldb = p.K;
+  q.tiles_m = (int)tiles_m;
+  q.tiles_n = (int)tiles_n;
+  q.buf = span_ok(OP != 2, C::BM, lda) && span_ok(OP == 0, C::BN, p.K);
+  q.g = p;
+  hipLaunchKernelGGL((gemm_split_kernel<C, OP != 2, OP == 0, 0, GroupedGemm<OP>>),
+                     dim3((unsigned)blocks, OP == 2 ? 1 : p.cuts), dim3(C::kThreads), 0, st, q,
+                     DxParams{});
   return check_launch("grouped_matmul");
 }
 

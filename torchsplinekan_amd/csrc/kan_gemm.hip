@@ -2204,13 +2204,14 @@ inline unsigned flat_blocks(int64_t count) {
 }  // namespace
 
 namespace {
-// The large tile where its tiles fill the chip; the narrow one for up to 64
-// columns.  (Half of a group's last row tile is empty on average.)
-int grouped_cfg_f32(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
-  const int64_t cols = op == 0 ? N : K;
-  if (cols <= 64) return 2;
-  const int64_t tiles_m = op == 2 ? ceil_div(N, 256) * E : T / 256 + E / 2;
-  return tiles_m * ceil_div(cols, 256) >= device_cu_count() ? 0 : 1;
+// The 128 x 128 tile, whose smaller empty parts and finer rounds decide: forward
+// of 16384 rows over 8 experts of 1024 x 1024 242 us against 305 on 256 x 256,
+// 32768 over 16 of 2048 x 1024 836 against 850.  Weight gradients have no empty
+// rows: the large tile where groups are long and its tiles fill the chip (the
+// latter sizes 750 us against 797; 5000 rows over 16 of 1024 x 1024 118 against 79).
+bool grouped_takes_big(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+  return op == 2 && T >= 1024 * E &&
+         E * ceil_div(N, 256) * ceil_div(K, 256) >= device_cu_count();
 }
 
 template <class C, int OP>
@@ -2240,42 +2241,29 @@ int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
                      DxParams{});
   return check_launch("grouped_matmul");
 }
-
-template <class C>
-int launch_grouped_op(int op, const GroupedParams& p, hipStream_t st) {
-  if (op == 0) return launch_grouped_cfg<C, 0>(p, st);
-  if (op == 1) return launch_grouped_cfg<C, 1>(p, st);
-  return launch_grouped_cfg<C, 2>(p, st);
-}
 }  // namespace
 
-// (a tile's share of the engine's 220 TFLOP/s, 150 on the narrow tile)
+// (a tile's share of the engine's 220 TFLOP/s)
 int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K) {
   const int cus = device_cu_count();
-  switch (grouped_cfg_f32(2, T, E, N, K)) {
-    case 0:
-      return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 256), {cus, 0.15, 10.0});
-    case 1:
-      return weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.076, 5.0});
-    default:
-      return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 64), {2 * cus, 0.11, 5.0});
-  }
+  if (grouped_takes_big(2, T, E, N, K))
+    return weight_run(T, E, N, K, ceil_div(N, 256) * ceil_div(K, 256), {cus, 0.15, 10.0});
+  return weight_run(T, E, N, K, ceil_div(N, 128) * ceil_div(K, 128), {2 * cus, 0.076, 5.0});
 }
 
-// (16 k of a 128 x 128 or 256 x 64 tile alone take about 0.9 us)
+// (16 k of a 128 x 128 tile alone take about 0.9 us)
 int grouped_f32_cuts(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
-  const int cfg = grouped_cfg_f32(op, T, E, N, K);
-  if (cfg == 0) return 1;
   const int64_t cols = op == 0 ? N : K, depth = op == 0 ? K : N;
-  const double tiles = row_tiles(T, E, cfg == 1 ? 128 : 256) * (double)ceil_div(cols, cfg == 1 ? 128 : 64);
-  return sum_cuts(tiles, 2 * device_cu_count(), ceil_div(depth, 64), 3.6);
+  return sum_cuts(row_tiles(T, E, 128) * (double)ceil_div(cols, 128), 2 * device_cu_count(),
+                  ceil_div(depth, 64), 3.6);
 }
 
 int launch_grouped_f32(int op, const GroupedParams& p, hipStream_t st) {
-  const int cfg = grouped_cfg_f32(op, p.T, p.E, p.N, p.K);
-  const int rc = cfg == 0   ? launch_grouped_op<CfgF32Big>(op, p, st)
-                 : cfg == 1 ? launch_grouped_op<CfgF32Small>(op, p, st)
-                            : launch_grouped_op<CfgF32Narrow>(op, p, st);
+  const int rc = op == 0 ? launch_grouped_cfg<CfgF32Small, 0>(p, st)
+                 : op == 1 ? launch_grouped_cfg<CfgF32Small, 1>(p, st)
+                 : grouped_takes_big(op, p.T, p.E, p.N, p.K)
+                     ? launch_grouped_cfg<CfgF32Big, 2>(p, st)
+                     : launch_grouped_cfg<CfgF32Small, 2>(p, st);
   if (rc != KAN_OK) return rc;
   return op == 2 ? launch_grouped_sum<float>(p, st)
                  : launch_grouped_cuts<float>(p, op == 0 ? p.N : p.K, st);

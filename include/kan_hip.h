@@ -464,7 +464,8 @@ int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* s
  * Rows from offsets[E] on get zeros.  T < 2^30, N and K <= 2^22, E <= 65535.  The weight product also takes b as 8-bit
  * rows (b_format, with b_scale and b_group as kan_hip_act8_quantize keeps
  * them; KAN_ACT8_NONE otherwise).  The workspace depends on the operands'
- * alignment, so its query takes their addresses (which it does not read). */
+ * alignment, so its query takes their addresses (which it does not read); it
+ * lies on 16 bytes. */
 #define KAN_GROUPED_FORWARD 0
 #define KAN_GROUPED_INPUT 1
 #define KAN_GROUPED_WEIGHT 2

@@ -40,7 +40,7 @@ def _native(who: str):
     return _C._lib
 
 
-@dataclass
+@dataclass(eq=False)
 class Activation8:
     """A tensor in 8 bits: q (int8 or float8_e4m3fn, the tensor's shape), scale
     [..., ceil(C / group)] float32, and the type it had.  A group that held an

@@ -25,7 +25,8 @@ struct Act8Params {
   float* scale;     // [rows, parts]
   void* out;        // [rows, C]
   int64_t rows, C, parts;
-  int group, vec;   // vec: rows start on whole vectors
+  int group, vec;   // vec: rows are whole vectors, on their alignment
+  int flat;         // groups are whole and follow each other in memory
 };
 
 template <int FORMAT>
@@ -60,19 +61,31 @@ struct Act8<KAN_ACT8_E4M3> {
   }
 };
 
-// Row, group and first column of this lane (false past the last group).
+struct __attribute__((packed, aligned(1))) LooseBytes {
+  uint2 v;
+};
+
+// This lane's place (false past the last group).
 struct Lane {
-  int64_t row, part, c;
-  int n;  // its values, 0..8
+  int64_t x, q, scale;  // offsets of its values and of its group's scale
+  int n;                // its values, 0..8
 };
 __device__ __forceinline__ bool lane_place(const Act8Params& p, Lane* l) {
   const int lpg = p.group / kActVals;
   const int64_t t = (int64_t)blockIdx.x * (kActThreads / lpg) + threadIdx.x / lpg;
   if (t >= p.rows * p.parts) return false;
-  l->row = t / p.parts;
-  l->part = t - l->row * p.parts;
-  l->c = l->part * p.group + (threadIdx.x % lpg) * kActVals;
-  l->n = (int)max((int64_t)0, min((int64_t)kActVals, p.C - l->c));
+  const int in = (threadIdx.x % lpg) * kActVals;
+  l->scale = t;
+  if (p.flat) {
+    l->x = l->q = t * p.group + in;
+    l->n = kActVals;
+    return true;
+  }
+  const int64_t row = t < 0x80000000ll ? (int64_t)((uint32_t)t / (uint32_t)p.parts) : t / p.parts;
+  const int64_t c = (t - row * p.parts) * p.group + in;
+  l->x = row * p.ldx + c;
+  l->q = row * p.C + c;
+  l->n = (int)max((int64_t)0, min((int64_t)kActVals, p.C - c));
   return true;
 }
 
@@ -83,9 +96,10 @@ __global__ __launch_bounds__(kActThreads) void quantize_kernel(Act8Params p) {
   const bool in = lane_place(p, &l);
   float v[kActVals] = {};
   if (in) {
-    const T* src = static_cast<const T*>(p.x) + l.row * p.ldx + l.c;
-    if (p.vec && l.n == kActVals) {
-      load_f32<T, kActVals>(src, v);
+    const T* src = static_cast<const T*>(p.x) + l.x;
+    if (l.n == kActVals) {
+      if (p.vec) load_f32<T, kActVals>(src, v);
+      else load_f32<T, kActVals, false>(src, v);
     } else {
 #pragma unroll
       for (int j = 0; j < kActVals; ++j)
@@ -106,15 +120,16 @@ __global__ __launch_bounds__(kActThreads) void quantize_kernel(Act8Params p) {
 #pragma unroll
   for (int j = 0; j < kActVals; ++j) u[j] = inv == 0.0f ? 0.0f : v[j] * inv;
   const uint32_t lo = F::pack4(u), hi = F::pack4(u + 4);
-  uint8_t* dst = p.q + l.row * p.C + l.c;
-  if (p.vec && l.n == kActVals) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+  uint8_t* dst = p.q + l.q;
+  if (l.n == kActVals) {
+    if (p.vec) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    else reinterpret_cast<LooseBytes*>(dst)->v = make_uint2(lo, hi);
   } else {
 #pragma unroll
     for (int j = 0; j < kActVals; ++j)
       if (j < l.n) dst[j] = (uint8_t)((j < 4 ? lo : hi) >> (8 * (j & 3)));
   }
-  if (threadIdx.x % (p.group / kActVals) == 0) p.scale[l.row * p.parts + l.part] = scale;
+  if (threadIdx.x % (p.group / kActVals) == 0) p.scale[l.scale] = scale;
 }
 
 template <typename T, int FORMAT>
@@ -122,10 +137,11 @@ __global__ __launch_bounds__(kActThreads) void dequantize_kernel(Act8Params p) {
   typedef Act8<FORMAT> F;
   Lane l;
   if (!lane_place(p, &l)) return;
-  const uint8_t* src = p.q + l.row * p.C + l.c;
+  const uint8_t* src = p.q + l.q;
   uint32_t lo = 0, hi = 0;
-  if (p.vec && l.n == kActVals) {
-    const uint2 w = *reinterpret_cast<const uint2*>(src);
+  if (l.n == kActVals) {
+    const uint2 w = p.vec ? *reinterpret_cast<const uint2*>(src)
+                          : reinterpret_cast<const LooseBytes*>(src)->v;
     lo = w.x;
     hi = w.y;
   } else {
@@ -133,15 +149,16 @@ __global__ __launch_bounds__(kActThreads) void dequantize_kernel(Act8Params p) {
     for (int j = 0; j < kActVals; ++j)
       if (j < l.n) (j < 4 ? lo : hi) |= (uint32_t)src[j] << (8 * (j & 3));
   }
-  const float scale = p.scale[l.row * p.parts + l.part];
+  const float scale = p.scale[l.scale];
   float u[kActVals];
   F::unpack4(lo, u);
   F::unpack4(hi, u + 4);
 #pragma unroll
   for (int j = 0; j < kActVals; ++j) u[j] *= scale;
-  T* dst = static_cast<T*>(p.out) + l.row * p.C + l.c;
-  if (p.vec && l.n == kActVals) {
-    store_f32<T, kActVals>(dst, u);
+  T* dst = static_cast<T*>(p.out) + l.q;
+  if (l.n == kActVals) {
+    if (p.vec) store_f32<T, kActVals>(dst, u);
+    else store_f32<T, kActVals, false>(dst, u);
   } else {
 #pragma unroll
     for (int j = 0; j < kActVals; ++j)
@@ -183,6 +200,7 @@ int run_act8(const char* who, int dtype, int format, Act8Params p, bool quantize
   const uintptr_t at = reinterpret_cast<uintptr_t>(quantize ? p.x : p.out);
   p.vec = p.C % kActVals == 0 && (!quantize || p.ldx % kActVals == 0) &&
           at % (value < 16 ? value : 16) == 0 && reinterpret_cast<uintptr_t>(p.q) % 8 == 0;
+  p.flat = p.C % p.group == 0 && (!quantize || p.ldx == p.C || p.rows == 1);
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassOther, st,
                     (double)p.rows * (p.C * (1.0 + dtype_bytes(dtype)) + 4.0 * p.parts));

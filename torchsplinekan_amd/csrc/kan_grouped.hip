@@ -883,6 +883,8 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(KAN_ERR_WORKSPACE, "grouped_matmul: needs %zu bytes of workspace, got %zu",
                      need, workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+    return set_error(KAN_ERR_INVALID, "grouped_matmul: the workspace lies on 16 bytes");
   char* ws = static_cast<char*>(workspace);
   GroupedParams p{};
   p.A = a;

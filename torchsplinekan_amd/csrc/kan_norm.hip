@@ -301,17 +301,30 @@ struct Pieces {
   __device__ __forceinline__ static int64_t at(int i) {
     return (int64_t)(i * TPR + (int)threadIdx.x % TPR) * VEC;
   }
-  __device__ __forceinline__ static void load(float (&v)[NV][VEC], const T* __restrict__ row,
-                                              int64_t C) {
+  typedef typename VecOf<T, VEC>::type vec;
+  __device__ __forceinline__ static void fetch(vec (&v)[NV], const T* __restrict__ row, int64_t C) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       if (at(i) + VEC <= C) {
-        load_f32<T, VEC, WHOLE>(row + at(i), v[i]);
+        if constexpr (WHOLE) v[i] = *reinterpret_cast<const vec*>(row + at(i));
+        else v[i] = reinterpret_cast<const LooseVec<T, VEC>*>(row + at(i))->v;
       } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = !WHOLE && at(i) + j < C ? (float)row[at(i) + j] : 0.0f;
+        for (int j = 0; j < VEC; ++j) v[i][j] = !WHOLE && at(i) + j < C ? row[at(i) + j] : (T)0.0f;
       }
     }
+  }
+  __device__ __forceinline__ static void unpack(float (&v)[NV][VEC], const vec (&raw)[NV]) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = (float)raw[i][j];
+  }
+  __device__ __forceinline__ static void load(float (&v)[NV][VEC], const T* __restrict__ row,
+                                              int64_t C) {
+    vec raw[NV];
+    fetch(raw, row, C);
+    unpack(v, raw);
   }
   __device__ __forceinline__ static void store(const float (&v)[NV][VEC], T* __restrict__ row,
                                                int64_t C) {
@@ -431,9 +444,12 @@ __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __rest
 }
 
 // Four waves a SIMD (128 registers; a float32 row of 512 lanes with a gate would
-// spill there and takes two).  dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
-// sum serves both, and a weight's factor is applied after it, so a lane keeps
-// only pre and scale * post, and two sums (three with a gate row's).
+// spill there and takes two).  dpost = scale * (sum of D a yh) and dscale = post *
+// (the same sum): one column sum serves both, a weight's factor applied after
+// it.  A gate row's gradient comes from the sum of D yh, times scale, post and
+// a'(g), and what its rows add to the first sum is a(g) times the same: two sums
+// a row.  In 16 bits the next row's
+// loads are in flight while a row is worked on (but beside a gate's values).
 template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::kThreads) __attribute__((
     amdgpu_waves_per_eu(sizeof(TY) == 4 && TPR == 512 && GATE != 0 ? 2 : 4))) void
@@ -441,6 +457,7 @@ norm_grad_kernel(NormParams p) {
   typedef RowShape<TPR> S;
   typedef Pieces<TX, TPR, VEC, NV, WHOLE> PX;
   typedef Pieces<TY, TPR, VEC, NV, WHOLE> PY;
+  constexpr bool kAhead = sizeof(TX) == 2 && GATE != 1;
   constexpr int kCols = S::kRows > 1 ? NV * VEC * S::kThreads : 1;
   __shared__ float red[4 * S::kWaves];
   __shared__ float cols[kCols];
@@ -448,53 +465,88 @@ norm_grad_kernel(NormParams p) {
   const float inv_c = 1.0f / (float)p.C;
   const bool branch = p.y != nullptr, normed = p.post != nullptr, with_h = p.dh != nullptr;
   const bool one = GATE == 0 && p.gate_kind != kGateNone;
-  float a[NV][VEC], slope[NV][VEC];
-  float sp[NV][VEC], pre[NV][VEC];
+  float sp[NV][VEC], pre[NV][VEC];  // scale * post (a gate row: times a(g)); pre
   float s_pre[NV][VEC] = {}, s_branch[NV][VEC] = {}, s_gate[NV][VEC] = {};
-  if (branch) {
-    load_weight<TPR, WHOLE>(sp, p.post, p.wdtype, p.C, 1.0f);
-    load_weight<TPR, WHOLE>(pre, p.scale, p.wdtype, p.C, p.scale_const);
-    KAN_EACH sp[i][j] *= pre[i][j];
-  }
+  auto load_sp = [&](float (&v)[NV][VEC]) __attribute__((always_inline)) {
+    float t[NV][VEC];
+    load_weight<TPR, WHOLE>(v, p.post, p.wdtype, p.C, 1.0f);
+    load_weight<TPR, WHOLE>(t, p.scale, p.wdtype, p.C, p.scale_const);
+    KAN_EACH v[i][j] *= t[i][j];
+  };
+  if (branch && GATE != 2) load_sp(sp);
   if (with_h) load_weight<TPR, WHOLE>(pre, p.pre, p.wdtype, p.C, 1.0f);
+
+  const TX *xs = static_cast<const TX*>(p.x), *dxs = static_cast<const TX*>(p.dxo);
+  const TY *ys = static_cast<const TY*>(p.y), *dhs = static_cast<const TY*>(p.dh);
+  const TY* gs = static_cast<const TY*>(p.gate);
+  struct Row {  // as loaded
+    typename PX::vec d[NV], x[NV];
+    typename PY::vec y[NV], dh[NV];
+  };
+  auto fetch = [&](Row& r, int64_t row) __attribute__((always_inline)) {
+    if (p.dxo != nullptr) PX::fetch(r.d, dxs + row * p.C, p.C);
+    if (with_h) {
+      PX::fetch(r.x, xs + row * p.C, p.C);
+      PY::fetch(r.dh, dhs + row * p.C, p.C);
+    }
+    if (branch) PY::fetch(r.y, ys + row * p.C, p.C);
+  };
+
   const RowRange rr = row_range(p, blockIdx.x);
+  const int mine = threadIdx.x / TPR;
+  Row in;
   for (int64_t seg = rr.lo; seg < rr.hi;) {  // (one turn but for gate rows)
     const int64_t end = GATE == 2 ? min(rr.hi, (seg / p.L + 1) * p.L) : rr.hi;
     if constexpr (GATE == 2) {
+      float a[NV][VEC];
+      load_sp(sp);
       PY::load(a, static_cast<const TY*>(p.gate) + seg / p.L * p.C, p.C);
-      KAN_EACH act_both(a[i][j], p.act, &a[i][j], &slope[i][j]);
+      KAN_EACH sp[i][j] *= act_of(a[i][j], p.act);
     }
+    if (kAhead && seg + mine < end) fetch(in, seg + mine);
     for (int64_t r0 = seg; r0 < end; r0 += S::kRows) {
-      const int64_t row = r0 + threadIdx.x / TPR;
+      const int64_t row = r0 + mine;
       if (S::kRows > 1 && row >= end) break;
-      float d[NV][VEC], x[NV][VEC], y[NV][VEC], dh[NV][VEC];
-      float r1 = 1.0f, r2 = 0.0f, a1 = 1.0f, slope1 = 0.0f;
-      if (p.dxo != nullptr) PX::load(d, static_cast<const TX*>(p.dxo) + row * p.C, p.C);
-      else KAN_EACH d[i][j] = 0.0f;
-      if (with_h) {
-        PX::load(x, static_cast<const TX*>(p.x) + row * p.C, p.C);
-        PY::load(dh, static_cast<const TY*>(p.dh) + row * p.C, p.C);
-        r2 = p.rstd[p.n + row];
+      float d[NV][VEC], x[NV][VEC], y[NV][VEC], dh[NV][VEC], a[NV][VEC], slope[NV][VEC];
+      float a1 = 1.0f, slope1 = 0.0f, r1 = 1.0f, r2 = 0.0f;
+      if constexpr (kAhead) {
+        PX::unpack(d, in.d);
+        PX::unpack(x, in.x);
+        PY::unpack(y, in.y);
+        PY::unpack(dh, in.dh);
+      } else {
+        if (p.dxo != nullptr) PX::load(d, dxs + row * p.C, p.C);
+        if (with_h) {
+          PX::load(x, xs + row * p.C, p.C);
+          PY::load(dh, dhs + row * p.C, p.C);
+        }
+        if (branch) PY::load(y, ys + row * p.C, p.C);
       }
+      if (p.dxo == nullptr) KAN_EACH d[i][j] = 0.0f;
+      if (with_h) r2 = p.rstd[p.n + row];
       if (branch) {
-        PY::load(y, static_cast<const TY*>(p.y) + row * p.C, p.C);
         if (normed) r1 = p.rstd[row];
         if constexpr (GATE == 1) {
-          PY::load(a, static_cast<const TY*>(p.gate) + row * p.C, p.C);
+          PY::load(a, gs + row * p.C, p.C);
           KAN_EACH act_both(a[i][j], p.act, &a[i][j], &slope[i][j]);
-        } else if (one) {
-          act_both((float)static_cast<const TY*>(p.gate)[row / p.L], p.act, &a1, &slope1);
         }
+        if (one) act_both((float)gs[row / p.L], p.act, &a1, &slope1);
         KAN_EACH y[i][j] *= r1;  // yh (y itself without post)
       }
+      if (kAhead && row + S::kRows < end) fetch(in, row + S::kRows);
+      // a(g), and scale * post * a(g)
       auto gate_of = [&](int i, int j) __attribute__((always_inline)) {
-        if constexpr (GATE != 0) return a[i][j];
+        if constexpr (GATE == 1) return a[i][j];
         else return a1;
+      };
+      auto factor = [&](int i, int j) __attribute__((always_inline)) {
+        if constexpr (GATE == 2) return sp[i][j];
+        else return sp[i][j] * gate_of(i, j);
       };
       if (with_h) {
         float s[1] = {0.0f};
         KAN_EACH {
-          if (branch) x[i][j] += gate_of(i, j) * (y[i][j] * sp[i][j]);
+          if (branch) x[i][j] += y[i][j] * factor(i, j);
           x[i][j] *= r2;  // xh
           s_pre[i][j] += dh[i][j] * x[i][j];
           dh[i][j] *= pre[i][j];  // t
@@ -508,12 +560,12 @@ norm_grad_kernel(NormParams p) {
       if (!branch) continue;
       float s[2] = {0.0f, 0.0f};  // of w yh; of the gate's gradient
       KAN_EACH {
-        const float da = d[i][j] * gate_of(i, j);
-        s_branch[i][j] += da * y[i][j];
-        if constexpr (GATE == 0) s[1] += d[i][j] * y[i][j] * sp[i][j];
-        else if constexpr (GATE == 1) slope[i][j] *= d[i][j] * y[i][j] * sp[i][j];
-        else s_gate[i][j] += d[i][j] * y[i][j];
-        d[i][j] = da * sp[i][j];  // w
+        const float dy = d[i][j] * y[i][j];
+        if constexpr (GATE == 2) s_gate[i][j] += dy;
+        else s_branch[i][j] += dy * gate_of(i, j);
+        if constexpr (GATE == 0) s[1] += dy * sp[i][j];
+        if constexpr (GATE == 1) slope[i][j] *= dy * sp[i][j];
+        d[i][j] *= factor(i, j);  // w
         s[0] += d[i][j] * y[i][j];
       }
       if constexpr (GATE == 1) {
@@ -529,10 +581,19 @@ norm_grad_kernel(NormParams p) {
       KAN_EACH d[i][j] = r1 * (d[i][j] - y[i][j] * m1);
       PY::store(d, static_cast<TY*>(p.dy) + row * p.C, p.C);
     }
-    if (GATE == 2 && p.dgate != nullptr) {
-      const int64_t at = p.nchunk > 1 ? (int64_t)blockIdx.x : seg / p.L;
-      KAN_EACH s_gate[i][j] *= sp[i][j] * slope[i][j];
-      flush_columns<TPR, WHOLE>(s_gate, p.part_gate + at * p.C, p.C, cols);
+    if constexpr (GATE == 2) {
+      float a[NV][VEC], slope[NV][VEC];
+      load_sp(sp);
+      PY::load(a, static_cast<const TY*>(p.gate) + seg / p.L * p.C, p.C);
+      KAN_EACH {
+        act_both(a[i][j], p.act, &a[i][j], &slope[i][j]);
+        s_branch[i][j] += a[i][j] * s_gate[i][j];
+        s_gate[i][j] *= sp[i][j] * slope[i][j];
+      }
+      if (p.dgate != nullptr) {
+        const int64_t at = p.nchunk > 1 ? (int64_t)blockIdx.x : seg / p.L;
+        flush_columns<TPR, WHOLE>(s_gate, p.part_gate + at * p.C, p.C, cols);
+      }
       KAN_EACH s_gate[i][j] = 0.0f;
     }
     seg = end;

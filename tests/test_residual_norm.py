@@ -261,7 +261,7 @@ TYPES = [(F32, F32), (BF16, BF16), (F16, F16), (F32, BF16), (F32, F16)]
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("xdt,ydt", TYPES)
-@pytest.mark.parametrize("C", [1, 2, 7, 64, 301, 512, 1000, 1024, 1025, 2048, 4096, 4104, 8192,
+@pytest.mark.parametrize("C", [1, 2, 7, 64, 65, 120, 128, 301, 512, 1000, 1024, 1025, 2048, 4096, 4104, 8192,
                                8200, 16385])
 def test_widths(C, xdt, ydt):
     _run_case((5, C), xdt, ydt, (5, C), "sigmoid", True)

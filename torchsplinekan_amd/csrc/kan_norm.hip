@@ -251,14 +251,14 @@ __global__ __launch_bounds__(kRowThreads) void norm_rows_grad_kernel(NormParams 
 
 // ---- rows held in registers ---------------------------------------------------
 // TPR lanes share a row, each with 8 of its values in NV pieces of VEC; a block
-// is one row's lanes, or four waves with a row each, and runs through its rows,
-// the weights staying in registers.  Every value is read once: the
+// is one row's lanes, or four waves with a row (8 or 4 narrow ones) each, and
+// runs through its rows, the weights staying in registers.  Every value is read once: the
 // passes above happen on registers, a row's sums cross its waves through LDS.
 template <int TPR>
 struct RowShape {
-  static constexpr int kThreads = TPR == 64 ? 256 : TPR;
-  static constexpr int kRows = kThreads / TPR;  // rows at once
-  static constexpr int kWaves = TPR / 64;       // of a row
+  static constexpr int kThreads = TPR <= 64 ? 256 : TPR;
+  static constexpr int kRows = kThreads / TPR;          // rows at once
+  static constexpr int kWaves = TPR <= 64 ? 1 : TPR / 64;  // of a row
   static_assert(kRows == 1 || kWaves == 1, "rows side by side share no barrier");
 };
 
@@ -268,7 +268,10 @@ struct RowShape {
 template <int TPR, int M>
 __device__ __forceinline__ void row_sums(float (&v)[M], float* red, int& turn) {
 #pragma unroll
-  for (int m = 0; m < M; ++m) v[m] = wave_sum(v[m]);
+  for (int m = 0; m < M; ++m) {
+    if constexpr (TPR >= 64) v[m] = wave_sum(v[m]);
+    else v[m] = lane_sum<TPR>(v[m]);
+  }
   constexpr int W = RowShape<TPR>::kWaves;
   if constexpr (W > 1) {
     float* buf = red + turn * (2 * W) + 0;
@@ -671,6 +674,7 @@ constexpr int64_t kMaxGridY = 65535;
 constexpr int64_t kMaxHeld = 8192;
 int held_tpr(int64_t C) {
   if (C > kMaxHeld) return 256;
+  if (C <= 128) return C <= 64 ? 8 : 16;
   int tpr = 64;
   while (tpr * 8 < C) tpr *= 2;
   return tpr;
@@ -684,7 +688,7 @@ struct RowPlan {
 constexpr int kGradWaves = 16;  // waves a CU (one block of the widest shape)
 RowPlan row_plan(int64_t n, int64_t C, int kind, int64_t L, int waves_per_cu) {
   const int tpr = held_tpr(C);
-  const int threads = tpr == 64 ? 256 : tpr, at_once = threads / tpr;
+  const int threads = tpr <= 64 ? 256 : tpr, at_once = threads / tpr;
   const int64_t target = device_cu_count() * (int64_t)std::max(1, 64 * waves_per_cu / threads);
   RowPlan g{};
   const int64_t want = std::max<int64_t>(1, ceil_div(n, target));
@@ -744,6 +748,8 @@ int launch_held(NormParams p, int64_t grad_blocks, hipStream_t st) {
 template <typename TX, typename TY, int GATE, bool WHOLE>
 int launch_tpr(const NormParams& p, int64_t grad_blocks, hipStream_t st) {
   switch (held_tpr(p.C)) {
+    case 8: return launch_held<TX, TY, 8, GATE, WHOLE>(p, grad_blocks, st);
+    case 16: return launch_held<TX, TY, 16, GATE, WHOLE>(p, grad_blocks, st);
     case 64: return launch_held<TX, TY, 64, GATE, WHOLE>(p, grad_blocks, st);
     case 128: return launch_held<TX, TY, 128, GATE, WHOLE>(p, grad_blocks, st);
     case 256: return launch_held<TX, TY, 256, GATE, WHOLE>(p, grad_blocks, st);

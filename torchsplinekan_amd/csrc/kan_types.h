@@ -101,4 +101,15 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// Sum over aligned groups of 8 or 16 lanes, in each of them.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+  static_assert(LANES == 8 || LANES == 16, "groups within a row of 16 lanes");
+  v += dpp_or_zero<0xB1>(v);
+  v += dpp_or_zero<0x4E>(v);
+  v += dpp_or_zero<0x141>(v);
+  if constexpr (LANES == 16) v += dpp_or_zero<0x140>(v);
+  return v;
+}
+
 }  // namespace kan

@@ -101,6 +101,8 @@ __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __rest
   Pieces<float, TPR, VEC, NV, WHOLE>::store(v, out, C);
 }
 
+// Bound by HBM: 16384 x 4096 bf16 with a gate row for 2048 rows 178 us (805 MB
+// and 25 of partial sums, 4.6 TB/s); 32768 x 1024 float32 150 us, 5.4 TB/s.
 // Four waves a SIMD (128 registers; a float32 row of 512 lanes with a gate would
 // spill there and takes two).  dpost = scale * (sum of D a yh) and dscale = post *
 // (the same sum): one column sum serves both, a weight's factor applied after
@@ -262,7 +264,7 @@ norm_grad_kernel(NormParams p) {
 }
 
 // Column sums of partial rows in a fixed order: 16 lanes of rows a column,
-// their sums added in order.
+// their sums added in order.  (512 partial rows of 4096 columns, two sums: 6 us.)
 constexpr int kSumRowLanes = 16;
 __device__ __forceinline__ bool column_sum(const float* __restrict__ part, int64_t rows, int64_t C,
                                            int64_t* col, float* sum) {

@@ -172,6 +172,17 @@ def test_views(C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [2048, 2047])
+def test_values_past_32_bit_offsets(C):
+    x = torch.zeros(1100000, C, dtype=BF16, device="cuda")
+    x[-300:] = _values(300, C, BF16).cuda()
+    a, b = quantize_activation(x), quantize_activation(x[-300:].clone())
+    assert torch.equal(a.q[-300:], b.q) and torch.equal(a.scale[-300:], b.scale)
+    back = a.dequantize()
+    assert torch.equal(back[-300:], b.dequantize()) and not bool(back[:-300].any())
+
+
+@pytest.mark.gpu
 def test_special_groups_on_the_device():
     test_special_groups("int8")
     test_special_groups("e4m3")

@@ -305,6 +305,60 @@ def test_values_that_are_not_finite(K, N, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows", [40, 4000])
+def test_weights_past_32_bit_offsets(dtype, rows):
+    """2.3e9 weight values; the last expert has the rows."""
+    E, N, K = 70, 4096, 8064
+    w = torch.zeros(E, N, K, dtype=dtype, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w[-1] = (torch.randn(N, K, generator=g, device="cuda") * K ** -0.5).to(dtype)
+    x = torch.randn(rows, K, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(rows, N, generator=g, device="cuda").to(dtype)
+    off = _offsets([0] * (E - 1) + [rows]).cuda()
+    y = grouped_linear(x, w, off)
+    want = torch.mm(x.double(), w[-1].double().t())
+    assert float((y.double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype] + 1e-6
+    xg = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(grouped_linear(xg, w, off), xg, dy)
+    want = torch.mm(dy.double(), w[-1].double())
+    assert float((dx.double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype] + 1e-6
+    del w
+    wg = torch.empty(E, N, K, dtype=dtype, device="cuda").requires_grad_()
+    dw, = torch.autograd.grad(grouped_linear(x, wg, off), wg, dy)
+    want = torch.mm(dy.double().t(), x.double())
+    assert float((dw[-1].double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype] + 1e-6
+    assert not bool(dw[:-1].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_past_32_bit_offsets(dtype):
+    """Outputs and inputs of more than 2^31 values; the last rows are compared."""
+    T, E, K, N = 1100000, 2, 2048, 72
+    x = torch.zeros(T, K, dtype=dtype, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x[-500:] = torch.randn(500, K, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(E, N, K, generator=g, device="cuda") * K ** -0.5).to(dtype)
+    off = _offsets([T - 400, 400]).cuda()
+    y = grouped_linear(x, w, off)
+    want = torch.cat([torch.mm(x[-500:-400].double(), w[0].double().t()),
+                      torch.mm(x[-400:].double(), w[1].double().t())])
+    assert float((y[-500:].double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype] + 1e-6
+    assert not bool(y[:-500].any())
+    wt = w.transpose(1, 2).contiguous().requires_grad_()       # [E, 2048, 72]
+    z = torch.zeros(T, N, dtype=dtype, device="cuda")
+    z[-500:] = y[-500:]
+    out = grouped_linear(z, wt, off)                           # [T, 2048]
+    want = torch.mm(z[-400:].double(), wt[1].detach().double().t())
+    assert float((out[-400:].detach().double() - want).norm() / want.norm()) \
+        < 2 * HALF_ULP[dtype] + 1e-6
+    dw, = torch.autograd.grad(out, wt, x)
+    want = torch.mm(x[-400:].double().t(), z[-400:].double())
+    assert float((dw[1].double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype] + 1e-6
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_same_bits_every_time(dtype):
     x, w, dy = _inputs(2000, 9, 200, 264, dtype)

@@ -349,6 +349,28 @@ def test_values_that_are_not_finite_stay_in_their_row(C):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("C", [2048, 2047])
+def test_rows_past_32_bit_offsets(C):
+    """More than 2^31 values; the last rows against the same rows alone."""
+    n, last = 1100000, 300
+    g = torch.Generator(device="cuda").manual_seed(0)
+    parts = [torch.randn(last, C, generator=g, device="cuda").to(BF16) for _ in range(4)]
+    x, y, dn, dh = (torch.zeros(n, C, dtype=BF16, device="cuda") for _ in range(4))
+    for whole, part in zip((x, y, dn, dh), parts):
+        whole[-last:] = part
+    w = torch.ones(C, device="cuda", dtype=BF16)
+
+    def once(x, y, dn, dh):
+        x, y = x.requires_grad_(), y.requires_grad_()
+        new, h = residual_norm(x, y, post_weight=w, pre_weight=w)
+        return [new, h, *torch.autograd.grad([new, h], [x, y], [dn, dh])]
+
+    for u, v in zip(once(x, y, dn, dh), once(*parts)):
+        assert torch.equal(u[-last:], v)
+        assert not bool(u[:-last].any())
+
+
+@pytest.mark.gpu
 def test_same_bits_every_time_and_on_another_stream():
     t, dnew, dh = _make((4, 600, 520), BF16, BF16, (4, 1, 520), True)
     dev = {k: None if v is None else v.cuda().requires_grad_() for k, v in t.items()}

@@ -220,6 +220,33 @@ def test_kept_rows(K, N, group, format, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("T,E,K,N", [(12000, 2, 1032, 4104), (9000, 3, 1024, 5001),
+                                     (20001, 2, 1283, 520)])
+def test_kept_rows_of_long_products(T, E, K, N, format, dtype):
+    """Products that are long enough to restore their 8-bit rows in a pass of
+    their own, and ones that bring odd rows onto whole chunks."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(T, K, generator=g, device="cuda").to(dtype)
+    w = torch.zeros(E, N, K, dtype=dtype, device="cuda").requires_grad_()
+    dy = torch.randn(T, N, generator=g, device="cuda").to(dtype)
+    counts = _counts(T, E, seed=3)
+    y = grouped_linear(x, w, _offsets(counts).cuda(), checkpoint=format)
+    dw, = torch.autograd.grad(y, w, dy)
+    kept = quantize_activation(x, 128, format).dequantize(F32).double()
+    lo = 0
+    for e, c in enumerate(counts):
+        X, D = kept[lo:lo + c], dy[lo:lo + c].double()
+        want, mag = torch.mm(D.t(), X), torch.mm(D.abs().t(), X.abs())
+        tol = (c + 16) * 2.0 ** -24 * mag + HALF_ULP[dtype] * (want.abs() + mag) + 2.0 ** -25
+        assert bool(((dw[e].double() - want).abs() <= tol).all())
+        # (a value's rounding to 16 bits is independent of the next one's)
+        assert float((dw[e].double() - want).norm() / want.norm()) < 2 * HALF_ULP[dtype]
+        lo += c
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("offsets,ends", [
     ([0, 10, 30, 30], [10, 30, 30]),          # rows past the last group

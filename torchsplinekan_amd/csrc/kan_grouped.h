@@ -76,31 +76,20 @@ struct GroupScan {
   }
 };
 
-// Number of row tiles of all groups.
-__device__ __forceinline__ int count_tiles(const GroupedParams& p, int bm) {
-  GroupScan s;
-  for (int base = 0; base <= p.E; base += 64) s.step(p, base, bm);
-  return s.carry_tiles;
-}
-
 // Group (E: none) and rows [m0, m1) of a row tile.
 struct RowTile {
   int e, m0, m1;
 };
-__device__ __forceinline__ RowTile find_tile(const GroupedParams& p, int tile, int bm) {
-  GroupScan s;
-  RowTile r{p.E, 0, 0};
-  for (int base = 0; base <= p.E; base += 64) {
-    s.step(p, base, bm);
-    if (tile >= s.carry_tiles) continue;
-    const int l = __builtin_ctzll(__ballot(tile < s.last));
-    r.e = base + l;
-    const int before = __builtin_amdgcn_readlane(s.last - s.tiles, l);
-    r.m0 = __builtin_amdgcn_readlane(s.begin, l) + (tile - before) * bm;
-    r.m1 = min(__builtin_amdgcn_readlane(s.end, l), r.m0 + bm);
-    break;
-  }
-  return r;
+// The tile from the scan of its 64 groups from `base` on (false: not one of them).
+__device__ __forceinline__ bool take_tile(const GroupScan& s, int base, int tile, int bm,
+                                          RowTile* r) {
+  if (tile >= s.carry_tiles) return false;
+  const int l = __builtin_ctzll(__ballot(tile < s.last));
+  const int before = __builtin_amdgcn_readlane(s.last - s.tiles, l);
+  r->e = base + l;
+  r->m0 = __builtin_amdgcn_readlane(s.begin, l) + (tile - before) * bm;
+  r->m1 = min(__builtin_amdgcn_readlane(s.end, l), r->m0 + bm);
+  return true;
 }
 
 // Rows [begin, end) of group e.
@@ -277,13 +266,21 @@ int launch_grouped_sum(const GroupedParams& p, hipStream_t st) {
 constexpr int kGroupedM = 8;
 __device__ __forceinline__ bool row_tile(const GroupedParams& p, int bm, int tiles_n, RowTile* t,
                                          int* tn) {
-  const int tiles_m = count_tiles(p, bm), total = tiles_m * tiles_n;
+  GroupScan s;  // the number of row tiles first
+  for (int base = 0; base <= p.E; base += 64) s.step(p, base, bm);
+  const int tiles_m = s.carry_tiles, total = tiles_m * tiles_n;
   if ((int)blockIdx.x >= total) return false;
   const int id = xcd_remap(blockIdx.x, total), group = kGroupedM * tiles_n;
   const int first = id / group * kGroupedM, in = id % group;
   const int gm = min(tiles_m - first, kGroupedM);
   *tn = __builtin_amdgcn_readfirstlane(in / gm);
-  *t = find_tile(p, __builtin_amdgcn_readfirstlane(first + in % gm), bm);
+  const int tile = __builtin_amdgcn_readfirstlane(first + in % gm);
+  if (p.E < 64) return take_tile(s, 0, tile, bm, t);  // (one scan has them all)
+  GroupScan again;
+  for (int base = 0; base <= p.E; base += 64) {
+    again.step(p, base, bm);
+    if (take_tile(again, base, tile, bm, t)) break;
+  }
   return true;
 }
 inline int64_t row_grid(const GroupedParams& p, int64_t bm, int64_t tiles_n) {

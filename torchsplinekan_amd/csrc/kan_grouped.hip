@@ -814,11 +814,22 @@ int check_grouped(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K)
   return KAN_OK;
 }
 
+// Whether a weight gradient in 16 bits restores its 8-bit rows once, in a pass of
+// their own, rather than in every tile that reads them: the tiles then run as on
+// 16-bit rows, about a fifth faster (16384 rows, 8 experts of 4096 x 4096: 605 us
+// from int8, 501 from bf16 and 32 for the pass), which pays from some 1800
+// outputs on.  The rows' 16-bit copy lives for the call only.
+bool restores_first(int64_t T, int64_t N, int64_t K) {
+  const double saved_us = 0.2 * 2.0 * (double)T * (double)N * (double)K / 1.05e9;
+  return K % 8 == 0 && saved_us > 5.0 + 3.0 * (double)(T * K) / 4.5e6;
+}
+
 // A call's workspace: rows brought onto 16 bytes (16-bit types) or restored from
-// 8 bits (fp32, whose engine takes floats), then the partial sums.
+// 8 bits (always in fp32, whose engine takes floats), then the partial sums.
 struct Workspace {
   HalfPlan plan;
   AlignPlan align;
+  bool restore;
   size_t rows_bytes, part_bytes;  // (part from a multiple of 16 bytes on)
 };
 Workspace plan_call(int dtype, int op, int format, const void* A, const void* B, int64_t T,
@@ -833,11 +844,15 @@ Workspace plan_call(int dtype, int op, int format, const void* A, const void* B,
   if (dtype == KAN_DTYPE_F32) {
     if (op == KAN_GROUPED_WEIGHT) w.plan.run = grouped_f32_run(T, E, N, K);
     else w.plan.cuts = grouped_f32_cuts(op, T, E, N, K);
-    if (format != KAN_ACT8_NONE) w.rows_bytes = 4 * (size_t)(T * K);
+    w.restore = format != KAN_ACT8_NONE;
+    if (w.restore) w.rows_bytes = 4 * (size_t)(T * K);
   } else {
     w.plan = half_plan(op, T, E, N, K);
-    w.align = align_plan(op, format, A, B, T, E, N, K);
-    w.rows_bytes = w.align.a_bytes + w.align.b_bytes;
+    w.restore = format != KAN_ACT8_NONE && restores_first(T, N, K);
+    // (restored rows lie on 16 bytes; those of A come behind them)
+    if (w.restore) w.rows_bytes = (size_t)round_up(2 * T * K, 16);
+    w.align = align_plan(op, format, A, w.restore ? nullptr : B, T, E, N, K);
+    w.rows_bytes += w.align.a_bytes + w.align.b_bytes;
   }
   w.rows_bytes = (size_t)round_up((int64_t)w.rows_bytes, 16);
   if (op == KAN_GROUPED_WEIGHT) w.part_bytes = 4 * (size_t)weight_part_elems(T, E, N, K, w.plan.run);
@@ -919,15 +934,14 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
     return dtype == KAN_DTYPE_F32    ? launch_few<float>(p, st)
            : dtype == KAN_DTYPE_BF16 ? launch_few<bf16>(p, st)
                                      : launch_few<f16>(p, st);
-  if (dtype == KAN_DTYPE_F32) {
-    if (w.rows_bytes > 0) {
-      const int e =
-          kan_hip_act8_dequantize(dtype, b_format, b, b_scale, T, K, b_group, ws, stream);
-      if (e != KAN_OK) return e;
-      p.B = ws;
-    }
-    return launch_grouped_f32(op, p, st);
+  if (w.restore) {
+    const int e = kan_hip_act8_dequantize(dtype, b_format, b, b_scale, T, K, b_group, ws, stream);
+    if (e != KAN_OK) return e;
+    p.B = ws;
+    p.format = KAN_ACT8_NONE;
+    ws += round_up((int64_t)dtype_bytes(dtype) * T * K, 16);
   }
+  if (dtype == KAN_DTYPE_F32) return launch_grouped_f32(op, p, st);
   return dtype == KAN_DTYPE_BF16 ? launch_half<bf16>(op, p, w.plan, w.align, ws, st)
                                  : launch_half<f16>(op, p, w.plan, w.align, ws, st);
 }

@@ -247,6 +247,32 @@ def test_kept_rows_of_long_products(T, E, K, N, format, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("T,E,K,N", [(200, 3, 96, 72), (200, 3, 77, 65), (12000, 2, 1032, 4104)])
+def test_kept_rows_at_the_end_of_the_range(T, E, K, N, format):
+    """Groups that hold bfloat16's largest values, whose scale times 128 is above
+    float32's: restored on their way into the tiles, and in a pass of their own.
+    (Bounds of test_kept_rows_of_long_products; dy's are 2^-110 of unit size.)"""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(T, K, generator=g, device="cuda").to(BF16)
+    top = torch.finfo(BF16).max
+    x[3, 0], x[3, 1], x[T - 2, K - 1] = top, -top, -top
+    w = torch.zeros(E, N, K, dtype=BF16, device="cuda").requires_grad_()
+    dy = (torch.randn(T, N, generator=g, device="cuda") * 2.0 ** -110).to(BF16)
+    counts = _counts(T, E, seed=3)
+    y = grouped_linear(x, w, _offsets(counts).cuda(), checkpoint=format, group=32)
+    dw, = torch.autograd.grad(y, w, dy)
+    kept = quantize_activation(x, 32, format).dequantize(F32).double()
+    lo = 0
+    for e, c in enumerate(counts):
+        X, D = kept[lo:lo + c], dy[lo:lo + c].double()
+        want, mag = torch.mm(D.t(), X), torch.mm(D.abs().t(), X.abs())
+        tol = (c + 16) * 2.0 ** -24 * mag + HALF_ULP[BF16] * (want.abs() + mag)
+        assert bool(((dw[e].double() - want).abs() <= tol).all())
+        lo += c
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("offsets,ends", [
     ([0, 10, 30, 30], [10, 30, 30]),          # rows past the last group

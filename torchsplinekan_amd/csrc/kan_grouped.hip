@@ -216,17 +216,13 @@ struct Operand {
       *reinterpret_cast<u32x4*>(lds + (p * NT + threadIdx.x) * 16) = v;
     }
   }
-  // 8 values q * scale rounded to T.  (int8: the bytes plus 128 convert in one
-  // operation each; (q + 128) s - 128 s in one rounding is q s.)
+  // 8 values q * scale rounded to T.  (int8: no detour over q + 128, whose product
+  // with a scale above FLT_MAX / 128 is infinite.)
   __device__ __forceinline__ static u32x4 restore(u32x4 q, float s) {
     typename Half<T>::frag f;
     if constexpr (MODE == kInt8) {
-      const float back = -128.0f * s;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t w = q[j >> 2] ^ 0x80808080u;
-        f[j] = (T)__builtin_fmaf((float)(uint8_t)(w >> (8 * (j & 3))), s, back);
-      }
+      for (int j = 0; j < 8; ++j) f[j] = (T)((float)(int8_t)(q[j >> 2] >> (8 * (j & 3))) * s);
     } else {
       typedef float f32x2 __attribute__((ext_vector_type(2)));
 #pragma unroll

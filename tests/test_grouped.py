@@ -426,6 +426,22 @@ def test_same_bits_every_time(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("leaf", [0, 1])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_forward_mode_is_refused(leaf, checkpoint):
+    from torch.autograd import forward_ad
+    x, w, _ = _inputs(9, 2, 32, 5, F32)
+    args, off = [x.cuda(), w.cuda()], _offsets([4, 5]).cuda()
+    want = grouped_linear(*args, off)
+    with forward_ad.dual_level():
+        got = grouped_linear(*args, off, checkpoint=checkpoint)
+        assert torch.equal(got, want) and not got.requires_grad
+        args[leaf] = forward_ad.make_dual(args[leaf], torch.ones_like(args[leaf]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            grouped_linear(*args, off, checkpoint=checkpoint)
+
+
+@pytest.mark.gpu
 def test_float64_and_other_devices_are_refused():
     x = torch.zeros(2, 4, dtype=torch.float64, device="cuda")
     off = _offsets([2]).cuda()

@@ -399,6 +399,25 @@ def test_float64_is_refused_on_the_device():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("leaf", NAMES)
+def test_forward_mode_is_refused(leaf):
+    """A dual tensor raises, with and without gradients; other tensors inside a
+    level give what they give outside."""
+    from torch.autograd import forward_ad
+    t, _, _ = _make((6, 40), F32, F32, (6, 1), True)
+    dev = {k: v.cuda() for k, v in t.items()}
+    new, h = _call(dev, "silu", None)
+    with forward_ad.dual_level():
+        for u, v in zip(_call(dev, "silu", None), (new, h)):
+            assert torch.equal(u, v) and not u.requires_grad
+        dev[leaf] = forward_ad.make_dual(dev[leaf], torch.ones_like(dev[leaf]))
+        with pytest.raises(RuntimeError, match="jvp"):
+            _call(dev, "silu", None)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="jvp"):
+            _call(dev, "silu", None)
+
+
+@pytest.mark.gpu
 def test_second_derivatives_are_refused():
     x = torch.randn(2, 8, device="cuda", requires_grad=True)
     w = torch.ones(8, device="cuda", requires_grad=True)

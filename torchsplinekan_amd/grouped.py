@@ -8,6 +8,7 @@ import ctypes
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -130,8 +131,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     never below the one before.)
     checkpoint "int8" or "e4m3": the weight's gradient reads x from 8 bits
     (groups of `group` values, quantize_activation) and x itself is not kept.
-    Sums are held in float32.  Gradients (first order) reach x and weight;
-    sums over rows have a fixed order."""
+    Sums are held in float32.  Gradients (first order) reach x and weight
+    (device tensors refuse forward mode); sums over rows have a fixed order."""
     _req(x.dim() == 2 and weight.dim() == 3, "x must be [T, K] and weight [E, N, K], got ",
          list(x.shape), " and ", list(weight.shape))
     _req(weight.shape[2] == x.shape[1], "weight.size(2)=", weight.shape[2], " must equal K=",
@@ -149,6 +150,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
         return _composite(x, weight, offsets, checkpoint, group)
     _native().operator_dtype_code(x.dtype, "grouped_linear")
     x, weight, offsets = x.contiguous(), weight.contiguous(), offsets.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+            or _forward_ad._current_level >= 0):  # (apply refuses forward-mode derivatives)
         return _GroupedLinear.apply(x, weight, offsets, checkpoint, group)
     return _GroupedLinear.forward(None, x, weight, offsets, None, group)

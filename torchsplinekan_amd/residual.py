@@ -13,6 +13,7 @@ import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -131,7 +132,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *,
     scale: residual scale, [C] or a number.
     dtype: type of h without y (default: x's).
     post_weight, pre_weight and a scale tensor share a type.  First-order
-    gradients reach every tensor; x' is not kept for them (the backward
+    gradients reach every tensor (device tensors refuse forward mode); x' is not kept for them (the backward
     evaluates it again from x and y)."""
     _req(x.dim() >= 1, "x must have at least one dimension")
     shape, C, device = x.shape, x.shape[-1], x.device
@@ -196,7 +197,7 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *,
                for t in (x, y, gate, post_weight, pre_weight, scale_t)]
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
     args = (gate_rows, scale_const, GATE_ACTS[gate_act], float(eps), dtype, wdtype, save)
-    if save:
+    if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
         new, h = _ResidualNorm.apply(*tensors, *args)
     else:
         new, h = _ResidualNorm.forward(None, *tensors, *args)

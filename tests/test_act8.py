@@ -125,6 +125,49 @@ def test_checkpoint_other_calls():
     torch.testing.assert_close(gx, (2 * w).expand(3, 24).detach())
 
 
+@pytest.mark.parametrize("around", ["both", "forward", "backward"])
+def test_checkpoint_keeps_the_forward_pass_autocast(around):
+    """Gradients are those of the layer at the restored input under the forward
+    pass's autocast, whatever surrounds the backward pass."""
+    net, x = _net(), _values(9, 24, F32).requires_grad_()
+    inputs = [x, *net.parameters()]
+    g = torch.randn(9, 8)
+
+    def cast(on):
+        return torch.autocast("cpu", dtype=BF16, enabled=on)
+
+    xr = quantize_activation(x, 32).dequantize().requires_grad_()
+    with cast(around != "backward"):
+        plain, want = net(x), net(xr)
+    with cast(around != "backward"):
+        y = checkpoint_8bit(net, x, group=32)
+    assert y.dtype == (F32 if around == "backward" else BF16) and torch.equal(y, plain)
+    with cast(around != "forward"):  # (which the products of both backward passes see)
+        want = torch.autograd.grad(want, [xr, *net.parameters()], g.to(y.dtype))
+        got = torch.autograd.grad(y, inputs, g.to(y.dtype))
+    for u, v in zip(got, want):
+        assert u.dtype == v.dtype and torch.equal(u, v)
+
+
+def test_checkpoint_leaves_autocast_of_other_calls():
+    """The layer used beside its checkpoint, in one autocast region, keeps its
+    gradients (casts of weights made without gradients are not kept for it)."""
+    net, x = _net(), _values(9, 24, F32)
+    with torch.autocast("cpu", dtype=BF16):
+        first = checkpoint_8bit(net, x, group=32)
+        beside = net(x)
+        got = torch.autograd.grad(beside.float().sum() + first.float().sum(),
+                                  list(net.parameters()))
+    for v in got:
+        assert bool(v.any())
+    with torch.autocast("cpu", dtype=BF16):
+        a = torch.autograd.grad(net(x).float().sum(), list(net.parameters()))
+        xr = quantize_activation(x, 32).dequantize()
+        b = torch.autograd.grad(net(xr).float().sum(), list(net.parameters()))
+    for v, u, w in zip(got, a, b):
+        assert torch.equal(v, u + w)
+
+
 # ---------------------------------------------------------------------------
 # GPU
 # ---------------------------------------------------------------------------

@@ -9,6 +9,7 @@ Device tensors run on the kernels of csrc/kan_act8.hip, CPU tensors on the same
 formulas in torch.
 """
 
+from contextlib import ExitStack
 from dataclasses import dataclass
 from typing import Callable, Optional, Sequence
 
@@ -121,20 +122,38 @@ def quantize_activation(x: torch.Tensor, group: int = 128, format: str = "int8")
     return Activation8(q, scale, group, format, x.dtype)
 
 
+def _autocast_of(device_type: str):
+    """(device type, enabled, type) of autocast on device_type and the CPU."""
+    return [(t, torch.is_autocast_enabled(t), torch.get_autocast_dtype(t))
+            for t in {device_type, "cpu"}]
+
+
+def _autocast(state) -> ExitStack:
+    """Autocast as in `state`.  Casts of weights are not kept where it is on: those of
+    a pass without gradients would serve calls beside it, which then lost theirs."""
+    stack = ExitStack()
+    for device_type, on, dtype in state:
+        if on or torch.is_autocast_enabled(device_type):
+            stack.enter_context(torch.autocast(device_type, dtype=dtype, enabled=on,
+                                               cache_enabled=False))
+    return stack
+
+
 class _Checkpoint8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, fn, args, group, format, x, *params):
         ctx.fn, ctx.args = fn, args
         ctx.kept = quantize_activation(x, group, format)
         ctx.params = params
-        with torch.no_grad():
+        ctx.autocast = _autocast_of(x.device.type)
+        with torch.no_grad(), _autocast(ctx.autocast):
             return fn(x, *args)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
         x = ctx.kept.dequantize().requires_grad_(ctx.needs_input_grad[4])
-        with torch.enable_grad():
+        with torch.enable_grad(), _autocast(ctx.autocast):
             out = ctx.fn(x, *ctx.args)
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
         pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
@@ -149,10 +168,11 @@ class _Checkpoint8(torch.autograd.Function):
 def checkpoint_8bit(fn: Callable, x: torch.Tensor, *args, group: int = 128, format: str = "int8",
                     params: Optional[Sequence[torch.Tensor]] = None):
     """fn(x, *args), keeping x in 8 bits for the backward pass and nothing that
-    fn makes: the backward restores x and runs fn again, so gradients are those
-    of fn at the restored x (the output is exact).  Gradients reach x and
-    `params` (default: fn.parameters() of a module; args are taken as
-    constants).  fn must give the same result each time: no random numbers."""
+    fn makes: the backward restores x and runs fn again, under the call's
+    autocast, so gradients are those of fn at the restored x (the output is
+    exact).  Gradients reach x and `params` (default: fn.parameters() of a
+    module; args are taken as constants).  fn must give the same result each
+    time: no random numbers."""
     check_format("checkpoint_8bit", group, format)
     if params is None:
         params = tuple(fn.parameters()) if isinstance(fn, nn.Module) else ()

@@ -98,6 +98,17 @@ def test_cpu_checkpoint():
     torch.testing.assert_close(dx[4:], dy[4:] @ w[1])
 
 
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_cpu_sums_under_autocast(checkpoint):
+    """Products in float32, as on the device."""
+    x, w, _ = _inputs(9, 2, 40, 5, F32)
+    off = _offsets([4, 5])
+    want = grouped_linear(x, w, off, checkpoint=checkpoint)
+    with torch.autocast("cpu", dtype=BF16):
+        got = grouped_linear(x, w, off, checkpoint=checkpoint)
+    assert got.dtype == F32 and torch.equal(got, want)
+
+
 @pytest.mark.parametrize("x,w,off,kw,text", [
     (torch.zeros(4), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32), {}, "must be"),
     (torch.zeros(4, 5), torch.zeros(2, 3, 4), torch.zeros(3, dtype=torch.int32), {}, "equal K"),

@@ -108,14 +108,15 @@ def _composite(x, weight, offsets, checkpoint, group):
     T, E = x.shape[0], weight.shape[0]
     parts, lo = [], 0
     ends = [min(max(int(v), 0), T) for v in offsets.tolist()[1:]]
-    for e in range(E):
-        hi = max(lo, ends[e])
-        xe, we = x[lo:hi].to(wide), weight[e].to(wide)
-        if checkpoint is None:
-            parts.append(xe @ we.t())
-        else:
-            parts.append(_KeptRows.apply(xe, we, group, checkpoint))
-        lo = hi
+    with torch.autocast(x.device.type, enabled=False):  # (whose products would be narrower)
+        for e in range(E):
+            hi = max(lo, ends[e])
+            xe, we = x[lo:hi].to(wide), weight[e].to(wide)
+            if checkpoint is None:
+                parts.append(xe @ we.t())
+            else:
+                parts.append(_KeptRows.apply(xe, we, group, checkpoint))
+            lo = hi
     parts.append(x.new_zeros(T - lo, weight.shape[1], dtype=wide))
     return torch.cat(parts).to(x.dtype)
 
@@ -131,8 +132,9 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     never below the one before.)
     checkpoint "int8" or "e4m3": the weight's gradient reads x from 8 bits
     (groups of `group` values, quantize_activation) and x itself is not kept.
-    Sums are held in float32.  Gradients (first order) reach x and weight
-    (device tensors refuse forward mode); sums over rows have a fixed order."""
+    Sums are held in float32, also under autocast, which casts nothing here.
+    Gradients (first order) reach x and weight (device tensors refuse forward
+    mode); sums over rows have a fixed order."""
     _req(x.dim() == 2 and weight.dim() == 3, "x must be [T, K] and weight [E, N, K], got ",
          list(x.shape), " and ", list(weight.shape))
     _req(weight.shape[2] == x.shape[1], "weight.size(2)=", weight.shape[2], " must equal K=",

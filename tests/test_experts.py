@@ -82,6 +82,26 @@ def test_stack_trains_on_the_cpu():
     assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in net.parameters())
 
 
+def _same_under_autocast(net, x):
+    """Output and gradients bit for bit those outside autocast."""
+    g = torch.randn(x.shape[:-1] + (x.shape[-1],), device=x.device)
+    want, wgrads = _grads(net, x, g)
+    with torch.autocast(x.device.type, dtype=torch.bfloat16):
+        got = net(x)
+    assert got.dtype == torch.float32 and torch.equal(got, want)
+    for u, v in zip(torch.autograd.grad(got, [x, *net.parameters()], g), wgrads):
+        assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("form", [None, "int8"])
+def test_autocast_changes_nothing(form):
+    torch.manual_seed(2)
+    net = KANExpertStack(12, 2, 4, top_k=2, checkpoint=form, group=32)
+    _same_under_autocast(net, torch.randn(40, 12).requires_grad_())
+    _same_under_autocast(KANExperts(12, 12, 3, checkpoint=form),
+                         torch.randn(40, 12).requires_grad_())
+
+
 def test_refusals():
     with pytest.raises(ValueError, match="top_k"):
         KANExperts(4, 4, 2, top_k=3)
@@ -123,6 +143,14 @@ def test_stack_on_the_device_against_float64(width, depth, experts, top_k, rows)
     for u, v in zip([got, *grads], [want, *wgrads]):
         assert float((u.detach().cpu().double() - v.detach()).norm()) < 1e-4 * max(
             1e-12, float(v.detach().norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", [None, "int8"])
+def test_autocast_changes_nothing_on_the_device(form):
+    torch.manual_seed(2)
+    net = KANExpertStack(48, 2, 4, top_k=2, checkpoint=form).cuda()
+    _same_under_autocast(net, torch.randn(200, 48, device="cuda").requires_grad_())
 
 
 @pytest.mark.gpu

@@ -46,8 +46,8 @@ class KANExperts(nn.Module):
     Parameters: router [E, I], base_weight [E, O, I], spline_weight
     [E, O, I, R] (R = grid_size + spline_order); buffer grid [I, G + 2k + 1].
     checkpoint: None, "int8" or "e4m3" (with `group` values a scale): what the
-    backward pass keeps of the routed rows.  First-order gradients only; device
-    inputs are float32."""
+    backward pass keeps of the routed rows (in float32 only).  First-order
+    gradients only; device inputs are float32, and autocast changes nothing."""
 
     def __init__(self, in_features: int, out_features: int, num_experts: int, top_k: int = 2,
                  grid_size: int = 5, spline_order: int = 3, scale_noise: float = 0.1,
@@ -91,6 +91,10 @@ class KANExperts(nn.Module):
                                   offsets)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        with torch.autocast(x.device.type, enabled=False):
+            return self._forward(x)
+
+    def _forward(self, x: torch.Tensor) -> torch.Tensor:
         lead, I, k = x.shape[:-1], self.in_features, self.top_k
         xf = x.reshape(-1, I)
         weights, order, offsets = route(F.linear(xf, self.router), k)
@@ -136,6 +140,10 @@ class KANExpertStack(nn.Module):
         self.eps = eps
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        with torch.autocast(x.device.type, enabled=False):
+            return self._forward(x)
+
+    def _forward(self, x: torch.Tensor) -> torch.Tensor:
         x, h = residual_norm(x, pre_weight=self.blocks[0].pre_weight, eps=self.eps)
         for block, after in zip(self.blocks, [*self.blocks[1:], None]):
             x, h = residual_norm(

@@ -7,6 +7,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+from _saved import check_kept_is_saved
 from torchsplinekan_amd import KANLinear, checkpoint_8bit, quantize_activation
 from torchsplinekan_amd.act8 import FORMATS, GROUPS
 
@@ -166,6 +167,19 @@ def test_checkpoint_leaves_autocast_of_other_calls():
         b = torch.autograd.grad(net(xr).float().sum(), list(net.parameters()))
     for v, u, w in zip(got, a, b):
         assert torch.equal(v, u + w)
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+def test_checkpoint_saves_what_it_keeps(format):
+    net, x, shift = _net(), _values(9, 24, F32).requires_grad_(), torch.zeros(8)
+    params = list(net.parameters())
+    check_kept_is_saved(
+        lambda: checkpoint_8bit(lambda v, s: net(v) + s, x, shift, format=format, params=params),
+        [x, *params], torch.randn(9, 8), in_place=[params[0], params[3], shift])
+    with pytest.raises(RuntimeError, match="second time"):
+        y = checkpoint_8bit(net, x)
+        for _ in range(2):
+            y.sum().backward()
 
 
 # ---------------------------------------------------------------------------

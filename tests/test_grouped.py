@@ -7,6 +7,7 @@ plus one rounding to the result's type."""
 import pytest
 import torch
 
+from _saved import check_kept_is_saved
 from torchsplinekan_amd import grouped_linear, quantize_activation
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -107,6 +108,19 @@ def test_cpu_sums_under_autocast(checkpoint):
     with torch.autocast("cpu", dtype=BF16):
         got = grouped_linear(x, w, off, checkpoint=checkpoint)
     assert got.dtype == F32 and torch.equal(got, want)
+
+
+def _check_saved(format, dev):
+    x, w, dy = (t.to(dev) for t in _inputs(9, 2, 40, 5, F32))
+    off = _offsets([4, 5]).to(dev)
+    x.requires_grad_(), w.requires_grad_()
+    check_kept_is_saved(lambda: grouped_linear(x, w, off, checkpoint=format), [x, w], dy,
+                        in_place=[w] if dev == "cpu" else [w, off])
+
+
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+def test_cpu_kept_rows_are_saved_tensors(format):
+    _check_saved(format, "cpu")
 
 
 @pytest.mark.parametrize("x,w,off,kw,text", [
@@ -434,6 +448,12 @@ def test_same_bits_every_time(dtype):
         runs.append([y, *torch.autograd.grad(y, [xd, wd], dy.cuda())])
     for u, v in zip(*runs):
         assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+def test_kept_rows_are_saved_tensors(format):
+    _check_saved(format, "cuda")
 
 
 @pytest.mark.gpu

@@ -142,9 +142,13 @@ def _autocast(state) -> ExitStack:
 class _Checkpoint8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, fn, args, group, format, x, *params):
-        ctx.fn, ctx.args = fn, args
-        ctx.kept = quantize_activation(x, group, format)
-        ctx.params = params
+        kept = quantize_activation(x, group, format)
+        tensors = [a for a in args if isinstance(a, torch.Tensor)]
+        ctx.fn, ctx.form = fn, (group, format, x.dtype)
+        ctx.args = [None if isinstance(a, torch.Tensor) else (a,) for a in args]
+        ctx.save_for_backward(kept.q, kept.scale, *tensors)
+        # (fn holds its parameters: references and versions are enough)
+        ctx.params, ctx.versions = params, [p._version for p in params]
         ctx.autocast = _autocast_of(x.device.type)
         with torch.no_grad(), _autocast(ctx.autocast):
             return fn(x, *args)
@@ -152,9 +156,14 @@ class _Checkpoint8(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
-        x = ctx.kept.dequantize().requires_grad_(ctx.needs_input_grad[4])
+        q, scale, *tensors = ctx.saved_tensors
+        _req([p._version for p in ctx.params] == ctx.versions, "checkpoint_8bit: a parameter was "
+             "changed in place between the forward and the backward pass")
+        x = Activation8(q, scale, *ctx.form).dequantize().requires_grad_(ctx.needs_input_grad[4])
+        rest = iter(tensors)
+        args = [next(rest) if a is None else a[0] for a in ctx.args]
         with torch.enable_grad(), _autocast(ctx.autocast):
-            out = ctx.fn(x, *ctx.args)
+            out = ctx.fn(x, *args)
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
         pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
         wanted = [t for t, need in zip((x, *ctx.params), ctx.needs_input_grad[4:]) if need]

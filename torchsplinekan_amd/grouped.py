@@ -60,18 +60,20 @@ class _GroupedLinear(torch.autograd.Function):
         if ctx is None:
             return y
         need_x, need_w = ctx.needs_input_grad[:2]
-        keep = x if need_w else None
+        keep, scale = x if need_w else None, None
         if need_w and checkpoint is not None:
-            keep, ctx.kept = None, quantize_activation(x, group, checkpoint)
+            kept = quantize_activation(x, group, checkpoint)
+            keep, scale = kept.q, kept.scale
         ctx.sizes = (T, E, N, K)
+        ctx.form = (group, checkpoint)
         ctx.like = x.new_empty(0)
-        ctx.save_for_backward(keep, weight if need_x else None, offsets)
+        ctx.save_for_backward(keep, scale, weight if need_x else None, offsets)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, weight, offsets = ctx.saved_tensors
+        x, scale, weight, offsets = ctx.saved_tensors
         T, E, N, K = ctx.sizes
         need_x, need_w = ctx.needs_input_grad[:2]
         dy = dy.contiguous()
@@ -79,8 +81,9 @@ class _GroupedLinear(torch.autograd.Function):
         if need_x:
             dx = _matmul(INPUT, dy, weight, offsets, ctx.like.new_empty(T, K), T, E, N, K)
         if need_w:
-            dw = _matmul(WEIGHT, dy, x if x is not None else ctx.kept, offsets,
-                         ctx.like.new_empty(E, N, K), T, E, N, K)
+            if scale is not None:
+                x = Activation8(x, scale, *ctx.form, dy.dtype)
+            dw = _matmul(WEIGHT, dy, x, offsets, ctx.like.new_empty(E, N, K), T, E, N, K)
         return dx, dw, None, None, None
 
 
@@ -91,15 +94,15 @@ class _KeptRows(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group, format):
         kept = quantize_activation(x, group, format)
-        ctx.save_for_backward(weight)
-        ctx.kept = kept
+        ctx.save_for_backward(weight, kept.q, kept.scale)
+        ctx.form = (group, format, x.dtype)
         return x @ weight.t()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        weight, = ctx.saved_tensors
-        return dy @ weight, dy.t() @ ctx.kept.dequantize(), None, None
+        weight, q, scale = ctx.saved_tensors
+        return dy @ weight, dy.t() @ Activation8(q, scale, *ctx.form).dequantize(), None, None
 
 
 def _composite(x, weight, offsets, checkpoint, group):

@@ -158,7 +158,8 @@ struct Operand {
     for (int p = 0; p < kPer; ++p)
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
                        to + p * NT * 16),
-                   "v"(off[p]), "s"(src));
+                   "v"(off[p]), "s"(src)
+                   : "m0");
   }
 
   // A slab into registers.  GUARD: k from kend on is zero, and chunks that lie

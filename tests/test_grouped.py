@@ -4,6 +4,8 @@ Bounds: a sum of L products in float32 is off by at most L + 16 roundings of
 2^-24 of the sum of magnitudes (16: what a matrix instruction truncates inside),
 plus one rounding to the result's type."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -159,6 +161,16 @@ def test_c_entry_refusals():
              None) == lib.KAN_ERR_LIMIT
     assert f(2, 0, None, None, 0, None, 0, None, 0, 0, 2, 16, 16, None, None, 0,
              None) == lib.KAN_OK
+
+
+def test_workspace_of_sizes_whose_product_passes_64_bits():
+    """Restored rows are counted also where T E N K is a multiple of 2^64."""
+    lib = pytest.importorskip("torchsplinekan_amd._lib")
+    nbytes = ctypes.c_size_t()
+    T, E, N, K = 1 << 29, 1 << 13, 1 << 11, 1 << 11
+    lib.check(lib.LIB.kan_hip_grouped_matmul_workspace(0, 2, None, None, 1, T, E, N, K,
+                                                       ctypes.byref(nbytes)))
+    assert nbytes.value >= 4 * T * K
 
 
 # ---------------------------------------------------------------------------

@@ -833,7 +833,7 @@ Workspace plan_call(int dtype, int op, int format, const void* A, const void* B,
                     int64_t E, int64_t N, int64_t K) {
   Workspace w{};
   w.plan = {kSmall, 1, kNoRuns};
-  if (T * E * N * K == 0) return w;
+  if (T == 0 || E == 0 || N == 0 || K == 0) return w;  // (their product can pass 64 bits)
   if (takes_few(dtype, op, T, E)) {
     w.plan.cfg = kFew;
     return w;

@@ -92,18 +92,6 @@ __device__ __forceinline__ bool take_tile(const GroupScan& s, int base, int tile
   return true;
 }
 
-// Rows [begin, end) of group e.
-__device__ __forceinline__ void group_rows(const GroupedParams& p, int e, int* begin, int* end) {
-  GroupScan s;
-  for (int base = 0; base <= e; base += 64) {
-    s.step(p, base, 1);
-    if (e < base + 64) {
-      *begin = __builtin_amdgcn_readlane(s.begin, e - base);
-      *end = __builtin_amdgcn_readlane(s.end, e - base);
-    }
-  }
-}
-
 // ---- tiles of the weight gradient -------------------------------------------
 // A group's rows are cut into items of `run` rows and a rest; every item has
 // all tiles of [N, K].  Items cost what their rows are many: whole runs come

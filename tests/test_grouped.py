@@ -284,6 +284,22 @@ def test_kept_rows_of_long_products(T, E, K, N, format, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("format", ["int8", "e4m3"])
+@pytest.mark.parametrize("K,N", [(96, 72), (77, 65)])
+def test_kept_rows_one_to_an_expert(K, N, format, dtype):
+    """Nothing is added up: a product of the restored value in x's type (exact in
+    float32), rounded once."""
+    E = 20
+    x, w, dy = _inputs(E, E, K, N, dtype)
+    wd = w.cuda().requires_grad_()
+    y = grouped_linear(x.cuda(), wd, _offsets([1] * E).cuda(), checkpoint=format, group=32)
+    dw, = torch.autograd.grad(y, wd, dy.cuda())
+    kept = quantize_activation(x, 32, format).dequantize()
+    assert torch.equal(dw.cpu(), (dy.float().unsqueeze(2) * kept.float().unsqueeze(1)).to(dtype))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("format", ["int8", "e4m3"])
 @pytest.mark.parametrize("T,E,K,N", [(200, 3, 96, 72), (200, 3, 77, 65), (12000, 2, 1032, 4104)])
 def test_kept_rows_at_the_end_of_the_range(T, E, K, N, format):

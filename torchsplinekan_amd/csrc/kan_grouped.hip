@@ -217,8 +217,12 @@ struct Operand {
       *reinterpret_cast<u32x4*>(lds + (p * NT + threadIdx.x) * 16) = v;
     }
   }
-  // 8 values q * scale rounded to T.  (int8: no detour over q + 128, whose product
-  // with a scale above FLT_MAX / 128 is infinite.)
+  // 8 values q * scale rounded to T: MFMA takes 16-bit operands, and what the rounding
+  // leaves out would be a product of its own, twice the time.  In bf16 a result is
+  // off by 0.0023 normwise where its own rounding alone makes 0.0017 (1 to 256 rows
+  // an expert alike), and the 8 bits themselves have cost 0.006 (int8) or 0.026 (e4m3).
+  // (int8: no detour over q + 128, whose product with a scale above FLT_MAX / 128
+  // is infinite.)
   __device__ __forceinline__ static u32x4 restore(u32x4 q, float s) {
     typename Half<T>::frag f;
     if constexpr (MODE == kInt8) {
@@ -631,7 +635,11 @@ int launch_few_cols(const GroupedParams& p, hipStream_t st) {
 // six times): 128 rows, 16 experts of 1024 x 1024, 8.4 us against 11.9 on tiles
 // in bf16, 14.8 against 32 in fp32; at 16 rows a group (64 rows, 4 experts of
 // 4096 x 4096, bf16) 42 against 33, at 32 in fp32 (512 rows, 16 experts of 1024 x
-// 1024) 30.6 against 35.5.
+// 1024) 30.6 against 35.5.  The mean decides, so one expert may get all rows and its
+// weights are read once for every 16 of them, from the caches: never slower than
+// equal groups of the same rows, up to twice the tiles' time for that expert alone
+// (512 rows, 64 experts of 1024 x 1024, bf16: equal 25.0 us, all at one 15.5, tiles
+// 12.5; 2048 rows, 64 experts, fp32: 102, 96 and 50).
 bool takes_few(int dtype, int op, int64_t T, int64_t E) {
   return op == KAN_GROUPED_FORWARD && T <= (dtype == KAN_DTYPE_F32 ? 32 : 8) * E;
 }

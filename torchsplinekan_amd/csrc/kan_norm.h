@@ -148,10 +148,11 @@ struct RowView {
 };
 
 // ---- rows held in registers ---------------------------------------------------
-// TPR lanes share a row, each with 8 of its values in NV pieces of VEC; a block
-// is one row's lanes, or four waves with a row (8 or 4 narrow ones) each, and
-// runs through its rows, the weights staying in registers.  Every value is read once: the
-// passes above happen on registers, a row's sums cross its waves through LDS.
+// TPR lanes share a row, each with 8 of its values (16 in rows of more than 8192)
+// in NV pieces of VEC; a block is one row's lanes, or four waves with a row (8 or 4
+// narrow ones) each, and runs through its rows, the weights staying in registers.
+// Every value is read once: the passes above happen on registers, a row's sums
+// cross its waves through LDS.
 template <int TPR>
 struct RowShape {
   static constexpr int kThreads = TPR <= 64 ? 256 : TPR;
@@ -257,8 +258,8 @@ __device__ __forceinline__ void load_weight(float (&v)[NV][VEC], const void* __r
   }
 }
 
-// Lanes that share a row of C values, 8 each (rows past kMaxHeld stay in memory,
-// on blocks of 256).
+// Lanes that share a row of C values, 8 each (16 past 8192; rows past kMaxHeld
+// stay in memory, on blocks of 256).
 constexpr int64_t kMaxHeld = 16384;
 inline int held_tpr(int64_t C) {
   if (C > kMaxHeld) return 256;

@@ -103,12 +103,16 @@ __device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __rest
 
 // Bound by HBM: 16384 x 4096 bf16 with a gate row for 2048 rows 178 us (805 MB
 // and 25 of partial sums, 4.6 TB/s); 32768 x 1024 float32 150 us, 5.4 TB/s.
-// Four waves a SIMD (128 registers; a float32 row of 512 lanes with a gate would
-// spill there and takes two).  dpost = scale * (sum of D a yh) and dscale = post *
-// (the same sum): one column sum serves both, a weight's factor applied after
-// it.  A gate row's gradient comes from the sum of D yh, times scale, post and
-// a'(g), and what its rows add to the first sum is a(g) times the same: two sums
-// a row.  In 16 bits the next row's
+// Four waves a SIMD, two for a float32 row of 512 lanes with a gate.  In the 128
+// registers that four leave not every row fits; the compiler keeps in scratch, a
+// lane: 52 to 92 bytes of 16-bit rows with a gate row (76 at the size above), up to
+// 28 without; 44 to 120 of a float32 stream with a 16-bit gate for every element;
+// 92 to 388 of float32 rows of 8 or 16 lanes, up to 28 of longer ones; and 196 to 584 of
+// all rows of more than 8192 columns (4096 x 16384 bf16 0.58 ms, their bytes 0.17).
+// dpost = scale * (sum of D a yh) and dscale = post * (the same sum): one column
+// sum serves both, a weight's factor applied after it.  A gate row's gradient
+// comes from the sum of D yh, times scale, post and a'(g), and what its rows add to
+// the first sum is a(g) times the same: two sums a row.  In 16 bits the next row's
 // loads are in flight while a row is worked on (but beside a gate's values).
 template <typename TX, typename TY, int TPR, int VEC, int NV, int GATE, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::kThreads) __attribute__((

@@ -135,6 +135,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     never below the one before.)
     checkpoint "int8" or "e4m3": the weight's gradient reads x from 8 bits
     (groups of `group` values, quantize_activation) and x itself is not kept.
+    On the device the restored values take part rounded to x's type, as
+    Activation8.dequantize gives them; on the CPU in float32.
     Sums are held in float32, also under autocast, which casts nothing here.
     Gradients (first order) reach x and weight (device tensors refuse forward
     mode); sums over rows have a fixed order."""

@@ -471,6 +471,14 @@ int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* s
 #define KAN_GROUPED_WEIGHT 2
 int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const void* b, int b_format,
                                      int64_t T, int64_t E, int64_t N, int64_t K, size_t* bytes);
+/* What the product runs on (host only, for tests and measurements): plan[0] rows
+ * of its tiles (16: the kernel for groups of a few rows), plan[1] cuts of its sums,
+ * plan[2] rows of an item of the weight product (0: an expert's rows are one),
+ * plan[3] 1 if 8-bit rows are restored in a pass of their own, plan[4] and plan[5]
+ * operands brought onto 16 bytes first and, in 16 bits, operands that reach LDS
+ * past the registers (1: a, 2: b, 3: both). */
+int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b, int b_format,
+                                int64_t T, int64_t E, int64_t N, int64_t K, int64_t* plan);
 int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,

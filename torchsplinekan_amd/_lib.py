@@ -107,6 +107,8 @@ SIGNATURES = {
     "kan_hip_act8_dequantize": (_int, [_int, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     "kan_hip_grouped_matmul_workspace": (_int, [_int, _int, _vp, _vp, _int] + [_i64] * 4
                                          + [ctypes.POINTER(_sz)]),
+    "kan_hip_grouped_matmul_plan": (_int, [_int, _int, _vp, _vp, _int] + [_i64] * 4
+                                    + [ctypes.POINTER(_i64)]),
     "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
                                + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
     "kan_hip_timing_enable": (_int, [_int]),

@@ -2243,6 +2243,10 @@ int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
 }
 }  // namespace
 
+int grouped_f32_rows(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+  return grouped_takes_big(op, T, E, N, K) ? 256 : 128;
+}
+
 // (a tile's share of the engine's 220 TFLOP/s)
 int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K) {
   const int cus = device_cu_count();

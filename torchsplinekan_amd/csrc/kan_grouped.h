@@ -325,7 +325,8 @@ int launch_grouped_cuts(const GroupedParams& p, int64_t cols, hipStream_t st) {
 }
 
 // fp32 products on the split contraction engine's tiles (kan_gemm.hip); the rows
-// of an item and the cuts of a sum there.
+// of a tile and of an item and the cuts of a sum there.
+int grouped_f32_rows(int op, int64_t T, int64_t E, int64_t N, int64_t K);
 int grouped_f32_run(int64_t T, int64_t E, int64_t N, int64_t K);
 int grouped_f32_cuts(int op, int64_t T, int64_t E, int64_t N, int64_t K);
 int launch_grouped_f32(int op, const GroupedParams& p, hipStream_t st);

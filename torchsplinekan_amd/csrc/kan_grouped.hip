@@ -884,6 +884,30 @@ int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const voi
   return KAN_OK;
 }
 
+int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b, int b_format,
+                                int64_t T, int64_t E, int64_t N, int64_t K, int64_t* plan) {
+  if (plan == nullptr)
+    return set_error(KAN_ERR_INVALID, "grouped_matmul_plan: plan must not be NULL");
+  const int rc = check_grouped(dtype, op, T, E, N, K);
+  if (rc != KAN_OK) return rc;
+  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
+  const bool f32 = dtype == KAN_DTYPE_F32, few = w.plan.cfg == kFew;
+  const int rows[] = {256, 192, 128, kFewRows};  // by HalfCfg
+  plan[0] = f32 && !few ? grouped_f32_rows(op, T, E, N, K) : rows[w.plan.cfg];
+  plan[1] = w.plan.cuts;
+  plan[2] = w.plan.run == kNoRuns ? 0 : w.plan.run;
+  plan[3] = w.restore;
+  plan[4] = (w.align.a ? 1 : 0) + (w.align.b ? 2 : 0);
+  plan[5] = 0;
+  if (!f32 && !few) {
+    const bool whole_a = w.align.a || whole_rows(a, op == KAN_GROUPED_FORWARD ? K : N);
+    const bool bytes = b_format != KAN_ACT8_NONE && !w.restore;
+    const bool whole_b = w.restore || w.align.b || whole_rows(b, K);
+    plan[5] = bytes ? (whole_a ? 1 : 0) : whole_a && whole_b ? 3 : 0;
+  }
+  return KAN_OK;
+}
+
 int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,

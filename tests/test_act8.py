@@ -267,3 +267,31 @@ def test_checkpointed_kan_layer():
     want = torch.autograd.grad(layer(xr), [xr, *layer.parameters()], g)
     for u, v in zip(got, want):
         assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("inside", [True, False])
+def test_checkpoint_under_autocast_on_the_device(inside):
+    """As on the CPU, the backward pass running on a thread of its own: gradients of
+    the layer at the restored input under the call's autocast, and a layer used
+    beside its checkpoint keeps its own."""
+    net, x = _net("cuda"), _values(64, 24, F32).cuda().requires_grad_()
+    params, g = list(net.parameters()), torch.randn(64, 8, device="cuda").to(BF16)
+    xr = quantize_activation(x, 32).dequantize().requires_grad_()
+    with torch.autocast("cuda", dtype=BF16):
+        want = net(xr)
+        y = checkpoint_8bit(net, x, group=32)
+        assert y.dtype == BF16 and torch.equal(y, net(x))
+        if inside:
+            got = torch.autograd.grad(y, [x, *params], g)
+            want = torch.autograd.grad(want, [xr, *params], g)
+    if not inside:
+        got = torch.autograd.grad(y, [x, *params], g)
+        want = torch.autograd.grad(want, [xr, *params], g)
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
+    with torch.autocast("cuda", dtype=BF16):
+        checkpoint_8bit(net, x, group=32)
+        beside = net(x)
+    for v in torch.autograd.grad(beside, params, g):
+        assert bool(v.any())

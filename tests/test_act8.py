@@ -150,6 +150,14 @@ def test_checkpoint_keeps_the_forward_pass_autocast(around):
         assert u.dtype == v.dtype and torch.equal(u, v)
 
 
+def test_checkpoint_counts_a_parameter_once():
+    """A tied weight that stands in params twice has one gradient."""
+    x, w = _values(6, 24, F32), torch.randn(24, requires_grad=True)
+    y = checkpoint_8bit(lambda v: v * w, x, group=32, params=[w, w])
+    got, = torch.autograd.grad(y.sum(), [w])
+    torch.testing.assert_close(got, quantize_activation(x, 32).dequantize().sum(0))
+
+
 def test_checkpoint_leaves_autocast_of_other_calls():
     """The layer used beside its checkpoint, in one autocast region, keeps its
     gradients (casts of weights made without gradients are not kept for it)."""

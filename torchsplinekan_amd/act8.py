@@ -185,7 +185,7 @@ def checkpoint_8bit(fn: Callable, x: torch.Tensor, *args, group: int = 128, form
     check_format("checkpoint_8bit", group, format)
     if params is None:
         params = tuple(fn.parameters()) if isinstance(fn, nn.Module) else ()
-    params = tuple(p for p in params if p.requires_grad)
+    params = tuple({id(p): p for p in params if p.requires_grad}.values())
     if not (torch.is_grad_enabled() and (x.requires_grad or params)):
         return fn(x, *args)
     return _Checkpoint8.apply(fn, args, group, format, x, *params)

@@ -158,6 +158,28 @@ def test_checkpoint_counts_a_parameter_once():
     torch.testing.assert_close(got, quantize_activation(x, 32).dequantize().sum(0))
 
 
+def test_checkpoint_passes_tensor_arguments():
+    """Gradients reach tensor arguments, alone or beside x's, and one that fn gives
+    back stays the caller's own."""
+    x, s = _values(6, 24, F32), torch.randn(24, requires_grad=True)
+    back = quantize_activation(x, 32).dequantize()
+    for need_x in (False, True):
+        xr = x.clone().requires_grad_(need_x)
+        y = checkpoint_8bit(lambda v, t, n: (v * t * n).sin(), xr, s, 2.0, group=32)
+        assert torch.equal(y, (x * s * 2).sin())
+        got, = torch.autograd.grad(y.sum(), [s], retain_graph=need_x)
+        torch.testing.assert_close(got, (2 * back * (2 * back * s).cos()).sum(0))
+        if need_x:
+            torch.testing.assert_close(torch.autograd.grad(y.sum(), [xr])[0],
+                                       2 * s.detach() * (2 * back * s.detach()).cos())
+    xr, t = x.clone().requires_grad_(), torch.ones(3)
+    y, out = checkpoint_8bit(lambda v, t: (v * 2, t), xr, t, group=32)
+    assert t.is_leaf and not t.requires_grad and torch.equal(out, t)
+    z = s * 3                                   # (not a leaf)
+    y = checkpoint_8bit(lambda v, t: v * t, xr, z, group=32)
+    torch.testing.assert_close(torch.autograd.grad(y.sum(), [s])[0], 3 * back.sum(0))
+
+
 def test_checkpoint_leaves_autocast_of_other_calls():
     """The layer used beside its checkpoint, in one autocast region, keeps its
     gradients (casts of weights made without gradients are not kept for it)."""

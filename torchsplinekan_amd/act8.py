@@ -139,14 +139,22 @@ def _autocast(state) -> ExitStack:
     return stack
 
 
+def _fill(rest, tensors):
+    """(rest with `tensors` in the places of its Nones, the tensors left over)"""
+    left = iter(tensors)
+    return [next(left) if r is None else r[0] for r in rest], list(left)
+
+
 class _Checkpoint8(torch.autograd.Function):
+    """Inputs beside x: the tensors among fn's further arguments (rest has None in
+    their places, the others as (value,)), then the parameters."""
+
     @staticmethod
-    def forward(ctx, fn, args, group, format, x, *params):
+    def forward(ctx, fn, rest, group, format, x, *tensors):
+        args, params = _fill(rest, tensors)
         kept = quantize_activation(x, group, format)
-        tensors = [a for a in args if isinstance(a, torch.Tensor)]
-        ctx.fn, ctx.form = fn, (group, format, x.dtype)
-        ctx.args = [None if isinstance(a, torch.Tensor) else (a,) for a in args]
-        ctx.save_for_backward(kept.q, kept.scale, *tensors)
+        ctx.fn, ctx.rest, ctx.form = fn, rest, (group, format, x.dtype)
+        ctx.save_for_backward(kept.q, kept.scale, *tensors[:len(tensors) - len(params)])
         # (fn holds its parameters: references and versions are enough)
         ctx.params, ctx.versions = params, [p._version for p in params]
         ctx.autocast = _autocast_of(x.device.type)
@@ -159,19 +167,18 @@ class _Checkpoint8(torch.autograd.Function):
         q, scale, *tensors = ctx.saved_tensors
         _req([p._version for p in ctx.params] == ctx.versions, "checkpoint_8bit: a parameter was "
              "changed in place between the forward and the backward pass")
-        x = Activation8(q, scale, *ctx.form).dequantize().requires_grad_(ctx.needs_input_grad[4])
-        rest = iter(tensors)
-        args = [next(rest) if a is None else a[0] for a in ctx.args]
+        needs = ctx.needs_input_grad[4:]
+        x = Activation8(q, scale, *ctx.form).dequantize().requires_grad_(needs[0])
+        tensors = [t.detach().requires_grad_(need) for t, need in zip(tensors, needs[1:])]
         with torch.enable_grad(), _autocast(ctx.autocast):
-            out = ctx.fn(x, *args)
+            out = ctx.fn(x, *_fill(ctx.rest, tensors)[0])
         outs = [out] if isinstance(out, torch.Tensor) else list(out)
         pairs = [(o, g) for o, g in zip(outs, grads) if g is not None and o.requires_grad]
-        wanted = [t for t, need in zip((x, *ctx.params), ctx.needs_input_grad[4:]) if need]
+        wanted = [t for t, need in zip((x, *tensors, *ctx.params), needs) if need]
         got = iter(torch.autograd.grad([o for o, _ in pairs], wanted, [g for _, g in pairs],
                                        allow_unused=True) if pairs and wanted
                    else [None] * len(wanted))
-        return (None, None, None, None,
-                *(next(got) if need else None for need in ctx.needs_input_grad[4:]))
+        return (None, None, None, None, *(next(got) if need else None for need in needs))
 
 
 def checkpoint_8bit(fn: Callable, x: torch.Tensor, *args, group: int = 128, format: str = "int8",
@@ -179,13 +186,16 @@ def checkpoint_8bit(fn: Callable, x: torch.Tensor, *args, group: int = 128, form
     """fn(x, *args), keeping x in 8 bits for the backward pass and nothing that
     fn makes: the backward restores x and runs fn again, under the call's
     autocast, so gradients are those of fn at the restored x (the output is
-    exact).  Gradients reach x and `params` (default: fn.parameters() of a
-    module; args are taken as constants).  fn must give the same result each
-    time: no random numbers."""
+    exact).  Gradients reach x, tensors in args and `params` (default:
+    fn.parameters() of a module), nothing else that fn uses.  fn must give the
+    same result each time: no random numbers."""
     check_format("checkpoint_8bit", group, format)
     if params is None:
         params = tuple(fn.parameters()) if isinstance(fn, nn.Module) else ()
     params = tuple({id(p): p for p in params if p.requires_grad}.values())
-    if not (torch.is_grad_enabled() and (x.requires_grad or params)):
+    tensors = tuple(a for a in args if isinstance(a, torch.Tensor))
+    if not (torch.is_grad_enabled()
+            and (x.requires_grad or params or any(t.requires_grad for t in tensors))):
         return fn(x, *args)
-    return _Checkpoint8.apply(fn, args, group, format, x, *params)
+    rest = [None if isinstance(a, torch.Tensor) else (a,) for a in args]
+    return _Checkpoint8.apply(fn, rest, group, format, x, *tensors, *params)

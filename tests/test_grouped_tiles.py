@@ -137,6 +137,34 @@ def test_products(code, op, kept, T, E, N, K, plan):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("code", [0, 2])
+@pytest.mark.parametrize("op", [FORWARD, INPUT, WEIGHT])
+def test_as_many_experts_as_there_may_be(op, code):
+    """65535 experts, most of them without rows."""
+    T, E, N, K = 300, 65535, 8, 12
+    dtype = {0: F32, 2: BF16}[code]
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randn(T, K, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(T, N, generator=g, device="cuda").to(dtype)
+    w = torch.randn(E, N, K, generator=g, device="cuda").to(dtype)
+    ids = torch.randint(0, E, (T,), generator=g, device="cuda").sort().values
+    off = torch.searchsorted(ids, torch.arange(E + 1, device="cuda"))
+    shape = {FORWARD: (T, N), INPUT: (T, K), WEIGHT: (E, N, K)}[op]
+    out = _matmul(op, x if op == FORWARD else dy, x if op == WEIGHT else w, off,
+                  torch.empty(shape, dtype=dtype, device="cuda"), T, E, N, K)
+    X, D, W = x.double(), dy.double(), w[ids].double()
+    if op == WEIGHT:
+        want = torch.zeros(E, N, K, dtype=torch.float64, device="cuda")
+        want.index_add_(0, ids, D.unsqueeze(2) * X.unsqueeze(1))
+    else:
+        want = (W * (X.unsqueeze(1) if op == FORWARD else D.unsqueeze(2))).sum(
+            2 if op == FORWARD else 1)
+    # (12 products at most, of values up to 5 each)
+    tol = (12 + 16) * 2.0 ** -24 * 12 * 25 + HALF_ULP[dtype] * want.abs()
+    assert bool(((out.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("op,N,K", [(FORWARD, 2, 1 << 22), (INPUT, 1 << 22, 2)])
 def test_float32_rows_past_a_buffer_resource(op, N, K):
     """Rows whose tile spans more than 2^31 bytes take 64-bit addresses.  (A sum of

@@ -73,3 +73,9 @@ def test_short_sequences(seqs, L):
     (9000, 2, 700), (9000, 400, 2), (9001, 5, 111), (16384, 3, 200)])
 def test_gate_rows_of_rows_that_waves_share(C, seqs, L, xdt, ydt):
     base._run_case((seqs, L, C), xdt, ydt, (seqs, 1, C), "tanh", True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,cols", [(8, 8), (300, 300), (8, 1)])
+def test_more_gate_rows_than_a_grid_is_high(C, cols):
+    base._run_case((70000, 2, C), F32, F32, (70000, 1, cols), "sigmoid", True)

@@ -438,6 +438,21 @@ int kan_hip_residual_norm_backward(int xdtype, int ydtype, int wdtype, const voi
                                    void* grad_scale, void* workspace, size_t workspace_bytes,
                                    void* stream);
 
+/* Layer norm of n rows of C values, y = weight * (x - m) r + bias with m =
+ * mean(x) and r = 1 / sqrt(mean((x - m)^2) + eps).  x is in xdtype (ydtype or
+ * FP32), y in ydtype, weight and bias [C] in wdtype (either may be NULL: 1 and
+ * 0).  stats [2, n] (optional) receives m and r; the backward reads it.  In the
+ * backward any output may be NULL; the workspace serves the sums of grad_weight
+ * and grad_bias and lies on 16 bytes.  With n = 0 nothing is written. */
+int kan_hip_layer_norm(int xdtype, int ydtype, int wdtype, const void* x, const void* weight,
+                       const void* bias, int64_t n, int64_t C, double eps, void* y, float* stats,
+                       void* stream);
+int kan_hip_layer_norm_backward_workspace(int64_t n, int64_t C, size_t* bytes);
+int kan_hip_layer_norm_backward(int xdtype, int ydtype, int wdtype, const void* grad_y,
+                                const void* x, const void* weight, const float* stats, int64_t n,
+                                int64_t C, void* grad_x, void* grad_weight, void* grad_bias,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
 /* Activations kept in 8 bits: rows of C values cut into groups of `group` (32,
  * 64, 128 or 256; the last of a row may be short), scale [rows,
  * ceil(C / group)] = max|x| * (1 / qmax) (127 for int8, 448 for e4m3) and q [rows, C]

@@ -103,6 +103,10 @@ SIGNATURES = {
     "kan_hip_residual_norm_backward_workspace": (_int, [_i64] * 4 + [ctypes.POINTER(_sz)]),
     "kan_hip_residual_norm_backward": (_int, [_int] * 3 + [_vp] * 8 + [_dbl, _int] + [_i64] * 4
                                        + [_vp] * 8 + [_sz, _vp]),
+    "kan_hip_layer_norm": (_int, [_int] * 3 + [_vp] * 3 + [_i64] * 2 + [_dbl] + [_vp] * 3),
+    "kan_hip_layer_norm_backward_workspace": (_int, [_i64] * 2 + [ctypes.POINTER(_sz)]),
+    "kan_hip_layer_norm_backward": (_int, [_int] * 3 + [_vp] * 4 + [_i64] * 2 + [_vp] * 4
+                                    + [_sz, _vp]),
     "kan_hip_act8_quantize": (_int, [_int, _int, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
     "kan_hip_act8_dequantize": (_int, [_int, _int, _vp, _vp, _i64, _i64, _i64, _vp, _vp]),
     "kan_hip_grouped_matmul_workspace": (_int, [_int, _int, _vp, _vp, _int] + [_i64] * 4
@@ -173,8 +177,8 @@ OPERATOR_DTYPES = {torch.float32: KAN_DTYPE_F32, torch.bfloat16: KAN_DTYPE_BF16,
 
 
 def operator_dtype_code(dtype: torch.dtype, who: str) -> int:
-    """dtype code of the operators beside the KAN layers (residual norm, 8-bit
-    activations, grouped products)."""
+    """dtype code of the operators beside the KAN layers (norms, 8-bit
+    activations, grouped and gated products, losses)."""
     code = OPERATOR_DTYPES.get(dtype)
     if code is None:
         raise RuntimeError(f"{who}: only FP32, BF16 and FP16 tensors are supported, got {dtype}")

@@ -258,6 +258,50 @@ __device__ __forceinline__ void load_weight(float (&v)[NV][VEC], const void* __r
   }
 }
 
+// This block's column sums into one partial row: rows that were handled side
+// by side are added through LDS in order.
+template <int TPR, bool WHOLE, int VEC, int NV>
+__device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __restrict__ out,
+                                              int64_t C, float* lds) {
+  typedef RowShape<TPR> S;
+  const int r = threadIdx.x / TPR, t = threadIdx.x % TPR;
+  if constexpr (S::kRows > 1) {
+    __syncthreads();
+    KAN_EACH lds[(i * VEC + j) * S::kThreads + threadIdx.x] = v[i][j];
+    __syncthreads();
+    if (r != 0) return;
+    KAN_EACH {
+#pragma unroll
+      for (int q = 1; q < S::kRows; ++q)
+        v[i][j] += lds[(i * VEC + j) * S::kThreads + q * TPR + t];
+    }
+  }
+  Pieces<float, TPR, VEC, NV, WHOLE>::store(v, out, C);
+}
+
+// Column sums of partial rows in a fixed order: 16 lanes of rows a column,
+// their sums added in order.  (512 partial rows of 4096 columns, two sums: 6 us.)
+constexpr int kSumRowLanes = 16;
+__device__ __forceinline__ bool column_sum(const float* __restrict__ part, int64_t rows, int64_t C,
+                                           int64_t* col, float* sum) {
+  __shared__ float red[kSumRowLanes][64];
+  const int lane = threadIdx.x & 63, rl = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.0f;
+  if (c < C) {
+#pragma unroll 4
+    for (int64_t r = rl; r < rows; r += kSumRowLanes) s += part[r * C + c];
+  }
+  red[rl][lane] = s;
+  __syncthreads();
+  if (rl != 0 || c >= C) return false;
+#pragma unroll
+  for (int w = 1; w < kSumRowLanes; ++w) s += red[w][lane];
+  *col = c;
+  *sum = s;
+  return true;
+}
+
 // Lanes that share a row of C values, 8 each (16 past 8192; rows past kMaxHeld
 // stay in memory, on blocks of 256).
 constexpr int64_t kMaxHeld = 16384;

@@ -80,27 +80,6 @@ __global__ __launch_bounds__(kRowThreads) void norm_rows_grad_kernel(NormParams 
   }
 }
 
-// This block's column sums into one partial row: rows that were handled side
-// by side are added through LDS in order.
-template <int TPR, bool WHOLE, int VEC, int NV>
-__device__ __forceinline__ void flush_columns(float (&v)[NV][VEC], float* __restrict__ out,
-                                              int64_t C, float* lds) {
-  typedef RowShape<TPR> S;
-  const int r = threadIdx.x / TPR, t = threadIdx.x % TPR;
-  if constexpr (S::kRows > 1) {
-    __syncthreads();
-    KAN_EACH lds[(i * VEC + j) * S::kThreads + threadIdx.x] = v[i][j];
-    __syncthreads();
-    if (r != 0) return;
-    KAN_EACH {
-#pragma unroll
-      for (int q = 1; q < S::kRows; ++q)
-        v[i][j] += lds[(i * VEC + j) * S::kThreads + q * TPR + t];
-    }
-  }
-  Pieces<float, TPR, VEC, NV, WHOLE>::store(v, out, C);
-}
-
 // Bound by HBM: 16384 x 4096 bf16 with a gate row for 2048 rows 178 us (805 MB
 // and 25 of partial sums, 4.6 TB/s); 32768 x 1024 float32 150 us, 5.4 TB/s.
 // Four waves a SIMD, two for a float32 row of 512 lanes with a gate.  In the 128
@@ -265,29 +244,6 @@ norm_grad_kernel(NormParams p) {
   const int64_t at = (int64_t)blockIdx.x * p.C;
   if (p.part_pre != nullptr) flush_columns<TPR, WHOLE>(s_pre, p.part_pre + at, p.C, cols);
   if (p.part_branch != nullptr) flush_columns<TPR, WHOLE>(s_branch, p.part_branch + at, p.C, cols);
-}
-
-// Column sums of partial rows in a fixed order: 16 lanes of rows a column,
-// their sums added in order.  (512 partial rows of 4096 columns, two sums: 6 us.)
-constexpr int kSumRowLanes = 16;
-__device__ __forceinline__ bool column_sum(const float* __restrict__ part, int64_t rows, int64_t C,
-                                           int64_t* col, float* sum) {
-  __shared__ float red[kSumRowLanes][64];
-  const int lane = threadIdx.x & 63, rl = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.0f;
-  if (c < C) {
-#pragma unroll 4
-    for (int64_t r = rl; r < rows; r += kSumRowLanes) s += part[r * C + c];
-  }
-  red[rl][lane] = s;
-  __syncthreads();
-  if (rl != 0 || c >= C) return false;
-#pragma unroll
-  for (int w = 1; w < kSumRowLanes; ++w) s += red[w][lane];
-  *col = c;
-  *sum = s;
-  return true;
 }
 
 // grid y 0: dpre; 1: dpost and dscale from their common sum.

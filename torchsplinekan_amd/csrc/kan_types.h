@@ -1,5 +1,5 @@
-// The 16-bit types of the operators beside the KAN layers (residual norm,
-// 8-bit activations, grouped products): storage types, conversions, vectors
+// The 16-bit types of the operators beside the KAN layers (norms, 8-bit
+// activations, grouped and gated products, losses): storage types, conversions, vectors
 // and wave sums.
 #pragma once
 
@@ -101,14 +101,15 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
-// Sum over aligned groups of 8 or 16 lanes, in each of them.
+// Sum over aligned groups of 8, 16 or 32 lanes, in each of them.
 template <int LANES>
 __device__ __forceinline__ float lane_sum(float v) {
-  static_assert(LANES == 8 || LANES == 16, "groups within a row of 16 lanes");
+  static_assert(LANES == 8 || LANES == 16 || LANES == 32, "groups of lanes in a wave");
   v += dpp_or_zero<0xB1>(v);
   v += dpp_or_zero<0x4E>(v);
   v += dpp_or_zero<0x141>(v);
-  if constexpr (LANES == 16) v += dpp_or_zero<0x140>(v);
+  if constexpr (LANES >= 16) v += dpp_or_zero<0x140>(v);
+  if constexpr (LANES == 32) v += __shfl_xor(v, 16);
   return v;
 }
 

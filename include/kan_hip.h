@@ -417,6 +417,8 @@ int kan_hip_refit_gram(int dtype, const void* x_t, const void* grid_old, const v
 #define KAN_GATE_SIGMOID 1
 #define KAN_GATE_TANH 2
 #define KAN_GATE_SILU 3
+#define KAN_GATE_GELU 4 /* gated products only, as is the next */
+#define KAN_GATE_RELU 5
 int kan_hip_residual_norm(int xdtype, int ydtype, int wdtype, const void* x, const void* y,
                           const void* gate, const void* post_weight, const void* pre_weight,
                           const void* scale, double scale_const, int gate_act, int64_t gate_rows,
@@ -470,7 +472,8 @@ int kan_hip_act8_dequantize(int dtype, int format, const void* q, const float* s
 /* Products grouped by expert: rows sorted by expert, expert e having the rows
  * offsets[e] .. offsets[e + 1] - 1 of T (offsets [E + 1] on the device, int32
  * or int64, ascending from 0; each is taken within 0 .. T and as the running
- * maximum, so that no value of theirs leads outside the operands).  With
+ * maximum, so that no value of theirs leads outside the operands; NULL with E = 1:
+ * all rows).  With
  * weights w [E, N, K]:
  *   KAN_GROUPED_FORWARD  a = x [T, K],  b = w:  out y [T, N],  y[t] = w[e] x[t]
  *   KAN_GROUPED_INPUT    a = dy [T, N], b = w:  out dx [T, K], dx[t] = w[e]^T dy[t]
@@ -498,6 +501,25 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,
                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gated products: h = act(g) * u with g = x gate^T and u = x up^T, rows x [T, K]
+ * of E experts (offsets as above; NULL with E = 1: all rows) and weights w
+ * [E, 2, N, K], an expert's gate before its up.  Rows from offsets[E] on get g =
+ * u = 0.  kept (optional; kan_hip_gated_kept bytes, on 16 bytes) receives what the
+ * backward pass needs of g and u: in FP32 themselves, otherwise 20 bits (BF16) or 24
+ * (FP16) of each.
+ * The backward's first part turns grad_h [T, N] into grad_pre [T, 2 N], the
+ * gradients of g and u; grouped products over w as [E, 2 N, K] make those of x and w
+ * of it.  N <= 2^21, other limits as above.  keep: whether the call will be given
+ * kept.  The workspace lies on 16 bytes. */
+int kan_hip_gated_kept(int dtype, int64_t T, int64_t N, size_t* bytes);
+int kan_hip_gated_workspace(int dtype, const void* x, const void* w, int64_t T, int64_t E, int64_t N,
+                            int64_t K, int keep, size_t* bytes);
+int kan_hip_gated(int dtype, int act, const void* x, const void* w, const void* offsets,
+                  int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* h, void* kept,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* kept, int64_t T,
+                           int64_t N, void* grad_pre, void* stream);
 
 /* Kernel-level timing (measurement support; no counterpart in the
  * reference, whose benchmarks time with torch.profiler,

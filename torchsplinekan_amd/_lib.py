@@ -115,6 +115,12 @@ SIGNATURES = {
                                     + [ctypes.POINTER(_i64)]),
     "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
                                + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
+    "kan_hip_gated_kept": (_int, [_int] + [_i64] * 2 + [ctypes.POINTER(_sz)]),
+    "kan_hip_gated_workspace": (_int, [_int, _vp, _vp] + [_i64] * 4
+                                + [_int, ctypes.POINTER(_sz)]),
+    "kan_hip_gated": (_int, [_int, _int, _vp, _vp, _vp, _int] + [_i64] * 4 + [_vp] * 3
+                      + [_sz, _vp]),
+    "kan_hip_gated_backward": (_int, [_int, _int, _vp, _vp, _i64, _i64, _vp, _vp]),
     "kan_hip_timing_enable": (_int, [_int]),
     "kan_hip_timing_read": (_int, [_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i64),
                                    ctypes.POINTER(ctypes.c_double)]),

@@ -20,8 +20,10 @@ struct GroupedParams {
   int group, format;      // of 8-bit rows (KAN_ACT8_NONE: B is in the products' type)
   int run;                // op 2: rows of an item of work; the sums of a group of
   float* part;            // several items go to part [T / run + E, N, K]
-  int cuts;               // op 0, 1: the sums are cut into this many (grid y), whose
-                          // results go to part [cuts, T, columns] if there are several
+  int cuts;               // op 0, 1: the sums are cut into this many (grid y); with part,
+                          // their results go to part [cuts, T, columns], and their sum
+                          // to C if C is given
+  const float* scale;     // a factor of the result (16-bit products; null: 1)
 };
 
 // ---- which rows a tile has --------------------------------------------------
@@ -51,9 +53,10 @@ __device__ __forceinline__ int scan_max(int v) {
 }
 
 // End of group e's rows as stored, within 0 .. T; the rows past the last
-// group's are a group E of their own that ends at T.
+// group's are a group E of their own that ends at T.  Without offsets (one
+// group) all rows are its own.
 __device__ __forceinline__ int group_end(const GroupedParams& p, int e) {
-  if (e >= p.E) return (int)p.T;
+  if (e >= p.E || p.offsets == nullptr) return (int)p.T;
   const int64_t v = p.offsets64 ? static_cast<const int64_t*>(p.offsets)[e + 1]
                                 : (int64_t)static_cast<const int*>(p.offsets)[e + 1];
   return (int)max((int64_t)0, min(p.T, v));
@@ -231,13 +234,14 @@ __global__ __launch_bounds__(256) void grouped_sum_kernel(GroupedParams p) {
   if (slots <= 1) return;
   const int64_t count = p.N * p.K;
   const float* part = p.part + first * count;
+  const float factor = p.scale == nullptr ? 1.0f : *p.scale;
   T* out = static_cast<T*>(p.C) + e * count;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count;
        i += (int64_t)gridDim.x * 256) {
     float v = part[i];
 #pragma unroll 8
     for (int q = 1; q < slots; ++q) v += part[q * count + i];
-    out[i] = (T)v;
+    out[i] = (T)(v * factor);
   }
 }
 template <typename T>
@@ -306,23 +310,57 @@ __device__ __forceinline__ void cut_range(const GroupedParams& p, int64_t* kbeg,
 // out = the sum of `cuts` slices of `count` values, in order.
 template <typename T>
 __global__ __launch_bounds__(256) void grouped_cuts_kernel(const float* __restrict__ part, int cuts,
-                                                           int64_t count, T* __restrict__ out) {
+                                                           int64_t count, const float* scale,
+                                                           T* __restrict__ out) {
+  const float factor = scale == nullptr ? 1.0f : *scale;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count;
        i += (int64_t)gridDim.x * 256) {
     float v = part[i];
 #pragma unroll 8
     for (int q = 1; q < cuts; ++q) v += part[q * count + i];
-    out[i] = (T)v;
+    out[i] = (T)(v * factor);
   }
 }
 template <typename T>
 int launch_grouped_cuts(const GroupedParams& p, int64_t cols, hipStream_t st) {
-  if (p.cuts <= 1) return KAN_OK;
+  if (p.part == nullptr || p.C == nullptr) return KAN_OK;
   const int64_t count = p.T * cols;
   grouped_cuts_kernel<T><<<dim3((unsigned)std::min<int64_t>(ceil_div(count, 256), 8192)), 256, 0,
-                           st>>>(p.part, p.cuts, count, static_cast<T*>(p.C));
+                           st>>>(p.part, p.cuts, count, p.scale, static_cast<T*>(p.C));
   return check_launch("grouped_matmul sum");
 }
+
+// What a product in 16 bits runs on (kan_grouped.hip).
+enum HalfCfg { kBig, kMid, kSmall, kFew };
+struct HalfPlan {
+  HalfCfg cfg;
+  int cuts, run;
+};
+HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K);
+constexpr int kFewRows = 16;
+bool takes_few(int dtype, int op, int64_t T, int64_t E);
+
+// Operands brought onto 16 bytes first, where that saves more than it takes.
+struct AlignPlan {
+  bool a, b;
+  int64_t a_rows, a_cols, b_rows, b_cols;
+  int b_value;  // bytes of a value of B
+  size_t a_bytes, b_bytes;
+};
+AlignPlan align_plan(int op, int format, const void* A, const void* B, int64_t T, int64_t E,
+                     int64_t N, int64_t K);
+double align_saves_us(int op, int64_t T, int64_t N, int64_t K);
+AlignPlan align_operands(const void* A, int64_t a_rows, int64_t a_cols, const void* B,
+                         int64_t b_rows, int64_t b_cols, int b_value, double saved_us);
+// Copies the operands that `al` names to ws, one behind the other, and has p take
+// them from there.
+int launch_aligned(const AlignPlan& al, GroupedParams* p, char* ws, hipStream_t st);
+
+// A product as planned: p's operands, sizes, part (of product_part_bytes) and scale
+// are set.  fp32 operands are contiguous.
+HalfPlan product_plan(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K);
+size_t product_part_bytes(int op, const HalfPlan& pl, int64_t T, int64_t E, int64_t N, int64_t K);
+int launch_product(int dtype, int op, GroupedParams p, const HalfPlan& pl, hipStream_t st);
 
 // fp32 products on the split contraction engine's tiles (kan_gemm.hip); the rows
 // of a tile and of an item and the cuts of a sum there.

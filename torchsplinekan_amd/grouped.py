@@ -31,7 +31,8 @@ def _native():
 
 
 def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
-    """One grouped product into `out`; b may be an Activation8 (WEIGHT)."""
+    """One grouped product into `out`; b may be an Activation8 (WEIGHT), offsets None
+    with one group."""
     lib = _native()
     if out.numel() == 0:
         return out
@@ -46,7 +47,8 @@ def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
     if nbytes.value:
         ws = torch.empty(nbytes.value, dtype=torch.uint8, device=out.device)
     lib.launch(lib.LIB.kan_hip_grouped_matmul, out.device, code, op, pa, pb, form, scale, group,
-               lib.ptr(offsets), int(offsets.dtype == torch.int64), T, E, N, K, out.data_ptr(),
+               lib.ptr(offsets),
+               int(offsets is not None and offsets.dtype == torch.int64), T, E, N, K, out.data_ptr(),
                lib.ptr(ws), nbytes.value)
     return out
 

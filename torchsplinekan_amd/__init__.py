@@ -12,11 +12,13 @@ from .experts import KANExperts, KANExpertStack
 from .act8 import Activation8, checkpoint_8bit, quantize_activation
 from .grouped import grouped_linear
 from .gated import gated_linear
+from .losses import linear_cross_entropy, linear_distillation
 from .residual import residual_norm
 from .layernorm import layer_norm
 
 __version__ = "0.1.0"
 
 __all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "Activation8", "checkpoint_8bit",
-           "quantize_activation", "grouped_linear", "gated_linear", "residual_norm", "layer_norm", "KANExperts",
+           "quantize_activation", "grouped_linear", "gated_linear", "residual_norm", "layer_norm", "linear_cross_entropy",
+           "linear_distillation", "KANExperts",
            "KANExpertStack", "__version__"]

@@ -20,7 +20,7 @@ LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["kan_capi.hip", "kan_basis.hip", "kan_gemm.hip", "kan_edge.hip", "kan_edge_mfma.hip",
            "kan_edge_mfma64.hip", "kan_span.hip", "kan_refit.hip", "kan_stream.hip", "kan_reg.hip",
            "kan_norm.hip", "kan_norm_grad.hip", "kan_layernorm.hip", "kan_act8.hip",
-           "kan_grouped.hip", "kan_gated.hip"]
+           "kan_grouped.hip", "kan_gated.hip", "kan_vocab.hip"]
 ARCH = "gfx950"
 
 COMMON_FLAGS = [

@@ -1,0 +1,928 @@
+// Losses of logits z = x W^T, x [T, D], W [V, D], that are never kept whole.  Row t
+// has a target distribution p on a few ids (one with p = 1 for the cross entropy, a
+// teacher's top ids for distillation) and a temperature tau; with q = softmax(z / tau)
+// over all V
+//   loss_t = tau^2 sum_j p_j (log p_j - log q_{id_j})
+//   dz_t   = g_t tau (q - sum_j p_j e_{id_j}),   dx = dz W,   dW = dz^T x.
+// (tau = 1 and one id: lse(z) - z_id and g_t (q - e_id).)
+//
+// Forward: the product's tiles end in each row's maximum, sum of exponentials and
+// sum of p z over the tile's columns; a second kernel joins a row's tiles.  Backward:
+// piece by piece of the vocabulary the product again, whose tiles end in dz in the
+// operands' type, and dx += dz W, dW = dz^T x from that piece.  4/3 of the
+// operations that kept logits would take, and 2 bytes a logit of one piece.
+//
+// A row's logits are taken from its maximum before the exponential, and p before
+// the rounding to 16 bits: where q is nearly p what is left keeps its accuracy.
+// dz is rounded to 16 bits as (q - p) w with w = 1 in rows that all count alike (in
+// f16 2^15, so that probabilities of 1e-8 still are normal numbers); the common
+// factor g tau is applied to the float32 sums of dx and dW.
+//
+// Everything is added in a fixed order; no atomics.
+#include "kan_grouped.h"
+#include "kan_tile.h"
+
+namespace kan {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNoId = 0x7fffffff;  // past every column
+
+struct VocabParams {
+  const void *x, *w;
+  int64_t T, V, D, k;
+  int64_t ldx, ldw;
+  float tau;
+  // kept for the backward pass
+  float *top, *total;  // [T]: a row's maximum and its sum of exp((z - top) / tau)
+  float* flag;         // [T]: 1; 0: the row does not count; NaN: an id that is no column
+  float* count;        // rows that count
+  int* ids;            // [T, k]: ascending (kNoId: absent)
+  float* prob;         // [T, k]: p
+  // of a call
+  float* entropy;      // [T]: sum_j p_j log p_j
+  float* stats;        // [3, tiles, T]
+  int tiles;           // of all pieces
+  float* weight;       // [T]: w
+  float* z;            // fp32: [T, cols] logits, then dz of a piece
+  void* G;             // 16 bits: [T, ldg] dz of a piece, zeros behind its columns
+  int64_t ldg;
+  int64_t v0, cols;    // the piece
+};
+
+// ---- targets ----------------------------------------------------------------------
+__global__ __launch_bounds__(256) void vocab_targets_kernel(VocabParams p, const void* target,
+                                                            int is64, int64_t ignore) {
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= p.T) return;
+  const int64_t id = is64 ? static_cast<const int64_t*>(target)[t]
+                          : (int64_t)static_cast<const int*>(target)[t];
+  const bool in = id >= 0 && id < p.V && id != ignore;
+  p.ids[t] = in ? (int)id : kNoId;
+  p.prob[t] = in ? 1.0f : 0.0f;
+  p.flag[t] = in ? 1.0f : id == ignore ? 0.0f : NAN;
+  p.entropy[t] = 0.0f;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+
+// One wave a row: p = softmax(teacher / tau) over its ids, sorted by id (a place is the
+// number of smaller ones, so equal ids keep their order).
+constexpr int64_t kMaxTop = 1024;
+__global__ __launch_bounds__(64) void vocab_teacher_kernel(VocabParams p, const void* ids, int is64,
+                                                           const float* __restrict__ teacher) {
+  __shared__ int id_of[kMaxTop];
+  __shared__ float value_of[kMaxTop];
+  const int64_t t = blockIdx.x, base = t * p.k;
+  const int k = (int)p.k, lane = threadIdx.x;
+  float top = -INFINITY;
+  bool bad = false;
+  for (int j = lane; j < k; j += 64) {
+    const int64_t id = is64 ? static_cast<const int64_t*>(ids)[base + j]
+                            : (int64_t)static_cast<const int*>(ids)[base + j];
+    const bool in = id >= 0 && id < p.V;
+    const float v = in ? teacher[base + j] / p.tau : -INFINITY;
+    bad |= id >= p.V;
+    id_of[j] = in ? (int)id : kNoId;
+    value_of[j] = v;
+    top = fmaxf(top, v);
+  }
+  top = wave_max(top);
+  if (top == -INFINITY) top = 0.0f;
+  float sum = 0.0f;
+  for (int j = lane; j < k; j += 64) {
+    const float e = expf(value_of[j] - top);
+    sum += e;
+  }
+  sum = wave_sum(sum);
+  const float log_sum = logf(sum);
+  __syncthreads();
+  float entropy = 0.0f;
+  for (int j = lane; j < k; j += 64) {
+    const int id = id_of[j];
+    const float v = value_of[j], e = expf(v - top);
+    const float prob = sum == 0.0f ? 0.0f : e / sum;
+    if (!(prob == 0.0f)) entropy += prob * (v - top - log_sum);
+    int place = 0;
+    for (int i = 0; i < k; ++i) place += id_of[i] < id || (id_of[i] == id && i < j);
+    p.ids[base + place] = id;
+    p.prob[base + place] = prob;
+  }
+  entropy = wave_sum(entropy);
+  bad = __any(bad);
+  if (lane == 0) {
+    p.entropy[t] = entropy;
+    p.flag[t] = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f;
+  }
+}
+
+// The first of a row's k ascending ids that is `from` or more.
+__device__ __forceinline__ int first_id(const int* __restrict__ ids, int k, int from) {
+  int lo = 0, hi = k;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ids[mid] < from) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// ---- tiles in 16 bits -------------------------------------------------------------
+// A lane holds rows 32 i + (lane & 31) of its wave's and 32 columns: 32 j + 8 q +
+// 4 (lane >> 5) + s at acc[i][j][4 q + s].
+template <typename T, class G, int MODE, bool GRAD>
+__global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, GroupedParams g,
+                                                           int tiles_n) {
+  constexpr int BM = G::BM, BN = G::BN, FM = G::FM, WN = G::WN;
+  static_assert(G::FN == 2, "a wave has 64 columns");
+  __shared__ __align__(16) char lds[2 * G::kBuf];
+  __shared__ int first[BM], last[BM];
+  __shared__ float row_top[GRAD ? BM : 1], row_part[GRAD ? BM : 1], row_weight[GRAD ? BM : 1];
+  RowTile t;
+  int tn;
+  if (!row_tile(g, BM, tiles_n, &t, &tn)) return;
+  const int64_t n0 = (int64_t)tn * BN;
+  const float c = kLog2e / p.tau;
+  for (int r = threadIdx.x; r < BM; r += G::NT) {
+    const int64_t row = t.m0 + r;
+    int lo = 0, hi = 0;
+    if (row < t.m1) {
+      const int* ids = p.ids + row * p.k;
+      const int from = (int)(p.v0 + n0);
+      lo = first_id(ids, (int)p.k, from);
+      hi = lo;
+      while (hi < p.k && ids[hi] < from + BN) ++hi;
+      if constexpr (GRAD) {
+        row_top[r] = p.top[row];
+        row_part[r] = 1.0f / p.total[row];
+        row_weight[r] = p.weight[row];
+      }
+    }
+    first[r] = lo;
+    last[r] = hi;
+  }
+  Operand<T, BM, true, MODE, G::NT> a;
+  Operand<T, BN, true, MODE, G::NT> b;
+  a.init(p.x, p.ldx, t.m0, t.m1 - t.m0);
+  b.init(p.w, p.ldw, p.v0 + n0, p.cols - n0);
+  f32x16 acc[FM][2];
+  tile_loop<T, G, true, true>(a, b, 0, p.D, lds, acc);
+  __syncthreads();
+
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int64_t left = p.cols - n0 - wn * 64;  // columns from the wave's first on
+  auto col_of = [&](int j, int v) { return 32 * j + 8 * (v >> 2) + 4 * half + (v & 3); };
+  // f(entry) for the row's ids in the wave's columns, the same number of turns in all lanes
+  auto entries = [&](int r, int64_t row, auto f) __attribute__((always_inline)) {
+    const int lo = first[r], hi = last[r];
+    for (int e = lo; __any(e < hi); ++e) {
+      int at = -1;
+      float prob = 0.0f;
+      if (e < hi) {
+        at = p.ids[row * p.k + e] - (int)(p.v0 + n0) - wn * 64;
+        prob = p.prob[row * p.k + e];
+      }
+      f(at, prob);
+    }
+  };
+  if constexpr (!GRAD) {
+    float* red = reinterpret_cast<float*>(lds);  // [3][WN][BM]
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int r = (wm * FM + i) * 32 + (lane & 31);
+      if (left < 64) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (col_of(j, v) >= left) acc[i][j][v] = -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, acc[i][j][v]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float from = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f((acc[i][j][v] - from) * c);
+      sum += __shfl_xor(sum, 32);
+      float dot = 0.0f;
+      entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
+        if (at < 0 || at >= 64 || ((at >> 2) & 1) != half || prob == 0.0f) return;
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (col_of(j, v) == at) z = acc[i][j][v];
+        dot += prob * z;
+      });
+      dot += __shfl_xor(dot, 32);
+      if (half == 0) {
+        red[wn * BM + r] = top;
+        red[(WN + wn) * BM + r] = sum;
+        red[(2 * WN + wn) * BM + r] = dot;
+      }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < BM; r += G::NT) {
+      if (t.m0 + r >= t.m1) break;
+      float top = -INFINITY, sum = 0.0f, dot = 0.0f;
+#pragma unroll
+      for (int q = 0; q < WN; ++q) top = fmaxf(top, red[q * BM + r]);
+      const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int q = 0; q < WN; ++q) {
+        sum += red[(WN + q) * BM + r] * __builtin_amdgcn_exp2f((red[q * BM + r] - from) * c);
+        dot += red[(2 * WN + q) * BM + r];
+      }
+      float* out = p.stats + (int64_t)tn * p.T + t.m0 + r;
+      out[0] = top;
+      out[p.tiles * p.T] = sum;
+      out[2 * p.tiles * p.T] = dot;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int r = (wm * FM + i) * 32 + (lane & 31);
+      const float top = row_top[r], part = row_part[r], weight = row_weight[r];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          acc[i][j][v] = __builtin_amdgcn_exp2f((acc[i][j][v] - top) * c) * part;
+      entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[i][j][v] -= col_of(j, v) == at ? prob : 0.0f;
+      });
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          acc[i][j][v] = weight == 0.0f || col_of(j, v) >= left ? 0.0f : acc[i][j][v] * weight;
+    }
+    // through LDS, to become whole 16-byte pieces of rows
+    constexpr int kWaveRows = FM * 32, kRowBytes = 128, kChunks = 8;
+    char* stage = lds + wave * kWaveRows * kRowBytes;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int r = i * 32 + (lane & 31);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          t4 v;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) v[u] = (T)acc[i][j][4 * q + u];
+          const int ch = (4 * j + q) ^ (r & (kChunks - 1));
+          *reinterpret_cast<t4*>(stage + r * kRowBytes + ch * 16 + half * 8) = v;
+        }
+    }
+    const int64_t row0 = t.m0 + wm * kWaveRows, col0 = n0 + wn * 64;
+#pragma unroll 4
+    for (int it = 0; it < kWaveRows / 8; ++it) {
+      const int r = it * 8 + lane / kChunks, ch = lane % kChunks;
+      const u32x4 v =
+          *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + ((ch ^ (r & (kChunks - 1))) * 16));
+      const int64_t row = row0 + r, col = col0 + 8 * ch;
+      if (row < t.m1 && col < p.ldg)
+        *reinterpret_cast<u32x4*>(static_cast<T*>(p.G) + row * p.ldg + col) = v;
+    }
+  }
+}
+
+// ---- fp32: logits of a piece in memory ----------------------------------------------
+// A wave has kSpan columns of a row, column lane + 64 i at v[i].
+constexpr int kSpan = 1024, kSpanValues = kSpan / 64;
+template <bool GRAD>
+__global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= p.T) return;
+  const float c = kLog2e / p.tau;
+  for (int64_t n0 = (int64_t)blockIdx.y * kSpan; n0 < p.cols; n0 += (int64_t)gridDim.y * kSpan) {
+    float* z = p.z + row * p.cols + n0;
+    const int64_t left = p.cols - n0;
+    float v[kSpanValues];
+#pragma unroll
+    for (int i = 0; i < kSpanValues; ++i) v[i] = lane + 64 * i < left ? z[lane + 64 * i] : -INFINITY;
+    const int* ids = p.ids + row * p.k;
+    const float* prob = p.prob + row * p.k;
+    const int from = (int)(p.v0 + n0), k = (int)p.k;
+    int e = first_id(ids, k, from);
+    if constexpr (!GRAD) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kSpanValues; ++i) top = fmaxf(top, v[i]);
+      top = wave_max(top);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSpanValues; ++i) sum += exp2f((v[i] - base) * c);
+      sum = wave_sum(sum);
+      float dot = 0.0f;
+      for (; e < k && ids[e] < from + kSpan; ++e)
+        if (prob[e] != 0.0f) dot += prob[e] * z[ids[e] - from];
+      if (lane == 0) {
+        float* out = p.stats + ((p.v0 + n0) / kSpan) * p.T + row;
+        out[0] = top;
+        out[p.tiles * p.T] = sum;
+        out[2 * p.tiles * p.T] = dot;
+      }
+    } else {
+      const float top = p.top[row], part = 1.0f / p.total[row], weight = p.weight[row];
+#pragma unroll
+      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f((v[i] - top) * c) * part;
+      for (; e < k && ids[e] < from + kSpan; ++e) {
+        const int at = ids[e] - from;
+#pragma unroll
+        for (int i = 0; i < kSpanValues; ++i) v[i] -= lane + 64 * i == at ? prob[e] : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < kSpanValues; ++i)
+        if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * weight;
+    }
+  }
+}
+
+// ---- rows ---------------------------------------------------------------------------
+// A row's tiles joined: 16 lanes of tiles a row, then their results in order.
+constexpr int kTileLanes = 16;
+__device__ __forceinline__ void join(float* top, float* sum, float m, float s, float c) {
+  const float most = fmaxf(*top, m), from = most == -INFINITY ? 0.0f : most;
+  *sum = *sum * exp2f((*top - from) * c) + s * exp2f((m - from) * c);
+  *top = most;
+}
+__global__ __launch_bounds__(64 * kTileLanes) void vocab_rows_kernel(VocabParams p,
+                                                                     float* __restrict__ loss) {
+  __shared__ float red[3][kTileLanes][64];
+  const int lane = threadIdx.x & 63, tl = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 64 + lane;
+  const float c = kLog2e / p.tau;
+  float top = -INFINITY, sum = 0.0f, dot = 0.0f;
+  if (row < p.T) {
+    for (int i = tl; i < p.tiles; i += kTileLanes) {
+      const float* at = p.stats + (int64_t)i * p.T + row;
+      join(&top, &sum, at[0], at[p.tiles * p.T], c);
+      dot += at[2 * p.tiles * p.T];
+    }
+  }
+  red[0][tl][lane] = top;
+  red[1][tl][lane] = sum;
+  red[2][tl][lane] = dot;
+  __syncthreads();
+  if (tl != 0 || row >= p.T) return;
+#pragma unroll
+  for (int i = 1; i < kTileLanes; ++i) {
+    join(&top, &sum, red[0][i][lane], red[1][i][lane], c);
+    dot += red[2][i][lane];
+  }
+  const float flag = p.flag[row];
+  p.top[row] = top;
+  p.total[row] = sum;
+  loss[row] = flag == 0.0f ? 0.0f
+              : flag != flag ? flag
+                             : p.tau * p.tau * (p.entropy[row] + (top - dot) / p.tau + logf(sum));
+}
+
+constexpr int kOneBlock = 1024;
+template <typename V>
+__device__ __forceinline__ V block_total(V v, V* red) {
+  __syncthreads();
+  red[threadIdx.x] = v;
+  __syncthreads();
+  for (int m = kOneBlock / 2; m > 0; m /= 2) {
+    if (threadIdx.x < m) red[threadIdx.x] += red[threadIdx.x + m];
+    __syncthreads();
+  }
+  return red[0];
+}
+// The sum or mean of the rows that count.
+__global__ __launch_bounds__(kOneBlock) void vocab_sum_kernel(VocabParams p,
+                                                              const float* __restrict__ rows,
+                                                              int mean, float* __restrict__ loss) {
+  __shared__ double red[kOneBlock];
+  double sum = 0.0, count = 0.0;
+  for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock) {
+    sum += rows[t];
+    count += p.flag[t] == 0.0f ? 0.0 : 1.0;
+  }
+  sum = block_total(sum, red);
+  count = block_total(count, red);
+  if (threadIdx.x != 0) return;
+  *p.count = (float)count;
+  *loss = (float)(mean ? sum / (count > 0.0 ? count : 1.0) : sum);
+}
+
+// w and the common factor from the gradient of the loss: of a scalar loss g is one
+// value (over the count for a mean) and w = flag; of the rows' losses (one block)
+// w = g_t / max|g|; w times `unit`, a power of 2.  fp32: w is the whole factor.
+__global__ __launch_bounds__(kOneBlock) void vocab_weights_kernel(VocabParams p,
+                                                                  const float* __restrict__ g,
+                                                                  int reduction, int fp32,
+                                                                  float unit,
+                                                                  float* __restrict__ scale) {
+  __shared__ float red[kOneBlock];
+  const bool rows = reduction == KAN_REDUCE_NONE;
+  float common = p.tau, most = 1.0f;
+  if (!rows) {
+    common *= *g;
+    if (reduction == KAN_REDUCE_MEAN) common /= fmaxf(*p.count, 1.0f);
+  } else if (!fp32) {
+    most = 0.0f;
+    for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock)
+      if (p.flag[t] != 0.0f) most = fmaxf(most, fabsf(g[t]));
+    red[threadIdx.x] = most;
+    __syncthreads();
+    for (int m = kOneBlock / 2; m > 0; m /= 2) {
+      if (threadIdx.x < m) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + m]);
+      __syncthreads();
+    }
+    most = red[0] == 0.0f ? 1.0f : red[0];
+    common *= most;
+  }
+  for (int64_t t = (int64_t)blockIdx.x * kOneBlock + threadIdx.x; t < p.T;
+       t += (int64_t)gridDim.x * kOneBlock) {
+    const float flag = p.flag[t];
+    const float w = rows ? flag * g[t] / most : flag;
+    p.weight[t] = flag == 0.0f ? 0.0f : w * (fp32 ? common : unit);
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = common / unit;
+}
+
+// x's rows for the weight's gradient, those that do not count as zeros: what they hold
+// may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld], zeros behind D.
+template <typename T>
+__global__ __launch_bounds__(256) void vocab_copy_kernel(VocabParams p, T* __restrict__ out,
+                                                         int64_t ld, int whole) {
+  constexpr int V = 16 / sizeof(T);
+  typedef typename VecOf<T, V>::type vec;
+  const int64_t per = ceil_div(ld, V), total = p.T * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, c = (i - row * per) * V;
+    const T* src = static_cast<const T*>(p.x) + row * p.D + c;
+    const bool on = p.flag[row] != 0.0f;
+    vec v;
+    if (on && c + V <= p.D) {
+      v = reinterpret_cast<const LooseVec<T, V>*>(src)->v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = on && c + j < p.D ? src[j] : (T)0.0f;
+    }
+    if (whole) {
+      *reinterpret_cast<vec*>(out + row * ld + c) = v;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (c + j < ld) out[row * ld + c + j] = v[j];
+    }
+  }
+}
+
+// acc (+)= the sum of `cuts` slices; the last piece's call gives out = acc * scale.
+template <typename T>
+__global__ __launch_bounds__(256) void vocab_add_kernel(const float* __restrict__ part, int cuts,
+                                                        int64_t count, float* __restrict__ acc,
+                                                        int start, const float* __restrict__ scale,
+                                                        T* __restrict__ out) {
+  const float factor = scale == nullptr ? 1.0f : *scale;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count;
+       i += (int64_t)gridDim.x * 256) {
+    float v = part[i];
+#pragma unroll 8
+    for (int q = 1; q < cuts; ++q) v += part[q * count + i];
+    if (!start) v += acc[i];
+    if (out == nullptr) acc[i] = v;
+    else out[i] = (T)(v * factor);
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------
+// Places in a workspace, each on 16 bytes.
+struct Places {
+  char* base;
+  size_t bytes;
+  template <typename T = char>
+  T* take(size_t count) {
+    T* at = reinterpret_cast<T*>(base + bytes);
+    bytes = (size_t)round_up((int64_t)(bytes + count * sizeof(T)), 16);
+    return at;
+  }
+};
+
+// 512 MiB of a piece's logits or dz: 8192 rows of 32768 columns in 16 bits, products
+// that are as long as the tiles can use.
+constexpr int64_t kPieceBytes = (int64_t)1 << 29;
+int64_t piece_columns(int dtype, int64_t T, int64_t V) {
+  const int64_t most =
+      std::max<int64_t>(kSpan, kPieceBytes / (T * (int64_t)dtype_bytes(dtype)) / kSpan * kSpan);
+  if (most >= V) return V;
+  return round_up(ceil_div(V, ceil_div(V, most)), kSpan);
+}
+size_t kept_floats(int64_t T, int64_t k) { return (size_t)(3 * T + 4 + 2 * T * k); }
+void set_kept(VocabParams* p, void* kept) {
+  p->top = static_cast<float*>(kept);
+  p->total = p->top + p->T;
+  p->flag = p->total + p->T;
+  p->count = p->flag + p->T;
+  p->prob = p->count + 4;
+  p->ids = reinterpret_cast<int*>(p->prob + p->T * p->k);
+}
+GroupedParams product_of(int64_t T, int64_t N, int64_t K) {
+  GroupedParams g{};
+  g.E = 1;
+  g.T = T;
+  g.N = N;
+  g.K = K;
+  g.lda = g.ldb = K;
+  return g;
+}
+// (the products' own rule for few rows does not hold here: those tiles end in sums)
+HalfCfg tile_of(int64_t T, int64_t cols, int64_t D) {
+  return half_plan(KAN_GROUPED_FORWARD, T, 1, cols, D).cfg;
+}
+int64_t tile_columns(HalfCfg cfg) { return cfg == kSmall ? 128 : 256; }
+
+template <typename T, class G, bool GRAD>
+int launch_vocab_tile(const VocabParams& p, hipStream_t st) {
+  GroupedParams g = product_of(p.T, p.cols, p.D);
+  const int64_t tiles_n = ceil_div(p.cols, G::BN), blocks = row_grid(g, G::BM, tiles_n);
+  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "vocab_loss: too many tiles");
+  if (whole_rows(p.x, p.ldx) && whole_rows(p.w, p.ldw))
+    vocab_tile_kernel<T, G, kDirect, GRAD>
+        <<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, g, (int)tiles_n);
+  else
+    vocab_tile_kernel<T, G, kGuarded, GRAD>
+        <<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, g, (int)tiles_n);
+  return check_launch("vocab_loss");
+}
+template <typename T, bool GRAD>
+int launch_vocab_half(const VocabParams& p, HalfCfg cfg, hipStream_t st) {
+  return cfg == kBig   ? launch_vocab_tile<T, TileBig, GRAD>(p, st)
+         : cfg == kMid ? launch_vocab_tile<T, TileMid, GRAD>(p, st)
+                       : launch_vocab_tile<T, TileSmall, GRAD>(p, st);
+}
+template <bool GRAD>
+int launch_vocab_tiles(int dtype, const VocabParams& p, HalfCfg cfg, hipStream_t st) {
+  return dtype == KAN_DTYPE_BF16 ? launch_vocab_half<bf16, GRAD>(p, cfg, st)
+                                 : launch_vocab_half<f16, GRAD>(p, cfg, st);
+}
+template <bool GRAD>
+int launch_vocab_span(const VocabParams& p, hipStream_t st) {
+  const int64_t spans = std::min<int64_t>(ceil_div(p.cols, kSpan), 65535);
+  vocab_span_kernel<GRAD><<<dim3((unsigned)ceil_div(p.T, 4), (unsigned)spans), 256, 0, st>>>(p);
+  return check_launch("vocab_loss");
+}
+
+int check_vocab(const char* who, int dtype, int64_t T, int64_t V, int64_t D, int64_t k, double tau,
+                int reduction) {
+  if (!dtype_is_operator(dtype))
+    return set_error(KAN_ERR_INVALID, "%s: dtype must be FP32, BF16 or FP16 (code %d)", who, dtype);
+  if (T < 0 || V < 1 || D < 1 || k < 1)
+    return set_error(KAN_ERR_INVALID, "%s: sizes must be positive", who);
+  if (!(tau > 0.0) || tau > 1e30 || tau < 1e-30)
+    return set_error(KAN_ERR_INVALID, "%s: the temperature must be positive and finite", who);
+  if (reduction < KAN_REDUCE_NONE || reduction > KAN_REDUCE_MEAN)
+    return set_error(KAN_ERR_INVALID, "%s: unknown reduction %d", who, reduction);
+  if (T > 0x3fffffff || V > (1 << 22) || D > (1 << 22) || k > kMaxTop)
+    return set_error(KAN_ERR_LIMIT,
+                     "%s: at most 2^30 - 1 rows, 2^22 columns and inputs and %d ids a row", who,
+                     (int)kMaxTop);
+  return KAN_OK;
+}
+
+// ---- a call's workspace ------------------------------------------------------------------
+struct ForwardPlan {
+  HalfCfg cfg;
+  AlignPlan align;
+  int64_t piece;
+  HalfPlan product;  // fp32
+  char* aligned;
+  float *stats, *entropy, *rows, *z, *part;
+  int tiles;
+  size_t bytes;
+};
+ForwardPlan plan_forward(int dtype, const void* x, const void* w, int64_t T, int64_t V, int64_t D,
+                         char* ws) {
+  ForwardPlan f{};
+  Places at{ws, 0};
+  if (dtype == KAN_DTYPE_F32) {
+    f.piece = piece_columns(dtype, T, V);
+    f.tiles = (int)ceil_div(V, kSpan);
+    f.product = product_plan(dtype, KAN_GROUPED_FORWARD, T, 1, f.piece, D);
+    f.z = at.take<float>((size_t)(T * f.piece));
+    // (a shorter last piece may be cut more often, but never into more values)
+    size_t part = product_part_bytes(KAN_GROUPED_FORWARD, f.product, T, 1, f.piece, D);
+    const int64_t rest = V % f.piece;
+    if (rest != 0)
+      part = std::max(part, product_part_bytes(KAN_GROUPED_FORWARD,
+                                               product_plan(dtype, KAN_GROUPED_FORWARD, T, 1, rest, D),
+                                               T, 1, rest, D));
+    f.part = part == 0 ? nullptr : at.take<float>(part / 4);
+  } else {
+    f.piece = V;
+    f.cfg = tile_of(T, V, D);
+    f.tiles = (int)ceil_div(V, tile_columns(f.cfg));
+    f.align = align_operands(x, T, D, w, V, D, 2, align_saves_us(KAN_GROUPED_FORWARD, T, V, D));
+    f.aligned = at.take(f.align.a_bytes + f.align.b_bytes);
+  }
+  f.stats = at.take<float>((size_t)(3 * T) * (size_t)f.tiles);
+  f.entropy = at.take<float>((size_t)T);
+  f.rows = at.take<float>((size_t)T);
+  f.bytes = at.bytes;
+  return f;
+}
+
+struct BackwardPlan {
+  HalfCfg cfg;
+  AlignPlan align;
+  int64_t piece, ldg, ldx;
+  char *rows, *aligned, *G;  // rows: x's for the weight's gradient
+  float *weight, *scale, *part, *slices, *acc;
+  size_t bytes;
+};
+BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, int64_t V, int64_t D,
+                           bool dx, bool dw, char* ws) {
+  BackwardPlan b{};
+  Places at{ws, 0};
+  const bool half = dtype != KAN_DTYPE_F32;
+  b.piece = piece_columns(dtype, T, V);
+  b.ldg = half ? round_up(b.piece, 8) : b.piece;
+  if (half) {
+    b.cfg = tile_of(T, b.piece, D);
+    double saved = align_saves_us(KAN_GROUPED_FORWARD, T, V, D);
+    if (dx) saved += align_saves_us(KAN_GROUPED_INPUT, T, V, D);
+    if (dw) saved += align_saves_us(KAN_GROUPED_WEIGHT, T, V, D);
+    // (rows copied for dw lie on 16 bytes)
+    b.align = align_operands(dw ? nullptr : x, T, dw ? round_up(D, 8) : D, w, V, D, 2, saved);
+    b.aligned = at.take(b.align.a_bytes + b.align.b_bytes);
+  }
+  b.ldx = half ? round_up(D, 8) : D;
+  if (dw) b.rows = at.take((size_t)(T * b.ldx) * dtype_bytes(dtype));
+  b.weight = at.take<float>((size_t)T);
+  b.scale = at.take<float>(1);
+  b.G = at.take((size_t)(T * b.ldg) * dtype_bytes(dtype));
+  size_t part = 0, slices = 0;
+  const int64_t rest = V % b.piece;
+  for (const int64_t cols : {b.piece, rest}) {
+    if (cols == 0) continue;
+    auto need = [&](int op) {
+      return product_part_bytes(op, product_plan(dtype, op, T, 1, cols, D), T, 1, cols, D);
+    };
+    if (!half) part = std::max(part, need(KAN_GROUPED_FORWARD));
+    if (dw) part = std::max(part, need(KAN_GROUPED_WEIGHT));
+    if (dx && (!half || b.piece == V)) part = std::max(part, need(KAN_GROUPED_INPUT));
+    else if (dx) slices = std::max(slices, need(KAN_GROUPED_INPUT));
+  }
+  if (dx && b.piece < V) {
+    slices = std::max(slices, 4 * (size_t)(T * D));
+    b.slices = at.take<float>(slices / 4);
+    b.acc = at.take<float>((size_t)(T * D));
+  }
+  b.part = part == 0 ? nullptr : at.take<float>(part / 4);
+  b.bytes = at.bytes;
+  return b;
+}
+
+template <typename T>
+void launch_copy(const VocabParams& p, char* out, int64_t ld, hipStream_t st) {
+  constexpr int64_t V = 16 / sizeof(T);
+  const int64_t blocks = std::min<int64_t>(ceil_div(p.T * ceil_div(ld, V), 256), 1 << 16);
+  vocab_copy_kernel<T><<<dim3((unsigned)blocks), 256, 0, st>>>(p, reinterpret_cast<T*>(out), ld,
+                                                               ld % V == 0);
+}
+template <typename T>
+void launch_add(const float* part, int cuts, int64_t count, float* acc, bool start,
+                const float* scale, void* out, hipStream_t st) {
+  vocab_add_kernel<T><<<dim3((unsigned)std::min<int64_t>(ceil_div(count, 256), 8192)), 256, 0, st>>>(
+      part, cuts, count, acc, start ? 1 : 0, scale, static_cast<T*>(out));
+}
+
+}  // namespace
+}  // namespace kan
+
+using namespace kan;
+
+extern "C" {
+
+int kan_hip_vocab_loss_kept(int64_t T, int64_t k, size_t* bytes) {
+  if (bytes == nullptr) return set_error(KAN_ERR_INVALID, "vocab_loss_kept: bytes must not be NULL");
+  const int rc = check_vocab("vocab_loss_kept", KAN_DTYPE_F32, T, 1, 1, k, 1.0, 0);
+  if (rc != KAN_OK) return rc;
+  *bytes = 4 * kept_floats(T, k);
+  return KAN_OK;
+}
+
+int kan_hip_vocab_loss_workspace(int dtype, const void* x, const void* w, int64_t T, int64_t V,
+                                 int64_t D, size_t* bytes) {
+  if (bytes == nullptr)
+    return set_error(KAN_ERR_INVALID, "vocab_loss_workspace: bytes must not be NULL");
+  const int rc = check_vocab("vocab_loss_workspace", dtype, T, V, D, 1, 1.0, 0);
+  if (rc != KAN_OK) return rc;
+  *bytes = T == 0 ? 0 : plan_forward(dtype, x, w, T, V, D, nullptr).bytes;
+  return KAN_OK;
+}
+
+int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids, int ids64,
+                       const float* teacher, int64_t T, int64_t V, int64_t D, int64_t k,
+                       int64_t ignore_index, double temperature, int reduction, float* loss,
+                       void* kept, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "vocab_loss";
+  const int rc = check_vocab(who, dtype, T, V, D, k, temperature, reduction);
+  if (rc != KAN_OK) return rc;
+  if (teacher == nullptr && k != 1)
+    return set_error(KAN_ERR_INVALID, "%s: without a teacher a row has one id", who);
+  if (T == 0) return KAN_OK;
+  if (x == nullptr || w == nullptr || ids == nullptr || loss == nullptr || kept == nullptr)
+    return set_error(KAN_ERR_INVALID, "%s: operands must not be NULL", who);
+  if (!aligned16(kept) || !aligned16(workspace))
+    return set_error(KAN_ERR_INVALID, "%s: kept values and the workspace lie on 16 bytes", who);
+  const ForwardPlan f = plan_forward(dtype, x, w, T, V, D, static_cast<char*>(workspace));
+  if (workspace == nullptr || workspace_bytes < f.bytes)
+    return set_error(KAN_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, f.bytes,
+                     workspace == nullptr ? (size_t)0 : workspace_bytes);
+  VocabParams p{};
+  p.x = x;
+  p.w = w;
+  p.T = T;
+  p.V = V;
+  p.D = p.ldx = p.ldw = D;
+  p.k = k;
+  p.tau = (float)temperature;
+  set_kept(&p, kept);
+  p.entropy = f.entropy;
+  p.stats = f.stats;
+  p.tiles = f.tiles;
+  p.cols = V;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * (double)V * (double)D);
+  if (teacher == nullptr)
+    vocab_targets_kernel<<<dim3((unsigned)ceil_div(T, 256)), 256, 0, st>>>(p, ids, ids64,
+                                                                         ignore_index);
+  else
+    vocab_teacher_kernel<<<dim3((unsigned)T), 64, 0, st>>>(p, ids, ids64, teacher);
+  int e = check_launch(who);
+  if (e != KAN_OK) return e;
+  if (dtype != KAN_DTYPE_F32) {
+    GroupedParams g = product_of(T, V, D);
+    g.A = x;
+    g.B = w;
+    e = launch_aligned(f.align, &g, f.aligned, st);
+    if (e != KAN_OK) return e;
+    p.x = g.A;
+    p.w = g.B;
+    p.ldx = g.lda;
+    p.ldw = g.ldb;
+    e = launch_vocab_tiles<false>(dtype, p, f.cfg, st);
+    if (e != KAN_OK) return e;
+  }
+  for (p.v0 = 0; dtype == KAN_DTYPE_F32 && p.v0 < V; p.v0 += f.piece) {
+    p.cols = std::min(f.piece, V - p.v0);
+    p.z = f.z;
+    GroupedParams g = product_of(T, p.cols, D);
+    g.A = x;
+    g.B = static_cast<const float*>(w) + p.v0 * D;
+    g.C = f.z;
+    const HalfPlan pl = product_plan(dtype, KAN_GROUPED_FORWARD, T, 1, p.cols, D);
+    g.part = pl.cuts > 1 ? f.part : nullptr;
+    e = launch_product(dtype, KAN_GROUPED_FORWARD, g, pl, st);
+    if (e == KAN_OK) e = launch_vocab_span<false>(p, st);
+    if (e != KAN_OK) return e;
+  }
+  float* rows = reduction == KAN_REDUCE_NONE ? loss : f.rows;
+  vocab_rows_kernel<<<dim3((unsigned)ceil_div(T, 64)), 64 * kTileLanes, 0, st>>>(p, rows);
+  if (reduction != KAN_REDUCE_NONE)
+    vocab_sum_kernel<<<1, kOneBlock, 0, st>>>(p, rows, reduction == KAN_REDUCE_MEAN, loss);
+  return check_launch(who);
+}
+
+int kan_hip_vocab_loss_backward_workspace(int dtype, const void* x, const void* w, int64_t T,
+                                          int64_t V, int64_t D, int with_dx, int with_dw,
+                                          size_t* bytes) {
+  if (bytes == nullptr)
+    return set_error(KAN_ERR_INVALID, "vocab_loss_backward_workspace: bytes must not be NULL");
+  const int rc = check_vocab("vocab_loss_backward_workspace", dtype, T, V, D, 1, 1.0, 0);
+  if (rc != KAN_OK) return rc;
+  *bytes = T == 0 ? 0 : plan_backward(dtype, x, w, T, V, D, with_dx != 0, with_dw != 0, nullptr).bytes;
+  return KAN_OK;
+}
+
+int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x, const void* w,
+                                const void* kept, int64_t T, int64_t V, int64_t D, int64_t k,
+                                double temperature, int reduction, void* grad_x, void* grad_w,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "vocab_loss_backward";
+  const int rc = check_vocab(who, dtype, T, V, D, k, temperature, reduction);
+  if (rc != KAN_OK) return rc;
+  if (T == 0 || (grad_x == nullptr && grad_w == nullptr)) return KAN_OK;
+  if (grad_loss == nullptr || x == nullptr || w == nullptr || kept == nullptr)
+    return set_error(KAN_ERR_INVALID, "%s: operands must not be NULL", who);
+  if (!aligned16(kept) || !aligned16(workspace))
+    return set_error(KAN_ERR_INVALID, "%s: kept values and the workspace lie on 16 bytes", who);
+  const BackwardPlan b = plan_backward(dtype, x, w, T, V, D, grad_x != nullptr, grad_w != nullptr,
+                                       static_cast<char*>(workspace));
+  if (workspace == nullptr || workspace_bytes < b.bytes)
+    return set_error(KAN_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, b.bytes,
+                     workspace == nullptr ? (size_t)0 : workspace_bytes);
+  const bool half = dtype != KAN_DTYPE_F32;
+  const int64_t value = (int64_t)dtype_bytes(dtype);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  TimedLaunch timed(kClassContraction, st, 6.0 * (double)T * (double)V * (double)D);
+  VocabParams p{};
+  p.T = T;
+  p.V = V;
+  p.D = D;
+  p.k = k;
+  p.tau = (float)temperature;
+  set_kept(&p, const_cast<void*>(kept));
+  p.weight = b.weight;
+  p.x = x;
+  GroupedParams in = product_of(T, V, D);
+  in.A = x;
+  in.B = w;
+  if (grad_w != nullptr) {
+    in.A = b.rows;
+    in.lda = b.ldx;
+    if (dtype == KAN_DTYPE_F32) launch_copy<float>(p, b.rows, b.ldx, st);
+    else if (dtype == KAN_DTYPE_BF16) launch_copy<bf16>(p, b.rows, b.ldx, st);
+    else launch_copy<f16>(p, b.rows, b.ldx, st);
+  }
+  int e = launch_aligned(b.align, &in, b.aligned, st);
+  if (e != KAN_OK) return e;
+  p.x = in.A;
+  p.w = in.B;
+  p.ldx = in.lda;
+  p.ldw = in.ldb;
+  p.G = b.G;
+  p.z = reinterpret_cast<float*>(b.G);
+  const bool one = half && reduction == KAN_REDUCE_NONE;
+  vocab_weights_kernel<<<dim3(one ? 1 : (unsigned)ceil_div(T, kOneBlock)), kOneBlock, 0, st>>>(
+      p, grad_loss, reduction, half ? 0 : 1, dtype == KAN_DTYPE_F16 ? 32768.0f : 1.0f, b.scale);
+  e = check_launch(who);
+  for (p.v0 = 0; e == KAN_OK && p.v0 < V; p.v0 += b.piece) {
+    p.cols = std::min(b.piece, V - p.v0);
+    const char* wp = static_cast<const char*>(p.w) + p.v0 * p.ldw * value;
+    auto product = [&](int op, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
+                       float* part) {
+      GroupedParams g = product_of(T, p.cols, D);
+      g.A = A;
+      g.B = B;
+      g.lda = lda;
+      g.ldb = ldb;
+      g.C = C;
+      g.scale = half ? b.scale : nullptr;
+      const HalfPlan pl = product_plan(dtype, op, T, 1, p.cols, D);
+      g.part = C == nullptr || product_part_bytes(op, pl, T, 1, p.cols, D) > 0 ? part : nullptr;
+      return launch_product(dtype, op, g, pl, st);
+    };
+    // dz of the piece
+    if (half) {
+      p.ldg = round_up(p.cols, 8);
+      e = launch_vocab_tiles<true>(dtype, p, b.cfg, st);
+    } else {
+      p.ldg = p.cols;
+      e = product(KAN_GROUPED_FORWARD, p.x, D, wp, D, p.z, b.part);
+      if (e == KAN_OK) e = launch_vocab_span<true>(p, st);
+    }
+    if (e == KAN_OK && grad_w != nullptr)
+      e = product(KAN_GROUPED_WEIGHT, p.G, p.ldg, p.x, p.ldx,
+                  static_cast<char*>(grad_w) + p.v0 * D * value, b.part);
+    if (e != KAN_OK || grad_x == nullptr) continue;
+    if (b.piece == V) {
+      e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, grad_x, b.part);
+      continue;
+    }
+    int cuts = 1;
+    if (half) {
+      e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, nullptr, b.slices);
+      cuts = product_plan(dtype, KAN_GROUPED_INPUT, T, 1, p.cols, D).cuts;
+    } else {
+      e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, b.slices, b.part);
+    }
+    if (e != KAN_OK) return e;
+    void* out = p.v0 + b.piece >= V ? grad_x : nullptr;
+    const float* scale = half ? b.scale : nullptr;
+    if (dtype == KAN_DTYPE_F32) launch_add<float>(b.slices, cuts, T * D, b.acc, p.v0 == 0, scale, out, st);
+    else if (dtype == KAN_DTYPE_BF16) launch_add<bf16>(b.slices, cuts, T * D, b.acc, p.v0 == 0, scale, out, st);
+    else launch_add<f16>(b.slices, cuts, T * D, b.acc, p.v0 == 0, scale, out, st);
+    e = check_launch(who);
+  }
+  return e;
+}
+
+}  // extern "C"

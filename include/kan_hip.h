@@ -524,22 +524,23 @@ int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* k
 /* Losses of logits z = x w^T (x [T, D], w [V, D]) that are never kept whole.  With
  * p a row's distribution on k ids, tau the temperature and q = softmax(z / tau):
  *   loss_t = tau^2 sum_j p_j (log p_j - log q_{id_j}).
- * teacher NULL: cross entropy, k = 1, p = 1; rows whose id is ignore_index do not
- * count.  teacher [T, k]: p = softmax(teacher / tau) over the row's ids; ids below 0
+ * teacher NULL: cross entropy, k = 0, ids [T] with p = 1 each; rows whose id is
+ * ignore_index do not count.  teacher [T, k]: p = softmax(teacher / tau) over the row's ids; ids below 0
  * are absent, equal ids add, and rows without any do not count.  ids [T, k] are int32 or int64
  * (ids64); one that is neither a column nor such makes its row's loss and its
  * gradients NaN.  A row that does not count may hold
  * anything.  reduction: the rows' losses [T] (0 where a row does not count),
  * their sum, or their mean over the rows that count (0 without any).  kept
  * (kan_hip_vocab_loss_kept bytes) is written by the forward and read by the
- * backward.  grad_x [T, D], grad_w [V, D], either of which may be NULL (with_dx,
+ * backward, which takes a cross entropy's ids again too.  (The logits of at most 64
+ * columns are kept.)  grad_x [T, D], grad_w [V, D], either of which may be NULL (with_dx,
  * with_dw: whether it will be given).  V and D are positive, T < 2^30, V and D <=
  * 2^22, k <= 1024.  Workspaces depend on the operands' alignment; they and kept lie
  * on 16 bytes.  With T = 0 nothing is written. */
 #define KAN_REDUCE_NONE 0
 #define KAN_REDUCE_SUM 1
 #define KAN_REDUCE_MEAN 2
-int kan_hip_vocab_loss_kept(int64_t T, int64_t k, size_t* bytes);
+int kan_hip_vocab_loss_kept(int64_t T, int64_t V, int64_t k, size_t* bytes);
 int kan_hip_vocab_loss_workspace(int dtype, const void* x, const void* w, int64_t T, int64_t V,
                                  int64_t D, size_t* bytes);
 int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids, int ids64,
@@ -550,9 +551,10 @@ int kan_hip_vocab_loss_backward_workspace(int dtype, const void* x, const void* 
                                           int64_t V, int64_t D, int with_dx, int with_dw,
                                           size_t* bytes);
 int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x, const void* w,
-                                const void* kept, int64_t T, int64_t V, int64_t D, int64_t k,
-                                double temperature, int reduction, void* grad_x, void* grad_w,
-                                void* workspace, size_t workspace_bytes, void* stream);
+                                const void* ids, int ids64, const void* kept, int64_t T, int64_t V,
+                                int64_t D, int64_t k, int64_t ignore_index, double temperature,
+                                int reduction, void* grad_x, void* grad_w, void* workspace,
+                                size_t workspace_bytes, void* stream);
 
 /* Kernel-level timing (measurement support; no counterpart in the
  * reference, whose benchmarks time with torch.profiler,

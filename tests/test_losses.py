@@ -221,13 +221,13 @@ def test_c_entry_refusals():
     from torchsplinekan_amd import _lib as lib
     L, n, p = lib.LIB, ctypes.c_size_t(), 4096
 
-    def call(dtype=2, x=p, ids=p, teacher=None, T=4, V=8, D=8, k=1, tau=1.0, red=2, loss=p, kept=p,
+    def call(dtype=2, x=p, ids=p, teacher=None, T=4, V=8, D=8, k=0, tau=1.0, red=2, loss=p, kept=p,
              ws=p, size=1 << 40):
         return L.kan_hip_vocab_loss(dtype, x, p, ids, 1, teacher, T, V, D, k, -100, tau, red, loss,
                                     kept, ws, size, None)
 
     bad = [dict(dtype=1), dict(x=None), dict(ids=None), dict(loss=None), dict(kept=None), dict(T=-1),
-           dict(V=0), dict(D=0), dict(k=0), dict(k=2), dict(tau=0.0), dict(tau=-1.0),
+           dict(V=0), dict(D=0), dict(k=-1), dict(k=1), dict(teacher=p), dict(tau=0.0), dict(tau=-1.0),
            dict(tau=float("nan")), dict(tau=float("inf")), dict(red=3), dict(kept=p + 4),
            dict(ws=p + 8)]
     for kw in bad:
@@ -236,16 +236,19 @@ def test_c_entry_refusals():
                dict(k=1025, teacher=p)):
         assert call(**kw) == lib.KAN_ERR_LIMIT, kw
     assert call(T=0, x=None, ids=None, loss=None, kept=None, ws=None) == lib.KAN_OK
-    assert L.kan_hip_vocab_loss_kept(5, 3, ctypes.byref(n)) == lib.KAN_OK
+    assert L.kan_hip_vocab_loss_kept(5, 99, 3, ctypes.byref(n)) == lib.KAN_OK
     assert n.value == 4 * (3 * 5 + 4 + 2 * 15)
-    assert L.kan_hip_vocab_loss_kept(5, 3, None) == lib.KAN_ERR_INVALID
+    assert L.kan_hip_vocab_loss_kept(5, 10, 0, ctypes.byref(n)) == lib.KAN_OK
+    assert n.value == 4 * (3 * 5 + 4 + 50)              # (few classes: their logits)
+    assert L.kan_hip_vocab_loss_kept(5, 99, 3, None) == lib.KAN_ERR_INVALID
     assert L.kan_hip_vocab_loss_workspace(2, p, p, 4, 8, 8, None) == lib.KAN_ERR_INVALID
 
-    def back(g=p, dx=p, dw=p, ws=p, size=1 << 40, T=4):
-        return L.kan_hip_vocab_loss_backward(2, g, p, p, p, T, 8, 8, 1, 1.0, 2, dx, dw, ws, size,
-                                             None)
+    def back(g=p, ids=p, dx=p, dw=p, ws=p, size=1 << 40, T=4):
+        return L.kan_hip_vocab_loss_backward(2, g, p, p, ids, 1, p, T, 8, 8, 0, -100, 1.0, 2, dx, dw,
+                                             ws, size, None)
 
     assert back(g=None) == lib.KAN_ERR_INVALID
+    assert back(ids=None) == lib.KAN_ERR_INVALID
     assert back(ws=p + 8) == lib.KAN_ERR_INVALID
     assert back(dx=None, dw=None) == lib.KAN_OK
     assert back(T=0) == lib.KAN_OK
@@ -257,7 +260,7 @@ def test_c_entry_refusals():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("V,D", [(1, 1), (2, 8), (10, 33), (64, 64), (128, 72), (129, 1), (1000, 200),
+@pytest.mark.parametrize("V,D", [(1, 1), (2, 8), (10, 33), (17, 40), (64, 64), (65, 64), (128, 72), (129, 1), (1000, 200),
                                  (1025, 40), (2049, 17)])
 @pytest.mark.parametrize("T", [1, 5, 33, 130, 300])
 def test_cross_entropy_sizes(T, V, D, dtype):
@@ -268,7 +271,7 @@ def test_cross_entropy_sizes(T, V, D, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("T,V,D,k", [(1, 2, 8, 1), (5, 10, 33, 10), (33, 300, 64, 7),
+@pytest.mark.parametrize("T,V,D,k", [(1, 2, 8, 1), (5, 10, 33, 10), (40, 30, 257, 9), (33, 300, 64, 7),
                                      (130, 1000, 72, 64), (70, 2049, 40, 65), (3, 1024, 16, 1024),
                                      (300, 515, 24, 33)])
 @pytest.mark.parametrize("tau", [1.0, 2.5])

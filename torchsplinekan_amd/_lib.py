@@ -121,14 +121,14 @@ SIGNATURES = {
     "kan_hip_gated": (_int, [_int, _int, _vp, _vp, _vp, _int] + [_i64] * 4 + [_vp] * 3
                       + [_sz, _vp]),
     "kan_hip_gated_backward": (_int, [_int, _int, _vp, _vp, _i64, _i64, _vp, _vp]),
-    "kan_hip_vocab_loss_kept": (_int, [_i64] * 2 + [ctypes.POINTER(_sz)]),
+    "kan_hip_vocab_loss_kept": (_int, [_i64] * 3 + [ctypes.POINTER(_sz)]),
     "kan_hip_vocab_loss_workspace": (_int, [_int, _vp, _vp] + [_i64] * 3 + [ctypes.POINTER(_sz)]),
     "kan_hip_vocab_loss": (_int, [_int] + [_vp] * 3 + [_int, _vp] + [_i64] * 5 + [_dbl, _int]
                            + [_vp] * 3 + [_sz, _vp]),
     "kan_hip_vocab_loss_backward_workspace": (_int, [_int, _vp, _vp] + [_i64] * 3
                                               + [_int, _int, ctypes.POINTER(_sz)]),
-    "kan_hip_vocab_loss_backward": (_int, [_int] + [_vp] * 4 + [_i64] * 4 + [_dbl, _int]
-                                    + [_vp] * 3 + [_sz, _vp]),
+    "kan_hip_vocab_loss_backward": (_int, [_int] + [_vp] * 4 + [_int, _vp] + [_i64] * 5
+                                    + [_dbl, _int] + [_vp] * 3 + [_sz, _vp]),
     "kan_hip_timing_enable": (_int, [_int]),
     "kan_hip_timing_read": (_int, [_int, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_i64),
                                    ctypes.POINTER(ctypes.c_double)]),

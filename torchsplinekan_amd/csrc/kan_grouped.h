@@ -275,6 +275,22 @@ __device__ __forceinline__ bool row_tile(const GroupedParams& p, int bm, int til
   }
   return true;
 }
+// The same of rows that are all of one group, whose tiles need no scan (a grid of
+// dense_grid blocks).
+__device__ __forceinline__ void dense_tile(int64_t T, int bm, int tiles_n, RowTile* t, int* tn) {
+  const int tiles_m = (int)((T + bm - 1) / bm);
+  const int id = xcd_remap(blockIdx.x, tiles_m * tiles_n), group = kGroupedM * tiles_n;
+  const int first = id / group * kGroupedM, in = id % group;
+  const int gm = min(tiles_m - first, kGroupedM);
+  *tn = __builtin_amdgcn_readfirstlane(in / gm);
+  const int tile = __builtin_amdgcn_readfirstlane(first + in % gm);
+  t->e = 0;
+  t->m0 = tile * bm;
+  t->m1 = (int)min(T, (int64_t)t->m0 + bm);
+}
+inline int64_t dense_grid(int64_t T, int64_t bm, int64_t tiles_n) {
+  return ceil_div(T, bm) * tiles_n;
+}
 inline int64_t row_grid(const GroupedParams& p, int64_t bm, int64_t tiles_n) {
   return (p.T / bm + p.E + 1) * tiles_n;
 }
@@ -340,6 +356,7 @@ struct HalfPlan {
   int cuts, run;
 };
 HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K);
+HalfPlan long_plan(int64_t T, int64_t N, int64_t K);
 constexpr int kFewRows = 16;
 bool takes_few(int dtype, int op, int64_t T, int64_t E);
 

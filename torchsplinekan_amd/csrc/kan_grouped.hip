@@ -72,15 +72,28 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
   if (OP == 2 ? slot >= 0 : p.part != nullptr) {  // an item of several, a cut's part
     float* part =
         p.part + (OP == 2 ? (int64_t)slot * p.N * p.K : (int64_t)blockIdx.y * p.T * n_end);
+    // (4 columns of a row lie side by side in a lane; value by value the stores of a
+    // whole tile took 100 us and more)
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const bool four = n_end % 4 == 0;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
+        for (int q = 0; q < 4; ++q) {
           const int64_t row = m0 + (wm * FM + i) * 32 + (lane & 31);
-          const int64_t col = n0 + (wn * FN + j) * 32 + 8 * (v >> 2) + 4 * (lane >> 5) + (v & 3);
-          if (row < m_end && col < n_end) part[row * n_end + col] = acc[i][j][v];
+          const int64_t col = n0 + (wn * FN + j) * 32 + 8 * q + 4 * (lane >> 5);
+          if (row >= m_end || col >= n_end) continue;
+          float* at = part + row * n_end + col;
+          if (four) {
+            *reinterpret_cast<f4*>(at) = {acc[i][j][4 * q], acc[i][j][4 * q + 1],
+                                          acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          } else {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              if (col + s < n_end) at[s] = acc[i][j][4 * q + s];
+          }
         }
     return;
   }
@@ -269,6 +282,31 @@ HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K) {
     if (t[c] < t[pl.cfg]) pl.cfg = (HalfCfg)c;
   if (pl.cfg == kSmall) pl.cuts = sum_cuts(small, 2 * cus, ceil_div(depth, kDepth), 0.7);
   return pl;
+}
+
+// The same of one group's long sums over few outputs (dx of a piece of a vocabulary),
+// where cuts pay on every tile: 4096 x 1024 outputs of 65536 terms in bf16 took 738
+// us on 128 x 128 in 2 cuts, 560 on 256 x 256 in 4.  A slab takes 1.7 us on the
+// largest tile; a cut's results are written and read again at 4 TB/s.
+HalfPlan long_plan(int64_t T, int64_t N, int64_t K) {
+  const int cus = device_cu_count();
+  const double slab_us[3] = {1.73, 1.4, 2.0};
+  const int64_t rows[3] = {256, 192, 128}, columns[3] = {256, 256, 128}, slabs = ceil_div(N, kDepth);
+  HalfPlan best{kSmall, 1, kNoRuns};
+  double least = 1e30;
+  for (int c = 0; c < 3; ++c) {
+    const double tiles = (double)ceil_div(T, rows[c]) * (double)ceil_div(K, columns[c]);
+    for (int cuts = 1; cuts <= 32 && (cuts == 1 || slabs / cuts >= 8); ++cuts) {
+      double t = slab_us[c] * rounds(tiles * cuts, c == 2 ? 2.0 * cus : cus) *
+                 (double)ceil_div(slabs, cuts);
+      if (cuts > 1) t += 5.0 + (double)cuts * (double)(T * K) * 8.0 / 4.0e6;
+      if (t < least) {
+        least = t;
+        best = {(HalfCfg)c, cuts, kNoRuns};
+      }
+    }
+  }
+  return best;
 }
 
 namespace {

@@ -285,12 +285,16 @@ __device__ __forceinline__ void slab_barrier() {
   asm volatile("" ::: "memory");
 }
 
+struct Nothing {
+  __device__ __forceinline__ void operator()() const {}
+};
 // acc = the tile's product over k in kbeg .. kend - 1 (KA, KB: K-contiguous
 // operands).  lds: 2 G::kBuf bytes on 16; waves are done with their reads of it
-// only after a barrier.
-template <typename T, class G, bool KA, bool KB, class A, class B>
+// only after a barrier.  meanwhile(): what else a block has to look up, called
+// while its first slab is on its way and before a barrier.
+template <typename T, class G, bool KA, bool KB, class A, class B, class F = Nothing>
 __device__ __forceinline__ void tile_loop(A& a, B& b, int64_t kbeg, int64_t kend, char* lds,
-                                          f32x16 (&acc)[G::FM][G::FN]) {
+                                          f32x16 (&acc)[G::FM][G::FN], const F& meanwhile = F()) {
   constexpr int BM = G::BM, BN = G::BN, FM = G::FM, FN = G::FN;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / G::WN, wn = wave % G::WN;
@@ -387,6 +391,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, int64_t kbeg, int64_t kend
     constexpr std::false_type full{};
     if (whole > 0) start(0, lds, full);
     else start(0, lds, rest);
+    meanwhile();
     finish(lds);
     slab_barrier();
     if (whole > 1) start(1, lds + G::kBuf, full);

@@ -12,8 +12,10 @@
 // operands' type, and dx += dz W, dW = dz^T x from that piece.  4/3 of the
 // operations that kept logits would take, and 2 bytes a logit of one piece.
 //
-// A row's logits are taken from its maximum before the exponential, and p before
-// the rounding to 16 bits: where q is nearly p what is left keeps its accuracy.
+// Exponentials are 2^(z log2(e) / tau - top) from one fused product and difference,
+// so that top, rounded once, is the exact reference of all of a row's; and p is
+// subtracted before the rounding to 16 bits: where q is nearly p what is left keeps
+// its accuracy.
 // dz is rounded to 16 bits as (q - p) w with w = 1 in rows that all count alike (in
 // f16 2^15, so that probabilities of 1e-8 still are normal numbers); the common
 // factor g tau is applied to the float32 sums of dx and dW.
@@ -34,11 +36,17 @@ struct VocabParams {
   int64_t T, V, D, k;
   int64_t ldx, ldw;
   float tau;
+  // cross entropy (k = 1); null: distillation
+  const void* target;  // [T]
+  int target64;
+  int64_t ignore;
   // kept for the backward pass
-  float *top, *total;  // [T]: a row's maximum and its sum of exp((z - top) / tau)
+  float *top, *total;  // [T]: a row's largest z / tau in powers of 2, and its sum of
+                       // 2^(z log2(e) / tau - top)
   float* flag;         // [T]: 1; 0: the row does not count; NaN: an id that is no column
   float* count;        // rows that count
-  int* ids;            // [T, k]: ascending (kNoId: absent)
+  float* logits;       // [T, V] of few classes
+  int* ids;            // [T, k] of distillation: ascending (kNoId: absent)
   float* prob;         // [T, k]: p
   // of a call
   float* entropy;      // [T]: sum_j p_j log p_j
@@ -46,23 +54,20 @@ struct VocabParams {
   int tiles;           // of all pieces
   float* weight;       // [T]: w
   float* z;            // fp32: [T, cols] logits, then dz of a piece
-  void* G;             // 16 bits: [T, ldg] dz of a piece, zeros behind its columns
+  void* G;             // 16 bits: [T, ldg] dz of a piece, zeros behind its columns as far
+                       // as 16 bytes go
   int64_t ldg;
   int64_t v0, cols;    // the piece
 };
 
 // ---- targets ----------------------------------------------------------------------
-__global__ __launch_bounds__(256) void vocab_targets_kernel(VocabParams p, const void* target,
-                                                            int is64, int64_t ignore) {
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= p.T) return;
-  const int64_t id = is64 ? static_cast<const int64_t*>(target)[t]
-                          : (int64_t)static_cast<const int*>(target)[t];
-  const bool in = id >= 0 && id < p.V && id != ignore;
-  p.ids[t] = in ? (int)id : kNoId;
-  p.prob[t] = in ? 1.0f : 0.0f;
-  p.flag[t] = in ? 1.0f : id == ignore ? 0.0f : NAN;
-  p.entropy[t] = 0.0f;
+// Cross entropy: the row's column (kNoId: none) and its flag.
+__device__ __forceinline__ int target_of(const VocabParams& p, int64_t row, float* flag) {
+  const int64_t id = p.target64 ? static_cast<const int64_t*>(p.target)[row]
+                                : (int64_t)static_cast<const int*>(p.target)[row];
+  const bool in = id >= 0 && id < p.V && id != p.ignore;
+  *flag = in ? 1.0f : id == p.ignore ? 0.0f : NAN;
+  return in ? (int)id : kNoId;
 }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -136,57 +141,66 @@ __device__ __forceinline__ int first_id(const int* __restrict__ ids, int k, int 
 // A lane holds rows 32 i + (lane & 31) of its wave's and 32 columns: 32 j + 8 q +
 // 4 (lane >> 5) + s at acc[i][j][4 q + s].
 template <typename T, class G, int MODE, bool GRAD>
-__global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, GroupedParams g,
-                                                           int tiles_n) {
+__global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int tiles_n) {
   constexpr int BM = G::BM, BN = G::BN, FM = G::FM, WN = G::WN;
   static_assert(G::FN == 2, "a wave has 64 columns");
   __shared__ __align__(16) char lds[2 * G::kBuf];
-  __shared__ int first[BM], last[BM];
-  __shared__ float row_top[GRAD ? BM : 1], row_part[GRAD ? BM : 1], row_weight[GRAD ? BM : 1];
+  __shared__ int first[BM], last[BM];  // the row's ids in the tile's columns; its target
+  __shared__ float row_from[GRAD ? BM : 1], row_weight[GRAD ? BM : 1];
   RowTile t;
   int tn;
-  if (!row_tile(g, BM, tiles_n, &t, &tn)) return;
+  dense_tile(p.T, BM, tiles_n, &t, &tn);
   const int64_t n0 = (int64_t)tn * BN;
+  const int col0 = (int)(p.v0 + n0);
   const float c = kLog2e / p.tau;
-  for (int r = threadIdx.x; r < BM; r += G::NT) {
-    const int64_t row = t.m0 + r;
-    int lo = 0, hi = 0;
-    if (row < t.m1) {
-      const int* ids = p.ids + row * p.k;
-      const int from = (int)(p.v0 + n0);
-      lo = first_id(ids, (int)p.k, from);
-      hi = lo;
-      while (hi < p.k && ids[hi] < from + BN) ++hi;
-      if constexpr (GRAD) {
-        row_top[r] = p.top[row];
-        row_part[r] = 1.0f / p.total[row];
-        row_weight[r] = p.weight[row];
+  auto look_up = [&]() __attribute__((always_inline)) {
+    for (int r = threadIdx.x; r < BM; r += G::NT) {
+      const int64_t row = t.m0 + r;
+      int lo = 0, hi = 0;
+      if (row < t.m1) {
+        if (p.target != nullptr) {
+          float flag;
+          lo = target_of(p, row, &flag);
+        } else {
+          const int* ids = p.ids + row * p.k;
+          hi = lo = first_id(ids, (int)p.k, col0);
+          while (hi < p.k && ids[hi] < col0 + BN) ++hi;
+        }
+        if constexpr (GRAD) {
+          row_from[r] = p.top[row] + __builtin_amdgcn_logf(p.total[row]);
+          row_weight[r] = p.weight[row];
+        }
       }
+      first[r] = lo;
+      last[r] = hi;
     }
-    first[r] = lo;
-    last[r] = hi;
-  }
+  };
   Operand<T, BM, true, MODE, G::NT> a;
   Operand<T, BN, true, MODE, G::NT> b;
   a.init(p.x, p.ldx, t.m0, t.m1 - t.m0);
-  b.init(p.w, p.ldw, p.v0 + n0, p.cols - n0);
+  b.init(p.w, p.ldw, col0, p.cols - n0);
   f32x16 acc[FM][2];
-  tile_loop<T, G, true, true>(a, b, 0, p.D, lds, acc);
+  tile_loop<T, G, true, true>(a, b, 0, p.D, lds, acc, look_up);
   __syncthreads();
 
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int64_t left = p.cols - n0 - wn * 64;  // columns from the wave's first on
+  const int left = (int)min(p.cols - n0 - wn * 64, (int64_t)64);  // the wave's columns that exist
   auto col_of = [&](int j, int v) { return 32 * j + 8 * (v >> 2) + 4 * half + (v & 3); };
-  // f(entry) for the row's ids in the wave's columns, the same number of turns in all lanes
+  // f(column of the wave's, p) for the row's ids, the same number of turns in all lanes
   auto entries = [&](int r, int64_t row, auto f) __attribute__((always_inline)) {
     const int lo = first[r], hi = last[r];
+    if (p.target != nullptr) {
+      const int at = lo - col0 - wn * 64;
+      if (__any(at >= 0 && at < 64)) f(at, 1.0f);
+      return;
+    }
     for (int e = lo; __any(e < hi); ++e) {
       int at = -1;
       float prob = 0.0f;
       if (e < hi) {
-        at = p.ids[row * p.k + e] - (int)(p.v0 + n0) - wn * 64;
+        at = p.ids[row * p.k + e] - col0 - wn * 64;
         prob = p.prob[row * p.k + e];
       }
       f(at, prob);
@@ -210,12 +224,14 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, Groupe
 #pragma unroll
         for (int v = 0; v < 16; ++v) top = fmaxf(top, acc[i][j][v]);
       top = fmaxf(top, __shfl_xor(top, 32));
+      top *= c;
       const float from = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f((acc[i][j][v] - from) * c);
+        for (int v = 0; v < 16; ++v)
+          sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], c, -from));
       sum += __shfl_xor(sum, 32);
       float dot = 0.0f;
       entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
@@ -244,7 +260,7 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, Groupe
       const float from = top == -INFINITY ? 0.0f : top;
 #pragma unroll
       for (int q = 0; q < WN; ++q) {
-        sum += red[(WN + q) * BM + r] * __builtin_amdgcn_exp2f((red[q * BM + r] - from) * c);
+        sum += red[(WN + q) * BM + r] * __builtin_amdgcn_exp2f(red[q * BM + r] - from);
         dot += red[(2 * WN + q) * BM + r];
       }
       float* out = p.stats + (int64_t)tn * p.T + t.m0 + r;
@@ -256,12 +272,12 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, Groupe
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int r = (wm * FM + i) * 32 + (lane & 31);
-      const float top = row_top[r], part = row_part[r], weight = row_weight[r];
+      const float from = row_from[r], weight = row_weight[r];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          acc[i][j][v] = __builtin_amdgcn_exp2f((acc[i][j][v] - top) * c) * part;
+          acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], c, -from));
       entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -271,8 +287,14 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, Groupe
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          acc[i][j][v] = weight == 0.0f || col_of(j, v) >= left ? 0.0f : acc[i][j][v] * weight;
+        for (int v = 0; v < 16; ++v) acc[i][j][v] *= weight;
+      if (left < 64 || __any(weight == 0.0f)) {  // (a row that does not count may hold NaN)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v)
+            if (weight == 0.0f || col_of(j, v) >= left) acc[i][j][v] = 0.0f;
+      }
     }
     // through LDS, to become whole 16-byte pieces of rows
     constexpr int kWaveRows = FM * 32, kRowBytes = 128, kChunks = 8;
@@ -320,23 +342,33 @@ __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
     float v[kSpanValues];
 #pragma unroll
     for (int i = 0; i < kSpanValues; ++i) v[i] = lane + 64 * i < left ? z[lane + 64 * i] : -INFINITY;
-    const int* ids = p.ids + row * p.k;
-    const float* prob = p.prob + row * p.k;
-    const int from = (int)(p.v0 + n0), k = (int)p.k;
-    int e = first_id(ids, k, from);
+    const int from = (int)(p.v0 + n0);
+    // f(column of the span's, p) for the row's ids
+    auto entries = [&](auto f) __attribute__((always_inline)) {
+      if (p.target != nullptr) {
+        float flag;
+        const int at = target_of(p, row, &flag) - from;
+        if (at >= 0 && at < kSpan) f(at, 1.0f);
+        return;
+      }
+      const int* ids = p.ids + row * p.k;
+      for (int e = first_id(ids, (int)p.k, from); e < p.k && ids[e] < from + kSpan; ++e)
+        f(ids[e] - from, p.prob[row * p.k + e]);
+    };
     if constexpr (!GRAD) {
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kSpanValues; ++i) top = fmaxf(top, v[i]);
-      top = wave_max(top);
+      top = wave_max(top) * c;
       const float base = top == -INFINITY ? 0.0f : top;
       float sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) sum += exp2f((v[i] - base) * c);
+      for (int i = 0; i < kSpanValues; ++i) sum += exp2f(__builtin_fmaf(v[i], c, -base));
       sum = wave_sum(sum);
       float dot = 0.0f;
-      for (; e < k && ids[e] < from + kSpan; ++e)
-        if (prob[e] != 0.0f) dot += prob[e] * z[ids[e] - from];
+      entries([&](int at, float prob) {
+        if (prob != 0.0f) dot += prob * z[at];
+      });
       if (lane == 0) {
         float* out = p.stats + ((p.v0 + n0) / kSpan) * p.T + row;
         out[0] = top;
@@ -346,12 +378,11 @@ __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
     } else {
       const float top = p.top[row], part = 1.0f / p.total[row], weight = p.weight[row];
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f((v[i] - top) * c) * part;
-      for (; e < k && ids[e] < from + kSpan; ++e) {
-        const int at = ids[e] - from;
+      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f(__builtin_fmaf(v[i], c, -top)) * part;
+      entries([&](int at, float prob) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kSpanValues; ++i) v[i] -= lane + 64 * i == at ? prob[e] : 0.0f;
-      }
+        for (int i = 0; i < kSpanValues; ++i) v[i] -= lane + 64 * i == at ? prob : 0.0f;
+      });
 #pragma unroll
       for (int i = 0; i < kSpanValues; ++i)
         if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * weight;
@@ -360,45 +391,158 @@ __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
 }
 
 // ---- rows ---------------------------------------------------------------------------
-// A row's tiles joined: 16 lanes of tiles a row, then their results in order.
-constexpr int kTileLanes = 16;
-__device__ __forceinline__ void join(float* top, float* sum, float m, float s, float c) {
+// The row's loss from its top, sum and dot = sum_j p_j z_j, and what is kept of it.
+__device__ __forceinline__ void finish_row(const VocabParams& p, int64_t row, float top, float sum,
+                                           float dot, float* __restrict__ loss) {
+  float flag, entropy = 0.0f;
+  if (p.target != nullptr) {
+    target_of(p, row, &flag);
+    p.flag[row] = flag;
+  } else {
+    flag = p.flag[row];
+    entropy = p.entropy[row];
+  }
+  p.top[row] = top;
+  p.total[row] = sum;
+  const float c = kLog2e / p.tau;
+  loss[row] = flag == 0.0f ? 0.0f
+              : flag != flag ? flag
+                             : p.tau * p.tau * (entropy + (top - dot * c) * 0.6931471805599453f +
+                                                logf(sum));
+}
+__device__ __forceinline__ void join(float* top, float* sum, float m, float s) {
   const float most = fmaxf(*top, m), from = most == -INFINITY ? 0.0f : most;
-  *sum = *sum * exp2f((*top - from) * c) + s * exp2f((m - from) * c);
+  *sum = *sum * exp2f(*top - from) + s * exp2f(m - from);
   *top = most;
 }
-__global__ __launch_bounds__(64 * kTileLanes) void vocab_rows_kernel(VocabParams p,
-                                                                     float* __restrict__ loss) {
-  __shared__ float red[3][kTileLanes][64];
-  const int lane = threadIdx.x & 63, tl = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * 64 + lane;
-  const float c = kLog2e / p.tau;
+// A row's tiles joined: 16 rows a block, 64 lanes of tiles a row, joined by fours in
+// a wave and then in the waves' order.
+constexpr int kBlockRows = 16, kRowWaves = 16;
+__global__ __launch_bounds__(64 * kRowWaves) void vocab_rows_kernel(VocabParams p,
+                                                                    float* __restrict__ loss) {
+  __shared__ float red[3][kRowWaves][kBlockRows];
+  const int r = threadIdx.x % kBlockRows, tl = threadIdx.x / kBlockRows, wave = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * kBlockRows + r;
   float top = -INFINITY, sum = 0.0f, dot = 0.0f;
   if (row < p.T) {
-    for (int i = tl; i < p.tiles; i += kTileLanes) {
+    for (int i = tl; i < p.tiles; i += 64 * kRowWaves / kBlockRows) {
       const float* at = p.stats + (int64_t)i * p.T + row;
-      join(&top, &sum, at[0], at[p.tiles * p.T], c);
+      join(&top, &sum, at[0], at[p.tiles * p.T]);
       dot += at[2 * p.tiles * p.T];
     }
   }
-  red[0][tl][lane] = top;
-  red[1][tl][lane] = sum;
-  red[2][tl][lane] = dot;
-  __syncthreads();
-  if (tl != 0 || row >= p.T) return;
 #pragma unroll
-  for (int i = 1; i < kTileLanes; ++i) {
-    join(&top, &sum, red[0][i][lane], red[1][i][lane], c);
-    dot += red[2][i][lane];
+  for (int m = kBlockRows; m < 64; m *= 2) {
+    const float other = __shfl_xor(top, m), s = __shfl_xor(sum, m);
+    join(&top, &sum, other, s);
+    dot += __shfl_xor(dot, m);
   }
-  const float flag = p.flag[row];
-  p.top[row] = top;
-  p.total[row] = sum;
-  loss[row] = flag == 0.0f ? 0.0f
-              : flag != flag ? flag
-                             : p.tau * p.tau * (p.entropy[row] + (top - dot) / p.tau + logf(sum));
+  if ((threadIdx.x & 63) < kBlockRows) {
+    red[0][wave][r] = top;
+    red[1][wave][r] = sum;
+    red[2][wave][r] = dot;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kBlockRows || row >= p.T) return;
+#pragma unroll
+  for (int i = 1; i < kRowWaves; ++i) {
+    join(&top, &sum, red[0][i][r], red[1][i][r]);
+    dot += red[2][i][r];
+  }
+  finish_row(p, row, top, sum, dot, loss);
 }
 
+// ---- few classes ----------------------------------------------------------------------
+// Up to kFewClasses columns: 16 rows and all columns a block, x and W straight from
+// memory into matrix instructions (few_rows), whose sums are a row's logits, its loss
+// and what is kept of it.  The logits are kept, being fewer than x's values.
+// 4096 rows of 256 -> 10 in fp32: @@ us and one launch; the product on a tile, the
+// span kernel and the rows' kernel took 32.
+constexpr int64_t kFewClasses = 64;
+template <typename T, int NC, bool WHOLE>
+__global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __restrict__ loss) {
+  typedef RowsMma<T> M;
+  __shared__ float red[4][kFewRows][16 * NC + 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m0 = (int64_t)blockIdx.x * kFewRows;
+  typename M::acc_t acc[NC];
+  const T* w[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    acc[c] = {0.0f, 0.0f, 0.0f, 0.0f};
+    w[c] = static_cast<const T*>(p.w) + min((int64_t)(16 * c + (lane & 15)), p.V - 1) * p.D;
+  }
+  const T* x = static_cast<const T*>(p.x) + min(m0 + (lane & 15), p.T - 1) * p.D;
+  few_rows<T, NC, WHOLE>(x, w, p.D, acc);
+#pragma unroll
+  for (int c = 0; c < NC; ++c)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) red[wave][lane & 15][16 * c + 4 * (lane >> 4) + v] = acc[c][v];
+  __syncthreads();
+  // 16 lanes a row, column 16 c + lane at z[c]
+  const int r = threadIdx.x >> 4, l = threadIdx.x & 15;
+  const int64_t row = m0 + r;
+  if (row >= p.T) return;
+  const float c2 = kLog2e / p.tau;
+  float z[NC], top = -INFINITY, sum = 0.0f, dot = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int v = 16 * c + l;
+    z[c] = -INFINITY;
+    if (v < p.V) {
+      z[c] = red[0][r][v] + red[1][r][v] + red[2][r][v] + red[3][r][v];
+      p.logits[row * p.V + v] = z[c];
+    }
+    top = fmaxf(top, z[c]);
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+  top *= c2;
+  const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) sum += exp2f(__builtin_fmaf(z[c], c2, -from));
+  auto add = [&](int id, float prob) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+      if (16 * c + l == id && prob != 0.0f) dot += prob * z[c];
+  };
+  if (p.target != nullptr) {
+    float flag;
+    add(target_of(p, row, &flag), 1.0f);
+  } else {
+    for (int e = 0; e < p.k; ++e) add(p.ids[row * p.k + e], p.prob[row * p.k + e]);
+  }
+  sum = lane_sum<16>(sum);
+  dot = lane_sum<16>(dot);
+  if (l == 0) finish_row(p, row, top, sum, dot, loss);
+}
+// dz from the kept logits, 16 lanes a row; in 16 bits zeros as far as 16 bytes go.
+template <typename T>
+__global__ __launch_bounds__(256) void vocab_few_grad_kernel(VocabParams p) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row >= p.T) return;
+  const float c = kLog2e / p.tau, top = p.top[row], part = 1.0f / p.total[row];
+  const float weight = p.weight[row];
+  const int64_t cols = sizeof(T) == 2 ? round_up(p.V, 8) : p.V;
+  float flag = 0.0f;
+  const int target = p.target == nullptr ? kNoId : target_of(p, row, &flag);
+  for (int64_t v = threadIdx.x & 15; v < cols; v += 16) {
+    float d = 0.0f;
+    if (v < p.V && weight != 0.0f) {
+      d = exp2f(__builtin_fmaf(p.logits[row * p.V + v], c, -top)) * part;
+      if (p.target != nullptr) {
+        d -= v == target ? 1.0f : 0.0f;
+      } else {
+        for (int e = 0; e < p.k; ++e)
+          d -= p.ids[row * p.k + e] == v ? p.prob[row * p.k + e] : 0.0f;
+      }
+      d *= weight;
+    }
+    static_cast<T*>(p.G)[row * p.ldg + v] = (T)d;
+  }
+}
+
+// ---- sums of the rows -------------------------------------------------------------------
 constexpr int kOneBlock = 1024;
 template <typename V>
 __device__ __forceinline__ V block_total(V v, V* red) {
@@ -429,51 +573,58 @@ __global__ __launch_bounds__(kOneBlock) void vocab_sum_kernel(VocabParams p,
 }
 
 // w and the common factor from the gradient of the loss: of a scalar loss g is one
-// value (over the count for a mean) and w = flag; of the rows' losses (one block)
-// w = g_t / max|g|; w times `unit`, a power of 2.  fp32: w is the whole factor.
-__global__ __launch_bounds__(kOneBlock) void vocab_weights_kernel(VocabParams p,
-                                                                  const float* __restrict__ g,
-                                                                  int reduction, int fp32,
-                                                                  float unit,
-                                                                  float* __restrict__ scale) {
+// value (over the count for a mean) and w = flag; of the rows' losses w = g_t /
+// max|g|, or in fp32 g_t; w times `unit`, a power of 2.  fp32: w is the whole factor.
+struct Upstream {
+  const float* g;
+  int reduction, fp32;
+  float unit;
+  const float* most;  // max|g| of the rows' losses in 16 bits
+  float* scale;
+};
+__device__ __forceinline__ float common_of(const VocabParams& p, const Upstream& u) {
+  if (u.reduction == KAN_REDUCE_NONE) return u.fp32 ? p.tau : p.tau * *u.most;
+  const float c = p.tau * *u.g;
+  return u.reduction == KAN_REDUCE_MEAN ? c / fmaxf(*p.count, 1.0f) : c;
+}
+__device__ __forceinline__ float weight_of(const VocabParams& p, const Upstream& u, int64_t row,
+                                           float common) {
+  const float flag = p.flag[row];
+  float w = flag;
+  if (u.reduction == KAN_REDUCE_NONE) w = u.fp32 ? flag * u.g[row] : flag * u.g[row] / *u.most;
+  return flag == 0.0f ? 0.0f : w * (u.fp32 ? common : u.unit);
+}
+__global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
+                                                               const float* __restrict__ g,
+                                                               float* __restrict__ out) {
   __shared__ float red[kOneBlock];
-  const bool rows = reduction == KAN_REDUCE_NONE;
-  float common = p.tau, most = 1.0f;
-  if (!rows) {
-    common *= *g;
-    if (reduction == KAN_REDUCE_MEAN) common /= fmaxf(*p.count, 1.0f);
-  } else if (!fp32) {
-    most = 0.0f;
-    for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock)
-      if (p.flag[t] != 0.0f) most = fmaxf(most, fabsf(g[t]));
-    red[threadIdx.x] = most;
+  float most = 0.0f;
+  for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock)
+    if (p.flag[t] != 0.0f) most = fmaxf(most, fabsf(g[t]));
+  red[threadIdx.x] = most;
+  __syncthreads();
+  for (int m = kOneBlock / 2; m > 0; m /= 2) {
+    if (threadIdx.x < m) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + m]);
     __syncthreads();
-    for (int m = kOneBlock / 2; m > 0; m /= 2) {
-      if (threadIdx.x < m) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + m]);
-      __syncthreads();
-    }
-    most = red[0] == 0.0f ? 1.0f : red[0];
-    common *= most;
   }
-  for (int64_t t = (int64_t)blockIdx.x * kOneBlock + threadIdx.x; t < p.T;
-       t += (int64_t)gridDim.x * kOneBlock) {
-    const float flag = p.flag[t];
-    const float w = rows ? flag * g[t] / most : flag;
-    p.weight[t] = flag == 0.0f ? 0.0f : w * (fp32 ? common : unit);
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) *scale = common / unit;
+  if (threadIdx.x == 0) *out = red[0] == 0.0f ? 1.0f : red[0];
 }
 
-// x's rows for the weight's gradient, those that do not count as zeros: what they hold
-// may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld], zeros behind D.
+// The rows' weights and, for the weight's gradient, x's rows, those that do not count
+// as zeros: what they hold may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld],
+// zeros behind D; ld 0: none.
 template <typename T>
-__global__ __launch_bounds__(256) void vocab_copy_kernel(VocabParams p, T* __restrict__ out,
-                                                         int64_t ld, int whole) {
+__global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstream u,
+                                                            T* __restrict__ out, int64_t ld,
+                                                            int whole) {
   constexpr int V = 16 / sizeof(T);
   typedef typename VecOf<T, V>::type vec;
+  const int64_t first = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
+  const float common = common_of(p, u);
+  if (first == 0) *u.scale = common / u.unit;
+  for (int64_t row = first; row < p.T; row += step) p.weight[row] = weight_of(p, u, row, common);
   const int64_t per = ceil_div(ld, V), total = p.T * per;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * 256) {
+  for (int64_t i = first; i < total; i += step) {
     const int64_t row = i / per, c = (i - row * per) * V;
     const T* src = static_cast<const T*>(p.x) + row * p.D + c;
     const bool on = p.flag[row] != 0.0f;
@@ -534,7 +685,13 @@ int64_t piece_columns(int dtype, int64_t T, int64_t V) {
   if (most >= V) return V;
   return round_up(ceil_div(V, ceil_div(V, most)), kSpan);
 }
-size_t kept_floats(int64_t T, int64_t k) { return (size_t)(3 * T + 4 + 2 * T * k); }
+// Values between rows of dz in 16 bits: an odd number of 128 bytes, so that a tile's
+// rows spread over the memory's channels.
+int64_t padded(int64_t cols) { return round_up(cols, 128) + 64; }
+// (k 0: cross entropy)
+size_t kept_floats(int64_t T, int64_t V, int64_t k) {
+  return (size_t)(3 * T + 4 + 2 * T * k) + (V <= kFewClasses ? (size_t)(T * V) : 0);
+}
 void set_kept(VocabParams* p, void* kept) {
   p->top = static_cast<float*>(kept);
   p->total = p->top + p->T;
@@ -542,6 +699,7 @@ void set_kept(VocabParams* p, void* kept) {
   p->count = p->flag + p->T;
   p->prob = p->count + 4;
   p->ids = reinterpret_cast<int*>(p->prob + p->T * p->k);
+  p->logits = p->prob + 2 * p->T * p->k;
 }
 GroupedParams product_of(int64_t T, int64_t N, int64_t K) {
   GroupedParams g{};
@@ -558,17 +716,19 @@ HalfCfg tile_of(int64_t T, int64_t cols, int64_t D) {
 }
 int64_t tile_columns(HalfCfg cfg) { return cfg == kSmall ? 128 : 256; }
 
+HalfPlan plan_product(int dtype, int op, int64_t T, int64_t cols, int64_t D) {
+  if (dtype != KAN_DTYPE_F32 && op == KAN_GROUPED_INPUT) return long_plan(T, cols, D);
+  return product_plan(dtype, op, T, 1, cols, D);
+}
+
 template <typename T, class G, bool GRAD>
 int launch_vocab_tile(const VocabParams& p, hipStream_t st) {
-  GroupedParams g = product_of(p.T, p.cols, p.D);
-  const int64_t tiles_n = ceil_div(p.cols, G::BN), blocks = row_grid(g, G::BM, tiles_n);
+  const int64_t tiles_n = ceil_div(p.cols, G::BN), blocks = dense_grid(p.T, G::BM, tiles_n);
   if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "vocab_loss: too many tiles");
   if (whole_rows(p.x, p.ldx) && whole_rows(p.w, p.ldw))
-    vocab_tile_kernel<T, G, kDirect, GRAD>
-        <<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, g, (int)tiles_n);
+    vocab_tile_kernel<T, G, kDirect, GRAD><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
   else
-    vocab_tile_kernel<T, G, kGuarded, GRAD>
-        <<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, g, (int)tiles_n);
+    vocab_tile_kernel<T, G, kGuarded, GRAD><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
   return check_launch("vocab_loss");
 }
 template <typename T, bool GRAD>
@@ -621,7 +781,9 @@ ForwardPlan plan_forward(int dtype, const void* x, const void* w, int64_t T, int
                          char* ws) {
   ForwardPlan f{};
   Places at{ws, 0};
-  if (dtype == KAN_DTYPE_F32) {
+  f.piece = V;
+  if (V <= kFewClasses) {
+  } else if (dtype == KAN_DTYPE_F32) {
     f.piece = piece_columns(dtype, T, V);
     f.tiles = (int)ceil_div(V, kSpan);
     f.product = product_plan(dtype, KAN_GROUPED_FORWARD, T, 1, f.piece, D);
@@ -635,7 +797,6 @@ ForwardPlan plan_forward(int dtype, const void* x, const void* w, int64_t T, int
                                                T, 1, rest, D));
     f.part = part == 0 ? nullptr : at.take<float>(part / 4);
   } else {
-    f.piece = V;
     f.cfg = tile_of(T, V, D);
     f.tiles = (int)ceil_div(V, tile_columns(f.cfg));
     f.align = align_operands(x, T, D, w, V, D, 2, align_saves_us(KAN_GROUPED_FORWARD, T, V, D));
@@ -653,7 +814,7 @@ struct BackwardPlan {
   AlignPlan align;
   int64_t piece, ldg, ldx;
   char *rows, *aligned, *G;  // rows: x's for the weight's gradient
-  float *weight, *scale, *part, *slices, *acc;
+  float *weight, *scale, *most, *part, *slices, *acc;
   size_t bytes;
 };
 BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, int64_t V, int64_t D,
@@ -662,7 +823,7 @@ BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, i
   Places at{ws, 0};
   const bool half = dtype != KAN_DTYPE_F32;
   b.piece = piece_columns(dtype, T, V);
-  b.ldg = half ? round_up(b.piece, 8) : b.piece;
+  b.ldg = half ? padded(b.piece) : b.piece;
   if (half) {
     b.cfg = tile_of(T, b.piece, D);
     double saved = align_saves_us(KAN_GROUPED_FORWARD, T, V, D);
@@ -676,15 +837,16 @@ BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, i
   if (dw) b.rows = at.take((size_t)(T * b.ldx) * dtype_bytes(dtype));
   b.weight = at.take<float>((size_t)T);
   b.scale = at.take<float>(1);
+  b.most = at.take<float>(1);
   b.G = at.take((size_t)(T * b.ldg) * dtype_bytes(dtype));
   size_t part = 0, slices = 0;
   const int64_t rest = V % b.piece;
   for (const int64_t cols : {b.piece, rest}) {
     if (cols == 0) continue;
     auto need = [&](int op) {
-      return product_part_bytes(op, product_plan(dtype, op, T, 1, cols, D), T, 1, cols, D);
+      return product_part_bytes(op, plan_product(dtype, op, T, cols, D), T, 1, cols, D);
     };
-    if (!half) part = std::max(part, need(KAN_GROUPED_FORWARD));
+    if (!half && V > kFewClasses) part = std::max(part, need(KAN_GROUPED_FORWARD));
     if (dw) part = std::max(part, need(KAN_GROUPED_WEIGHT));
     if (dx && (!half || b.piece == V)) part = std::max(part, need(KAN_GROUPED_INPUT));
     else if (dx) slices = std::max(slices, need(KAN_GROUPED_INPUT));
@@ -700,11 +862,31 @@ BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, i
 }
 
 template <typename T>
-void launch_copy(const VocabParams& p, char* out, int64_t ld, hipStream_t st) {
+void launch_prepare(const VocabParams& p, const Upstream& u, char* out, int64_t ld,
+                    hipStream_t st) {
   constexpr int64_t V = 16 / sizeof(T);
-  const int64_t blocks = std::min<int64_t>(ceil_div(p.T * ceil_div(ld, V), 256), 1 << 16);
-  vocab_copy_kernel<T><<<dim3((unsigned)blocks), 256, 0, st>>>(p, reinterpret_cast<T*>(out), ld,
-                                                               ld % V == 0);
+  const int64_t most = std::max(p.T, p.T * ceil_div(ld, V));
+  vocab_prepare_kernel<T><<<dim3((unsigned)std::min<int64_t>(ceil_div(most, 256), 1 << 16)), 256, 0,
+                            st>>>(p, u, reinterpret_cast<T*>(out), ld, ld % V == 0);
+}
+template <typename T, bool WHOLE>
+int launch_few_classes(const VocabParams& p, float* loss, hipStream_t st) {
+  const dim3 blocks((unsigned)ceil_div(p.T, kFewRows));
+  if (p.V <= 16) vocab_few_kernel<T, 1, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
+  else if (p.V <= 32) vocab_few_kernel<T, 2, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
+  else vocab_few_kernel<T, 4, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
+  return check_launch("vocab_loss");
+}
+template <typename T>
+int launch_few_forward(const VocabParams& p, float* loss, hipStream_t st) {
+  if (sizeof(T) == 2 && !(whole_rows(p.x, p.D) && whole_rows(p.w, p.D)))
+    return launch_few_classes<T, false>(p, loss, st);
+  return launch_few_classes<T, true>(p, loss, st);
+}
+template <typename T>
+int launch_few_grad(const VocabParams& p, hipStream_t st) {
+  vocab_few_grad_kernel<T><<<dim3((unsigned)ceil_div(p.T, 16)), 256, 0, st>>>(p);
+  return check_launch("vocab_loss_backward");
 }
 template <typename T>
 void launch_add(const float* part, int cuts, int64_t count, float* acc, bool start,
@@ -720,11 +902,11 @@ using namespace kan;
 
 extern "C" {
 
-int kan_hip_vocab_loss_kept(int64_t T, int64_t k, size_t* bytes) {
+int kan_hip_vocab_loss_kept(int64_t T, int64_t V, int64_t k, size_t* bytes) {
   if (bytes == nullptr) return set_error(KAN_ERR_INVALID, "vocab_loss_kept: bytes must not be NULL");
-  const int rc = check_vocab("vocab_loss_kept", KAN_DTYPE_F32, T, 1, 1, k, 1.0, 0);
+  const int rc = check_vocab("vocab_loss_kept", KAN_DTYPE_F32, T, V, 1, k + (k == 0), 1.0, 0);
   if (rc != KAN_OK) return rc;
-  *bytes = 4 * kept_floats(T, k);
+  *bytes = 4 * kept_floats(T, V, k);
   return KAN_OK;
 }
 
@@ -743,10 +925,10 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
                        int64_t ignore_index, double temperature, int reduction, float* loss,
                        void* kept, void* workspace, size_t workspace_bytes, void* stream) {
   const char* who = "vocab_loss";
-  const int rc = check_vocab(who, dtype, T, V, D, k, temperature, reduction);
+  const int rc = check_vocab(who, dtype, T, V, D, k + (k == 0), temperature, reduction);
   if (rc != KAN_OK) return rc;
-  if (teacher == nullptr && k != 1)
-    return set_error(KAN_ERR_INVALID, "%s: without a teacher a row has one id", who);
+  if ((teacher == nullptr) != (k == 0))
+    return set_error(KAN_ERR_INVALID, "%s: k is 0 without a teacher and positive with one", who);
   if (T == 0) return KAN_OK;
   if (x == nullptr || w == nullptr || ids == nullptr || loss == nullptr || kept == nullptr)
     return set_error(KAN_ERR_INVALID, "%s: operands must not be NULL", who);
@@ -771,14 +953,23 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
   p.cols = V;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * (double)V * (double)D);
-  if (teacher == nullptr)
-    vocab_targets_kernel<<<dim3((unsigned)ceil_div(T, 256)), 256, 0, st>>>(p, ids, ids64,
-                                                                         ignore_index);
-  else
+  int e = KAN_OK;
+  if (teacher == nullptr) {
+    p.target = ids;
+    p.target64 = ids64;
+    p.ignore = ignore_index;
+  } else {
     vocab_teacher_kernel<<<dim3((unsigned)T), 64, 0, st>>>(p, ids, ids64, teacher);
-  int e = check_launch(who);
+    e = check_launch(who);
+  }
+  float* rows = reduction == KAN_REDUCE_NONE ? loss : f.rows;
+  const bool few = V <= kFewClasses;
+  if (few && e == KAN_OK)
+    e = dtype == KAN_DTYPE_F32    ? launch_few_forward<float>(p, rows, st)
+        : dtype == KAN_DTYPE_BF16 ? launch_few_forward<bf16>(p, rows, st)
+                                  : launch_few_forward<f16>(p, rows, st);
   if (e != KAN_OK) return e;
-  if (dtype != KAN_DTYPE_F32) {
+  if (!few && dtype != KAN_DTYPE_F32) {
     GroupedParams g = product_of(T, V, D);
     g.A = x;
     g.B = w;
@@ -791,7 +982,7 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
     e = launch_vocab_tiles<false>(dtype, p, f.cfg, st);
     if (e != KAN_OK) return e;
   }
-  for (p.v0 = 0; dtype == KAN_DTYPE_F32 && p.v0 < V; p.v0 += f.piece) {
+  for (p.v0 = 0; !few && dtype == KAN_DTYPE_F32 && p.v0 < V; p.v0 += f.piece) {
     p.cols = std::min(f.piece, V - p.v0);
     p.z = f.z;
     GroupedParams g = product_of(T, p.cols, D);
@@ -804,8 +995,8 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
     if (e == KAN_OK) e = launch_vocab_span<false>(p, st);
     if (e != KAN_OK) return e;
   }
-  float* rows = reduction == KAN_REDUCE_NONE ? loss : f.rows;
-  vocab_rows_kernel<<<dim3((unsigned)ceil_div(T, 64)), 64 * kTileLanes, 0, st>>>(p, rows);
+  if (!few)
+    vocab_rows_kernel<<<dim3((unsigned)ceil_div(T, kBlockRows)), 64 * kRowWaves, 0, st>>>(p, rows);
   if (reduction != KAN_REDUCE_NONE)
     vocab_sum_kernel<<<1, kOneBlock, 0, st>>>(p, rows, reduction == KAN_REDUCE_MEAN, loss);
   return check_launch(who);
@@ -823,14 +1014,16 @@ int kan_hip_vocab_loss_backward_workspace(int dtype, const void* x, const void* 
 }
 
 int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x, const void* w,
-                                const void* kept, int64_t T, int64_t V, int64_t D, int64_t k,
-                                double temperature, int reduction, void* grad_x, void* grad_w,
-                                void* workspace, size_t workspace_bytes, void* stream) {
+                                const void* ids, int ids64, const void* kept, int64_t T, int64_t V,
+                                int64_t D, int64_t k, int64_t ignore_index, double temperature,
+                                int reduction, void* grad_x, void* grad_w, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   const char* who = "vocab_loss_backward";
-  const int rc = check_vocab(who, dtype, T, V, D, k, temperature, reduction);
+  const int rc = check_vocab(who, dtype, T, V, D, k + (k == 0), temperature, reduction);
   if (rc != KAN_OK) return rc;
   if (T == 0 || (grad_x == nullptr && grad_w == nullptr)) return KAN_OK;
-  if (grad_loss == nullptr || x == nullptr || w == nullptr || kept == nullptr)
+  if (grad_loss == nullptr || x == nullptr || w == nullptr || kept == nullptr ||
+      (k == 0 && ids == nullptr))
     return set_error(KAN_ERR_INVALID, "%s: operands must not be NULL", who);
   if (!aligned16(kept) || !aligned16(workspace))
     return set_error(KAN_ERR_INVALID, "%s: kept values and the workspace lie on 16 bytes", who);
@@ -849,18 +1042,28 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
   p.D = D;
   p.k = k;
   p.tau = (float)temperature;
+  if (k == 0) {
+    p.target = ids;
+    p.target64 = ids64;
+    p.ignore = ignore_index;
+  }
   set_kept(&p, const_cast<void*>(kept));
   p.weight = b.weight;
   p.x = x;
   GroupedParams in = product_of(T, V, D);
   in.A = x;
   in.B = w;
-  if (grad_w != nullptr) {
+  const Upstream up{grad_loss, reduction, half ? 0 : 1, dtype == KAN_DTYPE_F16 ? 32768.0f : 1.0f,
+                    b.most, b.scale};
+  if (half && reduction == KAN_REDUCE_NONE)
+    vocab_most_kernel<<<1, kOneBlock, 0, st>>>(p, grad_loss, b.most);
+  const int64_t ld = grad_w == nullptr ? 0 : b.ldx;
+  if (dtype == KAN_DTYPE_F32) launch_prepare<float>(p, up, b.rows, ld, st);
+  else if (dtype == KAN_DTYPE_BF16) launch_prepare<bf16>(p, up, b.rows, ld, st);
+  else launch_prepare<f16>(p, up, b.rows, ld, st);
+  if (ld > 0) {
     in.A = b.rows;
-    in.lda = b.ldx;
-    if (dtype == KAN_DTYPE_F32) launch_copy<float>(p, b.rows, b.ldx, st);
-    else if (dtype == KAN_DTYPE_BF16) launch_copy<bf16>(p, b.rows, b.ldx, st);
-    else launch_copy<f16>(p, b.rows, b.ldx, st);
+    in.lda = ld;
   }
   int e = launch_aligned(b.align, &in, b.aligned, st);
   if (e != KAN_OK) return e;
@@ -870,10 +1073,8 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
   p.ldw = in.ldb;
   p.G = b.G;
   p.z = reinterpret_cast<float*>(b.G);
-  const bool one = half && reduction == KAN_REDUCE_NONE;
-  vocab_weights_kernel<<<dim3(one ? 1 : (unsigned)ceil_div(T, kOneBlock)), kOneBlock, 0, st>>>(
-      p, grad_loss, reduction, half ? 0 : 1, dtype == KAN_DTYPE_F16 ? 32768.0f : 1.0f, b.scale);
-  e = check_launch(who);
+  if (e == KAN_OK) e = check_launch(who);
+  const bool few = V <= kFewClasses;
   for (p.v0 = 0; e == KAN_OK && p.v0 < V; p.v0 += b.piece) {
     p.cols = std::min(b.piece, V - p.v0);
     const char* wp = static_cast<const char*>(p.w) + p.v0 * p.ldw * value;
@@ -886,16 +1087,19 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
       g.ldb = ldb;
       g.C = C;
       g.scale = half ? b.scale : nullptr;
-      const HalfPlan pl = product_plan(dtype, op, T, 1, p.cols, D);
+      const HalfPlan pl = plan_product(dtype, op, T, p.cols, D);
       g.part = C == nullptr || product_part_bytes(op, pl, T, 1, p.cols, D) > 0 ? part : nullptr;
       return launch_product(dtype, op, g, pl, st);
     };
     // dz of the piece
-    if (half) {
-      p.ldg = round_up(p.cols, 8);
+    p.ldg = half ? padded(p.cols) : p.cols;
+    if (few) {
+      e = dtype == KAN_DTYPE_F32    ? launch_few_grad<float>(p, st)
+          : dtype == KAN_DTYPE_BF16 ? launch_few_grad<bf16>(p, st)
+                                    : launch_few_grad<f16>(p, st);
+    } else if (half) {
       e = launch_vocab_tiles<true>(dtype, p, b.cfg, st);
     } else {
-      p.ldg = p.cols;
       e = product(KAN_GROUPED_FORWARD, p.x, D, wp, D, p.z, b.part);
       if (e == KAN_OK) e = launch_vocab_span<true>(p, st);
     }
@@ -910,7 +1114,7 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
     int cuts = 1;
     if (half) {
       e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, nullptr, b.slices);
-      cuts = product_plan(dtype, KAN_GROUPED_INPUT, T, 1, p.cols, D).cuts;
+      cuts = plan_product(dtype, KAN_GROUPED_INPUT, T, p.cols, D).cuts;
     } else {
       e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, b.slices, b.part);
     }

@@ -41,15 +41,16 @@ def _workspace(lib, device, fn, *args):
 
 
 class _VocabLoss(torch.autograd.Function):
-    """x [T, D], weight [V, D], ids [T, k], teacher [T, k] float32 or None."""
+    """x [T, D], weight [V, D], ids [T, k], teacher [T, k] float32; cross entropy:
+    ids [T, 1], teacher None."""
 
     @staticmethod
     def forward(ctx, x, weight, ids, teacher, ignore, tau, reduction, save):
         lib = _native("linear_cross_entropy")
         T, D = x.shape
-        V, k = weight.shape[0], ids.shape[1]
+        V, k = weight.shape[0], 0 if teacher is None else ids.shape[1]
         code, L = lib.OPERATOR_DTYPES[x.dtype], lib.LIB
-        kept, _ = _workspace(lib, x.device, L.kan_hip_vocab_loss_kept, T, k)
+        kept, _ = _workspace(lib, x.device, L.kan_hip_vocab_loss_kept, T, V, k)
         px, pw = x.data_ptr(), weight.data_ptr()
         ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_workspace, code, px, pw, T, V, D)
         loss = torch.empty((T,) if reduction == 0 else (), dtype=torch.float32, device=x.device)
@@ -58,16 +59,16 @@ class _VocabLoss(torch.autograd.Function):
                    T, V, D, k, ignore, tau, reduction, loss.data_ptr(), kept.data_ptr(),
                    ws.data_ptr(), nbytes)
         if save:
-            ctx.args = (code, T, V, D, k, tau, reduction)
-            ctx.save_for_backward(x, weight, kept)
+            ctx.args = (code, T, V, D, k, ignore, tau, reduction)
+            ctx.save_for_backward(x, weight, ids if k == 0 else None, kept)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         lib = _native("linear_cross_entropy")
-        x, weight, kept = ctx.saved_tensors
-        code, T, V, D, k, tau, reduction = ctx.args
+        x, weight, ids, kept = ctx.saved_tensors
+        code, T, V, D, k, ignore, tau, reduction = ctx.args
         dx, dw = [torch.empty_like(t) if need else None
                   for t, need in zip((x, weight), ctx.needs_input_grad)]
         g = g.contiguous()
@@ -75,7 +76,9 @@ class _VocabLoss(torch.autograd.Function):
         ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_backward_workspace, code, px, pw,
                                 T, V, D, int(dx is not None), int(dw is not None))
         lib.launch(L.kan_hip_vocab_loss_backward, x.device, code, g.data_ptr(), px, pw,
-                   kept.data_ptr(), T, V, D, k, tau, reduction,
+                   None if ids is None else ids.data_ptr(),
+                   int(ids is not None and ids.dtype == torch.int64), kept.data_ptr(), T, V, D, k,
+                   ignore, tau, reduction,
                    None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
                    ws.data_ptr(), nbytes)
         return dx, dw, None, None, None, None, None, None

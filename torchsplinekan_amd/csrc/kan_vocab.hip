@@ -456,7 +456,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void vocab_rows_kernel(VocabParams 
 // Up to kFewClasses columns: 16 rows and all columns a block, x and W straight from
 // memory into matrix instructions (few_rows), whose sums are a row's logits, its loss
 // and what is kept of it.  The logits are kept, being fewer than x's values.
-// 4096 rows of 256 -> 10 in fp32: @@ us and one launch; the product on a tile, the
+// 4096 rows of 256 -> 10 in fp32: 5.2 us and one launch; the product on a tile, the
 // span kernel and the rows' kernel took 32.
 constexpr int64_t kFewClasses = 64;
 template <typename T, int NC, bool WHOLE>

@@ -6,7 +6,10 @@ knots they share; the routed rows' products run grouped by expert
 (``grouped_linear``), and with ``checkpoint`` the rows are kept in 8 bits and
 the basis, R + 1 times their size, is evaluated again in the backward pass
 (``checkpoint_8bit``).  ``KANExpertStack`` puts such blocks on a residual stream
-(``residual_norm``): norm, experts, norm, gate and residual scale.
+(``residual_norm``): norm, experts, norm, gate and residual scale; with a gated
+feed-forward block (``gated_linear``) beside the experts, a layer norm of what comes
+in (``layer_norm``) and a last layer of classes or tokens, whose losses never hold
+the logits (``linear_cross_entropy``, ``linear_distillation``).
 """
 
 import math
@@ -18,7 +21,10 @@ import torch.nn.functional as F
 
 from . import fused as _fused
 from .act8 import check_format, checkpoint_8bit
+from .gated import gated_linear
 from .grouped import grouped_linear
+from .layernorm import layer_norm
+from .losses import linear_cross_entropy, linear_distillation
 from .reference_backend import compute_basis
 from .residual import residual_norm
 
@@ -113,41 +119,95 @@ class KANExperts(nn.Module):
 
 
 class _Block(nn.Module):
-    def __init__(self, width: int, residual_scale: float, **experts) -> None:
+    def __init__(self, width: int, residual_scale: float, feed_forward: int, **experts) -> None:
         super().__init__()
         self.pre_weight = nn.Parameter(torch.ones(width))
         self.post_weight = nn.Parameter(torch.ones(width))
         self.scale = nn.Parameter(torch.full((width,), residual_scale))
         self.gate = nn.Linear(width, 1)
         self.experts = KANExperts(width, width, **experts)
+        self.gate_up = self.down = None
+        if feed_forward > 0:
+            self.gate_up = nn.Parameter(torch.empty(2, feed_forward, width))
+            self.down = nn.Parameter(torch.empty(width, feed_forward))
+            nn.init.normal_(self.gate_up, std=1.0 / math.sqrt(width))
+            nn.init.normal_(self.down, std=1.0 / math.sqrt(feed_forward))
+
+    def forward(self, h: torch.Tensor) -> torch.Tensor:
+        y = self.experts(h)
+        if self.down is not None:
+            y = y + F.linear(gated_linear(h, self.gate_up), self.down)
+        return y
 
 
 class KANExpertStack(nn.Module):
-    """depth residual blocks x' = x + scale * sigmoid(gate(h)) * norm(experts(h)),
+    """depth residual blocks x' = x + scale * sigmoid(gate(h)) * norm(block(h)),
     h = norm(x), and a norm of the last x'.  Each block's second norm, gate,
     scale and addition run in one pass with the next block's first norm.
-    Further arguments go to each KANExperts."""
+    feed_forward > 0: every block adds a gated feed-forward block of that many
+    outputs, which all rows pass, to its experts.  input_norm: x passes a layer
+    norm first.  num_classes: a last layer head [num_classes, width] for logits,
+    loss and distillation_loss.  Further arguments go to each KANExperts."""
 
     def __init__(self, width: int, depth: int, num_experts: int, residual_scale: float = 0.2,
-                 eps: float = 1e-6, **experts) -> None:
+                 eps: float = 1e-6, feed_forward: int = 0, input_norm: bool = False,
+                 num_classes: Optional[int] = None, **experts) -> None:
         super().__init__()
         if depth < 1:
             raise ValueError(f"depth must be >= 1, got {depth}")
+        if feed_forward < 0:
+            raise ValueError(f"feed_forward must be >= 0, got {feed_forward}")
+        if num_classes is not None and num_classes < 1:
+            raise ValueError(f"num_classes must be >= 1, got {num_classes}")
         self.blocks = nn.ModuleList([
-            _Block(width, residual_scale, num_experts=num_experts, **experts)
+            _Block(width, residual_scale, feed_forward, num_experts=num_experts, **experts)
             for _ in range(depth)])
         self.norm_weight = nn.Parameter(torch.ones(width))
         self.eps = eps
+        self.input_weight = self.input_bias = self.head = None
+        if input_norm:
+            self.input_weight = nn.Parameter(torch.ones(width))
+            self.input_bias = nn.Parameter(torch.zeros(width))
+        if num_classes is not None:
+            self.head = nn.Parameter(torch.empty(num_classes, width))
+            nn.init.normal_(self.head, std=1.0 / math.sqrt(width))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         with torch.autocast(x.device.type, enabled=False):
             return self._forward(x)
 
     def _forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.input_weight is not None:
+            x = layer_norm(x, self.input_weight, self.input_bias)
         x, h = residual_norm(x, pre_weight=self.blocks[0].pre_weight, eps=self.eps)
         for block, after in zip(self.blocks, [*self.blocks[1:], None]):
             x, h = residual_norm(
-                x, block.experts(h), post_weight=block.post_weight, gate=block.gate(h),
+                x, block(h), post_weight=block.post_weight, gate=block.gate(h),
                 gate_act="sigmoid", scale=block.scale, eps=self.eps,
                 pre_weight=self.norm_weight if after is None else after.pre_weight)
         return h
+
+    def _head(self) -> torch.Tensor:
+        if self.head is None:
+            raise RuntimeError("KANExpertStack: no last layer (num_classes)")
+        return self.head
+
+    def logits(self, x: torch.Tensor) -> torch.Tensor:
+        """head h of the stack's rows h, [..., num_classes]."""
+        head = self._head()
+        with torch.autocast(x.device.type, enabled=False):
+            return F.linear(self._forward(x), head)
+
+    def loss(self, x: torch.Tensor, target: torch.Tensor, **kw) -> torch.Tensor:
+        """linear_cross_entropy of the stack's rows against target [...]; further
+        arguments go to it."""
+        head = self._head()
+        return linear_cross_entropy(self(x), head, target, **kw)
+
+    def distillation_loss(self, x: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor,
+                          **kw) -> torch.Tensor:
+        """linear_distillation of the stack's rows from a teacher's logits at ids
+        [..., k] (`values, ids = teacher.logits(x).topk(k)`); further arguments go to
+        it."""
+        head = self._head()
+        return linear_distillation(self(x), head, ids, teacher, **kw)

@@ -212,14 +212,16 @@ def stream_of(device: torch.device) -> int:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def launch(fn, device: torch.device, *args) -> None:
     """fn(*args, stream) on `device` and its current stream, with the status
     checked.  (Short calls are bound by their host time: the stream's handle is
-    taken without building a Stream object, and the device is switched only
-    where it is another one.)"""
-    if device.index == torch.cuda.current_device():
+    taken without building a Stream object, the device's number without asking
+    whether torch has started, and the device is switched only where it is another
+    one.)"""
+    if device.index == _current_device():
         stream = stream_of(device) if _raw_stream is None else _raw_stream(device.index)
         status = fn(*args, stream)
     else:

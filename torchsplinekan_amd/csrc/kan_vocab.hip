@@ -516,32 +516,6 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __
   dot = lane_sum<16>(dot);
   if (l == 0) finish_row(p, row, top, sum, dot, loss);
 }
-// dz from the kept logits, 16 lanes a row; in 16 bits zeros as far as 16 bytes go.
-template <typename T>
-__global__ __launch_bounds__(256) void vocab_few_grad_kernel(VocabParams p) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= p.T) return;
-  const float c = kLog2e / p.tau, top = p.top[row], part = 1.0f / p.total[row];
-  const float weight = p.weight[row];
-  const int64_t cols = sizeof(T) == 2 ? round_up(p.V, 8) : p.V;
-  float flag = 0.0f;
-  const int target = p.target == nullptr ? kNoId : target_of(p, row, &flag);
-  for (int64_t v = threadIdx.x & 15; v < cols; v += 16) {
-    float d = 0.0f;
-    if (v < p.V && weight != 0.0f) {
-      d = exp2f(__builtin_fmaf(p.logits[row * p.V + v], c, -top)) * part;
-      if (p.target != nullptr) {
-        d -= v == target ? 1.0f : 0.0f;
-      } else {
-        for (int e = 0; e < p.k; ++e)
-          d -= p.ids[row * p.k + e] == v ? p.prob[row * p.k + e] : 0.0f;
-      }
-      d *= weight;
-    }
-    static_cast<T*>(p.G)[row * p.ldg + v] = (T)d;
-  }
-}
-
 // ---- sums of the rows -------------------------------------------------------------------
 constexpr int kOneBlock = 1024;
 template <typename V>
@@ -612,8 +586,9 @@ __global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
 
 // The rows' weights and, for the weight's gradient, x's rows, those that do not count
 // as zeros: what they hold may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld],
-// zeros behind D; ld 0: none.
-template <typename T>
+// zeros behind D; ld 0: none.  FEW: also dz of few classes from their kept logits, in 16
+// bits with zeros as far as 16 bytes go.
+template <typename T, bool FEW>
 __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstream u,
                                                             T* __restrict__ out, int64_t ld,
                                                             int whole) {
@@ -623,6 +598,27 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstr
   const float common = common_of(p, u);
   if (first == 0) *u.scale = common / u.unit;
   for (int64_t row = first; row < p.T; row += step) p.weight[row] = weight_of(p, u, row, common);
+  if constexpr (FEW) {
+    const float c = kLog2e / p.tau;
+    const int64_t cols = sizeof(T) == 2 ? round_up(p.V, 8) : p.V;
+    for (int64_t i = first; i < p.T * cols; i += step) {
+      const int64_t row = i / cols, v = i - row * cols;
+      const float weight = weight_of(p, u, row, common);
+      float d = 0.0f;
+      if (v < p.V && weight != 0.0f) {
+        d = exp2f(__builtin_fmaf(p.logits[row * p.V + v], c, -p.top[row])) / p.total[row];
+        if (p.target != nullptr) {
+          float flag;
+          d -= target_of(p, row, &flag) == v ? 1.0f : 0.0f;
+        } else {
+          for (int e = 0; e < p.k; ++e)
+            d -= p.ids[row * p.k + e] == v ? p.prob[row * p.k + e] : 0.0f;
+        }
+        d *= weight;
+      }
+      static_cast<T*>(p.G)[row * p.ldg + v] = (T)d;
+    }
+  }
   const int64_t per = ceil_div(ld, V), total = p.T * per;
   for (int64_t i = first; i < total; i += step) {
     const int64_t row = i / per, c = (i - row * per) * V;
@@ -865,9 +861,12 @@ template <typename T>
 void launch_prepare(const VocabParams& p, const Upstream& u, char* out, int64_t ld,
                     hipStream_t st) {
   constexpr int64_t V = 16 / sizeof(T);
-  const int64_t most = std::max(p.T, p.T * ceil_div(ld, V));
-  vocab_prepare_kernel<T><<<dim3((unsigned)std::min<int64_t>(ceil_div(most, 256), 1 << 16)), 256, 0,
-                            st>>>(p, u, reinterpret_cast<T*>(out), ld, ld % V == 0);
+  const bool few = p.V <= kFewClasses;
+  const int64_t most = p.T * std::max<int64_t>(ceil_div(ld, V), few ? p.V : 1);
+  const dim3 blocks((unsigned)std::min<int64_t>(ceil_div(most, 256), 1 << 16));
+  T* to = reinterpret_cast<T*>(out);
+  if (few) vocab_prepare_kernel<T, true><<<blocks, 256, 0, st>>>(p, u, to, ld, ld % V == 0);
+  else vocab_prepare_kernel<T, false><<<blocks, 256, 0, st>>>(p, u, to, ld, ld % V == 0);
 }
 template <typename T, bool WHOLE>
 int launch_few_classes(const VocabParams& p, float* loss, hipStream_t st) {
@@ -882,11 +881,6 @@ int launch_few_forward(const VocabParams& p, float* loss, hipStream_t st) {
   if (sizeof(T) == 2 && !(whole_rows(p.x, p.D) && whole_rows(p.w, p.D)))
     return launch_few_classes<T, false>(p, loss, st);
   return launch_few_classes<T, true>(p, loss, st);
-}
-template <typename T>
-int launch_few_grad(const VocabParams& p, hipStream_t st) {
-  vocab_few_grad_kernel<T><<<dim3((unsigned)ceil_div(p.T, 16)), 256, 0, st>>>(p);
-  return check_launch("vocab_loss_backward");
 }
 template <typename T>
 void launch_add(const float* part, int cuts, int64_t count, float* acc, bool start,
@@ -1050,6 +1044,9 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
   set_kept(&p, const_cast<void*>(kept));
   p.weight = b.weight;
   p.x = x;
+  p.G = b.G;
+  p.z = reinterpret_cast<float*>(b.G);
+  p.ldg = b.ldg;
   GroupedParams in = product_of(T, V, D);
   in.A = x;
   in.B = w;
@@ -1071,8 +1068,6 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
   p.w = in.B;
   p.ldx = in.lda;
   p.ldw = in.ldb;
-  p.G = b.G;
-  p.z = reinterpret_cast<float*>(b.G);
   if (e == KAN_OK) e = check_launch(who);
   const bool few = V <= kFewClasses;
   for (p.v0 = 0; e == KAN_OK && p.v0 < V; p.v0 += b.piece) {
@@ -1093,10 +1088,7 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
     };
     // dz of the piece
     p.ldg = half ? padded(p.cols) : p.cols;
-    if (few) {
-      e = dtype == KAN_DTYPE_F32    ? launch_few_grad<float>(p, st)
-          : dtype == KAN_DTYPE_BF16 ? launch_few_grad<bf16>(p, st)
-                                    : launch_few_grad<f16>(p, st);
+    if (few) {  // (the first kernel's)
     } else if (half) {
       e = launch_vocab_tiles<true>(dtype, p, b.cfg, st);
     } else {

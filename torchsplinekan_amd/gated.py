@@ -37,13 +37,13 @@ def _bytes(lib, fn, *args) -> int:
 
 
 class _GatedLinear(torch.autograd.Function):
-    """x [T, K], weight [E, 2, N, K]."""
+    """x [T, K], weight [E, 2, N, K], or [2, N, K] without offsets."""
 
     @staticmethod
     def forward(ctx, x, weight, offsets, act, save):
         lib = _native()
         T, K = x.shape
-        E, _, N, _ = weight.shape
+        N, E = weight.shape[-2], 1 if offsets is None else weight.shape[0]
         code = lib.OPERATOR_DTYPES[x.dtype]
         h = x.new_empty(T, N)
         kept = ws = None
@@ -78,7 +78,8 @@ class _GatedLinear(torch.autograd.Function):
         if need_x:
             dx = _matmul(INPUT, dpre, weight, offsets, dh.new_empty(T, K), T, E, 2 * N, K)
         if need_w:
-            dw = _matmul(WEIGHT, dpre, x, offsets, dh.new_empty(E, 2, N, K), T, E, 2 * N, K)
+            shape = (2, N, K) if offsets is None else (E, 2, N, K)
+            dw = _matmul(WEIGHT, dpre, x, offsets, dh.new_empty(shape), T, E, 2 * N, K)
         return dx, dw, None, None, None
 
 
@@ -122,29 +123,28 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
     Sums over rows have a fixed order."""
     _req(act in ACTS, "act must be None, 'sigmoid', 'tanh', 'silu', 'gelu' or 'relu', got ",
          repr(act))
-    lead = None
+    shape = weight.shape
     if offsets is None:
-        _req(weight.dim() == 3 and weight.shape[0] == 2, "weight must be [2, N, K], got ",
-             list(weight.shape))
+        _req(weight.dim() == 3 and shape[0] == 2, "weight must be [2, N, K], got ", list(shape))
         _req(x.dim() >= 1, "x must have at least one dimension")
-        lead, weight = x.shape[:-1], weight.unsqueeze(0)
     else:
-        _req(x.dim() == 2 and weight.dim() == 4 and weight.shape[1] == 2,
+        _req(x.dim() == 2 and weight.dim() == 4 and shape[1] == 2,
              "with offsets x must be [T, K] and weight [E, 2, N, K], got ", list(x.shape), " and ",
-             list(weight.shape))
-        _req(offsets.dim() == 1 and offsets.shape[0] == weight.shape[0] + 1,
-             "offsets must be [E + 1] = [", weight.shape[0] + 1, "], got ", list(offsets.shape))
+             list(shape))
+        _req(offsets.dim() == 1 and offsets.shape[0] == shape[0] + 1,
+             "offsets must be [E + 1] = [", shape[0] + 1, "], got ", list(offsets.shape))
         _req(offsets.dtype in (torch.int32, torch.int64), "offsets must be int32 or int64, got ",
              offsets.dtype)
         _req(offsets.device == x.device, "x, weight and offsets must be on one device")
-    _req(weight.shape[3] == x.shape[-1], "weight.size(-1)=", weight.shape[3], " must equal K=",
-         x.shape[-1])
+    _req(shape[-1] == x.shape[-1], "weight.size(-1)=", shape[-1], " must equal K=", x.shape[-1])
     _req(weight.dtype == x.dtype, "x and weight must share a dtype")
     _req(weight.device == x.device, "x, weight and offsets must be on one device")
-    if lead is not None:
-        x = x.reshape(lead.numel(), weight.shape[3])
+    lead = None
+    if x.dim() != 2:
+        lead = x.shape[:-1]
+        x = x.reshape(lead.numel(), shape[-1])
     if not x.is_cuda:
-        h = _composite(x, weight, offsets, act)
+        h = _composite(x, weight if offsets is not None else weight.unsqueeze(0), offsets, act)
     else:
         _native().operator_dtype_code(x.dtype, "gated_linear")
         x, weight = x.contiguous(), weight.contiguous()
@@ -154,4 +154,4 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
             h = _GatedLinear.apply(x, weight, offsets, ACTS[act], save)
         else:
             h = _GatedLinear.forward(None, x, weight, offsets, ACTS[act], False)
-    return h if lead is None else h.reshape(lead + (weight.shape[2],))
+    return h if lead is None else h.reshape(lead + (shape[-2],))

@@ -128,8 +128,9 @@ def _loss(who, x, weight, ids, teacher, ignore, tau, reduction):
     _req(weight.device == x.device and ids.device == x.device, who,
          ": tensors must be on one device")
     lead, code = x.shape[:-1], REDUCTIONS[reduction]
-    x = x.reshape(lead.numel(), x.shape[-1])
-    ids = ids.reshape(lead.numel(), ids.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(lead.numel(), x.shape[-1])
+        ids = ids.reshape(lead.numel(), ids.shape[-1])
     if teacher is not None:
         teacher = teacher.detach().reshape(ids.shape)
     if not x.is_cuda or x.numel() == 0 or ids.numel() == 0:
@@ -144,7 +145,7 @@ def _loss(who, x, weight, ids, teacher, ignore, tau, reduction):
             loss = _VocabLoss.apply(*args)
         else:
             loss = _VocabLoss.forward(None, *args)
-    return loss.reshape(lead) if code == 0 else loss
+    return loss.reshape(lead) if code == 0 and len(lead) != 1 else loss
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, *,

@@ -18,9 +18,8 @@ _C = _fused._C
 ACTS = {None: 0, "sigmoid": 1, "tanh": 2, "silu": 3, "gelu": 4, "relu": 5}
 
 
-def _req(cond: bool, *msg) -> None:
-    if not cond:
-        raise RuntimeError("gated_linear: " + "".join(str(m) for m in msg))
+def _refuse(*msg) -> None:
+    raise RuntimeError("gated_linear: " + "".join(str(m) for m in msg))
 
 
 def _native():
@@ -121,24 +120,30 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
     Gradients (first order) reach x and weight (device tensors refuse forward
     mode); for them 5 (bfloat16), 6 (float16) or 8 bytes an output are kept.
     Sums over rows have a fixed order."""
-    _req(act in ACTS, "act must be None, 'sigmoid', 'tanh', 'silu', 'gelu' or 'relu', got ",
-         repr(act))
+    if act not in ACTS:
+        _refuse("act must be None, 'sigmoid', 'tanh', 'silu', 'gelu' or 'relu', got ", repr(act))
     shape = weight.shape
     if offsets is None:
-        _req(weight.dim() == 3 and shape[0] == 2, "weight must be [2, N, K], got ", list(shape))
-        _req(x.dim() >= 1, "x must have at least one dimension")
+        if weight.dim() != 3 or shape[0] != 2:
+            _refuse("weight must be [2, N, K], got ", list(shape))
+        if x.dim() < 1:
+            _refuse("x must have at least one dimension")
     else:
-        _req(x.dim() == 2 and weight.dim() == 4 and shape[1] == 2,
-             "with offsets x must be [T, K] and weight [E, 2, N, K], got ", list(x.shape), " and ",
-             list(shape))
-        _req(offsets.dim() == 1 and offsets.shape[0] == shape[0] + 1,
-             "offsets must be [E + 1] = [", shape[0] + 1, "], got ", list(offsets.shape))
-        _req(offsets.dtype in (torch.int32, torch.int64), "offsets must be int32 or int64, got ",
-             offsets.dtype)
-        _req(offsets.device == x.device, "x, weight and offsets must be on one device")
-    _req(shape[-1] == x.shape[-1], "weight.size(-1)=", shape[-1], " must equal K=", x.shape[-1])
-    _req(weight.dtype == x.dtype, "x and weight must share a dtype")
-    _req(weight.device == x.device, "x, weight and offsets must be on one device")
+        if x.dim() != 2 or weight.dim() != 4 or shape[1] != 2:
+            _refuse("with offsets x must be [T, K] and weight [E, 2, N, K], got ", list(x.shape),
+                    " and ", list(shape))
+        if offsets.dim() != 1 or offsets.shape[0] != shape[0] + 1:
+            _refuse("offsets must be [E + 1] = [", shape[0] + 1, "], got ", list(offsets.shape))
+        if offsets.dtype not in (torch.int32, torch.int64):
+            _refuse("offsets must be int32 or int64, got ", offsets.dtype)
+        if offsets.device != x.device:
+            _refuse("x, weight and offsets must be on one device")
+    if shape[-1] != x.shape[-1]:
+        _refuse("weight.size(-1)=", shape[-1], " must equal K=", x.shape[-1])
+    if weight.dtype != x.dtype:
+        _refuse("x and weight must share a dtype")
+    if weight.device != x.device:
+        _refuse("x, weight and offsets must be on one device")
     lead = None
     if x.dim() != 2:
         lead = x.shape[:-1]

@@ -18,9 +18,8 @@ from . import fused as _fused
 _C = _fused._C
 
 
-def _req(cond: bool, *msg) -> None:
-    if not cond:
-        raise RuntimeError("layer_norm: " + "".join(str(m) for m in msg))
+def _refuse(*msg) -> None:
+    raise RuntimeError("layer_norm: " + "".join(str(m) for m in msg))
 
 
 def _native():
@@ -88,17 +87,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     Statistics and sums are held in float32.  First-order gradients reach x,
     weight and bias (device tensors refuse forward mode); sums over rows have a
     fixed order."""
-    _req(x.dim() >= 1, "x must have at least one dimension")
+    if x.dim() < 1:
+        _refuse("x must have at least one dimension")
     C, dtype = x.shape[-1], x.dtype if dtype is None else dtype
-    _req(x.dtype == dtype or x.dtype == torch.float32,
-         "x must be in the result's type or float32, got ", x.dtype, " and ", dtype)
+    if x.dtype != dtype and x.dtype != torch.float32:
+        _refuse("x must be in the result's type or float32, got ", x.dtype, " and ", dtype)
     for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            _req(t.dim() == 1 and t.shape[0] == C, name, " must have shape [", C, "], got ",
-                 list(t.shape))
-            _req(t.device == x.device, "tensors must be on one device")
-    _req(weight is None or bias is None or weight.dtype == bias.dtype,
-         "weight and bias must share a dtype")
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != C:
+            _refuse(name, " must have shape [", C, "], got ", list(t.shape))
+        if t.device != x.device:
+            _refuse("tensors must be on one device")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        _refuse("weight and bias must share a dtype")
     if not x.is_cuda or x.numel() == 0:
         return _composite(x, weight, bias, eps, dtype)
     lib = _native()
@@ -106,10 +108,12 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
         if t is not None and t.dtype not in lib.OPERATOR_DTYPES:
             lib.operator_dtype_code(t.dtype, "layer_norm")  # (raises)
     lib.operator_dtype_code(dtype, "layer_norm")
-    x, weight, bias = [t if t is None or t.is_contiguous() else t.contiguous()
-                       for t in (x, weight, bias)]
-    save = torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                           for t in (x, weight, bias))
+    x = x.contiguous()
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    save = torch.is_grad_enabled() and (
+        x.requires_grad or weight is not None and weight.requires_grad
+        or bias is not None and bias.requires_grad)
     if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
         return _LayerNorm.apply(x, weight, bias, float(eps), dtype, save)
     return _LayerNorm.forward(None, x, weight, bias, float(eps), dtype, save)

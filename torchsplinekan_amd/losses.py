@@ -20,9 +20,8 @@ REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 MAX_TOP = 1024
 
 
-def _req(cond: bool, *msg) -> None:
-    if not cond:
-        raise RuntimeError("".join(str(m) for m in msg))
+def _refuse(*msg) -> None:
+    raise RuntimeError("".join(str(m) for m in msg))
 
 
 def _native(who: str):
@@ -52,7 +51,8 @@ class _VocabLoss(torch.autograd.Function):
         code, L = lib.OPERATOR_DTYPES[x.dtype], lib.LIB
         kept, _ = _workspace(lib, x.device, L.kan_hip_vocab_loss_kept, T, V, k)
         px, pw = x.data_ptr(), weight.data_ptr()
-        ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_workspace, code, px, pw, T, V, D)
+        ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_workspace, code, px, pw, T, V,
+                                D)
         loss = torch.empty((T,) if reduction == 0 else (), dtype=torch.float32, device=x.device)
         lib.launch(L.kan_hip_vocab_loss, x.device, code, px, pw, ids.data_ptr(),
                    int(ids.dtype == torch.int64), None if teacher is None else teacher.data_ptr(),
@@ -73,8 +73,8 @@ class _VocabLoss(torch.autograd.Function):
                   for t, need in zip((x, weight), ctx.needs_input_grad)]
         g = g.contiguous()
         px, pw, L = x.data_ptr(), weight.data_ptr(), lib.LIB
-        ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_backward_workspace, code, px, pw,
-                                T, V, D, int(dx is not None), int(dw is not None))
+        ws, nbytes = _workspace(lib, x.device, L.kan_hip_vocab_loss_backward_workspace, code, px,
+                                pw, T, V, D, int(dx is not None), int(dw is not None))
         lib.launch(L.kan_hip_vocab_loss_backward, x.device, code, g.data_ptr(), px, pw,
                    None if ids is None else ids.data_ptr(),
                    int(ids is not None and ids.dtype == torch.int64), kept.data_ptr(), T, V, D, k,
@@ -117,16 +117,19 @@ def _composite(x, weight, ids, teacher, ignore, tau, reduction):
 
 def _loss(who, x, weight, ids, teacher, ignore, tau, reduction):
     """x [..., D], ids [..., k] as checked by the callers."""
-    _req(reduction in REDUCTIONS, who, ": reduction must be 'none', 'sum' or 'mean', got ",
-         repr(reduction))
-    _req(x.dim() >= 1 and weight.dim() == 2, who, ": x must be [..., D] and weight [V, D], got ",
-         list(x.shape), " and ", list(weight.shape))
-    _req(weight.shape[1] == x.shape[-1], who, ": weight.size(1)=", weight.shape[1],
-         " must equal D=", x.shape[-1])
-    _req(weight.shape[0] >= 1, who, ": weight must have at least one row")
-    _req(weight.dtype == x.dtype, who, ": x and weight must share a dtype")
-    _req(weight.device == x.device and ids.device == x.device, who,
-         ": tensors must be on one device")
+    if reduction not in REDUCTIONS:
+        _refuse(who, ": reduction must be 'none', 'sum' or 'mean', got ", repr(reduction))
+    if x.dim() < 1 or weight.dim() != 2:
+        _refuse(who, ": x must be [..., D] and weight [V, D], got ", list(x.shape), " and ",
+                list(weight.shape))
+    if weight.shape[1] != x.shape[-1]:
+        _refuse(who, ": weight.size(1)=", weight.shape[1], " must equal D=", x.shape[-1])
+    if weight.shape[0] < 1:
+        _refuse(who, ": weight must have at least one row")
+    if weight.dtype != x.dtype:
+        _refuse(who, ": x and weight must share a dtype")
+    if weight.device != x.device or ids.device != x.device:
+        _refuse(who, ": tensors must be on one device")
     lead, code = x.shape[:-1], REDUCTIONS[reduction]
     if x.dim() != 2:
         x = x.reshape(lead.numel(), x.shape[-1])
@@ -163,10 +166,11 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     mode); their products take the logits' gradient in x's type, and sums are held
     in float32, also under autocast, which casts nothing here."""
     who = "linear_cross_entropy"
-    _req(target.dtype in (torch.int32, torch.int64), who, ": target must be int32 or int64, got ",
-         target.dtype)
-    _req(x.dim() >= 1 and target.shape == x.shape[:-1], who, ": target must have x's leading shape ",
-         list(x.shape[:-1]), ", got ", list(target.shape))
+    if target.dtype not in (torch.int32, torch.int64):
+        _refuse(who, ": target must be int32 or int64, got ", target.dtype)
+    if x.dim() < 1 or target.shape != x.shape[:-1]:
+        _refuse(who, ": target must have x's leading shape ", list(x.shape[:-1]), ", got ",
+                list(target.shape))
     return _loss(who, x, weight, target.unsqueeze(-1), None, int(ignore_index), 1.0, reduction)
 
 
@@ -184,18 +188,21 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor
     teacher [..., k]: its logits at ids, float32, bfloat16 or float16; no gradient
     reaches it.  reduction, types and gradients as linear_cross_entropy."""
     who = "linear_distillation"
-    _req(ids.dtype in (torch.int32, torch.int64), who, ": ids must be int32 or int64, got ",
-         ids.dtype)
-    _req(x.dim() >= 1 and ids.dim() == x.dim() and ids.shape[:-1] == x.shape[:-1], who,
-         ": ids must have x's leading shape and k ids each, got ", list(ids.shape), " and ",
-         list(x.shape))
-    _req(1 <= ids.shape[-1] <= MAX_TOP, who, ": 1 to ", MAX_TOP, " ids a row, got ", ids.shape[-1])
-    _req(teacher.shape == ids.shape, who, ": teacher must have ids' shape ", list(ids.shape),
-         ", got ", list(teacher.shape))
-    _req(teacher.is_floating_point(), who, ": teacher must hold floating point logits, got ",
-         teacher.dtype)
-    _req(teacher.device == x.device, who, ": tensors must be on one device")
+    if ids.dtype not in (torch.int32, torch.int64):
+        _refuse(who, ": ids must be int32 or int64, got ", ids.dtype)
+    if x.dim() < 1 or ids.dim() != x.dim() or ids.shape[:-1] != x.shape[:-1]:
+        _refuse(who, ": ids must have x's leading shape and k ids each, got ", list(ids.shape),
+                " and ", list(x.shape))
+    if not 1 <= ids.shape[-1] <= MAX_TOP:
+        _refuse(who, ": 1 to ", MAX_TOP, " ids a row, got ", ids.shape[-1])
+    if teacher.shape != ids.shape:
+        _refuse(who, ": teacher must have ids' shape ", list(ids.shape), ", got ",
+                list(teacher.shape))
+    if not teacher.is_floating_point():
+        _refuse(who, ": teacher must hold floating point logits, got ", teacher.dtype)
+    if teacher.device != x.device:
+        _refuse(who, ": tensors must be on one device")
     temperature = float(temperature)
-    _req(1e-30 <= temperature <= 1e30, who, ": temperature must be positive and finite, got ",
-         temperature)
+    if not 1e-30 <= temperature <= 1e30:
+        _refuse(who, ": temperature must be positive and finite, got ", temperature)
     return _loss(who, x, weight, ids, teacher, -1, temperature, reduction)

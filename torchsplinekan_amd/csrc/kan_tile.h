@@ -144,15 +144,17 @@ struct Operand {
   // A whole slab straight into LDS.  (In assembly: the compiler would wait for
   // these loads before any transposing LDS read, taking it for a read of the
   // same bytes; slab_barrier waits for them.  They write no register.)
-  __device__ __forceinline__ void issue(int64_t k0, char* lds) const {
+  __device__ __forceinline__ void issue_part(int64_t k0, char* lds, int p) const {
     const uint32_t to = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds + (threadIdx.x >> 6) * 1024);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                     to + p * NT * 16),
+                 "v"(off[p]), "s"(slab(k0, p))
+                 : "m0");
+  }
+  __device__ __forceinline__ void issue(int64_t k0, char* lds) const {
 #pragma unroll
-    for (int p = 0; p < kPer; ++p)
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
-                       to + p * NT * 16),
-                   "v"(off[p]), "s"(slab(k0, p))
-                   : "m0");
+    for (int p = 0; p < kPer; ++p) issue_part(k0, lds, p);
   }
 
   // A slab into registers.  GUARD: k from kend on is zero, and chunks that lie
@@ -377,6 +379,28 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, int64_t kbeg, int64_t kend
     for (int st = 0; st + 1 < kSteps; ++st) {
       read_step(cur, st + 1);
       mma_step(st);
+    }
+    constexpr bool kStraight = A::kMode == kDirect && B::kMode == kDirect;
+    if constexpr (kStraight && !decltype(rest)::value) {
+      // (a whole slab in the midst of others: its loads and reads one by one under the
+      // step's MFMAs; the loads before them all, as the barrier leaves both of a
+      // SIMD's waves, kept its matrix unit waiting)
+      slab_barrier();
+      const int64_t k0 = kbeg + (int64_t)(kt + 2) * kDepth;
+      constexpr int kLoads = A::kPer + B::kPer, kSteps1 = (kSteps - 1) & 1;
+#pragma unroll
+      for (int q = 0; q < FM * FN || q < kLoads; ++q) {
+        if (q < FM * FN) {
+          const int i = q / FN, j = q % FN;
+          acc[i][j] = Half<T>::mma(bv[kSteps1][j], av[kSteps1][i], acc[i][j]);
+        }
+        if (q < FN) bv[0][q] = fb.read(nxt + kB, q, 0);
+        else if (q < FN + FM) av[0][q - FN] = fa.read(nxt, q - FN, 0);
+        if (q < A::kPer) a.issue_part(k0, cur, q);
+        else if (q < kLoads) b.issue_part(k0, cur + kB, q - A::kPer);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return;
     }
     if (next) {
       finish(nxt);

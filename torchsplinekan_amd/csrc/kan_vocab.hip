@@ -535,6 +535,7 @@ __global__ __launch_bounds__(kOneBlock) void vocab_sum_kernel(VocabParams p,
                                                               int mean, float* __restrict__ loss) {
   __shared__ double red[kOneBlock];
   double sum = 0.0, count = 0.0;
+#pragma unroll 8
   for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock) {
     sum += rows[t];
     count += p.flag[t] == 0.0f ? 0.0 : 1.0;
@@ -573,8 +574,9 @@ __global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
                                                                float* __restrict__ out) {
   __shared__ float red[kOneBlock];
   float most = 0.0f;
+#pragma unroll 8
   for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock)
-    if (p.flag[t] != 0.0f) most = fmaxf(most, fabsf(g[t]));
+    most = fmaxf(most, p.flag[t] != 0.0f ? fabsf(g[t]) : 0.0f);
   red[threadIdx.x] = most;
   __syncthreads();
   for (int m = kOneBlock / 2; m > 0; m /= 2) {

@@ -532,7 +532,7 @@ int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* k
  * anything.  reduction: the rows' losses [T] (0 where a row does not count),
  * their sum, or their mean over the rows that count (0 without any).  kept
  * (kan_hip_vocab_loss_kept bytes) is written by the forward and read by the
- * backward, which takes a cross entropy's ids again too.  (The logits of at most 64
+ * backward, which takes a cross entropy's ids again too.  (The logits of at most 32
  * columns are kept.)  grad_x [T, D], grad_w [V, D], either of which may be NULL (with_dx,
  * with_dw: whether it will be given).  V and D are positive, T < 2^30, V and D <=
  * 2^22, k <= 1024.  Workspaces depend on the operands' alignment; they and kept lie

@@ -353,6 +353,80 @@ def test_gradients_are_off_by_two_roundings(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,V", [(1, 10), (70, 32), (40, 33), (300, 1500), (3, 5000)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_rows_that_are_nearly_certain(T, V, ties, dtype):
+    """Logits without rounding (sixteenths), targets ahead of the rest by 8 to 25: what
+    is left of the loss, 1e-3 and below, is right in its own size, and so are gradients.
+    Each exponential's argument is rounded in its product with log2(e) and by log2(e)
+    itself, and comes out to 2 ulp: r = (3 |z - top| + 8) u; then a sum of V terms.
+    ties: a row's largest logit is there twice (loss log 2 and more)."""
+    g = torch.Generator().manual_seed(V + T)
+    w = torch.randint(-3, 4, (V, 64), generator=g).float()
+    w[:, 0] = 4
+    target = torch.randint(1, V, (T,), generator=g)
+    x = w[target] / 16
+    if ties:
+        w[0] = w[int(target[0])]
+    z = x.double() @ w.double().t()
+    top = z.amax(1, keepdim=True)
+    assert bool((z.gather(1, target[:, None]) == top).all()) or ties
+    e = (z - top).exp()
+    hit = F.one_hot(target, V).double()
+    rest = (e * (1 - hit)).sum(1, keepdim=True) if not ties else e.sum(1, keepdim=True) - 1
+    rows = (torch.log1p(rest) + top - z.gather(1, target[:, None]))[:, 0]
+    r = (3 * (z - top).amin().abs() + 8 + V) * U
+    xd, wd = (t.to("cuda", dtype).requires_grad_() for t in (x, w))
+    loss = linear_cross_entropy(xd, wd, target.cuda(), reduction="none")
+    _near(loss, (rows, 2 * r * rows + 2.0 ** -126), "loss")
+    dx, dw = torch.autograd.grad(loss, [xd, wd], torch.ones(T, device="cuda"))
+    # q - 1 = ((e - 1) - rest) / (1 + rest), without the difference of nearly equal numbers
+    d = ((e - hit) - hit * rest) / (1 + rest)
+    H = HALF_ULP[dtype]
+    # (float16: dz 2^15 times as large, subnormals 2^-24 apart)
+    Ed = d.abs() * (2 * r + (0 if dtype == F32 else H)) + (2.0 ** -39 if dtype == F16 else 0.0)
+    for got, a, E, b, terms in ((dx, d, Ed, w, V), (dw, d.t(), Ed.t(), x, T)):
+        value = a @ b.double()
+        err = (E + (2 * terms + 32) * U * (a.abs() + E)) @ b.double().abs()
+        tol = err + H * (value.abs() + err) + (2.0 ** -25 if dtype == F16 else 2.0 ** -126)
+        _near(got, (value, tol), "gradient")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T,V,D", [(1, 2, 115), (3, 120, 128), (64, 9000, 40), (65, 1000, 72),
+                                   (2048, 20, 64), (3, 100000, 64)])
+@pytest.mark.parametrize("k", [0, 2])
+def test_small_problems_round_their_gradients_once(T, V, D, k, dtype):
+    """Up to 64 rows, or 4096 and 2^31 products of values, dz goes into its products in two parts:
+    what is left of its rounding is H^2 of it, and the gradients' error their own
+    rounding.  2^15 dz in float16 has subnormals 2^-24 apart in its second part."""
+    x, w, ids, *teacher = _inputs(T, V, D, dtype, k, seed=V)
+    x, w, ids = x.cuda(), w.cuda(), ids.cuda()
+    teacher = teacher[0].cuda() if teacher else None
+    if teacher is None:
+        ids = ids[:, None]
+    xd, wd = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = _call(xd, wd, ids if k else ids[:, 0], teacher, 1.0, -100, "sum")
+    H = HALF_ULP[dtype]
+    got = torch.autograd.grad(loss, [xd, wd], torch.tensor(2.0, device="cuda"))
+    g = torch.full((T,), 2.0, dtype=torch.float64, device="cuda")
+    # the bound of float32 operands, with the second part's rounding and the last one
+    _, *want = _expected(x.float(), w.float(), ids, teacher, 1.0, -100, g, F32)
+    z = x.double() @ w.double().t()
+    p = torch.zeros_like(z).scatter_add_(1, ids, torch.ones_like(ids, dtype=torch.float64)
+                                         if teacher is None else teacher.double().softmax(1))
+    d = (2 * (z.softmax(1) - p)).abs()
+    part = 2 * H * H * d + (2.0 ** -38 if dtype == F16 else 0.0)
+    for a, (value, tol), left in zip(got, want, (part @ w.double().abs(),
+                                                 part.t() @ x.double().abs())):
+        err = tol + 2 * left
+        _near(a, (value, err + H * (value.abs() + err) + (2.0 ** -25 if dtype == F16 else 0.0)),
+              "gradient")
+
+
+@pytest.mark.gpu
 def test_half_precision_keeps_small_probabilities():
     """A vocabulary whose probabilities are below float16's smallest numbers."""
     T, V, D = 64, 60000, 32

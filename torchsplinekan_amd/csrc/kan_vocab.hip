@@ -6,16 +6,17 @@
 //   dz_t   = g_t tau (q - sum_j p_j e_{id_j}),   dx = dz W,   dW = dz^T x.
 // (tau = 1 and one id: lse(z) - z_id and g_t (q - e_id).)
 //
-// Forward: the product's tiles end in each row's maximum, sum of exponentials and
-// sum of p z over the tile's columns; a second kernel joins a row's tiles.  Backward:
+// Forward: the product's tiles end in each row's maximum, rest and sum of p z over the
+// tile's columns (see below); a second kernel joins a row's tiles.  Backward:
 // piece by piece of the vocabulary the product again, whose tiles end in dz in the
 // operands' type, and dx += dz W, dW = dz^T x from that piece.  4/3 of the
 // operations that kept logits would take, and 2 bytes a logit of one piece.
 //
-// Exponentials are 2^(z log2(e) / tau - top) from one fused product and difference,
-// so that top, rounded once, is the exact reference of all of a row's; and p is
-// subtracted before the rounding to 16 bits: where q is nearly p what is left keeps
-// its accuracy.
+// A row keeps its largest z, top, and rest = the sum of exp((z - top) / tau) over the
+// others (1 for each that equals top but one): lse = top / tau + log1p(rest), and
+//   q_j - p_j = ((e_j - p_j) - p_j rest) / (1 + rest),   e_j = exp((z_j - top) / tau),
+// so the small loss and gradient of a row that is nearly certain keep their accuracy,
+// which 1 + rest alone rounds away.
 // dz is rounded to 16 bits as (q - p) w with w = 1 in rows that all count alike (in
 // f16 2^15, so that probabilities of 1e-8 still are normal numbers); the common
 // factor g tau is applied to the float32 sums of dx and dW.
@@ -41,8 +42,7 @@ struct VocabParams {
   int target64;
   int64_t ignore;
   // kept for the backward pass
-  float *top, *total;  // [T]: a row's largest z / tau in powers of 2, and its sum of
-                       // 2^(z log2(e) / tau - top)
+  float *top, *rest;   // [T]
   float* flag;         // [T]: 1; 0: the row does not count; NaN: an id that is no column
   float* count;        // rows that count
   float* logits;       // [T, V] of few classes
@@ -55,7 +55,8 @@ struct VocabParams {
   float* weight;       // [T]: w
   float* z;            // fp32: [T, cols] logits, then dz of a piece
   void* G;             // 16 bits: [T, ldg] dz of a piece, zeros behind its columns as far
-                       // as 16 bytes go
+                       // as 16 bytes go; then, or null,
+  void* G2;            // [T, ldg]: what the rounding of G's values has left, rounded
   int64_t ldg;
   int64_t v0, cols;    // the piece
 };
@@ -137,16 +138,35 @@ __device__ __forceinline__ int first_id(const int* __restrict__ ids, int k, int 
   return lo;
 }
 
+// The part of `rest` of a value z, `from` the largest (or 0 for none), which is itself
+// counted in `most`.
+__device__ __forceinline__ float below(float z, float from, float c) {
+  return z == from ? 0.0f : __builtin_amdgcn_exp2f((z - from) * c);
+}
+// top and rest of two sets of logits as those of both (top -INFINITY: an empty set, whose
+// rest is 0).
+__device__ __forceinline__ void join(float* top, float* rest, float m, float s, float c) {
+  const bool more = m > *top;
+  const float most = more ? m : *top, least = more ? *top : m;
+  const float mine = more ? s : *rest, other = more ? *rest : s;
+  const float f = least == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((least - most) * c);
+  *rest = mine + (other + 1.0f) * f;
+  *top = most;
+}
+
 // ---- tiles in 16 bits -------------------------------------------------------------
 // A lane holds rows 32 i + (lane & 31) of its wave's and 32 columns: 32 j + 8 q +
 // 4 (lane >> 5) + s at acc[i][j][4 q + s].
-template <typename T, class G, int MODE, bool GRAD>
+// PARTS (0: the forward pass): of dz.  Only the smallest tile takes two: on the
+// largest the second time over its sums would not stay in registers.
+template <typename T, class G, int MODE, int PARTS>
 __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int tiles_n) {
   constexpr int BM = G::BM, BN = G::BN, FM = G::FM, WN = G::WN;
+  constexpr bool GRAD = PARTS > 0;
   static_assert(G::FN == 2, "a wave has 64 columns");
   __shared__ __align__(16) char lds[2 * G::kBuf];
   __shared__ int first[BM], last[BM];  // the row's ids in the tile's columns; its target
-  __shared__ float row_from[GRAD ? BM : 1], row_weight[GRAD ? BM : 1];
+  __shared__ float row_top[GRAD ? BM : 1], row_rest[GRAD ? BM : 1], row_weight[GRAD ? BM : 1];
   RowTile t;
   int tn;
   dense_tile(p.T, BM, tiles_n, &t, &tn);
@@ -167,8 +187,9 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
           while (hi < p.k && ids[hi] < col0 + BN) ++hi;
         }
         if constexpr (GRAD) {
-          row_from[r] = p.top[row] + __builtin_amdgcn_logf(p.total[row]);
+          row_top[r] = p.top[row];
           row_weight[r] = p.weight[row];
+          row_rest[r] = p.rest[row];
         }
       }
       first[r] = lo;
@@ -224,15 +245,19 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
 #pragma unroll
         for (int v = 0; v < 16; ++v) top = fmaxf(top, acc[i][j][v]);
       top = fmaxf(top, __shfl_xor(top, 32));
-      top *= c;
       const float from = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
+      float rest = 0.0f;
+      int most = 0;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v)
-          sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], c, -from));
-      sum += __shfl_xor(sum, 32);
+        for (int v = 0; v < 16; ++v) {
+          rest += below(acc[i][j][v], from, c);
+          most += acc[i][j][v] == from ? 1 : 0;
+        }
+      rest += __shfl_xor(rest, 32);
+      most += __shfl_xor(most, 32);
+      if (top > -INFINITY) rest += (float)(most - 1);
       float dot = 0.0f;
       entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
         if (at < 0 || at >= 64 || ((at >> 2) & 1) != half || prob == 0.0f) return;
@@ -247,47 +272,48 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
       dot += __shfl_xor(dot, 32);
       if (half == 0) {
         red[wn * BM + r] = top;
-        red[(WN + wn) * BM + r] = sum;
+        red[(WN + wn) * BM + r] = rest;
         red[(2 * WN + wn) * BM + r] = dot;
       }
     }
     __syncthreads();
     for (int r = threadIdx.x; r < BM; r += G::NT) {
       if (t.m0 + r >= t.m1) break;
-      float top = -INFINITY, sum = 0.0f, dot = 0.0f;
+      float top = red[r], rest = red[WN * BM + r], dot = red[2 * WN * BM + r];
 #pragma unroll
-      for (int q = 0; q < WN; ++q) top = fmaxf(top, red[q * BM + r]);
-      const float from = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int q = 0; q < WN; ++q) {
-        sum += red[(WN + q) * BM + r] * __builtin_amdgcn_exp2f(red[q * BM + r] - from);
+      for (int q = 1; q < WN; ++q) {
+        join(&top, &rest, red[q * BM + r], red[(WN + q) * BM + r], c);
         dot += red[(2 * WN + q) * BM + r];
       }
       float* out = p.stats + (int64_t)tn * p.T + t.m0 + r;
       out[0] = top;
-      out[p.tiles * p.T] = sum;
+      out[p.tiles * p.T] = rest;
       out[2 * p.tiles * p.T] = dot;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int r = (wm * FM + i) * 32 + (lane & 31);
-      const float from = row_from[r], weight = row_weight[r];
+      const float top = row_top[r], rest = row_rest[r], weight = row_weight[r];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
-          acc[i][j][v] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][v], c, -from));
+          acc[i][j][v] = __builtin_amdgcn_exp2f((acc[i][j][v] - top) * c);
       entries(r, t.m0 + r, [&](int at, float prob) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) acc[i][j][v] -= col_of(j, v) == at ? prob : 0.0f;
+          for (int v = 0; v < 16; ++v) {
+            const float here = col_of(j, v) == at ? prob : 0.0f;
+            acc[i][j][v] = __builtin_fmaf(-here, rest, acc[i][j][v] - here);
+          }
       });
+      const float part = weight / (1.0f + rest);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) acc[i][j][v] *= weight;
+        for (int v = 0; v < 16; ++v) acc[i][j][v] *= part;
       if (left < 64 || __any(weight == 0.0f)) {  // (a row that does not count may hold NaN)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
@@ -300,29 +326,39 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
     constexpr int kWaveRows = FM * 32, kRowBytes = 128, kChunks = 8;
     char* stage = lds + wave * kWaveRows * kRowBytes;
     typedef T t4 __attribute__((ext_vector_type(4)));
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int r = i * 32 + (lane & 31);
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          t4 v;
-#pragma unroll
-          for (int u = 0; u < 4; ++u) v[u] = (T)acc[i][j][4 * q + u];
-          const int ch = (4 * j + q) ^ (r & (kChunks - 1));
-          *reinterpret_cast<t4*>(stage + r * kRowBytes + ch * 16 + half * 8) = v;
-        }
-    }
     const int64_t row0 = t.m0 + wm * kWaveRows, col0 = n0 + wn * 64;
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part) {
+      T* to = static_cast<T*>(part == 0 ? p.G : p.G2);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = i * 32 + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            t4 v;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = (T)acc[i][j][4 * q + u];
+            const int ch = (4 * j + q) ^ (r & (kChunks - 1));
+            *reinterpret_cast<t4*>(stage + r * kRowBytes + ch * 16 + half * 8) = v;
+          }
+      }
 #pragma unroll 4
-    for (int it = 0; it < kWaveRows / 8; ++it) {
-      const int r = it * 8 + lane / kChunks, ch = lane % kChunks;
-      const u32x4 v =
-          *reinterpret_cast<const u32x4*>(stage + r * kRowBytes + ((ch ^ (r & (kChunks - 1))) * 16));
-      const int64_t row = row0 + r, col = col0 + 8 * ch;
-      if (row < t.m1 && col < p.ldg)
-        *reinterpret_cast<u32x4*>(static_cast<T*>(p.G) + row * p.ldg + col) = v;
+      for (int it = 0; it < kWaveRows / 8; ++it) {
+        const int r = it * 8 + lane / kChunks, ch = lane % kChunks;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(stage + r * kRowBytes +
+                                                        ((ch ^ (r & (kChunks - 1))) * 16));
+        const int64_t row = row0 + r, col = col0 + 8 * ch;
+        if (row < t.m1 && col < p.ldg) *reinterpret_cast<u32x4*>(to + row * p.ldg + col) = v;
+      }
+      if (part + 1 == PARTS) break;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) acc[i][j][v] -= (float)(T)acc[i][j][v];
     }
   }
 }
@@ -359,12 +395,17 @@ __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
       float top = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kSpanValues; ++i) top = fmaxf(top, v[i]);
-      top = wave_max(top) * c;
+      top = wave_max(top);
       const float base = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f;
+      float rest = 0.0f, most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) sum += exp2f(__builtin_fmaf(v[i], c, -base));
-      sum = wave_sum(sum);
+      for (int i = 0; i < kSpanValues; ++i) {
+        rest += below(v[i], base, c);
+        most += v[i] == base ? 1.0f : 0.0f;
+      }
+      rest = wave_sum(rest);
+      most = wave_sum(most);
+      if (top > -INFINITY) rest += most - 1.0f;
       float dot = 0.0f;
       entries([&](int at, float prob) {
         if (prob != 0.0f) dot += prob * z[at];
@@ -372,27 +413,31 @@ __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
       if (lane == 0) {
         float* out = p.stats + ((p.v0 + n0) / kSpan) * p.T + row;
         out[0] = top;
-        out[p.tiles * p.T] = sum;
+        out[p.tiles * p.T] = rest;
         out[2 * p.tiles * p.T] = dot;
       }
     } else {
-      const float top = p.top[row], part = 1.0f / p.total[row], weight = p.weight[row];
+      const float top = p.top[row], rest = p.rest[row], weight = p.weight[row];
+      const float part = weight / (1.0f + rest);
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f(__builtin_fmaf(v[i], c, -top)) * part;
+      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f((v[i] - top) * c);
       entries([&](int at, float prob) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kSpanValues; ++i) v[i] -= lane + 64 * i == at ? prob : 0.0f;
+        for (int i = 0; i < kSpanValues; ++i) {
+          const float here = lane + 64 * i == at ? prob : 0.0f;
+          v[i] = __builtin_fmaf(-here, rest, v[i] - here);
+        }
       });
 #pragma unroll
       for (int i = 0; i < kSpanValues; ++i)
-        if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * weight;
+        if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * part;
     }
   }
 }
 
 // ---- rows ---------------------------------------------------------------------------
-// The row's loss from its top, sum and dot = sum_j p_j z_j, and what is kept of it.
-__device__ __forceinline__ void finish_row(const VocabParams& p, int64_t row, float top, float sum,
+// The row's loss from its top, rest and dot = sum_j p_j z_j, and what is kept of it.
+__device__ __forceinline__ void finish_row(const VocabParams& p, int64_t row, float top, float rest,
                                            float dot, float* __restrict__ loss) {
   float flag, entropy = 0.0f;
   if (p.target != nullptr) {
@@ -403,17 +448,11 @@ __device__ __forceinline__ void finish_row(const VocabParams& p, int64_t row, fl
     entropy = p.entropy[row];
   }
   p.top[row] = top;
-  p.total[row] = sum;
-  const float c = kLog2e / p.tau;
+  if (top == INFINITY) rest = NAN;  // (inf - inf, as everywhere else in the row)
+  p.rest[row] = rest;
   loss[row] = flag == 0.0f ? 0.0f
               : flag != flag ? flag
-                             : p.tau * p.tau * (entropy + (top - dot * c) * 0.6931471805599453f +
-                                                logf(sum));
-}
-__device__ __forceinline__ void join(float* top, float* sum, float m, float s) {
-  const float most = fmaxf(*top, m), from = most == -INFINITY ? 0.0f : most;
-  *sum = *sum * exp2f(*top - from) + s * exp2f(m - from);
-  *top = most;
+                             : p.tau * p.tau * (entropy + (top - dot) / p.tau + log1pf(rest));
 }
 // A row's tiles joined: 16 rows a block, 64 lanes of tiles a row, joined by fours in
 // a wave and then in the waves' order.
@@ -423,42 +462,44 @@ __global__ __launch_bounds__(64 * kRowWaves) void vocab_rows_kernel(VocabParams 
   __shared__ float red[3][kRowWaves][kBlockRows];
   const int r = threadIdx.x % kBlockRows, tl = threadIdx.x / kBlockRows, wave = threadIdx.x >> 6;
   const int64_t row = (int64_t)blockIdx.x * kBlockRows + r;
-  float top = -INFINITY, sum = 0.0f, dot = 0.0f;
+  const float c = kLog2e / p.tau;
+  float top = -INFINITY, rest = 0.0f, dot = 0.0f;
   if (row < p.T) {
     for (int i = tl; i < p.tiles; i += 64 * kRowWaves / kBlockRows) {
       const float* at = p.stats + (int64_t)i * p.T + row;
-      join(&top, &sum, at[0], at[p.tiles * p.T]);
+      join(&top, &rest, at[0], at[p.tiles * p.T], c);
       dot += at[2 * p.tiles * p.T];
     }
   }
 #pragma unroll
   for (int m = kBlockRows; m < 64; m *= 2) {
-    const float other = __shfl_xor(top, m), s = __shfl_xor(sum, m);
-    join(&top, &sum, other, s);
+    const float other = __shfl_xor(top, m), s = __shfl_xor(rest, m);
+    join(&top, &rest, other, s, c);
     dot += __shfl_xor(dot, m);
   }
   if ((threadIdx.x & 63) < kBlockRows) {
     red[0][wave][r] = top;
-    red[1][wave][r] = sum;
+    red[1][wave][r] = rest;
     red[2][wave][r] = dot;
   }
   __syncthreads();
   if (threadIdx.x >= kBlockRows || row >= p.T) return;
 #pragma unroll
   for (int i = 1; i < kRowWaves; ++i) {
-    join(&top, &sum, red[0][i][r], red[1][i][r]);
+    join(&top, &rest, red[0][i][r], red[1][i][r], c);
     dot += red[2][i][r];
   }
-  finish_row(p, row, top, sum, dot, loss);
+  finish_row(p, row, top, rest, dot, loss);
 }
 
 // ---- few classes ----------------------------------------------------------------------
 // Up to kFewClasses columns: 16 rows and all columns a block, x and W straight from
 // memory into matrix instructions (few_rows), whose sums are a row's logits, its loss
 // and what is kept of it.  The logits are kept, being fewer than x's values.
-// 4096 rows of 256 -> 10 in fp32: 5.2 us and one launch; the product on a tile, the
-// span kernel and the rows' kernel took 32.
-constexpr int64_t kFewClasses = 64;
+// 4096 rows of 256 -> 10 in fp32: 4.6 us and one launch; the product on a tile, the
+// span kernel and the rows' kernel took 32.  65536 rows of 1024 -> 64 in bf16: 95 us
+// forward this way, 53 on tiles; forward and backward 249 and 252.
+constexpr int64_t kFewClasses = 32;
 template <typename T, int NC, bool WHOLE>
 __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __restrict__ loss) {
   typedef RowsMma<T> M;
@@ -484,7 +525,7 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __
   const int64_t row = m0 + r;
   if (row >= p.T) return;
   const float c2 = kLog2e / p.tau;
-  float z[NC], top = -INFINITY, sum = 0.0f, dot = 0.0f;
+  float z[NC], top = -INFINITY, rest = 0.0f, most = 0.0f, dot = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
     const int v = 16 * c + l;
@@ -497,10 +538,12 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __
   }
 #pragma unroll
   for (int m = 1; m < 16; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
-  top *= c2;
   const float from = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) sum += exp2f(__builtin_fmaf(z[c], c2, -from));
+  for (int c = 0; c < NC; ++c) {
+    rest += below(z[c], from, c2);
+    most += z[c] == from ? 1.0f : 0.0f;
+  }
   auto add = [&](int id, float prob) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -512,9 +555,11 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __
   } else {
     for (int e = 0; e < p.k; ++e) add(p.ids[row * p.k + e], p.prob[row * p.k + e]);
   }
-  sum = lane_sum<16>(sum);
+  rest = lane_sum<16>(rest);
+  most = lane_sum<16>(most);
+  if (top > -INFINITY) rest += most - 1.0f;
   dot = lane_sum<16>(dot);
-  if (l == 0) finish_row(p, row, top, sum, dot, loss);
+  if (l == 0) finish_row(p, row, top, rest, dot, loss);
 }
 // ---- sums of the rows -------------------------------------------------------------------
 constexpr int kOneBlock = 1024;
@@ -588,7 +633,7 @@ __global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
 
 // The rows' weights and, for the weight's gradient, x's rows, those that do not count
 // as zeros: what they hold may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld],
-// zeros behind D; ld 0: none.  FEW: also dz of few classes from their kept logits, in 16
+// zeros behind D; ld 0: none; a second time behind them with a second part of dz.  FEW: also dz of few classes from their kept logits, in 16
 // bits with zeros as far as 16 bytes go.
 template <typename T, bool FEW>
 __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstream u,
@@ -608,17 +653,21 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstr
       const float weight = weight_of(p, u, row, common);
       float d = 0.0f;
       if (v < p.V && weight != 0.0f) {
-        d = exp2f(__builtin_fmaf(p.logits[row * p.V + v], c, -p.top[row])) / p.total[row];
+        const float rest = p.rest[row];
+        auto take = [&](float prob) { d = __builtin_fmaf(-prob, rest, d - prob); };
+        d = exp2f((p.logits[row * p.V + v] - p.top[row]) * c);
         if (p.target != nullptr) {
           float flag;
-          d -= target_of(p, row, &flag) == v ? 1.0f : 0.0f;
+          if (target_of(p, row, &flag) == v) take(1.0f);
         } else {
           for (int e = 0; e < p.k; ++e)
-            d -= p.ids[row * p.k + e] == v ? p.prob[row * p.k + e] : 0.0f;
+            if (p.ids[row * p.k + e] == v) take(p.prob[row * p.k + e]);
         }
-        d *= weight;
+        d *= weight / (1.0f + rest);
       }
-      static_cast<T*>(p.G)[row * p.ldg + v] = (T)d;
+      const T whole = (T)d;
+      static_cast<T*>(p.G)[row * p.ldg + v] = whole;
+      if (p.G2 != nullptr) static_cast<T*>(p.G2)[row * p.ldg + v] = (T)(d - (float)whole);
     }
   }
   const int64_t per = ceil_div(ld, V), total = p.T * per;
@@ -633,12 +682,14 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstr
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = on && c + j < p.D ? src[j] : (T)0.0f;
     }
-    if (whole) {
-      *reinterpret_cast<vec*>(out + row * ld + c) = v;
-    } else {
+    for (int64_t to = row; to < p.T * (p.G2 != nullptr ? 2 : 1); to += p.T) {
+      if (whole) {
+        *reinterpret_cast<vec*>(out + to * ld + c) = v;
+      } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (c + j < ld) out[row * ld + c + j] = v[j];
+        for (int j = 0; j < V; ++j)
+          if (c + j < ld) out[to * ld + c + j] = v[j];
+      }
     }
   }
 }
@@ -692,8 +743,8 @@ size_t kept_floats(int64_t T, int64_t V, int64_t k) {
 }
 void set_kept(VocabParams* p, void* kept) {
   p->top = static_cast<float*>(kept);
-  p->total = p->top + p->T;
-  p->flag = p->total + p->T;
+  p->rest = p->top + p->T;
+  p->flag = p->rest + p->T;
   p->count = p->flag + p->T;
   p->prob = p->count + 4;
   p->ids = reinterpret_cast<int*>(p->prob + p->T * p->k);
@@ -714,31 +765,43 @@ HalfCfg tile_of(int64_t T, int64_t cols, int64_t D) {
 }
 int64_t tile_columns(HalfCfg cfg) { return cfg == kSmall ? 128 : 256; }
 
+// Whether dz is taken in two parts of 16 bits, one behind the other as 2 T rows of the
+// second products.  The error of a single rounding is spread over all values that a sum
+// takes in, and vanishes in the gradient's own; with few rows or columns there is little to
+// spread it over, and it made the gradients' error 1.5 to 3 times that of their own
+// rounding.  The second part costs little there (bf16, forward and backward; one row more
+// is one part): 64 rows of 4096 -> 131072 1.21 ms, 65 1.13; 512 of 512 -> 8192 150 us, 513
+// 145; 2000 of 1024 -> 1024 153 us.  131072 rows of 1024 -> 16 took 0.95 ms so and take 0.36.
+bool in_parts(int64_t T, int64_t V, int64_t D) {
+  return T <= 64 || (T <= 4096 && T * V <= ((int64_t)1 << 31) / D);
+}
 HalfPlan plan_product(int dtype, int op, int64_t T, int64_t cols, int64_t D) {
   if (dtype != KAN_DTYPE_F32 && op == KAN_GROUPED_INPUT) return long_plan(T, cols, D);
   return product_plan(dtype, op, T, 1, cols, D);
 }
 
-template <typename T, class G, bool GRAD>
+template <typename T, class G, int PARTS>
 int launch_vocab_tile(const VocabParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(p.cols, G::BN), blocks = dense_grid(p.T, G::BM, tiles_n);
   if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "vocab_loss: too many tiles");
   if (whole_rows(p.x, p.ldx) && whole_rows(p.w, p.ldw))
-    vocab_tile_kernel<T, G, kDirect, GRAD><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
+    vocab_tile_kernel<T, G, kDirect, PARTS><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
   else
-    vocab_tile_kernel<T, G, kGuarded, GRAD><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
+    vocab_tile_kernel<T, G, kGuarded, PARTS><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
   return check_launch("vocab_loss");
 }
-template <typename T, bool GRAD>
+template <typename T, int PARTS>
 int launch_vocab_half(const VocabParams& p, HalfCfg cfg, hipStream_t st) {
-  return cfg == kBig   ? launch_vocab_tile<T, TileBig, GRAD>(p, st)
-         : cfg == kMid ? launch_vocab_tile<T, TileMid, GRAD>(p, st)
-                       : launch_vocab_tile<T, TileSmall, GRAD>(p, st);
+  if constexpr (PARTS == 2) return launch_vocab_tile<T, TileSmall, 2>(p, st);
+  else
+    return cfg == kBig   ? launch_vocab_tile<T, TileBig, PARTS>(p, st)
+           : cfg == kMid ? launch_vocab_tile<T, TileMid, PARTS>(p, st)
+                         : launch_vocab_tile<T, TileSmall, PARTS>(p, st);
 }
-template <bool GRAD>
+template <int PARTS>
 int launch_vocab_tiles(int dtype, const VocabParams& p, HalfCfg cfg, hipStream_t st) {
-  return dtype == KAN_DTYPE_BF16 ? launch_vocab_half<bf16, GRAD>(p, cfg, st)
-                                 : launch_vocab_half<f16, GRAD>(p, cfg, st);
+  return dtype == KAN_DTYPE_BF16 ? launch_vocab_half<bf16, PARTS>(p, cfg, st)
+                                 : launch_vocab_half<f16, PARTS>(p, cfg, st);
 }
 template <bool GRAD>
 int launch_vocab_span(const VocabParams& p, hipStream_t st) {
@@ -811,6 +874,8 @@ struct BackwardPlan {
   HalfCfg cfg;
   AlignPlan align;
   int64_t piece, ldg, ldx;
+  int parts;        // of dz
+  bool sliced;      // dx is added from slices
   char *rows, *aligned, *G;  // rows: x's for the weight's gradient
   float *weight, *scale, *most, *part, *slices, *acc;
   size_t bytes;
@@ -821,6 +886,8 @@ BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, i
   Places at{ws, 0};
   const bool half = dtype != KAN_DTYPE_F32;
   b.piece = piece_columns(dtype, T, V);
+  b.parts = half && in_parts(T, V, D) ? 2 : 1;
+  b.sliced = b.piece < V || b.parts == 2;
   b.ldg = half ? padded(b.piece) : b.piece;
   if (half) {
     b.cfg = tile_of(T, b.piece, D);
@@ -832,27 +899,28 @@ BackwardPlan plan_backward(int dtype, const void* x, const void* w, int64_t T, i
     b.aligned = at.take(b.align.a_bytes + b.align.b_bytes);
   }
   b.ldx = half ? round_up(D, 8) : D;
-  if (dw) b.rows = at.take((size_t)(T * b.ldx) * dtype_bytes(dtype));
+  if (dw) b.rows = at.take((size_t)(b.parts * T * b.ldx) * dtype_bytes(dtype));
   b.weight = at.take<float>((size_t)T);
   b.scale = at.take<float>(1);
   b.most = at.take<float>(1);
-  b.G = at.take((size_t)(T * b.ldg) * dtype_bytes(dtype));
+  b.G = at.take((size_t)(b.parts * T * b.ldg) * dtype_bytes(dtype));
   size_t part = 0, slices = 0;
   const int64_t rest = V % b.piece;
   for (const int64_t cols : {b.piece, rest}) {
     if (cols == 0) continue;
     auto need = [&](int op) {
-      return product_part_bytes(op, plan_product(dtype, op, T, cols, D), T, 1, cols, D);
+      const int64_t rows = op == KAN_GROUPED_FORWARD ? T : b.parts * T;
+      return product_part_bytes(op, plan_product(dtype, op, rows, cols, D), rows, 1, cols, D);
     };
     if (!half && V > kFewClasses) part = std::max(part, need(KAN_GROUPED_FORWARD));
     if (dw) part = std::max(part, need(KAN_GROUPED_WEIGHT));
-    if (dx && (!half || b.piece == V)) part = std::max(part, need(KAN_GROUPED_INPUT));
+    if (dx && (!half || !b.sliced)) part = std::max(part, need(KAN_GROUPED_INPUT));
     else if (dx) slices = std::max(slices, need(KAN_GROUPED_INPUT));
   }
-  if (dx && b.piece < V) {
-    slices = std::max(slices, 4 * (size_t)(T * D));
+  if (dx && b.sliced) {
+    slices = std::max(slices, 4 * (size_t)(b.parts * T * D));
     b.slices = at.take<float>(slices / 4);
-    b.acc = at.take<float>((size_t)(T * D));
+    if (b.piece < V) b.acc = at.take<float>((size_t)(T * D));
   }
   b.part = part == 0 ? nullptr : at.take<float>(part / 4);
   b.bytes = at.bytes;
@@ -874,8 +942,7 @@ template <typename T, bool WHOLE>
 int launch_few_classes(const VocabParams& p, float* loss, hipStream_t st) {
   const dim3 blocks((unsigned)ceil_div(p.T, kFewRows));
   if (p.V <= 16) vocab_few_kernel<T, 1, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
-  else if (p.V <= 32) vocab_few_kernel<T, 2, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
-  else vocab_few_kernel<T, 4, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
+  else vocab_few_kernel<T, 2, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
   return check_launch("vocab_loss");
 }
 template <typename T>
@@ -975,7 +1042,7 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
     p.w = g.B;
     p.ldx = g.lda;
     p.ldw = g.ldb;
-    e = launch_vocab_tiles<false>(dtype, p, f.cfg, st);
+    e = launch_vocab_tiles<0>(dtype, p, f.cfg, st);
     if (e != KAN_OK) return e;
   }
   for (p.v0 = 0; !few && dtype == KAN_DTYPE_F32 && p.v0 < V; p.v0 += f.piece) {
@@ -1047,6 +1114,7 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
   p.weight = b.weight;
   p.x = x;
   p.G = b.G;
+  if (b.parts == 2) p.G2 = b.G + T * b.ldg * value;
   p.z = reinterpret_cast<float*>(b.G);
   p.ldg = b.ldg;
   GroupedParams in = product_of(T, V, D);
@@ -1077,22 +1145,25 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
     const char* wp = static_cast<const char*>(p.w) + p.v0 * p.ldw * value;
     auto product = [&](int op, const void* A, int64_t lda, const void* B, int64_t ldb, void* C,
                        float* part) {
-      GroupedParams g = product_of(T, p.cols, D);
+      const int64_t rows = op == KAN_GROUPED_FORWARD ? T : b.parts * T;
+      GroupedParams g = product_of(rows, p.cols, D);
       g.A = A;
       g.B = B;
       g.lda = lda;
       g.ldb = ldb;
       g.C = C;
       g.scale = half ? b.scale : nullptr;
-      const HalfPlan pl = plan_product(dtype, op, T, p.cols, D);
-      g.part = C == nullptr || product_part_bytes(op, pl, T, 1, p.cols, D) > 0 ? part : nullptr;
+      const HalfPlan pl = plan_product(dtype, op, rows, p.cols, D);
+      g.part = C == nullptr || product_part_bytes(op, pl, rows, 1, p.cols, D) > 0 ? part : nullptr;
       return launch_product(dtype, op, g, pl, st);
     };
     // dz of the piece
     p.ldg = half ? padded(p.cols) : p.cols;
+    if (b.parts == 2) p.G2 = b.G + T * p.ldg * value;
     if (few) {  // (the first kernel's)
     } else if (half) {
-      e = launch_vocab_tiles<true>(dtype, p, b.cfg, st);
+      e = b.parts == 2 ? launch_vocab_tiles<2>(dtype, p, b.cfg, st)
+                       : launch_vocab_tiles<1>(dtype, p, b.cfg, st);
     } else {
       e = product(KAN_GROUPED_FORWARD, p.x, D, wp, D, p.z, b.part);
       if (e == KAN_OK) e = launch_vocab_span<true>(p, st);
@@ -1101,14 +1172,15 @@ int kan_hip_vocab_loss_backward(int dtype, const float* grad_loss, const void* x
       e = product(KAN_GROUPED_WEIGHT, p.G, p.ldg, p.x, p.ldx,
                   static_cast<char*>(grad_w) + p.v0 * D * value, b.part);
     if (e != KAN_OK || grad_x == nullptr) continue;
-    if (b.piece == V) {
+    if (!b.sliced) {
       e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, grad_x, b.part);
       continue;
     }
     int cuts = 1;
     if (half) {
       e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, nullptr, b.slices);
-      cuts = plan_product(dtype, KAN_GROUPED_INPUT, T, p.cols, D).cuts;
+      // (a cut's slice has the parts' rows one behind the other)
+      cuts = b.parts * plan_product(dtype, KAN_GROUPED_INPUT, b.parts * T, p.cols, D).cuts;
     } else {
       e = product(KAN_GROUPED_INPUT, p.G, p.ldg, wp, p.ldw, b.slices, b.part);
     }

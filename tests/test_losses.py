@@ -485,6 +485,32 @@ def test_ids_that_are_no_columns_and_values_that_are_not_finite(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [20, 700])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(V, dtype):
+    x, w, target = (t.cuda() for t in _inputs(100, V, 40, dtype))
+    x.requires_grad_()
+    g = torch.rand(100, device="cuda") + 0.5
+    g[50] = 2.0
+    loss = linear_cross_entropy(x, w, target, reduction="none")
+    want, = torch.autograd.grad(loss, x, g, retain_graph=True)
+    others = torch.ones(100, dtype=torch.bool, device="cuda")
+    others[[3, 77]] = False
+    g[3], g[77] = torch.inf, torch.nan
+    got, = torch.autograd.grad(loss, x, g)
+    if dtype == F32:
+        # (a tile of the product that holds such values is evaluated a second time, without
+        # the split of its operands: each result lies within a sum's bound)
+        d = (x.double() @ w.double().t()).softmax(1).scatter_add_(
+            1, target[:, None], torch.ones(100, 1, dtype=torch.float64, device="cuda"))
+        tol = 2 * (V + 16) * U * ((2 * d) @ w.double().abs())
+        assert bool(((got.double() - want.double()).abs() <= tol)[others].all())
+    else:
+        assert torch.equal(got[others], want[others])
+    assert not bool(got[~others].isfinite().any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_no_row_counts(dtype):
     x, w, _ = (t.cuda() for t in _inputs(140, 300, 64, dtype))
     x.requires_grad_(), w.requires_grad_()

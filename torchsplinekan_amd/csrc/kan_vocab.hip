@@ -599,7 +599,7 @@ struct Upstream {
   const float* g;
   int reduction, fp32;
   float unit;
-  const float* most;  // max|g| of the rows' losses in 16 bits
+  const float* most;  // the largest finite |g| of the rows' losses in 16 bits
   float* scale;
 };
 __device__ __forceinline__ float common_of(const VocabParams& p, const Upstream& u) {
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
   float most = 0.0f;
 #pragma unroll 8
   for (int64_t t = threadIdx.x; t < p.T; t += kOneBlock)
-    most = fmaxf(most, p.flag[t] != 0.0f ? fabsf(g[t]) : 0.0f);
+    most = fmaxf(most, p.flag[t] != 0.0f && fabsf(g[t]) < INFINITY ? fabsf(g[t]) : 0.0f);
   red[threadIdx.x] = most;
   __syncthreads();
   for (int m = kOneBlock / 2; m > 0; m /= 2) {

@@ -1059,7 +1059,7 @@ __device__ __forceinline__ TileCoords grouped_coords(GroupedGemm<OP>& p) {
     tc.m0 = t.m0;
     tc.n0 = (int64_t)tn * C::BN;
     tc.kend = t.e == g.E ? 0 : OP == 0 ? g.K : g.N;
-    cut_range(g, &tc.kbeg, &tc.kend);
+    cut_range(g, blockIdx.y, &tc.kbeg, &tc.kend);
     p.M = t.m1;
     p.B += t.e * weights;
     if (g.cuts > 1) p.C = g.part + blockIdx.y * (g.T * p.N);

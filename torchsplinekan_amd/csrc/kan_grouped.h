@@ -254,15 +254,24 @@ int launch_grouped_sum(const GroupedParams& p, hipStream_t st) {
 
 // ---- tiles of the other two products ------------------------------------------
 // The row tiles of all groups in a row, kGroupedM of them at a time over all
-// columns; false past the last.
+// columns; false past the last.  cut (of a grid of p.cuts in y): a cut's tiles before
+// the next cut's, so that an XCD has a stretch of few cuts, whose operands its L2
+// serves to several tiles.
 constexpr int kGroupedM = 8;
 __device__ __forceinline__ bool row_tile(const GroupedParams& p, int bm, int tiles_n, RowTile* t,
-                                         int* tn) {
+                                         int* tn, int* cut = nullptr) {
   GroupScan s;  // the number of row tiles first
   for (int base = 0; base <= p.E; base += 64) s.step(p, base, bm);
   const int tiles_m = s.carry_tiles, total = tiles_m * tiles_n;
-  if ((int)blockIdx.x >= total) return false;
-  const int id = xcd_remap(blockIdx.x, total), group = kGroupedM * tiles_n;
+  const int block = cut == nullptr ? blockIdx.x : blockIdx.y * gridDim.x + blockIdx.x;
+  const int all = cut == nullptr ? total : total * p.cuts;
+  if (block >= all) return false;
+  int id = xcd_remap(block, all);
+  const int group = kGroupedM * tiles_n;
+  if (cut != nullptr) {
+    *cut = __builtin_amdgcn_readfirstlane(id / total);
+    id -= *cut * total;
+  }
   const int first = id / group * kGroupedM, in = id % group;
   const int gm = min(tiles_m - first, kGroupedM);
   *tn = __builtin_amdgcn_readfirstlane(in / gm);
@@ -317,12 +326,13 @@ inline int sum_cuts(double tiles, int places, int64_t slabs, double slab_us) {
   if (cuts < 2 || (double)(slabs - slabs / cuts) * slab_us < 10.0) return 1;
   return (int)std::min<int64_t>(cuts, 32);
 }
-// The k range of this block's cut, whole slabs of 64.
-__device__ __forceinline__ void cut_range(const GroupedParams& p, int64_t* kbeg, int64_t* kend) {
+// The k range of a cut, whole slabs of 64.
+__device__ __forceinline__ void cut_range(const GroupedParams& p, int cut, int64_t* kbeg,
+                                          int64_t* kend) {
   if (p.cuts <= 1) return;
   const int k = (int)*kend, each = ((k + p.cuts - 1) / p.cuts + 63) / 64 * 64;
   // (uniform values: the division runs in vector registers)
-  *kbeg = __builtin_amdgcn_readfirstlane(min(k, (int)blockIdx.y * each));
+  *kbeg = __builtin_amdgcn_readfirstlane(min(k, cut * each));
   *kend = __builtin_amdgcn_readfirstlane(min(k, (int)*kbeg + each));
 }
 

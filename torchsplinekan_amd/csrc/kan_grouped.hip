@@ -34,7 +34,7 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
   __shared__ __align__(16) char lds[2 * G::kBuf];
 
   // the tile: rows [m0, m_end) and columns [n0, n_end) of the output, k range
-  int e, tn, slot = -1;
+  int e, tn, slot = -1, cut = 0;
   int64_t m0, m_end, kbeg = 0, kend;
   if constexpr (OP == 2) {
     WeightTile t;
@@ -48,12 +48,12 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
     m_end = p.N;
   } else {
     RowTile t;
-    if (!row_tile(p, BM, tiles_n, &t, &tn)) return;
+    if (!row_tile(p, BM, tiles_n, &t, &tn, &cut)) return;
     e = t.e;
     m0 = t.m0;
     m_end = t.m1;
     kend = e == p.E ? 0 : OP == 0 ? p.K : p.N;
-    cut_range(p, &kbeg, &kend);
+    cut_range(p, cut, &kbeg, &kend);
   }
   const int64_t n_end = OP == 0 ? p.N : p.K, n0 = (int64_t)tn * BN;
   const int64_t weight = (int64_t)e * p.N * (OP == 2 ? p.K : p.ldb);
@@ -71,11 +71,9 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
 
   if (OP == 2 ? slot >= 0 : p.part != nullptr) {  // an item of several, a cut's part
     float* part =
-        p.part + (OP == 2 ? (int64_t)slot * p.N * p.K : (int64_t)blockIdx.y * p.T * n_end);
+        p.part + (OP == 2 ? (int64_t)slot * p.N * p.K : (int64_t)cut * p.T * n_end);
     // (4 columns of a row lie side by side in a lane; value by value the stores of a
     // whole tile took 100 us and more)
-    typedef float f4 __attribute__((ext_vector_type(4)));
-    const bool four = n_end % 4 == 0;
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -86,9 +84,9 @@ __global__ __launch_bounds__(G::NT) void grouped_tile_kernel(GroupedParams p, in
           const int64_t col = n0 + (wn * FN + j) * 32 + 8 * q + 4 * (lane >> 5);
           if (row >= m_end || col >= n_end) continue;
           float* at = part + row * n_end + col;
-          if (four) {
-            *reinterpret_cast<f4*>(at) = {acc[i][j][4 * q], acc[i][j][4 * q + 1],
-                                          acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          if (col + 4 <= n_end) {
+            reinterpret_cast<LooseVec<float, 4>*>(at)->v = {
+                acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
           } else {
 #pragma unroll
             for (int s = 0; s < 4; ++s)

@@ -265,8 +265,12 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (col_of(j, v) == at) z = acc[i][j][v];
+          for (int q = 0; q < 4; ++q)
+            if (__any(at >> 3 == 4 * j + q)) {
+#pragma unroll
+              for (int s = 0; s < 4; ++s)
+                if (col_of(j, 4 * q + s) == at) z = acc[i][j][4 * q + s];
+            }
         dot += prob * z;
       });
       dot += __shfl_xor(dot, 32);
@@ -304,10 +308,14 @@ __global__ __launch_bounds__(G::NT) void vocab_tile_kernel(VocabParams p, int ti
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const float here = col_of(j, v) == at ? prob : 0.0f;
-            acc[i][j][v] = __builtin_fmaf(-here, rest, acc[i][j][v] - here);
-          }
+          for (int q = 0; q < 4; ++q)
+            if (__any(at >> 3 == 4 * j + q)) {  // (of 8 such columns few waves need a second)
+#pragma unroll
+              for (int s = 0; s < 4; ++s) {
+                const float here = col_of(j, 4 * q + s) == at ? prob : 0.0f;
+                acc[i][j][4 * q + s] = __builtin_fmaf(-here, rest, acc[i][j][4 * q + s] - here);
+              }
+            }
       });
       const float part = weight / (1.0f + rest);
 #pragma unroll

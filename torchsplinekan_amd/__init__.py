@@ -20,6 +20,5 @@ __version__ = "0.1.0"
 
 __all__ = ["KANLinear", "KAN", "PruneResult", "prune_nodes", "Activation8", "checkpoint_8bit",
            "quantize_activation", "grouped_linear", "gated_linear", "residual_norm", "layer_norm",
-           "linear_cross_entropy",
-           "linear_distillation", "KANExperts",
-           "KANExpertStack", "__version__"]
+           "linear_cross_entropy", "linear_distillation", "KANExperts", "KANExpertStack",
+           "__version__"]

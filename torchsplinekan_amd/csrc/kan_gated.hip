@@ -157,6 +157,9 @@ __device__ __forceinline__ void finish_8(const GatedParams& p, int64_t row, int6
 }
 
 // ---- tiles in 16 bits -------------------------------------------------------------
+// Bound by MFMA at the power cap, and where K is short by the stores: 16384 rows of
+// 4096 -> 4096 in bf16 844 us (1.30 PFLOP/s); of 1024 -> 4096 275 us (1.0), and 358 with
+// the kept values, 3.5 times h's bytes behind 16 slabs of product.
 template <typename T, class G, int MODE>
 __global__ __launch_bounds__(G::NT) void gated_tile_kernel(GatedParams p, int tiles_n, int whole) {
   constexpr int BM = G::BM, BN = G::BN, FM = G::FM;
@@ -217,7 +220,8 @@ __global__ __launch_bounds__(G::NT) void gated_tile_kernel(GatedParams p, int ti
 
 // ---- few rows ---------------------------------------------------------------------
 // As the grouped products' kernel for groups of a few rows: 16 rows and 16 NP
-// outputs a block, bound by the weights' bytes.
+// outputs a block, bound by the weights' bytes: 8 rows of 1024 -> 4096 in bf16, 16.8 MB,
+// in 6 us (from the last-level cache); one row of 4096 -> 4096, 67 MB, in 13.
 template <typename T, int NP, bool WHOLE>
 __global__ __launch_bounds__(256) void gated_few_kernel(GatedParams p, int tiles_n) {
   typedef RowsMma<T> M;
@@ -303,7 +307,8 @@ __global__ __launch_bounds__(256) void gated_value_kernel(GatedParams p) {
   });
 }
 
-// [dg du] from dh (A) and what was kept; C: [T, 2 N].  Bound by HBM.
+// [dg du] from dh (A) and what was kept; C: [T, 2 N].  Bound by HBM: 16384 x 4096 in
+// bf16, 738 MB, 148 us (5.0 TB/s).
 template <typename T, int V>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedParams p) {
   each_output<V>(p.T, p.N, [&](int64_t row, int64_t n) {

@@ -155,6 +155,10 @@ __device__ __forceinline__ void join(float* top, float* rest, float m, float s, 
 }
 
 // ---- tiles in 16 bits -------------------------------------------------------------
+// Bound by MFMA at the power cap, and with few inputs by what follows the product (an
+// exponential of every logit): 8192 rows of 2048 -> 65536 in bf16 1.80 ms forward (1.22
+// PFLOP/s) and 2.0 for dz; 4096 of 1024 -> 65536 with 64 ids a row 0.59 and
+// 0.66 (without a teacher 0.50 forward); 33 of 1024 -> 32768 by W's bytes, 16 us.
 // A lane holds rows 32 i + (lane & 31) of its wave's and 32 columns: 32 j + 8 q +
 // 4 (lane >> 5) + s at acc[i][j][4 q + s].
 // PARTS (0: the forward pass): of dz.  Only the smallest tile takes two: on the
@@ -463,7 +467,7 @@ __device__ __forceinline__ void finish_row(const VocabParams& p, int64_t row, fl
                              : p.tau * p.tau * (entropy + (top - dot) / p.tau + log1pf(rest));
 }
 // A row's tiles joined: 16 rows a block, 64 lanes of tiles a row, joined by fours in
-// a wave and then in the waves' order.
+// a wave and then in the waves' order.  8192 rows of 256 tiles: 12 us; 33 rows 4.4, latency.
 constexpr int kBlockRows = 16, kRowWaves = 16;
 __global__ __launch_bounds__(64 * kRowWaves) void vocab_rows_kernel(VocabParams p,
                                                                     float* __restrict__ loss) {
@@ -641,8 +645,9 @@ __global__ __launch_bounds__(kOneBlock) void vocab_most_kernel(VocabParams p,
 
 // The rows' weights and, for the weight's gradient, x's rows, those that do not count
 // as zeros: what they hold may be anything, and 0 times NaN is NaN.  [T, D] -> [T, ld],
-// zeros behind D; ld 0: none; a second time behind them with a second part of dz.  FEW: also dz of few classes from their kept logits, in 16
-// bits with zeros as far as 16 bytes go.
+// zeros behind D (8192 x 2048 in bf16: 13 us); ld 0: none; a second time behind them with
+// a second part of dz.  FEW: also dz of few classes from their kept logits, in 16 bits with
+// zeros as far as 16 bytes go.
 template <typename T, bool FEW>
 __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabParams p, Upstream u,
                                                             T* __restrict__ out, int64_t ld,

@@ -367,6 +367,7 @@ struct HalfPlan {
 };
 HalfPlan half_plan(int op, int64_t T, int64_t E, int64_t N, int64_t K);
 HalfPlan long_plan(int64_t T, int64_t N, int64_t K);
+HalfPlan long_weight_plan(int64_t T, int64_t N, int64_t K);
 constexpr int kFewRows = 16;
 bool takes_few(int dtype, int op, int64_t T, int64_t E);
 
@@ -388,7 +389,9 @@ int launch_aligned(const AlignPlan& al, GroupedParams* p, char* ws, hipStream_t 
 
 // A product as planned: p's operands, sizes, part (of product_part_bytes) and scale
 // are set.  fp32 operands are contiguous.
-HalfPlan product_plan(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K);
+// dense: of one group without offsets, which has all rows.
+HalfPlan product_plan(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K,
+                      bool dense = false);
 size_t product_part_bytes(int op, const HalfPlan& pl, int64_t T, int64_t E, int64_t N, int64_t K);
 int launch_product(int dtype, int op, GroupedParams p, const HalfPlan& pl, hipStream_t st);
 

@@ -398,6 +398,32 @@ int launch_aligned(const AlignPlan& al, GroupedParams* p, char* ws, hipStream_t 
   return KAN_OK;
 }
 
+// The weight gradient of one group that has all rows, of fewer large tiles than CUs: runs
+// of rows on either tile.  16384 rows, 8192 x 1024 in bf16: 272 us on 128 x 128, 237 on
+// 256 x 256 in two runs; 65536 rows, 512 x 256: 55 us in the runs of groups, 48 in these.
+// (64 rows of two small tiles a CU take 1.14 us.)
+HalfPlan long_weight_plan(int64_t T, int64_t N, int64_t K) {
+  const int cus = device_cu_count();
+  const double slab_us[2] = {1.73, 1.14};
+  const int64_t side[2] = {256, 128};
+  HalfPlan best{kSmall, 1, kNoRuns};
+  double least = 1e30;
+  for (int c = 0; c < 2; ++c) {
+    const double tiles = (double)ceil_div(N, side[c]) * (double)ceil_div(K, side[c]);
+    for (int64_t runs = 1; runs <= 32 && (runs == 1 || T / runs >= 512); ++runs) {
+      const int64_t run = round_up(ceil_div(T, runs), kDepth);
+      double t = slab_us[c] * rounds(tiles * (double)ceil_div(T, run), (c + 1.0) * cus) *
+                 (double)(run / kDepth);
+      if (runs > 1) t += 5.0 + (double)runs * (double)(N * K) * 8.0 / 4.0e6;
+      if (t < least) {
+        least = t;
+        best = {c == 0 ? kBig : kSmall, 1, runs == 1 ? kNoRuns : (int)run};
+      }
+    }
+  }
+  return best;
+}
+
 namespace {
 
 template <typename T>
@@ -416,13 +442,14 @@ int launch_half(int op, const GroupedParams& p, const HalfPlan& plan, hipStream_
 
 }  // namespace
 
-HalfPlan product_plan(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K) {
+HalfPlan product_plan(int dtype, int op, int64_t T, int64_t E, int64_t N, int64_t K, bool dense) {
   HalfPlan pl{kSmall, 1, kNoRuns};
   if (T == 0 || E == 0 || N == 0 || K == 0) return pl;  // (their product can pass 64 bits)
   if (takes_few(dtype, op, T, E)) {
     pl.cfg = kFew;
   } else if (dtype != KAN_DTYPE_F32) {
     pl = half_plan(op, T, E, N, K);
+    if (dense && op == KAN_GROUPED_WEIGHT && pl.cfg == kSmall) pl = long_weight_plan(T, N, K);
   } else if (op == KAN_GROUPED_WEIGHT) {
     pl.run = grouped_f32_run(T, E, N, K);
   } else {
@@ -482,9 +509,9 @@ struct Workspace {
   size_t rows_bytes, part_bytes;  // (part from a multiple of 16 bytes on)
 };
 Workspace plan_call(int dtype, int op, int format, const void* A, const void* B, int64_t T,
-                    int64_t E, int64_t N, int64_t K) {
+                    int64_t E, int64_t N, int64_t K, bool dense = false) {
   Workspace w{};
-  w.plan = product_plan(dtype, op, T, E, N, K);
+  w.plan = product_plan(dtype, op, T, E, N, K, dense && E == 1 && format == KAN_ACT8_NONE);
   if (T == 0 || E == 0 || N == 0 || K == 0 || w.plan.cfg == kFew) return w;
   if (dtype == KAN_DTYPE_F32) {
     w.restore = format != KAN_ACT8_NONE;
@@ -517,6 +544,9 @@ int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const voi
   if (rc != KAN_OK) return rc;
   const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
   *bytes = w.rows_bytes + w.part_bytes;
+  // (a call without offsets may be planned otherwise)
+  const Workspace d = plan_call(dtype, op, b_format, a, b, T, E, N, K, true);
+  *bytes = std::max(*bytes, d.rows_bytes + d.part_bytes);
   return KAN_OK;
 }
 
@@ -567,7 +597,7 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   const bool some = op == KAN_GROUPED_WEIGHT ? T > 0 : E * N * K > 0;  // any term to add up
   if (out == nullptr || (some && (a == nullptr || b == nullptr)) || (E > 1 && offsets == nullptr))
     return set_error(KAN_ERR_INVALID, "grouped_matmul: operands must not be NULL");
-  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
+  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K, offsets == nullptr);
   const size_t need = w.rows_bytes + w.part_bytes;
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return set_error(KAN_ERR_WORKSPACE, "grouped_matmul: needs %zu bytes of workspace, got %zu",

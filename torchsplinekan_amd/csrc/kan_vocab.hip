@@ -790,7 +790,7 @@ bool in_parts(int64_t T, int64_t V, int64_t D) {
 }
 HalfPlan plan_product(int dtype, int op, int64_t T, int64_t cols, int64_t D) {
   if (dtype != KAN_DTYPE_F32 && op == KAN_GROUPED_INPUT) return long_plan(T, cols, D);
-  return product_plan(dtype, op, T, 1, cols, D);
+  return product_plan(dtype, op, T, 1, cols, D, true);
 }
 
 template <typename T, class G, int PARTS>

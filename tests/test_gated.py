@@ -234,6 +234,36 @@ def test_kinds_of_tiles(T, E, N, K, rows, align, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("counts,N,K,dense", [
+    ([17], 256, 4096, True), ([64], 512, 2048, True), ([33], 203, 4100, True),
+    ([200], 72, 8192, True), ([40], 8, 2051, True), ([60, 0, 90], 64, 2048, False),
+    ([0, 129, 2], 77, 3000, False)])
+def test_sums_in_cuts(counts, N, K, dense, dtype):
+    """Few tiles and long sums: partial sums that another kernel joins."""
+    T, E = sum(counts), len(counts)
+    x, w, dh = _inputs(T, E, K, N, dtype)
+    from torchsplinekan_amd import _lib as lib
+    nbytes = ctypes.c_size_t()
+    for keep in (0, 1):
+        lib.check(lib.LIB.kan_hip_gated_workspace(
+            lib.OPERATOR_DTYPES[dtype], 4096, 4096, T, E, N, K, keep, ctypes.byref(nbytes)))
+        assert nbytes.value >= 2 * 4 * T * 2 * N
+    _check(x, w, dh, None if dense else _offsets(counts), where="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_sums_in_cuts_of_rows_behind_the_last_expert(dtype):
+    x, w, _ = _inputs(90, 2, 2048, 40, dtype)
+    h = gated_linear(x.cuda(), w.cuda(), torch.tensor([0, 30, 70], device="cuda"), act="sigmoid")
+    assert bool(h[:70].any(1).all()) and not bool(h[70:].any())
+    for r, e in ((slice(0, 30), 0), (slice(30, 70), 1)):
+        want = _expected(x[r].double(), w[e].double(), torch.zeros(1, 40).double(), "sigmoid", dtype)
+        _near(h[r], tuple(v.cuda() for v in want["h"]), "h")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
 def test_gradients_are_off_by_two_roundings(dtype):
     """(An operand's rounding and the result's, each a uniform error of at most H:
     H (2 / 3)^(1/2) normwise; the kept values' bits leave no trace.)"""

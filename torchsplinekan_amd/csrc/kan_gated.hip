@@ -307,6 +307,44 @@ __global__ __launch_bounds__(256) void gated_value_kernel(GatedParams p) {
   });
 }
 
+// 16 bits: h and what is kept from the partial sums [cuts, T, 2 N] of a product on few
+// tiles, 8 outputs a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void gated_join_kernel(GatedParams p, int whole) {
+  const int64_t per = (p.N + 7) / 8, total = p.T * per, slice = p.T * 2 * p.N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, n = (i - row * per) * 8;
+    const int count = (int)min(p.N - n, (int64_t)8);
+    const float* at = p.part + row * 2 * p.N + n;
+    float g[8] = {}, u[8] = {};
+    if (whole) {
+#pragma unroll 4
+      for (int q = 0; q < p.cuts; ++q) {
+        float a[8], b[8];
+        load_f32<float, 4>(at + q * slice, reinterpret_cast<float(&)[4]>(a[0]));
+        load_f32<float, 4>(at + q * slice + 4, reinterpret_cast<float(&)[4]>(a[4]));
+        load_f32<float, 4>(at + q * slice + p.N, reinterpret_cast<float(&)[4]>(b[0]));
+        load_f32<float, 4>(at + q * slice + p.N + 4, reinterpret_cast<float(&)[4]>(b[4]));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          g[j] += a[j];
+          u[j] += b[j];
+        }
+      }
+    } else {
+      for (int q = 0; q < p.cuts; ++q)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < count) {
+            g[j] += at[q * slice + j];
+            u[j] += at[q * slice + p.N + j];
+          }
+    }
+    finish_8<T>(p, row, n, count, whole != 0, g, u);
+  }
+}
+
 // [dg du] from dh (A) and what was kept; C: [T, 2 N].  Bound by HBM: 16384 x 4096 in
 // bf16, 738 MB, 148 us (5.0 TB/s).
 template <typename T, int V>
@@ -397,13 +435,36 @@ int check_gated(const char* who, int dtype, int act, int64_t T, int64_t E, int64
   return KAN_OK;
 }
 
-// A forward call's workspace: 16 bits: operands brought onto 16 bytes.  fp32: g
-// and u where they are not kept, then the product's partial sums.
+// A forward call's workspace: 16 bits: operands brought onto 16 bytes, then the partial
+// sums of a product whose tiles would leave places idle.  fp32: g and u where they are
+// not kept, then the product's partial sums.
 struct GatedPlan {
   HalfPlan plan;
   AlignPlan align;
-  size_t pre_bytes, bytes;
+  size_t pre_bytes, bytes;  // before the partial sums; all
 };
+// Cuts of long sums on tiles of 128 x 128 that leave places idle: a slab takes 0.63 us, the
+// weights are read at 4.7 TB/s, and the cuts' sums written, read and joined at 4 TB/s by
+// one more launch, 7 us in all.  4096 -> 4096 in bf16, without cuts and in them: 64 rows
+// 41.3 and 23.2 us, 256 rows 43.0 and 34.7; 300 rows of 2048 -> 1000 19.2 and 17.7 (23.5 in
+// 8 cuts, as the grouped products' rule has it).
+int gated_cuts(int64_t T, int64_t E, int64_t N, int64_t K) {
+  const double tiles = row_tiles(T, E, 128) * (double)ceil_div(N, 64);
+  const double read = 4.0 * (double)std::min(E, T) * (double)N * (double)K / 4.7e6;
+  const int64_t slabs = ceil_div(K, kDepth);
+  int best = 1;
+  double least = 0.0;
+  for (int cuts = 1; cuts <= 32 && (cuts == 1 || slabs / cuts >= 4); ++cuts) {
+    const double turns = std::max(1.0, rounds(tiles * cuts, 2.0 * device_cu_count()));
+    double t = std::max(0.63 * turns * (double)ceil_div(slabs, cuts), read);
+    if (cuts > 1) t += 7.0 + (double)cuts * (double)(2 * T * N) * 8.0 / 4.0e6;
+    if (cuts == 1 || t < least) {
+      least = t;
+      best = cuts;
+    }
+  }
+  return best;
+}
 GatedPlan plan_gated(int dtype, const void* x, const void* w, int64_t T, int64_t E, int64_t N,
                      int64_t K, bool keep) {
   GatedPlan g{};
@@ -415,7 +476,9 @@ GatedPlan plan_gated(int dtype, const void* x, const void* w, int64_t T, int64_t
     g.bytes = g.pre_bytes + product_part_bytes(KAN_GROUPED_FORWARD, g.plan, T, E, 2 * N, K);
   } else {
     g.align = align_plan(KAN_GROUPED_FORWARD, KAN_ACT8_NONE, x, w, T, E, 2 * N, K);
-    g.bytes = g.align.a_bytes + g.align.b_bytes;
+    g.plan.cuts = g.plan.cfg == kSmall && E > 0 && K > 0 ? gated_cuts(T, E, N, K) : 1;
+    g.pre_bytes = (size_t)round_up((int64_t)(g.align.a_bytes + g.align.b_bytes), 16);
+    g.bytes = g.pre_bytes + product_part_bytes(KAN_GROUPED_FORWARD, g.plan, T, E, 2 * N, K);
   }
   return g;
 }
@@ -482,8 +545,22 @@ int kan_hip_gated(int dtype, int act, const void* x, const void* w, const void* 
            : dtype == KAN_DTYPE_BF16 ? launch_gated_few<bf16>(p, st)
                                      : launch_gated_few<f16>(p, st);
   if (dtype != KAN_DTYPE_F32) {
-    const int e = launch_aligned(g.align, &p, ws, st);
+    int e = launch_aligned(g.align, &p, ws, st);
     if (e != KAN_OK) return e;
+    if (g.plan.cuts > 1) {
+      p.part = reinterpret_cast<float*>(ws + g.pre_bytes);
+      p.cuts = g.plan.cuts;
+      GroupedParams q = p;
+      q.C = nullptr;
+      q.N = 2 * N;
+      e = launch_product(dtype, KAN_GROUPED_FORWARD, q, g.plan, st);
+      if (e != KAN_OK) return e;
+      const int whole = N % 8 == 0 && aligned16(h);
+      const unsigned blocks = flat_blocks(T * ceil_div(N, 8));
+      if (dtype == KAN_DTYPE_BF16) gated_join_kernel<bf16><<<blocks, 256, 0, st>>>(p, whole);
+      else gated_join_kernel<f16><<<blocks, 256, 0, st>>>(p, whole);
+      return check_launch("gated");
+    }
     return dtype == KAN_DTYPE_BF16 ? launch_gated_half<bf16>(p, g.plan.cfg, st)
                                    : launch_gated_half<f16>(p, g.plan.cfg, st);
   }

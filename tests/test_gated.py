@@ -397,3 +397,26 @@ def test_other_stream_and_graph(T):
         torch.cuda.synchronize()
         for a, b in zip(out, step()):
             assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_sums_in_cuts_in_two_graphs():
+    """Two captured calls, replayed in turn with eager ones between them: each has
+    partial sums of its own."""
+    w = _inputs(1, 1, 4096, 192, BF16)[1][0].cuda()
+    xs = [_inputs(T, 1, 4096, 192, BF16, seed=T)[0].cuda() for T in (48, 70)]
+    with torch.no_grad():
+        want = [gated_linear(x, w) for x in xs]
+        torch.cuda.synchronize()
+        graphs = [torch.cuda.CUDAGraph() for _ in xs]
+        out = []
+        for x, graph in zip(xs, graphs):
+            with torch.cuda.graph(graph):
+                out.append(gated_linear(x, w))
+        for _ in range(3):
+            for k in (0, 1):
+                graphs[k].replay()
+                assert torch.equal(gated_linear(xs[1 - k], w), want[1 - k])
+                torch.cuda.synchronize()
+                assert torch.equal(out[k], want[k])
+                out[k].zero_()

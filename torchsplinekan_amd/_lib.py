@@ -12,6 +12,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (must precede the CDLL open, see module docstring)
+from torch.autograd import forward_ad as _forward_ad
 
 from . import build_lib as _build_lib
 
@@ -229,6 +230,29 @@ def launch(fn, device: torch.device, *args) -> None:
             status = fn(*args, stream_of(device))
     if status != KAN_OK:
         check(status)
+
+
+_is_tracing, _dispatch_mode = torch._C._is_tracing, torch._C._get_dispatch_mode
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def traced() -> bool:
+    """Whether torch.jit.trace records the calls: it sees an autograd function's apply
+    and torch's own operations, and of a bare launch nothing but the empty results.
+    make_fx with real tensors looks below apply too and would record those empty
+    results: refused.  (With fake tensors there is no memory to launch on.)"""
+    if _dispatch_mode(_PROXY) is not None:
+        raise RuntimeError("the device kernels cannot be recorded by make_fx")
+    return _is_tracing()
+
+
+def call(function, save: bool, *args):
+    """`function`, an autograd function, of args: through apply where its backward pass
+    is wanted (save), under forward mode (which apply refuses) and where the call is
+    traced; otherwise its forward alone, which is shorter on the host."""
+    if traced() or save or _forward_ad._current_level >= 0:
+        return function.apply(*args)
+    return function.forward(None, *args)
 
 
 # routing switches of kan_hip_set_route (KAN_ROUTE_* in include/kan_hip.h) and

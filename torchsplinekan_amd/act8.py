@@ -41,6 +41,40 @@ def _native(who: str):
     return _C._lib
 
 
+class _Quantize(torch.autograd.Function):
+    """(q, scale) of a device tensor x, without a gradient: a function for the sake of
+    traced calls, as the next."""
+
+    @staticmethod
+    def forward(ctx, x, group, format):
+        lib = _native("quantize_activation")
+        C = x.shape[-1]
+        rows, ldx = x.numel() // C, C
+        if not x.is_contiguous():
+            if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C:
+                ldx = x.stride(0)
+            else:
+                x = x.contiguous()
+        code, _, qdtype = FORMATS[format]
+        q = torch.empty(x.shape, dtype=qdtype, device=x.device)
+        scale = torch.empty(x.shape[:-1] + (-(-C // group),), dtype=torch.float32, device=x.device)
+        lib.launch(lib.LIB.kan_hip_act8_quantize, x.device, lib.OPERATOR_DTYPES[x.dtype], code,
+                   x.data_ptr(), ldx, rows, C, group, q.data_ptr(), scale.data_ptr())
+        return q, scale
+
+
+class _Dequantize(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, scale, group, format, dtype):
+        lib = _native("dequantize_activation")
+        out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        C = out.shape[-1]
+        lib.launch(lib.LIB.kan_hip_act8_dequantize, out.device,
+                   lib.operator_dtype_code(dtype, "dequantize_activation"), FORMATS[format][0],
+                   q.data_ptr(), scale.data_ptr(), out.numel() // C, C, group, out.data_ptr())
+        return out
+
+
 @dataclass(eq=False)
 class Activation8:
     """A tensor in 8 bits: q (int8 or float8_e4m3fn, the tensor's shape), scale
@@ -63,14 +97,10 @@ class Activation8:
         dtype = self.dtype if dtype is None else dtype
         if not self.q.is_cuda or self.q.numel() == 0:
             return _dequantize_cpu(self, dtype)
-        lib = _native("dequantize_activation")
-        out = torch.empty(self.q.shape, dtype=dtype, device=self.q.device)
-        C = out.shape[-1]
-        lib.launch(lib.LIB.kan_hip_act8_dequantize, out.device,
-                   lib.operator_dtype_code(dtype, "dequantize_activation"),
-                   FORMATS[self.format][0], self.q.data_ptr(), self.scale.data_ptr(),
-                   out.numel() // C, C, self.group, out.data_ptr())
-        return out
+        args = (self.q, self.scale, self.group, self.format, dtype)
+        if _native("dequantize_activation").traced():
+            return _Dequantize.apply(*args)
+        return _Dequantize.forward(None, *args)
 
 
 def _quantize_cpu(x, group, format):
@@ -106,19 +136,10 @@ def quantize_activation(x: torch.Tensor, group: int = 128, format: str = "int8")
     if not x.is_cuda or x.numel() == 0:
         q, scale = _quantize_cpu(x.detach(), group, format)
         return Activation8(q, scale, group, format, x.dtype)
-    lib = _native(who)
-    C = x.shape[-1]
-    rows, ldx = x.numel() // C, C
-    if not x.is_contiguous():
-        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= C:
-            ldx = x.stride(0)
-        else:
-            x = x.contiguous()
-    code, _, qdtype = FORMATS[format]
-    q = torch.empty(x.shape, dtype=qdtype, device=x.device)
-    scale = torch.empty(x.shape[:-1] + (-(-C // group),), dtype=torch.float32, device=x.device)
-    lib.launch(lib.LIB.kan_hip_act8_quantize, x.device, lib.OPERATOR_DTYPES[x.dtype], code,
-               x.data_ptr(), ldx, rows, C, group, q.data_ptr(), scale.data_ptr())
+    if _native(who).traced():
+        q, scale = _Quantize.apply(x.detach(), group, format)
+    else:
+        q, scale = _Quantize.forward(None, x, group, format)
     return Activation8(q, scale, group, format, x.dtype)
 
 

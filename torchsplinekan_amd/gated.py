@@ -8,7 +8,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -39,8 +38,9 @@ class _GatedLinear(torch.autograd.Function):
     """x [T, K], weight [E, 2, N, K], or [2, N, K] without offsets."""
 
     @staticmethod
-    def forward(ctx, x, weight, offsets, act, save):
+    def forward(ctx, x, weight, offsets, act):
         lib = _native()
+        save = ctx is not None and any(ctx.needs_input_grad)
         T, K = x.shape
         N, E = weight.shape[-2], 1 if offsets is None else weight.shape[0]
         code = lib.OPERATOR_DTYPES[x.dtype]
@@ -79,7 +79,7 @@ class _GatedLinear(torch.autograd.Function):
         if need_w:
             shape = (2, N, K) if offsets is None else (E, 2, N, K)
             dw = _matmul(WEIGHT, dpre, x, offsets, dh.new_empty(shape), T, E, 2 * N, K)
-        return dx, dw, None, None, None
+        return dx, dw, None, None
 
 
 def _act(g: torch.Tensor, act: Optional[str]) -> torch.Tensor:
@@ -151,12 +151,10 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, offsets: Optional[torch.
     if not x.is_cuda:
         h = _composite(x, weight if offsets is not None else weight.unsqueeze(0), offsets, act)
     else:
-        _native().operator_dtype_code(x.dtype, "gated_linear")
+        lib = _native()
+        lib.operator_dtype_code(x.dtype, "gated_linear")
         x, weight = x.contiguous(), weight.contiguous()
         offsets = None if offsets is None else offsets.contiguous()
         save = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
-        if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
-            h = _GatedLinear.apply(x, weight, offsets, ACTS[act], save)
-        else:
-            h = _GatedLinear.forward(None, x, weight, offsets, ACTS[act], False)
+        h = lib.call(_GatedLinear, save, x, weight, offsets, ACTS[act])
     return h if lead is None else h.reshape(lead + (shape[-2],))

@@ -8,7 +8,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -157,9 +156,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
         check_format("grouped_linear", group, checkpoint)
     if not x.is_cuda:
         return _composite(x, weight, offsets, checkpoint, group)
-    _native().operator_dtype_code(x.dtype, "grouped_linear")
+    lib = _native()
+    lib.operator_dtype_code(x.dtype, "grouped_linear")
     x, weight, offsets = x.contiguous(), weight.contiguous(), offsets.contiguous()
-    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
-            or _forward_ad._current_level >= 0):  # (apply refuses forward-mode derivatives)
-        return _GroupedLinear.apply(x, weight, offsets, checkpoint, group)
-    return _GroupedLinear.forward(None, x, weight, offsets, None, group)
+    save = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
+    return lib.call(_GroupedLinear, save, x, weight, offsets, checkpoint, group)

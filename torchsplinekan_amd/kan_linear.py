@@ -220,6 +220,8 @@ class KANLinear(nn.Module):
         return out.reshape(lead + (self.out_features,))
 
     def _needs_autograd(self, xf: torch.Tensor) -> bool:
+        if _C._lib.traced():  # (an autograd function is what a trace records)
+            return True
         if not torch.is_grad_enabled():
             return False
         return xf.requires_grad or any(p.requires_grad for p in self.parameters())

@@ -10,7 +10,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -31,8 +30,9 @@ def _native():
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps, dtype, save):
+    def forward(ctx, x, weight, bias, eps, dtype):
         lib = _native()
+        save = ctx is not None and any(ctx.needs_input_grad)
         C = x.shape[-1]
         n = x.numel() // C
         y = torch.empty(x.shape, dtype=dtype, device=x.device)
@@ -63,7 +63,7 @@ class _LayerNorm(torch.autograd.Function):
         at = [None if t is None else t.data_ptr() for t in (dy, x, weight, stats, *grads, ws)]
         lib.launch(lib.LIB.kan_hip_layer_norm_backward, x.device, *codes, *at[:4], n, C, *at[4:],
                    nbytes.value)
-        return (*grads, None, None, None)
+        return (*grads, None, None)
 
 
 def _composite(x, weight, bias, eps, dtype):
@@ -114,6 +114,4 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     save = torch.is_grad_enabled() and (
         x.requires_grad or weight is not None and weight.requires_grad
         or bias is not None and bias.requires_grad)
-    if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
-        return _LayerNorm.apply(x, weight, bias, float(eps), dtype, save)
-    return _LayerNorm.forward(None, x, weight, bias, float(eps), dtype, save)
+    return lib.call(_LayerNorm, save, x, weight, bias, float(eps), dtype)

@@ -10,7 +10,6 @@ import ctypes
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -44,7 +43,7 @@ class _VocabLoss(torch.autograd.Function):
     ids [T, 1], teacher None."""
 
     @staticmethod
-    def forward(ctx, x, weight, ids, teacher, ignore, tau, reduction, save):
+    def forward(ctx, x, weight, ids, teacher, ignore, tau, reduction):
         lib = _native("linear_cross_entropy")
         T, D = x.shape
         V, k = weight.shape[0], 0 if teacher is None else ids.shape[1]
@@ -58,7 +57,7 @@ class _VocabLoss(torch.autograd.Function):
                    int(ids.dtype == torch.int64), None if teacher is None else teacher.data_ptr(),
                    T, V, D, k, ignore, tau, reduction, loss.data_ptr(), kept.data_ptr(),
                    ws.data_ptr(), nbytes)
-        if save:
+        if ctx is not None and any(ctx.needs_input_grad):
             ctx.args = (code, T, V, D, k, ignore, tau, reduction)
             ctx.save_for_backward(x, weight, ids if k == 0 else None, kept)
         return loss
@@ -81,7 +80,7 @@ class _VocabLoss(torch.autograd.Function):
                    ignore, tau, reduction,
                    None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
                    ws.data_ptr(), nbytes)
-        return dx, dw, None, None, None, None, None, None
+        return dx, dw, None, None, None, None, None
 
 
 def _composite(x, weight, ids, teacher, ignore, tau, reduction):
@@ -139,15 +138,12 @@ def _loss(who, x, weight, ids, teacher, ignore, tau, reduction):
     if not x.is_cuda or x.numel() == 0 or ids.numel() == 0:
         loss = _composite(x, weight, ids, teacher, ignore, tau, code)
     else:
-        _native(who).operator_dtype_code(x.dtype, who)
+        lib = _native(who)
+        lib.operator_dtype_code(x.dtype, who)
         x, weight, ids = x.contiguous(), weight.contiguous(), ids.contiguous()
         teacher = None if teacher is None else teacher.float().contiguous()
         save = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)
-        args = (x, weight, ids, teacher, ignore, tau, code, save)
-        if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
-            loss = _VocabLoss.apply(*args)
-        else:
-            loss = _VocabLoss.forward(None, *args)
+        loss = lib.call(_VocabLoss, save, x, weight, ids, teacher, ignore, tau, code)
     return loss.reshape(lead) if code == 0 and len(lead) != 1 else loss
 
 

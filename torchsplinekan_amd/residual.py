@@ -13,7 +13,6 @@ import ctypes
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import fused as _fused
@@ -47,9 +46,9 @@ def _gate_rows(gate: torch.Tensor, x: torch.Tensor) -> int:
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, y, gate, post, pre, scale, gate_rows, scale_const, act, eps, dtype, wdtype,
-                save):
+    def forward(ctx, x, y, gate, post, pre, scale, gate_rows, scale_const, act, eps, dtype, wdtype):
         lib = _native()
+        save = ctx is not None and any(ctx.needs_input_grad)
         C = x.shape[-1]
         n = x.numel() // C
         new = None if y is None else torch.empty_like(x)
@@ -90,7 +89,7 @@ class _ResidualNorm(torch.autograd.Function):
                         ws)]
         lib.launch(lib.LIB.kan_hip_residual_norm_backward, x.device, *codes, *at[:8], scale_const,
                    act, gate_rows, gate_cols, n, C, *at[8:], nbytes.value)
-        return (*grads, None, None, None, None, None, None, None)
+        return (*grads, None, None, None, None, None, None)
 
 
 def _composite(x, y, gate, post, pre, scale, scale_const, act, eps, dtype):
@@ -196,9 +195,6 @@ def residual_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *,
     tensors = [t if t is None or t.is_contiguous() else t.contiguous()
                for t in (x, y, gate, post_weight, pre_weight, scale_t)]
     save = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-    args = (gate_rows, scale_const, GATE_ACTS[gate_act], float(eps), dtype, wdtype, save)
-    if save or _forward_ad._current_level >= 0:  # (apply refuses forward-mode derivatives)
-        new, h = _ResidualNorm.apply(*tensors, *args)
-    else:
-        new, h = _ResidualNorm.forward(None, *tensors, *args)
+    args = (gate_rows, scale_const, GATE_ACTS[gate_act], float(eps), dtype, wdtype)
+    new, h = lib.call(_ResidualNorm, save, *tensors, *args)
     return (x if new is None else new), h

@@ -501,6 +501,12 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
                            const float* b_scale, int64_t b_group, const void* offsets,
                            int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,
                            void* workspace, size_t workspace_bytes, void* stream);
+/* INPUT and WEIGHT in 16 bits with every result times *scale (on the device), before it
+ * is rounded; a and b are in dtype, and the workspace is the plain product's. */
+int kan_hip_grouped_matmul_scaled(int dtype, int op, const void* a, const void* b,
+                                  const void* offsets, int offsets64, int64_t T, int64_t E,
+                                  int64_t N, int64_t K, const float* scale, void* out,
+                                  void* workspace, size_t workspace_bytes, void* stream);
 
 /* Gated products: h = act(g) * u with g = x gate^T and u = x up^T, rows x [T, K]
  * of E experts (offsets as above; NULL with E = 1: all rows) and weights w
@@ -511,7 +517,12 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
  * The backward's first part turns grad_h [T, N] into grad_pre [T, 2 N], the
  * gradients of g and u; grouped products over w as [E, 2 N, K] make those of x and w
  * of it.  N <= 2^21, other limits as above.  keep: whether the call will be given
- * kept.  The workspace lies on 16 bytes. */
+ * kept.  The workspace lies on 16 bytes.
+ * FP16: grad_pre holds what that type can of it; the scaled form writes it times a power of
+ * two, 1 where its largest finite value is within 1 .. 2^15 and otherwise the one that takes
+ * that to 2^14 .. 2^15, and one over that power to scale[0] for
+ * kan_hip_grouped_matmul_scaled (scale has room for KAN_GATED_SCALE_VALUES). */
+#define KAN_GATED_SCALE_VALUES 8192
 int kan_hip_gated_kept(int dtype, int64_t T, int64_t N, size_t* bytes);
 int kan_hip_gated_workspace(int dtype, const void* x, const void* w, int64_t T, int64_t E, int64_t N,
                             int64_t K, int keep, size_t* bytes);
@@ -520,6 +531,9 @@ int kan_hip_gated(int dtype, int act, const void* x, const void* w, const void* 
                   void* workspace, size_t workspace_bytes, void* stream);
 int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* kept, int64_t T,
                            int64_t N, void* grad_pre, void* stream);
+int kan_hip_gated_backward_scaled(int dtype, int act, const void* grad_h, const void* kept,
+                                  int64_t T, int64_t N, void* grad_pre, float* scale,
+                                  void* stream);
 
 /* Losses of logits z = x w^T (x [T, D], w [V, D]) that are never kept whole.  With
  * p a row's distribution on k ids, tau the temperature and q = softmax(z / tau):

@@ -22,6 +22,7 @@ KAN_DTYPE_F32 = 0
 KAN_DTYPE_F64 = 1
 KAN_DTYPE_BF16 = 2  # the operators beside the KAN layers only
 KAN_DTYPE_F16 = 3
+KAN_GATED_SCALE_VALUES = 8192
 KAN_OK = 0
 KAN_ERR_INVALID = 1
 KAN_ERR_LIMIT = 2
@@ -116,12 +117,15 @@ SIGNATURES = {
                                     + [ctypes.POINTER(_i64)]),
     "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
                                + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
+    "kan_hip_grouped_matmul_scaled": (_int, [_int, _int] + [_vp] * 3 + [_int] + [_i64] * 4
+                                      + [_vp] * 3 + [_sz, _vp]),
     "kan_hip_gated_kept": (_int, [_int] + [_i64] * 2 + [ctypes.POINTER(_sz)]),
     "kan_hip_gated_workspace": (_int, [_int, _vp, _vp] + [_i64] * 4
                                 + [_int, ctypes.POINTER(_sz)]),
     "kan_hip_gated": (_int, [_int, _int, _vp, _vp, _vp, _int] + [_i64] * 4 + [_vp] * 3
                       + [_sz, _vp]),
     "kan_hip_gated_backward": (_int, [_int, _int, _vp, _vp, _i64, _i64, _vp, _vp]),
+    "kan_hip_gated_backward_scaled": (_int, [_int, _int, _vp, _vp, _i64, _i64] + [_vp] * 3),
     "kan_hip_vocab_loss_kept": (_int, [_i64] * 3 + [ctypes.POINTER(_sz)]),
     "kan_hip_vocab_loss_workspace": (_int, [_int, _vp, _vp] + [_i64] * 3 + [ctypes.POINTER(_sz)]),
     "kan_hip_vocab_loss": (_int, [_int] + [_vp] * 3 + [_int, _vp] + [_i64] * 5 + [_dbl, _int]

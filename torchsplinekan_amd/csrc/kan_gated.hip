@@ -30,6 +30,8 @@ struct GatedParams : GroupedParams {  // N: outputs; B [E, 2 N, K]; C: h
   void* pre;  // null: not kept.  fp32: [T, 2 N]; 16 bits: words [T, 2 N]
   void* low;  // 16 bits: [T, N], the low bits of g before those of u
   int act;
+  float* factor;  // null, or [kScaleValues]: the gradients' factor, then largest values
+  int parts;      // how many of those
 };
 
 // bytes of the words, on 16
@@ -345,39 +347,102 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedParams p, int whol
   }
 }
 
-// [dg du] from dh (A) and what was kept; C: [T, 2 N].  Bound by HBM: 16384 x 4096 in
-// bf16, 738 MB, 148 us (5.0 TB/s).
+// V values of dg and du from dh (A) and what was kept.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void gated_grad_kernel(GatedParams p) {
-  each_output<V>(p.T, p.N, [&](int64_t row, int64_t n) {
-    float g[V], u[V], dh[V];
-    if constexpr (sizeof(T) == 4) {
-      const float* at = static_cast<const float*>(p.pre) + row * 2 * p.N + n;
-      load_f32<float, V>(at, g);
-      load_f32<float, V>(at + p.N, u);
-    } else {
-      const uint16_t* at = static_cast<const uint16_t*>(p.pre) + row * 2 * p.N + n;
-      typedef uint16_t words __attribute__((ext_vector_type(V)));
-      constexpr int kLow = Kept<T>::kLow;
-      typedef typename Kept<T>::low Low;
-      typedef typename VecOf<Low, V>::type lows;
-      const words hg = *reinterpret_cast<const words*>(at);
-      const words hu = *reinterpret_cast<const words*>(at + p.N);
-      const lows low =
-          *reinterpret_cast<const lows*>(static_cast<const Low*>(p.low) + row * p.N + n);
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        g[j] = from_kept<kLow>(hg[j], low[j] >> kLow);
-        u[j] = from_kept<kLow>(hu[j], low[j] & ((1 << kLow) - 1));
-      }
-    }
-    load_f32<T, V>(static_cast<const T*>(p.A) + row * p.N + n, dh);
+__device__ __forceinline__ void gated_grads(const GatedParams& p, int64_t row, int64_t n,
+                                            float (&g)[V], float (&u)[V]) {
+  float dh[V];
+  if constexpr (sizeof(T) == 4) {
+    const float* at = static_cast<const float*>(p.pre) + row * 2 * p.N + n;
+    load_f32<float, V>(at, g);
+    load_f32<float, V>(at + p.N, u);
+  } else {
+    const uint16_t* at = static_cast<const uint16_t*>(p.pre) + row * 2 * p.N + n;
+    typedef uint16_t words __attribute__((ext_vector_type(V)));
+    constexpr int kLow = Kept<T>::kLow;
+    typedef typename Kept<T>::low Low;
+    typedef typename VecOf<Low, V>::type lows;
+    const words hg = *reinterpret_cast<const words*>(at);
+    const words hu = *reinterpret_cast<const words*>(at + p.N);
+    const lows low = *reinterpret_cast<const lows*>(static_cast<const Low*>(p.low) + row * p.N + n);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      float a, slope;
-      gated_act<sizeof(T) == 2>(g[j], p.act, &a, &slope);
-      g[j] = dh[j] * u[j] * slope;
-      u[j] = dh[j] * a;
+      g[j] = from_kept<kLow>(hg[j], low[j] >> kLow);
+      u[j] = from_kept<kLow>(hu[j], low[j] & ((1 << kLow) - 1));
+    }
+  }
+  load_f32<T, V>(static_cast<const T*>(p.A) + row * p.N + n, dh);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    float a, slope;
+    gated_act<sizeof(T) == 2>(g[j], p.act, &a, &slope);
+    g[j] = dh[j] * u[j] * slope;
+    u[j] = dh[j] * a;
+  }
+}
+
+// [dg du]; C: [T, 2 N].  Bound by HBM: 16384 x 4096 in bf16, 738 MB, 148 us (5.0 TB/s).
+// MOST: the block's largest finite value too.
+__device__ __forceinline__ float block_most(float v) {
+  __shared__ float red[4];
+  v = wave_max(v);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+template <typename T, int V, bool MOST>
+__global__ __launch_bounds__(256) void gated_grad_kernel(GatedParams p) {
+  float most = 0.0f;
+  each_output<V>(p.T, p.N, [&](int64_t row, int64_t n) {
+    float g[V], u[V];
+    gated_grads<T, V>(p, row, n, g, u);
+    T* out = static_cast<T*>(p.C) + row * 2 * p.N + n;
+    store_f32<T, V>(out, g);
+    store_f32<T, V>(out + p.N, u);
+    if constexpr (MOST) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float a = fabsf(g[j]), b = fabsf(u[j]);
+        most = fmaxf(most, fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f));
+      }
+    }
+  });
+  if constexpr (MOST) {
+    most = block_most(most);
+    if (threadIdx.x == 0) p.factor[1 + blockIdx.x] = most;
+  }
+}
+
+// f16 has 30 binades of normal values.  Gradients of a mean over many rows lie below
+// them, and over small weights products lie above them whose sums do not: where the
+// largest of dg and du is not within 1 .. 2^15 they are written again, times the power of 2
+// that takes it to 2^14 .. 2^15, and the products behind them undo that on their
+// float32 sums.  (Within that range a value is off by 2^-25 at most, 2^-25 of the largest.)
+// 8192 x 1024: 4.2 us where nothing is written again, 18 where it is (19 for the kernel
+// before); 16384 x 4096: 6.7 and 155.  Scaled in every call, from a pass that only
+// looked for the largest: 13 and 155.
+constexpr int kScaleValues = KAN_GATED_SCALE_VALUES;
+template <typename T, int V>
+__global__ __launch_bounds__(256) void gated_rescale_kernel(GatedParams p) {
+  float most = 0.0f;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < p.parts; i += 256) most = fmaxf(most, p.factor[1 + i]);
+  most = block_most(most);
+  float unit = 1.0f;
+  if (most != 0.0f && (most < 1.0f || most >= 32768.0f)) {
+    int e;
+    frexpf(most, &e);  // (most < 2^e; one over the unit is a normal number)
+    unit = ldexpf(1.0f, min(max(15 - e, -126), 126));
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.factor = 1.0f / unit;
+  if (unit == 1.0f) return;
+  each_output<V>(p.T, p.N, [&](int64_t row, int64_t n) {
+    float g[V], u[V];
+    gated_grads<T, V>(p, row, n, g, u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      g[j] *= unit;
+      u[j] *= unit;
     }
     T* out = static_cast<T*>(p.C) + row * 2 * p.N + n;
     store_f32<T, V>(out, g);
@@ -421,6 +486,19 @@ int launch_gated_few(const GatedParams& p, hipStream_t st) {
     return wide ? launch_gated_few_cols<T, 2, false>(p, st)
                 : launch_gated_few_cols<T, 1, false>(p, st);
   return wide ? launch_gated_few_cols<T, 2, true>(p, st) : launch_gated_few_cols<T, 1, true>(p, st);
+}
+
+template <typename T, int V>
+int launch_gated_grad(GatedParams p, hipStream_t st) {
+  const unsigned blocks = flat_blocks(p.T * p.N / V);
+  if (p.factor == nullptr) {
+    gated_grad_kernel<T, V, false><<<blocks, 256, 0, st>>>(p);
+  } else if constexpr (std::is_same<T, f16>::value) {
+    p.parts = (int)std::min<unsigned>(blocks, kScaleValues - 1);
+    gated_grad_kernel<T, V, true><<<p.parts, 256, 0, st>>>(p);
+    gated_rescale_kernel<T, V><<<std::min<unsigned>(blocks, 8 * device_cu_count()), 256, 0, st>>>(p);
+  }
+  return check_launch("gated_backward");
 }
 
 int check_gated(const char* who, int dtype, int act, int64_t T, int64_t E, int64_t N, int64_t K) {
@@ -576,8 +654,8 @@ int kan_hip_gated(int dtype, int act, const void* x, const void* w, const void* 
   return check_launch("gated");
 }
 
-int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* kept, int64_t T,
-                           int64_t N, void* grad_pre, void* stream) {
+static int gated_backward(int dtype, int act, const void* grad_h, const void* kept, int64_t T,
+                          int64_t N, void* grad_pre, float* scale, void* stream) {
   const int rc = check_gated("gated_backward", dtype, act, T, 0, N, 0);
   if (rc != KAN_OK) return rc;
   if (T == 0 || N == 0) return KAN_OK;
@@ -593,22 +671,30 @@ int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* k
   p.T = T;
   p.N = N;
   p.act = act;
+  p.factor = scale;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassOther, st, (double)T * N * (dtype == KAN_DTYPE_F32 ? 20 : 11));
   const bool whole = aligned16(grad_h) && aligned16(grad_pre);
-  const unsigned wide = flat_blocks(T * N / (dtype == KAN_DTYPE_F32 ? 4 : 8)),
-                 one = flat_blocks(T * N);
-  if (dtype == KAN_DTYPE_F32) {
-    if (whole && N % 4 == 0) gated_grad_kernel<float, 4><<<wide, 256, 0, st>>>(p);
-    else gated_grad_kernel<float, 1><<<one, 256, 0, st>>>(p);
-  } else if (dtype == KAN_DTYPE_BF16) {
-    if (whole && N % 8 == 0) gated_grad_kernel<bf16, 8><<<wide, 256, 0, st>>>(p);
-    else gated_grad_kernel<bf16, 1><<<one, 256, 0, st>>>(p);
-  } else {
-    if (whole && N % 8 == 0) gated_grad_kernel<f16, 8><<<wide, 256, 0, st>>>(p);
-    else gated_grad_kernel<f16, 1><<<one, 256, 0, st>>>(p);
-  }
-  return check_launch("gated_backward");
+  if (dtype == KAN_DTYPE_F32)
+    return whole && N % 4 == 0 ? launch_gated_grad<float, 4>(p, st)
+                               : launch_gated_grad<float, 1>(p, st);
+  if (dtype == KAN_DTYPE_BF16)
+    return whole && N % 8 == 0 ? launch_gated_grad<bf16, 8>(p, st)
+                               : launch_gated_grad<bf16, 1>(p, st);
+  return whole && N % 8 == 0 ? launch_gated_grad<f16, 8>(p, st) : launch_gated_grad<f16, 1>(p, st);
+}
+
+int kan_hip_gated_backward(int dtype, int act, const void* grad_h, const void* kept, int64_t T,
+                           int64_t N, void* grad_pre, void* stream) {
+  return gated_backward(dtype, act, grad_h, kept, T, N, grad_pre, nullptr, stream);
+}
+
+int kan_hip_gated_backward_scaled(int dtype, int act, const void* grad_h, const void* kept,
+                                  int64_t T, int64_t N, void* grad_pre, float* scale,
+                                  void* stream) {
+  if (dtype != KAN_DTYPE_F16 || scale == nullptr)
+    return set_error(KAN_ERR_INVALID, "gated_backward_scaled: FP16 and a place for the factor");
+  return gated_backward(dtype, act, grad_h, kept, T, N, grad_pre, scale, stream);
 }
 
 }  // extern "C"

@@ -574,10 +574,11 @@ int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b,
   return KAN_OK;
 }
 
-int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
-                           const float* b_scale, int64_t b_group, const void* offsets,
-                           int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,
-                           void* workspace, size_t workspace_bytes, void* stream) {
+static int grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
+                          const float* b_scale, int64_t b_group, const void* offsets,
+                          int offsets64, int64_t T, int64_t E, int64_t N, int64_t K,
+                          const float* scale, void* out, void* workspace, size_t workspace_bytes,
+                          void* stream) {
   const int rc = check_grouped(dtype, op, T, E, N, K);
   if (rc != KAN_OK) return rc;
   if (b_format != KAN_ACT8_NONE) {
@@ -618,6 +619,7 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   p.K = K;
   p.group = (int)b_group;
   p.format = b_format;
+  p.scale = scale;
   hipStream_t st = static_cast<hipStream_t>(stream);
   TimedLaunch timed(kClassContraction, st, 2.0 * (double)T * N * K);
   p.lda = op == KAN_GROUPED_FORWARD ? K : N;
@@ -632,6 +634,25 @@ int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int 
   }
   const int e = launch_aligned(w.align, &p, ws, st);
   return e != KAN_OK ? e : launch_product(dtype, op, p, w.plan, st);
+}
+
+int kan_hip_grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,
+                           const float* b_scale, int64_t b_group, const void* offsets,
+                           int offsets64, int64_t T, int64_t E, int64_t N, int64_t K, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  return grouped_matmul(dtype, op, a, b, b_format, b_scale, b_group, offsets, offsets64, T, E, N, K,
+                        nullptr, out, workspace, workspace_bytes, stream);
+}
+
+int kan_hip_grouped_matmul_scaled(int dtype, int op, const void* a, const void* b,
+                                  const void* offsets, int offsets64, int64_t T, int64_t E,
+                                  int64_t N, int64_t K, const float* scale, void* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype == KAN_DTYPE_F32 || op == KAN_GROUPED_FORWARD || scale == nullptr)
+    return set_error(KAN_ERR_INVALID,
+                     "grouped_matmul_scaled: gradients' products in 16 bits and a factor");
+  return grouped_matmul(dtype, op, a, b, KAN_ACT8_NONE, nullptr, 0, offsets, offsets64, T, E, N, K,
+                        scale, out, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -101,6 +101,12 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+
 // Sum over aligned groups of 8, 16 or 32 lanes, in each of them.
 template <int LANES>
 __device__ __forceinline__ float lane_sum(float v) {

@@ -71,12 +71,6 @@ __device__ __forceinline__ int target_of(const VocabParams& p, int64_t row, floa
   return in ? (int)id : kNoId;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v = fmaxf(v, __shfl_xor(v, m));
-  return v;
-}
-
 // One wave a row: p = softmax(teacher / tau) over its ids, sorted by id (a place is the
 // number of smaller ones, so equal ids keep their order).
 constexpr int64_t kMaxTop = 1024;

@@ -71,14 +71,20 @@ class _GatedLinear(torch.autograd.Function):
         need_x, need_w = ctx.needs_input_grad[:2]
         dh = dh.contiguous()
         dpre = dh.new_empty(T, 2 * N)
-        lib.launch(lib.LIB.kan_hip_gated_backward, dh.device, lib.OPERATOR_DTYPES[dh.dtype], act,
-                   lib.ptr(dh), lib.ptr(kept), T, N, lib.ptr(dpre))
+        code, factor = lib.OPERATOR_DTYPES[dh.dtype], None
+        if dh.dtype == torch.float16 and dpre.numel():  # (small or large values would be lost)
+            factor = torch.empty(lib.KAN_GATED_SCALE_VALUES, dtype=torch.float32, device=dh.device)
+            lib.launch(lib.LIB.kan_hip_gated_backward_scaled, dh.device, code, act, lib.ptr(dh),
+                       lib.ptr(kept), T, N, lib.ptr(dpre), factor.data_ptr())
+        else:
+            lib.launch(lib.LIB.kan_hip_gated_backward, dh.device, code, act, lib.ptr(dh),
+                       lib.ptr(kept), T, N, lib.ptr(dpre))
         dx = dw = None
         if need_x:
-            dx = _matmul(INPUT, dpre, weight, offsets, dh.new_empty(T, K), T, E, 2 * N, K)
+            dx = _matmul(INPUT, dpre, weight, offsets, dh.new_empty(T, K), T, E, 2 * N, K, factor)
         if need_w:
             shape = (2, N, K) if offsets is None else (E, 2, N, K)
-            dw = _matmul(WEIGHT, dpre, x, offsets, dh.new_empty(shape), T, E, 2 * N, K)
+            dw = _matmul(WEIGHT, dpre, x, offsets, dh.new_empty(shape), T, E, 2 * N, K, factor)
         return dx, dw, None, None
 
 

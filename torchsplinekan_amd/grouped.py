@@ -29,9 +29,9 @@ def _native():
     return _C._lib
 
 
-def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
+def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int, factor=None):
     """One grouped product into `out`; b may be an Activation8 (WEIGHT), offsets None
-    with one group."""
+    with one group; factor: a float32 tensor whose first value all results are times."""
     lib = _native()
     if out.numel() == 0:
         return out
@@ -45,10 +45,14 @@ def _matmul(op: int, a, b, offsets, out, T: int, E: int, N: int, K: int):
                                                        ctypes.byref(nbytes)))
     if nbytes.value:
         ws = torch.empty(nbytes.value, dtype=torch.uint8, device=out.device)
+    off64 = int(offsets is not None and offsets.dtype == torch.int64)
+    if factor is not None:
+        lib.launch(lib.LIB.kan_hip_grouped_matmul_scaled, out.device, code, op, pa, pb,
+                   lib.ptr(offsets), off64, T, E, N, K, factor.data_ptr(), out.data_ptr(),
+                   lib.ptr(ws), nbytes.value)
+        return out
     lib.launch(lib.LIB.kan_hip_grouped_matmul, out.device, code, op, pa, pb, form, scale, group,
-               lib.ptr(offsets),
-               int(offsets is not None and offsets.dtype == torch.int64), T, E, N, K, out.data_ptr(),
-               lib.ptr(ws), nbytes.value)
+               lib.ptr(offsets), off64, T, E, N, K, out.data_ptr(), lib.ptr(ws), nbytes.value)
     return out
 
 

@@ -5,8 +5,9 @@
 //   dx = r (t - mean(t) - xh mean(t xh)),  dweight = sum_rows dy xh,  dbias = sum_rows dy.
 //
 // A row lies in the registers of 8 to 1024 lanes (kan_norm.h), so that the
-// variance is taken of the values less their mean without a second read.  All
-// arithmetic is in float32, rounded once where a result is stored.  The column
+// variance is taken of the values less their mean without a second read.  The mean of
+// what is left of the values goes into the mean: a constant row becomes zero, and rows far
+// from zero are off by the mean's own rounding.  All arithmetic is in float32, rounded once where a result is stored.  The column
 // sums go through one partial row a block, added in block order: no atomics, the
 // same bits every time.  Bound by HBM: 16384 rows of 4096 in bf16, forward 45 us (6.0
 // TB/s, part of it from the last-level cache), forward and backward 137 us for 671 MB;
@@ -43,6 +44,9 @@ inline Rows plan_rows(int64_t n, int64_t C, int waves_per_cu) {
   return {ceil_div(n, chunk), chunk};
 }
 
+// The squares of values less m + d are those less m, less d^2: taken so where d^2 is
+// below this part of the variance, and its rounding with it.
+constexpr float kShift = 1.0f / 1024;
 template <typename TX, typename TY, int TPR, int VEC, int NV, bool WHOLE>
 __global__ __launch_bounds__(RowShape<TPR>::kThreads) void layer_norm_kernel(LayerNormParams p) {
   typedef RowShape<TPR> S;
@@ -64,20 +68,33 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void layer_norm_kernel(Lay
     float s[1] = {0.0f};
     KAN_EACH s[0] += x[i][j];
     row_sums<TPR>(s, red, turn);
-    // (a division: a constant row's mean is that value, and the row becomes zero)
-    const float m = s[0] / (float)p.C;
-    s[0] = 0.0f;
+    float m = s[0] / (float)p.C;
+    float t[2] = {0.0f, 0.0f};
     KAN_EACH {
-      x[i][j] = PX::at(i) + j < p.C ? x[i][j] - m : 0.0f;
-      s[0] += x[i][j] * x[i][j];
+      const float d = PX::at(i) + j < p.C ? x[i][j] - m : 0.0f;
+      t[0] += d;
+      t[1] += d * d;
     }
-    row_sums<TPR>(s, red, turn);
-    const float r = 1.0f / sqrtf(s[0] * inv_c + p.eps);
+    row_sums<TPR>(t, red, turn);
+    // (the sum over C values was off by a few units in m's last place, and so is d)
+    const float d = t[0] * inv_c;
+    m += d;
+    float var = t[1] * inv_c - d * d;
+    if (!(d * d <= kShift * var)) {  // (all of a row alike; its squares may be beyond a float)
+      s[0] = 0.0f;
+      KAN_EACH {
+        const float v = PX::at(i) + j < p.C ? x[i][j] - m : 0.0f;
+        s[0] += v * v;
+      }
+      row_sums<TPR>(s, red, turn);
+      var = s[0] * inv_c;
+    }
+    const float r = 1.0f / sqrtf(var + p.eps);
     if (p.stats != nullptr && threadIdx.x % TPR == 0) {
       p.stats[row] = m;
       p.stats[p.n + row] = r;
     }
-    KAN_EACH x[i][j] = x[i][j] * r * w[i][j] + b[i][j];
+    KAN_EACH x[i][j] = (x[i][j] - m) * r * w[i][j] + b[i][j];
     PY::store(x, static_cast<TY*>(p.y) + row * p.C, p.C);
   }
 }
@@ -133,13 +150,25 @@ __global__ __launch_bounds__(kRowThreads) void layer_norm_rows_kernel(LayerNormP
     const TX* x = static_cast<const TX*>(p.x) + row * p.C;
     float s = 0.0f;
     for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) s += (float)x[c];
-    const float m = block_sum(s, red) / (float)p.C;
+    float m = block_sum(s, red) / (float)p.C, t = 0.0f;
     s = 0.0f;
     for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
-      const float d = (float)x[c] - m;
-      s += d * d;
+      const float v = (float)x[c] - m;
+      t += v;
+      s += v * v;
     }
-    const float r = 1.0f / sqrtf(block_sum(s, red) * inv_c + p.eps);
+    const float d = block_sum(t, red) * inv_c;
+    m += d;
+    float var = block_sum(s, red) * inv_c - d * d;
+    if (!(d * d <= kShift * var)) {  // (as above)
+      s = 0.0f;
+      for (int64_t c = threadIdx.x; c < p.C; c += kRowThreads) {
+        const float v = (float)x[c] - m;
+        s += v * v;
+      }
+      var = block_sum(s, red) * inv_c;
+    }
+    const float r = 1.0f / sqrtf(var + p.eps);
     if (p.stats != nullptr && threadIdx.x == 0) {
       p.stats[row] = m;
       p.stats[p.n + row] = r;

@@ -70,7 +70,8 @@ def _composite(x, weight, bias, eps, dtype):
     """The formula in torch (CPU tensors, empty tensors), in float32 or wider."""
     wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     v = x.to(wide)
-    v = v - v.mean(-1, keepdim=True)
+    m = v.mean(-1, keepdim=True)
+    v = v - (m + (v - m).mean(-1, keepdim=True))  # (a constant row becomes zero)
     v = v * (v.square().mean(-1, keepdim=True) + eps).rsqrt()
     if weight is not None:
         v = v * weight.to(wide)

@@ -254,7 +254,9 @@ def call(function, save: bool, *args):
     """`function`, an autograd function, of args: through apply where its backward pass
     is wanted (save), under forward mode (which apply refuses) and where the call is
     traced; otherwise its forward alone, which is shorter on the host."""
-    if traced() or save or _forward_ad._current_level >= 0:
+    if (save or _is_tracing() or _dispatch_mode(_PROXY) is not None
+            or _forward_ad._current_level >= 0):
+        traced()  # (raises under make_fx)
         return function.apply(*args)
     return function.forward(None, *args)
 

@@ -549,7 +549,7 @@ int kan_hip_gated_backward_scaled(int dtype, int act, const void* grad_h, const 
  * backward, which takes a cross entropy's ids again too.  (The logits of at most 32
  * columns are kept.)  grad_x [T, D], grad_w [V, D], either of which may be NULL (with_dx,
  * with_dw: whether it will be given).  V and D are positive, T < 2^30, V and D <=
- * 2^22, k <= 1024.  Workspaces depend on the operands' alignment; they and kept lie
+ * 2^22, k <= 1024; in 16 bits tiles of 128 x 128 logits number less than 2^24 (KAN_ERR_LIMIT).  Workspaces depend on the operands' alignment; they and kept lie
  * on 16 bytes.  With T = 0 nothing is written. */
 #define KAN_REDUCE_NONE 0
 #define KAN_REDUCE_SUM 1

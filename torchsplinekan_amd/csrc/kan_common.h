@@ -47,6 +47,8 @@ __device__ __forceinline__ int xcd_remap(int pid, int total) {
   return xcd * per + min(xcd, rem) + idx;
 }
 __host__ __device__ inline int64_t round_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
+// Whether a grid of `blocks` x 1 x 1 can be launched: 32 bits count its threads.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= 0xffffffff / threads; }
 
 // Width of one augmented basis row [H(n, 0..I*R-1) | silu(x(n, 0..I-1))],
 // padded to a multiple of 4 elements so that rows start 16-byte aligned.

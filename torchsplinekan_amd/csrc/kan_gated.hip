@@ -454,7 +454,7 @@ __global__ __launch_bounds__(256) void gated_rescale_kernel(GatedParams p) {
 template <typename T, class G>
 int launch_gated_tile(const GatedParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(p.N, G::BN / 2), blocks = row_grid(p, G::BM, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "gated: too many tiles");
+  if (!grid_fits(blocks, G::NT)) return set_error(KAN_ERR_LIMIT, "gated: too many tiles");
   const int whole = p.N % 8 == 0 && aligned16(p.C) && aligned16(p.pre);
   if (whole_rows(p.A, p.lda) && whole_rows(p.B, p.ldb))
     gated_tile_kernel<T, G, kDirect><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n,
@@ -474,7 +474,7 @@ int launch_gated_half(const GatedParams& p, HalfCfg cfg, hipStream_t st) {
 template <typename T, int NP, bool WHOLE>
 int launch_gated_few_cols(const GatedParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(p.N, 16 * NP), blocks = row_grid(p, kFewRows, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "gated: too many tiles");
+  if (!grid_fits(blocks, 256)) return set_error(KAN_ERR_LIMIT, "gated: too many tiles");
   gated_few_kernel<T, NP, WHOLE><<<dim3((unsigned)blocks), 256, 0, st>>>(p, (int)tiles_n);
   return check_launch("gated");
 }

@@ -2219,7 +2219,7 @@ int launch_grouped_cfg(const GroupedParams& p, hipStream_t st) {
   const int64_t cols = OP == 0 ? p.N : p.K, lda = OP == 0 ? p.K : p.N;
   const int64_t tiles_n = ceil_div(cols, C::BN), tiles_m = ceil_div(p.N, C::BM);
   const int64_t blocks = OP == 2 ? weight_grid(p, tiles_m * tiles_n) : row_grid(p, C::BM, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  if (!grid_fits(blocks, C::kThreads)) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
   // whole-slab byte offsets in 31 bits, as launch_cfg
   auto span_ok = [](bool kcont, int rows, int64_t ld) {
     return ((kcont ? rows * ld + C::BK : C::BK * ld + rows) * 4) < (int64_t)1 << 31;

@@ -144,7 +144,7 @@ int launch_tile(const GroupedParams& p, hipStream_t st) {
   const int64_t cols = OP == 0 ? p.N : p.K;
   const int64_t tiles_n = ceil_div(cols, G::BN), tiles_m = ceil_div(p.N, G::BM);
   const int64_t blocks = OP == 2 ? weight_grid(p, tiles_m * tiles_n) : row_grid(p, G::BM, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  if (!grid_fits(blocks, G::NT)) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
   grouped_tile_kernel<T, G, OP, MA, MB><<<dim3((unsigned)blocks, OP == 2 ? 1 : p.cuts), G::NT, 0,
                                          st>>>(
       p, (int)tiles_m, (int)tiles_n, cols % 8 == 0 && aligned16(p.C) ? 1 : 0);
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(256) void grouped_few_kernel(GroupedParams p, int t
 template <typename T, int NC, bool WHOLE>
 int launch_few_cols(const GroupedParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(p.N, 16 * NC), blocks = row_grid(p, kFewRows, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
+  if (!grid_fits(blocks, 256)) return set_error(KAN_ERR_LIMIT, "grouped_matmul: too many tiles");
   grouped_few_kernel<T, NC, WHOLE><<<dim3((unsigned)blocks), 256, 0, st>>>(p, (int)tiles_n);
   return check_launch("grouped_matmul");
 }

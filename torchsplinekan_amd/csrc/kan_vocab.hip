@@ -71,6 +71,13 @@ __device__ __forceinline__ int target_of(const VocabParams& p, int64_t row, floa
   return in ? (int)id : kNoId;
 }
 
+// Blocks of a kernel that takes rows in turns: a grid has fewer than 2^32 threads, which
+// T rows of a wave each pass from 2^26 on.
+constexpr int64_t kMaxBlocks = 1 << 20;
+unsigned row_blocks(int64_t rows, int64_t each) {
+  return (unsigned)std::min<int64_t>(ceil_div(rows, each), kMaxBlocks);
+}
+
 // One wave a row: p = softmax(teacher / tau) over its ids, sorted by id (a place is the
 // number of smaller ones, so equal ids keep their order).
 constexpr int64_t kMaxTop = 1024;
@@ -78,46 +85,49 @@ __global__ __launch_bounds__(64) void vocab_teacher_kernel(VocabParams p, const 
                                                            const float* __restrict__ teacher) {
   __shared__ int id_of[kMaxTop];
   __shared__ float value_of[kMaxTop];
-  const int64_t t = blockIdx.x, base = t * p.k;
   const int k = (int)p.k, lane = threadIdx.x;
-  float top = -INFINITY;
-  bool bad = false;
-  for (int j = lane; j < k; j += 64) {
-    const int64_t id = is64 ? static_cast<const int64_t*>(ids)[base + j]
-                            : (int64_t)static_cast<const int*>(ids)[base + j];
-    const bool in = id >= 0 && id < p.V;
-    const float v = in ? teacher[base + j] / p.tau : -INFINITY;
-    bad |= id >= p.V;
-    id_of[j] = in ? (int)id : kNoId;
-    value_of[j] = v;
-    top = fmaxf(top, v);
-  }
-  top = wave_max(top);
-  if (top == -INFINITY) top = 0.0f;
-  float sum = 0.0f;
-  for (int j = lane; j < k; j += 64) {
-    const float e = expf(value_of[j] - top);
-    sum += e;
-  }
-  sum = wave_sum(sum);
-  const float log_sum = logf(sum);
-  __syncthreads();
-  float entropy = 0.0f;
-  for (int j = lane; j < k; j += 64) {
-    const int id = id_of[j];
-    const float v = value_of[j], e = expf(v - top);
-    const float prob = sum == 0.0f ? 0.0f : e / sum;
-    if (!(prob == 0.0f)) entropy += prob * (v - top - log_sum);
-    int place = 0;
-    for (int i = 0; i < k; ++i) place += id_of[i] < id || (id_of[i] == id && i < j);
-    p.ids[base + place] = id;
-    p.prob[base + place] = prob;
-  }
-  entropy = wave_sum(entropy);
-  bad = __any(bad);
-  if (lane == 0) {
-    p.entropy[t] = entropy;
-    p.flag[t] = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f;
+  for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x) {
+    const int64_t base = t * p.k;
+    float top = -INFINITY;
+    bool bad = false;
+    for (int j = lane; j < k; j += 64) {
+      const int64_t id = is64 ? static_cast<const int64_t*>(ids)[base + j]
+                              : (int64_t)static_cast<const int*>(ids)[base + j];
+      const bool in = id >= 0 && id < p.V;
+      const float v = in ? teacher[base + j] / p.tau : -INFINITY;
+      bad |= id >= p.V;
+      id_of[j] = in ? (int)id : kNoId;
+      value_of[j] = v;
+      top = fmaxf(top, v);
+    }
+    top = wave_max(top);
+    if (top == -INFINITY) top = 0.0f;
+    float sum = 0.0f;
+    for (int j = lane; j < k; j += 64) {
+      const float e = expf(value_of[j] - top);
+      sum += e;
+    }
+    sum = wave_sum(sum);
+    const float log_sum = logf(sum);
+    __syncthreads();
+    float entropy = 0.0f;
+    for (int j = lane; j < k; j += 64) {
+      const int id = id_of[j];
+      const float v = value_of[j], e = expf(v - top);
+      const float prob = sum == 0.0f ? 0.0f : e / sum;
+      if (!(prob == 0.0f)) entropy += prob * (v - top - log_sum);
+      int place = 0;
+      for (int i = 0; i < k; ++i) place += id_of[i] < id || (id_of[i] == id && i < j);
+      p.ids[base + place] = id;
+      p.prob[base + place] = prob;
+    }
+    entropy = wave_sum(entropy);
+    bad = __any(bad);
+    if (lane == 0) {
+      p.entropy[t] = entropy;
+      p.flag[t] = bad ? NAN : sum == 0.0f ? 0.0f : 1.0f;
+    }
+    __syncthreads();  // (its ids may be the next row's)
   }
 }
 
@@ -375,68 +385,69 @@ constexpr int kSpan = 1024, kSpanValues = kSpan / 64;
 template <bool GRAD>
 __global__ __launch_bounds__(256) void vocab_span_kernel(VocabParams p) {
   const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= p.T) return;
   const float c = kLog2e / p.tau;
-  for (int64_t n0 = (int64_t)blockIdx.y * kSpan; n0 < p.cols; n0 += (int64_t)gridDim.y * kSpan) {
-    float* z = p.z + row * p.cols + n0;
-    const int64_t left = p.cols - n0;
-    float v[kSpanValues];
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < p.T;
+       row += (int64_t)gridDim.x * 4) {
+    for (int64_t n0 = (int64_t)blockIdx.y * kSpan; n0 < p.cols; n0 += (int64_t)gridDim.y * kSpan) {
+      float* z = p.z + row * p.cols + n0;
+      const int64_t left = p.cols - n0;
+      float v[kSpanValues];
 #pragma unroll
-    for (int i = 0; i < kSpanValues; ++i) v[i] = lane + 64 * i < left ? z[lane + 64 * i] : -INFINITY;
-    const int from = (int)(p.v0 + n0);
-    // f(column of the span's, p) for the row's ids
-    auto entries = [&](auto f) __attribute__((always_inline)) {
-      if (p.target != nullptr) {
-        float flag;
-        const int at = target_of(p, row, &flag) - from;
-        if (at >= 0 && at < kSpan) f(at, 1.0f);
-        return;
-      }
-      const int* ids = p.ids + row * p.k;
-      for (int e = first_id(ids, (int)p.k, from); e < p.k && ids[e] < from + kSpan; ++e)
-        f(ids[e] - from, p.prob[row * p.k + e]);
-    };
-    if constexpr (!GRAD) {
-      float top = -INFINITY;
+      for (int i = 0; i < kSpanValues; ++i) v[i] = lane + 64 * i < left ? z[lane + 64 * i] : -INFINITY;
+      const int from = (int)(p.v0 + n0);
+      // f(column of the span's, p) for the row's ids
+      auto entries = [&](auto f) __attribute__((always_inline)) {
+        if (p.target != nullptr) {
+          float flag;
+          const int at = target_of(p, row, &flag) - from;
+          if (at >= 0 && at < kSpan) f(at, 1.0f);
+          return;
+        }
+        const int* ids = p.ids + row * p.k;
+        for (int e = first_id(ids, (int)p.k, from); e < p.k && ids[e] < from + kSpan; ++e)
+          f(ids[e] - from, p.prob[row * p.k + e]);
+      };
+      if constexpr (!GRAD) {
+        float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) top = fmaxf(top, v[i]);
-      top = wave_max(top);
-      const float base = top == -INFINITY ? 0.0f : top;
-      float rest = 0.0f, most = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) {
-        rest += below(v[i], base, c);
-        most += v[i] == base ? 1.0f : 0.0f;
-      }
-      rest = wave_sum(rest);
-      most = wave_sum(most);
-      if (top > -INFINITY) rest += most - 1.0f;
-      float dot = 0.0f;
-      entries([&](int at, float prob) {
-        if (prob != 0.0f) dot += prob * z[at];
-      });
-      if (lane == 0) {
-        float* out = p.stats + ((p.v0 + n0) / kSpan) * p.T + row;
-        out[0] = top;
-        out[p.tiles * p.T] = rest;
-        out[2 * p.tiles * p.T] = dot;
-      }
-    } else {
-      const float top = p.top[row], rest = p.rest[row], weight = p.weight[row];
-      const float part = weight / (1.0f + rest);
-#pragma unroll
-      for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f((v[i] - top) * c);
-      entries([&](int at, float prob) __attribute__((always_inline)) {
+        for (int i = 0; i < kSpanValues; ++i) top = fmaxf(top, v[i]);
+        top = wave_max(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        float rest = 0.0f, most = 0.0f;
 #pragma unroll
         for (int i = 0; i < kSpanValues; ++i) {
-          const float here = lane + 64 * i == at ? prob : 0.0f;
-          v[i] = __builtin_fmaf(-here, rest, v[i] - here);
+          rest += below(v[i], base, c);
+          most += v[i] == base ? 1.0f : 0.0f;
         }
-      });
+        rest = wave_sum(rest);
+        most = wave_sum(most);
+        if (top > -INFINITY) rest += most - 1.0f;
+        float dot = 0.0f;
+        entries([&](int at, float prob) {
+          if (prob != 0.0f) dot += prob * z[at];
+        });
+        if (lane == 0) {
+          float* out = p.stats + ((p.v0 + n0) / kSpan) * p.T + row;
+          out[0] = top;
+          out[p.tiles * p.T] = rest;
+          out[2 * p.tiles * p.T] = dot;
+        }
+      } else {
+        const float top = p.top[row], rest = p.rest[row], weight = p.weight[row];
+        const float part = weight / (1.0f + rest);
 #pragma unroll
-      for (int i = 0; i < kSpanValues; ++i)
-        if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * part;
+        for (int i = 0; i < kSpanValues; ++i) v[i] = exp2f((v[i] - top) * c);
+        entries([&](int at, float prob) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < kSpanValues; ++i) {
+            const float here = lane + 64 * i == at ? prob : 0.0f;
+            v[i] = __builtin_fmaf(-here, rest, v[i] - here);
+          }
+        });
+#pragma unroll
+        for (int i = 0; i < kSpanValues; ++i)
+          if (lane + 64 * i < left) z[lane + 64 * i] = weight == 0.0f ? 0.0f : v[i] * part;
+      }
     }
   }
 }
@@ -467,35 +478,40 @@ __global__ __launch_bounds__(64 * kRowWaves) void vocab_rows_kernel(VocabParams 
                                                                     float* __restrict__ loss) {
   __shared__ float red[3][kRowWaves][kBlockRows];
   const int r = threadIdx.x % kBlockRows, tl = threadIdx.x / kBlockRows, wave = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * kBlockRows + r;
   const float c = kLog2e / p.tau;
-  float top = -INFINITY, rest = 0.0f, dot = 0.0f;
-  if (row < p.T) {
-    for (int i = tl; i < p.tiles; i += 64 * kRowWaves / kBlockRows) {
-      const float* at = p.stats + (int64_t)i * p.T + row;
-      join(&top, &rest, at[0], at[p.tiles * p.T], c);
-      dot += at[2 * p.tiles * p.T];
+  for (int64_t row0 = (int64_t)blockIdx.x * kBlockRows; row0 < p.T;
+       row0 += (int64_t)gridDim.x * kBlockRows) {
+    const int64_t row = row0 + r;
+    float top = -INFINITY, rest = 0.0f, dot = 0.0f;
+    if (row < p.T) {
+      for (int i = tl; i < p.tiles; i += 64 * kRowWaves / kBlockRows) {
+        const float* at = p.stats + (int64_t)i * p.T + row;
+        join(&top, &rest, at[0], at[p.tiles * p.T], c);
+        dot += at[2 * p.tiles * p.T];
+      }
     }
-  }
 #pragma unroll
-  for (int m = kBlockRows; m < 64; m *= 2) {
-    const float other = __shfl_xor(top, m), s = __shfl_xor(rest, m);
-    join(&top, &rest, other, s, c);
-    dot += __shfl_xor(dot, m);
-  }
-  if ((threadIdx.x & 63) < kBlockRows) {
-    red[0][wave][r] = top;
-    red[1][wave][r] = rest;
-    red[2][wave][r] = dot;
-  }
-  __syncthreads();
-  if (threadIdx.x >= kBlockRows || row >= p.T) return;
+    for (int m = kBlockRows; m < 64; m *= 2) {
+      const float other = __shfl_xor(top, m), s = __shfl_xor(rest, m);
+      join(&top, &rest, other, s, c);
+      dot += __shfl_xor(dot, m);
+    }
+    if ((threadIdx.x & 63) < kBlockRows) {
+      red[0][wave][r] = top;
+      red[1][wave][r] = rest;
+      red[2][wave][r] = dot;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBlockRows && row < p.T) {
 #pragma unroll
-  for (int i = 1; i < kRowWaves; ++i) {
-    join(&top, &rest, red[0][i][r], red[1][i][r], c);
-    dot += red[2][i][r];
+      for (int i = 1; i < kRowWaves; ++i) {
+        join(&top, &rest, red[0][i][r], red[1][i][r], c);
+        dot += red[2][i][r];
+      }
+      finish_row(p, row, top, rest, dot, loss);
+    }
+    __syncthreads();
   }
-  finish_row(p, row, top, rest, dot, loss);
 }
 
 // ---- few classes ----------------------------------------------------------------------
@@ -511,62 +527,67 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabParams p, float* __
   typedef RowsMma<T> M;
   __shared__ float red[4][kFewRows][16 * NC + 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m0 = (int64_t)blockIdx.x * kFewRows;
-  typename M::acc_t acc[NC];
-  const T* w[NC];
+  for (int64_t m0 = (int64_t)blockIdx.x * kFewRows; m0 < p.T;
+       m0 += (int64_t)gridDim.x * kFewRows) {
+    typename M::acc_t acc[NC];
+    const T* w[NC];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    acc[c] = {0.0f, 0.0f, 0.0f, 0.0f};
-    w[c] = static_cast<const T*>(p.w) + min((int64_t)(16 * c + (lane & 15)), p.V - 1) * p.D;
-  }
-  const T* x = static_cast<const T*>(p.x) + min(m0 + (lane & 15), p.T - 1) * p.D;
-  few_rows<T, NC, WHOLE>(x, w, p.D, acc);
-#pragma unroll
-  for (int c = 0; c < NC; ++c)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) red[wave][lane & 15][16 * c + 4 * (lane >> 4) + v] = acc[c][v];
-  __syncthreads();
-  // 16 lanes a row, column 16 c + lane at z[c]
-  const int r = threadIdx.x >> 4, l = threadIdx.x & 15;
-  const int64_t row = m0 + r;
-  if (row >= p.T) return;
-  const float c2 = kLog2e / p.tau;
-  float z[NC], top = -INFINITY, rest = 0.0f, most = 0.0f, dot = 0.0f;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int v = 16 * c + l;
-    z[c] = -INFINITY;
-    if (v < p.V) {
-      z[c] = red[0][r][v] + red[1][r][v] + red[2][r][v] + red[3][r][v];
-      p.logits[row * p.V + v] = z[c];
+    for (int c = 0; c < NC; ++c) {
+      acc[c] = {0.0f, 0.0f, 0.0f, 0.0f};
+      w[c] = static_cast<const T*>(p.w) + min((int64_t)(16 * c + (lane & 15)), p.V - 1) * p.D;
     }
-    top = fmaxf(top, z[c]);
-  }
-#pragma unroll
-  for (int m = 1; m < 16; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
-  const float from = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    rest += below(z[c], from, c2);
-    most += z[c] == from ? 1.0f : 0.0f;
-  }
-  auto add = [&](int id, float prob) __attribute__((always_inline)) {
+    const T* x = static_cast<const T*>(p.x) + min(m0 + (lane & 15), p.T - 1) * p.D;
+    few_rows<T, NC, WHOLE>(x, w, p.D, acc);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
-      if (16 * c + l == id && prob != 0.0f) dot += prob * z[c];
-  };
-  if (p.target != nullptr) {
-    float flag;
-    add(target_of(p, row, &flag), 1.0f);
-  } else {
-    for (int e = 0; e < p.k; ++e) add(p.ids[row * p.k + e], p.prob[row * p.k + e]);
+#pragma unroll
+      for (int v = 0; v < 4; ++v) red[wave][lane & 15][16 * c + 4 * (lane >> 4) + v] = acc[c][v];
+    __syncthreads();
+    // 16 lanes a row, column 16 c + lane at z[c]
+    const int r = threadIdx.x >> 4, l = threadIdx.x & 15;
+    const int64_t row = m0 + r;
+    if (row < p.T) {
+      const float c2 = kLog2e / p.tau;
+      float z[NC], top = -INFINITY, rest = 0.0f, most = 0.0f, dot = 0.0f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int v = 16 * c + l;
+        z[c] = -INFINITY;
+        if (v < p.V) {
+          z[c] = red[0][r][v] + red[1][r][v] + red[2][r][v] + red[3][r][v];
+          p.logits[row * p.V + v] = z[c];
+        }
+        top = fmaxf(top, z[c]);
+      }
+#pragma unroll
+      for (int m = 1; m < 16; m *= 2) top = fmaxf(top, __shfl_xor(top, m));
+      const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        rest += below(z[c], from, c2);
+        most += z[c] == from ? 1.0f : 0.0f;
+      }
+      auto add = [&](int id, float prob) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          if (16 * c + l == id && prob != 0.0f) dot += prob * z[c];
+      };
+      if (p.target != nullptr) {
+        float flag;
+        add(target_of(p, row, &flag), 1.0f);
+      } else {
+        for (int e = 0; e < p.k; ++e) add(p.ids[row * p.k + e], p.prob[row * p.k + e]);
+      }
+      rest = lane_sum<16>(rest);
+      most = lane_sum<16>(most);
+      if (top > -INFINITY) rest += most - 1.0f;
+      dot = lane_sum<16>(dot);
+      if (l == 0) finish_row(p, row, top, rest, dot, loss);
+    }
+    __syncthreads();
   }
-  rest = lane_sum<16>(rest);
-  most = lane_sum<16>(most);
-  if (top > -INFINITY) rest += most - 1.0f;
-  dot = lane_sum<16>(dot);
-  if (l == 0) finish_row(p, row, top, rest, dot, loss);
 }
+
 // ---- sums of the rows -------------------------------------------------------------------
 constexpr int kOneBlock = 1024;
 template <typename V>
@@ -733,7 +754,8 @@ struct Places {
 };
 
 // 512 MiB of a piece's logits or dz: 8192 rows of 32768 columns in 16 bits, products
-// that are as long as the tiles can use.
+// that are as long as the tiles can use; past 262144 rows (131072 in fp32) 1024 columns,
+// whatever they take.
 constexpr int64_t kPieceBytes = (int64_t)1 << 29;
 int64_t piece_columns(int dtype, int64_t T, int64_t V) {
   const int64_t most =
@@ -790,7 +812,7 @@ HalfPlan plan_product(int dtype, int op, int64_t T, int64_t cols, int64_t D) {
 template <typename T, class G, int PARTS>
 int launch_vocab_tile(const VocabParams& p, hipStream_t st) {
   const int64_t tiles_n = ceil_div(p.cols, G::BN), blocks = dense_grid(p.T, G::BM, tiles_n);
-  if (blocks > 0x7fffffff) return set_error(KAN_ERR_LIMIT, "vocab_loss: too many tiles");
+  if (!grid_fits(blocks, G::NT)) return set_error(KAN_ERR_LIMIT, "vocab_loss: too many tiles");
   if (whole_rows(p.x, p.ldx) && whole_rows(p.w, p.ldw))
     vocab_tile_kernel<T, G, kDirect, PARTS><<<dim3((unsigned)blocks), G::NT, 0, st>>>(p, (int)tiles_n);
   else
@@ -813,7 +835,7 @@ int launch_vocab_tiles(int dtype, const VocabParams& p, HalfCfg cfg, hipStream_t
 template <bool GRAD>
 int launch_vocab_span(const VocabParams& p, hipStream_t st) {
   const int64_t spans = std::min<int64_t>(ceil_div(p.cols, kSpan), 65535);
-  vocab_span_kernel<GRAD><<<dim3((unsigned)ceil_div(p.T, 4), (unsigned)spans), 256, 0, st>>>(p);
+  vocab_span_kernel<GRAD><<<dim3(row_blocks(p.T, 4), (unsigned)spans), 256, 0, st>>>(p);
   return check_launch("vocab_loss");
 }
 
@@ -947,7 +969,7 @@ void launch_prepare(const VocabParams& p, const Upstream& u, char* out, int64_t 
 }
 template <typename T, bool WHOLE>
 int launch_few_classes(const VocabParams& p, float* loss, hipStream_t st) {
-  const dim3 blocks((unsigned)ceil_div(p.T, kFewRows));
+  const unsigned blocks = row_blocks(p.T, kFewRows);
   if (p.V <= 16) vocab_few_kernel<T, 1, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
   else vocab_few_kernel<T, 2, WHOLE><<<blocks, 256, 0, st>>>(p, loss);
   return check_launch("vocab_loss");
@@ -1029,7 +1051,7 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
     p.target64 = ids64;
     p.ignore = ignore_index;
   } else {
-    vocab_teacher_kernel<<<dim3((unsigned)T), 64, 0, st>>>(p, ids, ids64, teacher);
+    vocab_teacher_kernel<<<row_blocks(T, 1), 64, 0, st>>>(p, ids, ids64, teacher);
     e = check_launch(who);
   }
   float* rows = reduction == KAN_REDUCE_NONE ? loss : f.rows;
@@ -1066,7 +1088,7 @@ int kan_hip_vocab_loss(int dtype, const void* x, const void* w, const void* ids,
     if (e != KAN_OK) return e;
   }
   if (!few)
-    vocab_rows_kernel<<<dim3((unsigned)ceil_div(T, kBlockRows)), 64 * kRowWaves, 0, st>>>(p, rows);
+    vocab_rows_kernel<<<row_blocks(T, kBlockRows), 64 * kRowWaves, 0, st>>>(p, rows);
   if (reduction != KAN_REDUCE_NONE)
     vocab_sum_kernel<<<1, kOneBlock, 0, st>>>(p, rows, reduction == KAN_REDUCE_MEAN, loss);
   return check_launch(who);

@@ -552,9 +552,9 @@ GatedPlan plan_gated(int dtype, const void* x, const void* w, int64_t T, int64_t
   if (dtype == KAN_DTYPE_F32) {
     if (!keep) g.pre_bytes = (size_t)round_up(8 * T * N, 16);
     g.bytes = g.pre_bytes + product_part_bytes(KAN_GROUPED_FORWARD, g.plan, T, E, 2 * N, K);
-  } else {
+  } else if (E > 0 && K > 0) {  // (without experts or inputs nothing is read)
     g.align = align_plan(KAN_GROUPED_FORWARD, KAN_ACT8_NONE, x, w, T, E, 2 * N, K);
-    g.plan.cuts = g.plan.cfg == kSmall && E > 0 && K > 0 ? gated_cuts(T, E, N, K) : 1;
+    g.plan.cuts = g.plan.cfg == kSmall ? gated_cuts(T, E, N, K) : 1;
     g.pre_bytes = (size_t)round_up((int64_t)(g.align.a_bytes + g.align.b_bytes), 16);
     g.bytes = g.pre_bytes + product_part_bytes(KAN_GROUPED_FORWARD, g.plan, T, E, 2 * N, K);
   }

@@ -115,6 +115,8 @@ SIGNATURES = {
                                          + [ctypes.POINTER(_sz)]),
     "kan_hip_grouped_matmul_plan": (_int, [_int, _int, _vp, _vp, _int] + [_i64] * 4
                                     + [ctypes.POINTER(_i64)]),
+    "kan_hip_grouped_matmul_dense_plan": (_int, [_int, _int, _vp, _vp] + [_i64] * 3
+                                          + [ctypes.POINTER(_i64)]),
     "kan_hip_grouped_matmul": (_int, [_int, _int, _vp, _vp, _int, _vp, _i64, _vp, _int]
                                + [_i64] * 4 + [_vp, _vp, _sz, _vp]),
     "kan_hip_grouped_matmul_scaled": (_int, [_int, _int] + [_vp] * 3 + [_int] + [_i64] * 4

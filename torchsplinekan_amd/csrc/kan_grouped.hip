@@ -550,13 +550,13 @@ int kan_hip_grouped_matmul_workspace(int dtype, int op, const void* a, const voi
   return KAN_OK;
 }
 
-int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b, int b_format,
-                                int64_t T, int64_t E, int64_t N, int64_t K, int64_t* plan) {
+static int report_plan(int dtype, int op, const void* a, const void* b, int b_format, int64_t T,
+                       int64_t E, int64_t N, int64_t K, bool dense, int64_t* plan) {
   if (plan == nullptr)
     return set_error(KAN_ERR_INVALID, "grouped_matmul_plan: plan must not be NULL");
   const int rc = check_grouped(dtype, op, T, E, N, K);
   if (rc != KAN_OK) return rc;
-  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K);
+  const Workspace w = plan_call(dtype, op, b_format, a, b, T, E, N, K, dense);
   const bool f32 = dtype == KAN_DTYPE_F32, few = w.plan.cfg == kFew;
   const int rows[] = {256, 192, 128, kFewRows};  // by HalfCfg
   plan[0] = f32 && !few ? grouped_f32_rows(op, T, E, N, K) : rows[w.plan.cfg];
@@ -572,6 +572,16 @@ int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b,
     plan[5] = bytes ? (whole_a ? 1 : 0) : whole_a && whole_b ? 3 : 0;
   }
   return KAN_OK;
+}
+
+int kan_hip_grouped_matmul_plan(int dtype, int op, const void* a, const void* b, int b_format,
+                                int64_t T, int64_t E, int64_t N, int64_t K, int64_t* plan) {
+  return report_plan(dtype, op, a, b, b_format, T, E, N, K, false, plan);
+}
+
+int kan_hip_grouped_matmul_dense_plan(int dtype, int op, const void* a, const void* b, int64_t T,
+                                      int64_t N, int64_t K, int64_t* plan) {
+  return report_plan(dtype, op, a, b, KAN_ACT8_NONE, T, 1, N, K, true, plan);
 }
 
 static int grouped_matmul(int dtype, int op, const void* a, const void* b, int b_format,

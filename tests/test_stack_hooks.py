@@ -1,0 +1,28 @@
+"""KANExpertStack's logits and losses go through the module's call, with its hooks."""
+
+import torch
+
+from torchsplinekan_amd import KANExpertStack
+
+
+def test_hooks_run_for_logits_and_losses():
+    torch.manual_seed(0)
+    net, seen = KANExpertStack(8, 1, 2, num_classes=5), []
+    net.register_forward_pre_hook(lambda m, args: seen.append("before"))
+    net.register_forward_hook(lambda m, args, out: 2 * out)
+    x = torch.randn(4, 8)
+    h = net(x)
+    torch.testing.assert_close(net.logits(x), h @ net.head.t())
+    values, ids = net.logits(x).topk(2)
+    net.loss(x, torch.tensor([0, 1, 2, 3]))
+    net.distillation_loss(x, ids, values.detach())
+    assert seen == ["before"] * 5
+
+
+def test_logits_under_autocast_are_those_without():
+    torch.manual_seed(0)
+    net, x = KANExpertStack(8, 1, 2, num_classes=5), torch.randn(4, 8)
+    want = net.logits(x)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        got = net.logits(x)
+    assert got.dtype == torch.float32 and torch.equal(got, want)

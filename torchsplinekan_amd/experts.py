@@ -195,8 +195,9 @@ class KANExpertStack(nn.Module):
     def logits(self, x: torch.Tensor) -> torch.Tensor:
         """head h of the stack's rows h, [..., num_classes]."""
         head = self._head()
+        h = self(x)
         with torch.autocast(x.device.type, enabled=False):
-            return F.linear(self._forward(x), head)
+            return F.linear(h, head)
 
     def loss(self, x: torch.Tensor, target: torch.Tensor, **kw) -> torch.Tensor:
         """linear_cross_entropy of the stack's rows against target [...]; further

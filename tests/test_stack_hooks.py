@@ -1,6 +1,8 @@
-"""KANExpertStack's logits and losses go through the module's call, with its hooks."""
+"""KANExpertStack's logits and losses go through the module's call, with its hooks, and its
+norms each have their eps."""
 
 import torch
+import torch.nn.functional as F
 
 from torchsplinekan_amd import KANExpertStack
 
@@ -26,3 +28,15 @@ def test_logits_under_autocast_are_those_without():
     with torch.autocast("cpu", dtype=torch.bfloat16):
         got = net.logits(x)
     assert got.dtype == torch.float32 and torch.equal(got, want)
+
+
+def test_the_input_norm_has_an_eps_of_its_own():
+    torch.manual_seed(0)
+    kw = dict(num_experts=2, eps=0.5, input_norm=True, input_eps=0.25)
+    net, x = KANExpertStack(8, 1, **kw).double(), torch.randn(4, 8, dtype=torch.float64)
+    plain = KANExpertStack(8, 1, num_experts=2, eps=0.5).double()
+    plain.load_state_dict(net.state_dict(), strict=False)
+    for eps in (0.25, 2.0):
+        net.input_eps = eps
+        torch.testing.assert_close(net(x), plain(F.layer_norm(x, (8,), eps=eps)))
+    assert KANExpertStack(8, 1, 2, input_norm=True).input_eps == 1e-5

@@ -146,12 +146,13 @@ class KANExpertStack(nn.Module):
     scale and addition run in one pass with the next block's first norm.
     feed_forward > 0: every block adds a gated feed-forward block of that many
     outputs, which all rows pass, to its experts.  input_norm: x passes a layer
-    norm first.  num_classes: a last layer head [num_classes, width] for logits,
-    loss and distillation_loss.  Further arguments go to each KANExperts."""
+    norm first, with input_eps (eps is the other norms').  num_classes: a last layer
+    head [num_classes, width] for logits, loss and distillation_loss.  Further
+    arguments go to each KANExperts."""
 
     def __init__(self, width: int, depth: int, num_experts: int, residual_scale: float = 0.2,
                  eps: float = 1e-6, feed_forward: int = 0, input_norm: bool = False,
-                 num_classes: Optional[int] = None, **experts) -> None:
+                 num_classes: Optional[int] = None, input_eps: float = 1e-5, **experts) -> None:
         super().__init__()
         if depth < 1:
             raise ValueError(f"depth must be >= 1, got {depth}")
@@ -163,7 +164,7 @@ class KANExpertStack(nn.Module):
             _Block(width, residual_scale, feed_forward, num_experts=num_experts, **experts)
             for _ in range(depth)])
         self.norm_weight = nn.Parameter(torch.ones(width))
-        self.eps = eps
+        self.eps, self.input_eps = eps, input_eps
         self.input_weight = self.input_bias = self.head = None
         if input_norm:
             self.input_weight = nn.Parameter(torch.ones(width))
@@ -178,7 +179,7 @@ class KANExpertStack(nn.Module):
 
     def _forward(self, x: torch.Tensor) -> torch.Tensor:
         if self.input_weight is not None:
-            x = layer_norm(x, self.input_weight, self.input_bias)
+            x = layer_norm(x, self.input_weight, self.input_bias, eps=self.input_eps)
         x, h = residual_norm(x, pre_weight=self.blocks[0].pre_weight, eps=self.eps)
         for block, after in zip(self.blocks, [*self.blocks[1:], None]):
             x, h = residual_norm(

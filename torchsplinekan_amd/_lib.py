@@ -238,8 +238,7 @@ def launch(fn, device: torch.device, *args) -> None:
         check(status)
 
 
-_is_tracing, _dispatch_mode = torch._C._is_tracing, torch._C._get_dispatch_mode
-_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_is_tracing, _dispatch_modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
 
 
 def traced() -> bool:
@@ -247,7 +246,8 @@ def traced() -> bool:
     and torch's own operations, and of a bare launch nothing but the empty results.
     make_fx with real tensors looks below apply too and would record those empty
     results: refused.  (With fake tensors there is no memory to launch on.)"""
-    if _dispatch_mode(_PROXY) is not None:
+    if (_dispatch_modes() and torch._C._get_dispatch_mode(
+            torch._C._TorchDispatchModeKey.PROXY) is not None):
         raise RuntimeError("the device kernels cannot be recorded by make_fx")
     return _is_tracing()
 
@@ -256,8 +256,7 @@ def call(function, save: bool, *args):
     """`function`, an autograd function, of args: through apply where its backward pass
     is wanted (save), under forward mode (which apply refuses) and where the call is
     traced; otherwise its forward alone, which is shorter on the host."""
-    if (save or _is_tracing() or _dispatch_mode(_PROXY) is not None
-            or _forward_ad._current_level >= 0):
+    if save or _is_tracing() or _dispatch_modes() or _forward_ad._current_level >= 0:
         traced()  # (raises under make_fx)
         return function.apply(*args)
     return function.forward(None, *args)

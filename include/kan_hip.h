@@ -524,7 +524,8 @@ int kan_hip_grouped_matmul_scaled(int dtype, int op, const void* a, const void* 
  * FP16: grad_pre holds what that type can of it; the scaled form writes it times a power of
  * two, 1 where its largest finite value is within 1 .. 2^15 and otherwise the one that takes
  * that to 2^14 .. 2^15, and one over that power to scale[0] for
- * kan_hip_grouped_matmul_scaled (scale has room for KAN_GATED_SCALE_VALUES). */
+ * kan_hip_grouped_matmul_scaled (scale has room for KAN_GATED_SCALE_VALUES; with T or N
+ * = 0 nothing is written). */
 #define KAN_GATED_SCALE_VALUES 8192
 int kan_hip_gated_kept(int dtype, int64_t T, int64_t N, size_t* bytes);
 int kan_hip_gated_workspace(int dtype, const void* x, const void* w, int64_t T, int64_t E, int64_t N,
@@ -543,7 +544,7 @@ int kan_hip_gated_backward_scaled(int dtype, int act, const void* grad_h, const 
  *   loss_t = tau^2 sum_j p_j (log p_j - log q_{id_j}).
  * teacher NULL: cross entropy, k = 0, ids [T] with p = 1 each; rows whose id is
  * ignore_index do not count.  teacher [T, k]: p = softmax(teacher / tau) over the row's ids; ids below 0
- * are absent, equal ids add, and rows without any do not count.  ids [T, k] are int32 or int64
+ * are absent, equal ids add, and rows without any, or with logits of -inf alone, do not count.  ids [T, k] are int32 or int64
  * (ids64); one that is neither a column nor such makes its row's loss and its
  * gradients NaN.  A row that does not count may hold
  * anything.  reduction: the rows' losses [T] (0 where a row does not count),

@@ -15,7 +15,8 @@
 // exponent and leading 7 bits of mantissa, and 4 (bf16) or 8 (f16) bits more of
 // each in a second array: 20 or 24 bits.  Gradients are then off by what the
 // operands of their products and their own rounding make (normwise 0.0023 in bf16,
-// 0.00030 in f16); with g and u in the type itself they would be off by 0.0029 and
+// 0.00030 in f16, where [dg du] is stored times a power of 2 if its largest value asks for
+// it); with g and u in the type itself they would be off by 0.0029 and
 // 0.00037, and in float32 the kept values and the bytes both passes move for them
 // would be 1.6 (1.3) times as many.
 #include "kan_grouped.h"
@@ -38,8 +39,8 @@ struct GatedParams : GroupedParams {  // N: outputs; B [E, 2 N, K]; C: h
 inline size_t word_bytes(int64_t T, int64_t N) { return (size_t)round_up(4 * T * N, 16); }
 
 // ---- activations --------------------------------------------------------------
-// For 16-bit results: exponentials and reciprocals of the hardware, a few units of
-// 2^-24 off.
+// For 16-bit results: exponentials and reciprocals of the hardware, off by a few units of
+// 2^-24 and by |v| more, for the rounding of the exponential's argument.
 __device__ __forceinline__ float quick_sigmoid(float v) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * v));
 }

@@ -470,40 +470,40 @@ __device__ __forceinline__ void few_rows(const T* x, const T* (&w)[NC], int64_t 
   typedef RowsMma<T> M;
   constexpr int V = 16 / sizeof(T), U = 4;  // values of a load, loads of a lane's turn
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-      auto load = [](const T* q) __attribute__((always_inline)) {
-        if constexpr (sizeof(T) == 2 && !WHOLE)
-          return __builtin_bit_cast(typename M::vec, load16_even(q));
-        else
-          return reinterpret_cast<const LooseVec<T, V>*>(q)->v;
-      };
-      constexpr int kTurn = 4 * U * V;
-      for (int64_t k0 = wave * kTurn; k0 < K; k0 += 4 * kTurn) {
-        typename M::vec a[NC][U], b[U];
-        const int64_t k = k0 + (lane >> 4) * V;
-        if (k0 + kTurn <= K) {
-  #pragma unroll
-          for (int u = 0; u < U; ++u) {
-  #pragma unroll
-            for (int c = 0; c < NC; ++c)
-              a[c][u] = load(w[c] + k + u * 4 * V);
-            b[u] = load(x + k + u * 4 * V);
-          }
-        } else {
-  #pragma unroll
-          for (int u = 0; u < U; ++u)
-  #pragma unroll
-            for (int j = 0; j < V; ++j) {
-              const int64_t at = k + u * 4 * V + j;
-  #pragma unroll
-              for (int c = 0; c < NC; ++c) a[c][u][j] = at < K ? w[c][at] : (T)0.0f;
-              b[u][j] = at < K ? x[at] : (T)0.0f;
-            }
-        }
-  #pragma unroll
-        for (int u = 0; u < U; ++u)
-  #pragma unroll
-          for (int c = 0; c < NC; ++c) acc[c] = M::mma(a[c][u], b[u], acc[c]);
+  auto load = [](const T* q) __attribute__((always_inline)) {
+    if constexpr (sizeof(T) == 2 && !WHOLE)
+      return __builtin_bit_cast(typename M::vec, load16_even(q));
+    else
+      return reinterpret_cast<const LooseVec<T, V>*>(q)->v;
+  };
+  constexpr int kTurn = 4 * U * V;
+  for (int64_t k0 = wave * kTurn; k0 < K; k0 += 4 * kTurn) {
+    typename M::vec a[NC][U], b[U];
+    const int64_t k = k0 + (lane >> 4) * V;
+    if (k0 + kTurn <= K) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          a[c][u] = load(w[c] + k + u * 4 * V);
+        b[u] = load(x + k + u * 4 * V);
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int64_t at = k + u * 4 * V + j;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) a[c][u][j] = at < K ? w[c][at] : (T)0.0f;
+          b[u][j] = at < K ? x[at] : (T)0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) acc[c] = M::mma(a[c][u], b[u], acc[c]);
+  }
 }
 
 // ---- host ---------------------------------------------------------------------

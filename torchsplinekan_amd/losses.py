@@ -179,8 +179,9 @@ def linear_distillation(x: torch.Tensor, weight: torch.Tensor, ids: torch.Tensor
     over all V, in float32 and without the student's logits.
 
     x [..., D]; weight [V, D]; ids [..., k], int32 or int64, k <= 1024: columns in
-    any order (equal ones add); those below 0 are absent, and a row without any
-    does not count.  An id from V on makes its row's loss and its gradients NaN.
+    any order (equal ones add); those below 0 are absent, and a row without any, or
+    with logits of -inf alone, does not count.  An id from V on makes its row's loss
+    and its gradients NaN.
     teacher [..., k]: its logits at ids, float32, bfloat16 or float16; no gradient
     reaches it.  reduction, types and gradients as linear_cross_entropy."""
     who = "linear_distillation"

@@ -9,9 +9,9 @@
 // what is left of the values goes into the mean: a constant row becomes zero, and rows far
 // from zero are off by the mean's own rounding.  All arithmetic is in float32, rounded once where a result is stored.  The column
 // sums go through one partial row a block, added in block order: no atomics, the
-// same bits every time.  Bound by HBM: 16384 rows of 4096 in bf16, forward 45 us (6.0
-// TB/s, part of it from the last-level cache), forward and backward 137 us for 671 MB;
-// 32768 x 1024 in float32 42 and 140 us.
+// same bits every time.  Bound by HBM: 16384 rows of 4096 in bf16, forward 47 us (5.7
+// TB/s, part of it from the last-level cache), forward and backward 138 us for 671 MB (135
+// without the mean's second part); 32768 x 1024 in float32 42 and 140 us.
 #include "kan_norm.h"
 
 namespace kan {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(RowShape<TPR>::kThreads) void layer_norm_grad_kerne
 }
 
 // Rows wider than registers hold, one at a time, read again in every pass (4096 x 16392
-// in bf16: forward 215 us, 16384 columns 50).
+// in bf16: forward 217 us, 16384 columns 52).
 template <typename TX, typename TY>
 __global__ __launch_bounds__(kRowThreads) void layer_norm_rows_kernel(LayerNormParams p) {
   __shared__ float red[kRowThreads / 64];
